@@ -365,6 +365,93 @@ int mz_qk_logits(const mz_kv_store* store, const void* query, long long q_stride
 int mz_av_output(const mz_kv_store* store, const void* weights, int w_dtype, int n_tokens, int q_heads,
                  void* out, int out_dtype, void* stream);
 
+/*
+ * ---- paged cache: rows of unlike lengths, pages that rows share, 4-bit codes (the reference has none: its store is one block per layer,
+ * muzero/cache/layer.py:183-217, and every batch entry has the same length).
+ *
+ * A row (sequence) of `length` tokens keeps its first Q = 64 * max(0, (length - residual) / 64) tokens in pages of 64 tokens and the others in
+ * 16 bits in its ring, token t at place t mod `ring`.  block_table[row][i] is the page of tokens 64 i .. 64 i + 63 in every layer, -1 where there
+ * is none; page_refs counts the rows that hold a page (0 = free).
+ *
+ * A page holds per kv head 72 * head_dim bytes: key codes [head_dim][32], key words [head_dim] of 32 bits, value codes [64][head_dim/64][32],
+ * value words [64][head_dim/64].  A row of 64 values (keys: a channel's 64 tokens, values: 64 channels of a token) has two codes to a byte, the
+ * earlier one in the lower half.  Code e stands for A + T * (book[z][e] - z) / 32.  Its word has T (f16) in the lower half, in the upper
+ * half z (0..127), or A (f16, |bits| >= 128) for a row that does not straddle zero: then z is 0 above zero, 127 below.  book[z] are the 16 levels of the
+ * zero-anchored log compander with alpha 2, in 127ths of the row's range (mz_paged_books).
+ *
+ * All index arrays are device memory (int32).  Errors that only the device can see are or-ed into *status and leave the memory alone:
+ */
+#define MZ_PAGED_NO_PAGES 1  /* extend: more pages needed than are free; nothing was changed */
+#define MZ_PAGED_TOO_LONG 2  /* extend: a row would outgrow its table row; nothing was changed */
+#define MZ_PAGED_BAD_INDEX 4 /* a row or page index outside the cache, or a row that is both source and target; skipped */
+
+typedef struct {
+  int layers, rows, pages, width;        /* width: entries of a row of the table */
+  int kv_heads, head_dim;                /* head_dim 64 or 128 */
+  int residual, ring;                    /* residual: a multiple of 64; ring >= residual + 64 */
+  int kv_dtype;                          /* MZ_F16 or MZ_BF16 */
+  void* store;                           /* [layers][pages][kv_heads][72 * head_dim] bytes */
+  long long store_stride_layer, store_stride_page;   /* bytes, multiples of 16 */
+  void* tail;                            /* [layers][rows][2 (key, value)][kv_heads][ring][head_dim] */
+  long long tail_stride_layer, tail_stride_row;      /* elements, multiples of 8 */
+  int *block_table, *lengths, *page_refs, *status;   /* [rows][width], [rows], [pages], [1] */
+} mz_paged_cache;
+
+/* book[128][16] and nearest[128][128] (the code of the level nearest r, ties to the lower code) as the kernels use them, on the host. */
+int mz_paged_books(unsigned char* book, unsigned char* nearest);
+
+/*
+ * Lengthens the rows rows[0..batch) (NULL: row i is i; distinct) by offsets[i+1] - offsets[i] tokens (NULL: one each) and gives them the pages that
+ * their new lengths need, the lowest free ones first, in the order of the list.  All or nothing.  batch <= 4096.
+ */
+int mz_paged_extend(const mz_paged_cache* cache, const int* rows, const int* offsets, int batch, void* stream);
+
+/*
+ * Writes the newest tokens of the rows (those that mz_paged_extend announced, with the same rows and offsets) of one layer: token j of list
+ * entry i is key/value token offsets[i] + j of `tokens`.  Whole groups that leave the residual window are quantized into their pages, the newest
+ * tokens go to the ring.  No entry brings more than max_new tokens.  Replaces the append + flush of muzero/cache/layer.py:351-459.
+ */
+int mz_paged_append(const mz_paged_cache* cache, int layer, const void* key, long long k_stride_token, long long k_stride_head, const void* value,
+                    long long v_stride_token, long long v_stride_head, const int* rows, const int* offsets, int batch, int tokens, int max_new,
+                    void* stream);
+
+/*
+ * out[b][l][h][:] (contiguous, the cache's type or fp32) = attention of query[b][l][h][:], the l-th of the newest q_len tokens of row rows[b], over the row's
+ * tokens up to its own.  Queries before the row's first token and rows without tokens give zeros.  q_heads is a multiple of kv_heads; batch <= 1024.
+ */
+typedef struct {
+  const void* query;
+  long long q_stride_b, q_stride_l, q_stride_h;      /* elements */
+  int batch, q_len, q_heads;
+  const int* rows;                                   /* NULL: row b is b */
+  float scaling;
+  void* out;
+  int out_dtype;
+  void* workspace;                                   /* 16-byte aligned */
+  size_t workspace_bytes;
+} mz_paged_attention_args;
+size_t mz_paged_attention_workspace_bytes(const mz_paged_cache* cache, int batch, int q_len, int q_heads);
+int mz_paged_attention(const mz_paged_cache* cache, int layer, const mz_paged_attention_args* args, void* stream);
+
+/*
+ * Row target[i] becomes a copy of row source[i], in all layers: what it held is released, the source's pages are shared (counted), its ring is
+ * copied as far as it is live.  Targets are distinct and no row is both.
+ */
+int mz_paged_fork(const mz_paged_cache* cache, const int* source, const int* target, int n, void* stream);
+
+/* Empties rows: their pages are released, those that no other row holds are free again. */
+int mz_paged_free(const mz_paged_cache* cache, const int* rows, int n, void* stream);
+
+/*
+ * Moves the live pages of the upper places into the free ones below, in all layers, the lowest to the lowest, so that n live pages stand in places
+ * 0 .. n-1, and rewrites the table and the counts.  workspace: mz_paged_compact_workspace_bytes() bytes.
+ */
+size_t mz_paged_compact_workspace_bytes(const mz_paged_cache* cache);
+int mz_paged_compact(const mz_paged_cache* cache, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Copies the contents of page source[i] to page target[i] in all layers (tables and counts stay).  No page is both, targets are distinct. */
+int mz_paged_copy_pages(const mz_paged_cache* cache, const int* source, const int* target, int n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ decode attention) as hand-written sm_100a CUDA behind the reference's plug-in AP
 from .config import MuZeroConfig
 from .quantizer import select_alpha, quantize_rows, dequantize_rows, roundtrip
 from .cache.layer import MuZeroCacheLayer
+from .cache.paged import MuZeroPagedCache
 from .cache.attention import get_mu_zero_decode_stats, mu_zero_decode_attention_forward, reset_mu_zero_decode_stats
 from .integrations.transformers_patch import MuZeroCache, patch_transformers
 
@@ -16,6 +17,7 @@ __all__ = [
     "MuZeroConfig",
     "MuZeroCacheLayer",
     "MuZeroCache",
+    "MuZeroPagedCache",
     "select_alpha",
     "quantize_rows",
     "dequantize_rows",

@@ -24,6 +24,8 @@ EXPORTS = (
     "mz_decode_attention_partial", "mz_lse_merge", "mz_qk_logits", "mz_av_output", "mz_decode_attention_static",
     "mz_decode_step", "mz_decode_step_workspace_bytes", "mz_flush_kv_parts", "mz_decode_workspace_bound", "mz_decode_attention_partial_packed", "mz_lse_merge_packed", "mz_store_gather_batch", "mz_debug_force_kernel", "mz_debug_fail_waits", "mz_debug_decode_kernel", "mz_bounds_violations",
     "mz_alpha_stats", "mz_alpha_stats_workspace_bytes", "mz_materialize_kv", "mz_roundtrip_kv", "mz_flush_kv_move",
+    "mz_paged_books", "mz_paged_extend", "mz_paged_append", "mz_paged_attention_workspace_bytes", "mz_paged_attention", "mz_paged_fork",
+    "mz_paged_free", "mz_paged_compact_workspace_bytes", "mz_paged_compact", "mz_paged_copy_pages",
 )
 
 
@@ -61,6 +63,33 @@ class DecodeArgs(Structure):
         ("out", c_void_p),
         ("out_dtype", c_int),
         ("splits", c_int),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class PagedCache(Structure):
+    _fields_ = [
+        ("layers", c_int), ("rows", c_int), ("pages", c_int), ("width", c_int),
+        ("kv_heads", c_int), ("head_dim", c_int),
+        ("residual", c_int), ("ring", c_int),
+        ("kv_dtype", c_int),
+        ("store", c_void_p),
+        ("store_stride_layer", c_longlong), ("store_stride_page", c_longlong),
+        ("tail", c_void_p),
+        ("tail_stride_layer", c_longlong), ("tail_stride_row", c_longlong),
+        ("block_table", c_void_p), ("lengths", c_void_p), ("page_refs", c_void_p), ("status", c_void_p),
+    ]
+
+
+class PagedAttentionArgs(Structure):
+    _fields_ = [
+        ("query", c_void_p),
+        ("q_stride_b", c_longlong), ("q_stride_l", c_longlong), ("q_stride_h", c_longlong),
+        ("batch", c_int), ("q_len", c_int), ("q_heads", c_int),
+        ("rows", c_void_p),
+        ("scaling", c_float),
+        ("out", c_void_p),
+        ("out_dtype", c_int),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t),
     ]
 
@@ -126,6 +155,19 @@ def load_library() -> ctypes.CDLL:
     lib.mz_alpha_stats_workspace_bytes.restype = c_size_t
     lib.mz_qk_logits.argtypes = [POINTER(KVStore), c_void_p, c_longlong, c_longlong, c_int, c_float, c_void_p, c_int, c_void_p]
     lib.mz_av_output.argtypes = [POINTER(KVStore), c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p]
+    lib.mz_paged_books.argtypes = [c_void_p, c_void_p]
+    lib.mz_paged_extend.argtypes = [POINTER(PagedCache), c_void_p, c_void_p, c_int, c_void_p]
+    lib.mz_paged_append.argtypes = [POINTER(PagedCache), c_int] + [c_void_p, c_longlong, c_longlong] * 2 + [c_void_p, c_void_p, c_int, c_int, c_int,
+                                                                                                            c_void_p]
+    lib.mz_paged_attention_workspace_bytes.argtypes = [POINTER(PagedCache), c_int, c_int, c_int]
+    lib.mz_paged_attention_workspace_bytes.restype = c_size_t
+    lib.mz_paged_attention.argtypes = [POINTER(PagedCache), c_int, POINTER(PagedAttentionArgs), c_void_p]
+    lib.mz_paged_fork.argtypes = [POINTER(PagedCache), c_void_p, c_void_p, c_int, c_void_p]
+    lib.mz_paged_free.argtypes = [POINTER(PagedCache), c_void_p, c_int, c_void_p]
+    lib.mz_paged_compact_workspace_bytes.argtypes = [POINTER(PagedCache)]
+    lib.mz_paged_compact_workspace_bytes.restype = c_size_t
+    lib.mz_paged_compact.argtypes = [POINTER(PagedCache), c_void_p, c_size_t, c_void_p]
+    lib.mz_paged_copy_pages.argtypes = [POINTER(PagedCache), c_void_p, c_void_p, c_int, c_void_p]
     _lib = lib
     return lib
 
