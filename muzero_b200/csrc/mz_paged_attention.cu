@@ -12,17 +12,28 @@
 //
 // Work.  A query row is one (token, head) that shares a kv head; NR of them (4, or 8 above 4) go through a step together, more take several
 // passes.  The steps of all (list entry, kv head, pass) pairs stand in one line that is cut evenly over the CTAs on the device, from the lengths it
-// finds there; a CTA leaves a record (m, l, out) per pair that it met, slot = CTA + pair.  The 16-bit tokens of the rings go to CTAs of their own in
-// the same launch (mma.sync), one record per pair.  A second kernel merges a pair's records.
+// finds there; a CTA leaves a record (m, l, out) per pair that it met, slot = CTA + pair.  The 16-bit tokens of the rings are shared out over the CTAs
+// as well; their records follow.  A second kernel merges a pair's records.
 //
-// A CTA that has steps: four warps expand keys, one step ahead, four warps have softmax and values.  MMAs are issued by one thread of each team.  Every
-// mbarrier wait is bounded; one that runs out makes the CTA's records NaN and ends its MMAs.
+// A CTA is four groups of four warps, two CTAs to an SM:
+//   keys     expand the keys' codes and scale the queries, up to two steps ahead of
+//   values   logits, softmax, expansion of the values, running output (thread = token, then channel)
+//   rings    16-bit tokens on mma.sync, from memory; they fill the gaps of the others
+//   service  a warp that walks the line, looks pages up and has them copied to shared memory (bulk copies: keys two steps ahead, values three),
+//            one that finds a step's largest T, and one each that issues the MMAs of the keys and of the values
+// mbarriers tie them together.  Every wait is bounded; one that runs out makes the CTA's records NaN and ends its MMAs.
 #include "mz_paged.cuh"
 
 namespace mzp {
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int THREADS = 256, MAX_BATCH = 1024;
+constexpr int THREADS = 512, MAX_BATCH = 1024, CTAS_PER_SM = 2;
 constexpr int SPIN_LIMIT = 1000000;              // looks of a wait before it gives up; afterwards one look each
+// registers: 4 x 32 threads each of keys (as launched), values, rings and service share 512 x 64
+template <int NR>
+struct Regs {
+  static constexpr int VALUES = NR == 4 ? 88 : 104, RINGS = NR == 4 ? 72 : 64, SERVICE = NR == 4 ? 32 : 24;
+  static_assert(64 + VALUES + RINGS + SERVICE <= 4 * 64, "register split");
+};
 constexpr int STEP = 2 * MZP_PAGE;
 
 struct Args {
@@ -33,6 +44,7 @@ struct Args {
   void* out;
   int out_dtype, layer, batch, q_len, q_heads, group;      // group: query heads per kv head
   int qrows, passes;                             // query rows per kv head, and how many passes of NR they take
+  int parts;                                     // that a ring's tiles are cut in
   float scaling;                                 // times log2(e)
   // workspace: header {CTAs with steps, pad, steps (64 bits)}, steps before each entry [batch + 1], records
   int* head;
@@ -58,9 +70,14 @@ __device__ __forceinline__ uint4 book128(uint32_t a) {      // constant after th
   asm("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
-__device__ __forceinline__ uint4 ldg128(const void* p) {    // pages are read once
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
 }
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -72,18 +89,32 @@ __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t n) { asm volatil
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.shared::cta.b64 t, [%0];\n\t}\n" ::"r"(bar) : "memory");
 }
-// Waits for the phase of this parity.  Who gives up says so before it goes on.
-__device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile int* s_failed, bool& failed) {
-  const int limit = failed ? 1 : SPIN_LIMIT;
-  for (int it = 0; it < limit; ++it) {
-    uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}\n"
-                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    if (done) return;
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;\n\t}\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+// global -> shared, 16-byte aligned, a multiple of 16 bytes
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}\n"
+               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+// Waits for the phase of this parity.  Who gives up says so before it goes on; the others notice.
+__device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile int* s_failed) {
+  for (int it = 0; it < SPIN_LIMIT; ++it) {
+    if (bar_test(bar, parity)) return;
+    if ((it & 255) == 255 && *s_failed) return;
   }
-  failed = true;
   *s_failed = 1;
 }
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 // shared-memory operand, not swizzled, major along the kept dimension: cores of 8 rows x 16 bytes, 128 bytes apart along the reduction,
 // `chunk` bytes apart along the kept dimension
 __device__ __forceinline__ uint64_t descriptor(uint32_t sa, uint32_t chunk) {
@@ -151,12 +182,12 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// a page's row of 64 codes -> 64 bytes, stored as four pieces of 16, `chunk` bytes apart.  A selector's top bit asks for the sign of a level, which is
-// zero: so the two permutes of a nibble are zero exactly where they are not meant, and their results are or-ed.
-__device__ __forceinline__ void expand_row(const uint4& lo, const uint4& hi, const uint4& book, uint32_t dst, uint32_t chunk) {
-  const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+// 32 codes of a row -> 32 bytes, two pieces of 16, `chunk` bytes apart.  A selector's top bit asks for the sign of a level, which is zero: so the two
+// permutes of a nibble are zero exactly where they are not meant, and their results are or-ed.
+__device__ __forceinline__ void expand_half(const uint4& codes, const uint4& book, uint32_t dst, uint32_t chunk) {
+  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < 2; ++q) {
     uint32_t o[4];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -167,47 +198,71 @@ __device__ __forceinline__ void expand_row(const uint4& lo, const uint4& hi, con
     sts128(dst + q * chunk, o[0], o[1], o[2], o[3]);
   }
 }
+// A row's 32 bytes of codes at `src` -> its 64 levels.  Of eight neighbouring threads the upper four take the second half first: then the
+// eight read from different banks.
+__device__ __forceinline__ void expand_row(uint32_t src, const uint4& book, uint32_t dst, uint32_t chunk, int lane) {
+  const uint32_t half = (lane >> 2) & 1;
+  const uint4 first = lds128(src + 16 * half), second = lds128(src + 16 - 16 * half);
+  expand_half(first, book, dst + 2 * half * chunk, chunk);
+  expand_half(second, book, dst + 2 * (1 - half) * chunk, chunk);
+}
 
 // shared memory of a CTA
+constexpr int K_STAGES = 2, V_STAGES = 3;
 template <int D, int NR>
 struct Smem {
   static constexpr int ROWS = D;                           // rows of the keys' operand = rows of the values' operand (D == 128: 128 tokens)
   static constexpr int CHUNK = ROWS * 16;
   static constexpr int A_BYTES = 8 * CHUNK;                // 128 positions
   static constexpr int B_BYTES = 2 * NR * 4 / 16 * CHUNK;  // 2 blocks x NR x 4 bytes
-  static constexpr int K_A = 0, V_A = A_BYTES, K_B = 2 * A_BYTES, V_B = K_B + B_BYTES;
-  static constexpr int OPERANDS = V_B + B_BYTES;
-  static constexpr int RINGS = 8 * NR * D * 4;             // a ring CTA's partial outputs lie over the operands
-  static constexpr int BOOK = OPERANDS > RINGS ? OPERANDS : RINGS;
-  static constexpr int TOTAL = BOOK + MZP_BOOKS * MZP_LEVELS;
+  static constexpr int SIDE = 36 * D;                      // keys or values of a page, as they come from memory
+  static constexpr int K_A = 0, V_A = A_BYTES, K_B = 2 * A_BYTES, V_B = K_B + B_BYTES, K_IN = V_B + B_BYTES;
+  static constexpr int V_IN = K_IN + K_STAGES * 2 * SIDE, BOOK = V_IN + V_STAGES * 2 * SIDE;
+  static constexpr int QUERY = BOOK + MZP_BOOKS * MZP_LEVELS;          // the ring warps' queries [8][D], rows 16 bytes apart in the banks
+  static constexpr int Q_ROW = 2 * D + 16;
+  static constexpr int TOTAL = QUERY + 8 * Q_ROW;
   static constexpr int N = 8 * NR, TM_S = 0, TM_O = 2 * N, TM_COLS = NR == 4 ? 128 : 256;
-  static constexpr int CTAS = NR == 4 ? 3 : 2;             // per SM
+};
+// what a step is, for those who work on it
+struct StepInfo {
+  int pair, fresh;                          // the pair's number; whether this is the CTA's first step of it
+  int count, see;                           // tokens of the step; the last position that the pair's first query token sees
+  int b, head, r0, valid;                   // list entry, kv head, first query row; bit p: page p is there
 };
 // exchange between the warps of a CTA
 template <int NR>
 struct Exchange {
-  float base[4][4][2 * NR];                 // constant terms of the logits, by step and key warp (keys run up to two steps ahead)
-  float fin[4][4 * NR];                     // end of a pair: sums of p, constant terms of the output
-  float qs[4][NR];                          // logit per unit of the scaled query, by pair
-  float qmax[4][4][NR];                     // largest |q|, by pair and warp
-  float vmax[2][4][NR];                     // largest logit, by step parity and warp
-  uint32_t kt[4][4], vt[2][4];              // largest T (bits) of the keys, by step and warp; of the values
-  float ring_m[8][NR], ring_l[8][NR];
-  unsigned long long bar[6];                // products of the keys done [2], their sums read [2], products of the values done, end
-  int warp_sum[8][2];
+  alignas(16) float base[4][4][2 * NR];     // constant terms of the logits, by step and key warp (keys run up to two steps ahead)
+  alignas(16) float fin[4][4 * NR];         // end of a pair: sums of p, constant terms of the output
+  alignas(16) float qs[4][NR];              // logit per unit of the scaled query, by pair
+  alignas(16) float vmax[2][4][NR];         // largest logit, by step parity and warp
+  alignas(16) StepInfo info[4];             // by step
+  float qmax[2][4][NR];                     // largest |q|, by pair and warp
+  uint32_t kt[4], vt[4];                    // largest T (bits) of the step's keys, values
+  // copied [stage], scaled [stage] and used [stage] of keys and values; operand written, products done [2], sums read [2] of the keys; operand
+  // written, products done of the values; end
+  unsigned long long bar[3 * (K_STAGES + V_STAGES) + 8];
+  int warp_sum[16];
   uint32_t tmem;
   int failed;
   int prefix[MAX_BATCH + 1];                // steps of the entries before
 };
-
-struct Cursor { int b, kp, step, steps; };
+template <int N>
+__device__ __forceinline__ void load_floats(float (&v)[N], const float* s) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const float4 f = *(const float4*)(s + i);
+    v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+  }
+}
 
 template <int D, bool BF, int NR>
-__global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel(const Args p, const uint8_t* __restrict__ book_table) {
+__global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const Args p, const uint8_t* __restrict__ book_table) {
   using S = Smem<D, NR>;
   constexpr int DT = BF ? MZ_BF16 : MZ_F16;
   constexpr int PB = 72 * D;                     // page bytes per kv head
   constexpr int RPT = D / 64;                    // rows of codes per thread, side and step
+  constexpr int STREAMS = D == 128 ? 2 : 4;      // records of a ring's part
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Exchange<NR> x;
   const mz_paged_cache& c = p.c;
@@ -215,54 +270,45 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   const uint32_t sbase = smem_u32(smem), sbook = sbase + S::BOOK;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t bars = smem_u32(x.bar);
-  const uint32_t k_done = bars, k_free = bars + 16, v_done = bars + 32, b_end = bars + 40;
+  const uint32_t k_full = bars, k_scaled = k_full + 8 * K_STAGES, k_used = k_scaled + 8 * K_STAGES;
+  const uint32_t v_full = k_used + 8 * K_STAGES, v_scaled = v_full + 8 * V_STAGES, v_used = v_scaled + 8 * V_STAGES;
+  const uint32_t k_ready = v_used + 8 * V_STAGES, k_done = k_ready + 8, k_free = k_done + 16, v_ready = k_free + 16, v_done = v_ready + 8, b_end = v_done + 8;
   if (tid == 0) {
     x.failed = 0;
-    bar_init(k_done, 2); bar_init(k_done + 8, 2);
-    bar_init(k_free, 128); bar_init(k_free + 8, 128);
-    bar_init(v_done, 1); bar_init(b_end, 1);
+    for (int i = 0; i < K_STAGES; ++i) { bar_init(k_full + 8 * i, 1); bar_init(k_scaled + 8 * i, 1); bar_init(k_used + 8 * i, 4); }
+    for (int i = 0; i < V_STAGES; ++i) { bar_init(v_full + 8 * i, 1); bar_init(v_scaled + 8 * i, 1); bar_init(v_used + 8 * i, 4); }
+    bar_init(k_ready, 4); bar_init(v_ready, 4);
+    for (int i = 0; i < 2; ++i) { bar_init(k_done + 8 * i, 2); bar_init(k_free + 8 * i, 4); }
+    bar_init(v_done, 1); bar_init(b_end, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  for (int i = tid; i < MZP_BOOKS * MZP_LEVELS / 16; i += THREADS) ((uint4*)(smem + S::BOOK))[i] = ((const uint4*)book_table)[i];
-  asm volatile("griddepcontrol.wait;" ::: "memory");        // what was before is written, and the records are read
+  if (tid < MZP_BOOKS * MZP_LEVELS / 16) ((uint4*)(smem + S::BOOK))[tid] = ((const uint4*)book_table)[tid];
 
-  // ---- the line of steps, and how many CTAs take rings
-  const int kp_all = c.kv_heads * p.passes;
-  auto length_of = [&](int b) {
-    const int row = p.rows ? p.rows[b] : b;
-    if (row < 0 || row >= c.rows) return 0;
-    return max(0, min(c.lengths[row], 0x7fffffff - STEP));
+  // ---- the line of steps
+  auto length_of = [&](int b, int& row) {
+    row = p.rows ? p.rows[b] : b;
+    return row < 0 || row >= c.rows ? 0 : max(0, min(c.lengths[row], 0x7fffffff - STEP));
   };
-  long long ring_tokens = 0;
-  int total_steps;
+  const int kp_all = c.kv_heads * p.passes;
+  int total_steps = 0;
   {
     constexpr int PER = MAX_BATCH / THREADS;
-    int st[PER], sum = 0, rt = 0;
+    int st[PER], sum = 0;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int b = tid * PER + k, len = b < p.batch ? length_of(b) : 0;
-      const int packed = mzp_packed(len, c.residual);
-      st[k] = (packed + STEP - 1) / STEP;
+      const int b = tid * PER + k;
+      int row;
+      st[k] = b < p.batch ? (mzp_packed(length_of(b, row), c.residual) + STEP - 1) / STEP : 0;
       sum += st[k];
-      rt += len - packed;
     }
-    int scan = sum, ring_sum = rt;
+    int scan = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, scan, o);
-      if (lane >= o) scan += y;
-      ring_sum += __shfl_xor_sync(0xffffffffu, ring_sum, o);
-    }
-    if (lane == 31) { x.warp_sum[warp][0] = scan; x.warp_sum[warp][1] = ring_sum; }
+    for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, scan, o); if (lane >= o) scan += y; }
+    if (lane == 31) x.warp_sum[warp] = scan;
     __syncthreads();
     int before = scan - sum;
-    total_steps = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      if (w < warp) before += x.warp_sum[w][0];
-      total_steps += x.warp_sum[w][0];
-      ring_tokens += x.warp_sum[w][1];
-    }
+    for (int w = 0; w < 16; ++w) { const int t = x.warp_sum[w]; if (w < warp) before += t; total_steps += t; }
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       const int b = tid * PER + k;
@@ -270,308 +316,74 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
       before += st[k];
     }
     if (tid == THREADS - 1 && p.batch == MAX_BATCH) x.prefix[MAX_BATCH] = before;
-    __syncthreads();
   }
   const long long T = (long long)total_steps * kp_all;
-  const int G = gridDim.x;
-  // cost of a ring: 16 per token, a step 1024 (measured; see the launch)
-  int n_ring = 0;
-  if (ring_tokens > 0) {
-    const double cr = (double)ring_tokens * kp_all * 16.0, cs = (double)T * 1024.0;
-    n_ring = (int)(G * cr / (cr + cs) + 0.5);
-    n_ring = max(1, min(n_ring, T > 0 ? G - 1 : G));
-  }
-  const int W = (int)min((long long)(G - n_ring), T);        // CTAs that share the steps: none is left without one
-  if (blockIdx.x == 0) {
-    if (tid == 0) { p.head[0] = W; *(long long*)(p.head + 2) = T; }
-    for (int b = tid; b <= p.batch; b += THREADS) p.head[4 + b] = x.prefix[b];
-  }
-  const long long ring_slots = (long long)G + p.pairs;
-
-  if ((int)blockIdx.x < n_ring) {
-    // ================= rings: a warp takes 16 tokens at a time; A = keys [token][channel], B = queries; A = values [channel][token], B = p in two parts
-    const int g = lane >> 2, t = lane & 3;
-    for (long long unit = blockIdx.x; unit < p.pairs; unit += n_ring) {
-      const int b = (int)(unit / kp_all), kp = (int)(unit % kp_all), head = kp / p.passes, r0 = kp % p.passes * NR;
-      const int row = p.rows ? p.rows[b] : b, len = length_of(b), packed = mzp_packed(len, c.residual);
-      if (len == packed) continue;
-      const int tokens = len - packed;
-      const uint16_t* ring_k = (const uint16_t*)c.tail + (long long)p.layer * c.tail_stride_layer + (long long)row * c.tail_stride_row + (long long)head * c.ring * D;
-      const uint16_t* ring_v = ring_k + (long long)c.kv_heads * c.ring * D;
-      const int ring0 = packed % c.ring;
-      auto place = [&](int i) { int r = ring0 + i; return r >= c.ring ? r - c.ring : r; };      // i < tokens <= ring
-      // queries: column g = query row r0 + g; a lane's 8 channels of each block of 32
-      uint4 qf[D / 32];
-      {
-        const int r = r0 + g;
-        const bool on = g < NR && r < p.qrows;
-        const int l = on ? r / p.group : 0, h = head * p.group + (on ? r % p.group : 0);
-        const uint16_t* qp = p.query + (long long)b * p.qsb + l * p.qsl + h * p.qsh + 8 * t;
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          qf[k] = make_uint4(0, 0, 0, 0);
-          if (on) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = (uint32_t)qp[32 * k + 2 * j] | (uint32_t)qp[32 * k + 2 * j + 1] << 16;
-            qf[k] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-      }
-      // columns 2t, 2t + 1 of the logits: the last token that the query sees, counted from the ring's first
-      int last[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) last[j] = len - p.q_len + (r0 + 2 * t + j) / p.group - packed;
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 16][4];
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
-      for (int tile = warp; tile * 16 < tokens; tile += 8) {
-        const int i0 = tile * 16;
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-        {
-          const uint16_t* ka = ring_k + (long long)place(min(i0 + g, tokens - 1)) * D + 8 * t;
-          const uint16_t* kb = ring_k + (long long)place(min(i0 + g + 8, tokens - 1)) * D + 8 * t;
-          uint4 va[D / 32], vb[D / 32];
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) { va[k] = *(const uint4*)(ka + 32 * k); vb[k] = *(const uint4*)(kb + 32 * k); }
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) {
-            mma16<BF>(s, va[k].x, vb[k].x, va[k].y, vb[k].y, qf[k].x, qf[k].y);
-            mma16<BF>(s, va[k].z, vb[k].z, va[k].w, vb[k].w, qf[k].z, qf[k].w);
-          }
-        }
-        // s[0], s[1]: token g, columns 2t, 2t + 1; s[2], s[3]: token g + 8
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int i = i0 + g + 8 * (k >> 1);
-          s[k] = i < tokens && i <= last[k & 1] ? s[k] * p.scaling : -INFINITY;
-        }
-        float pr[4], fix[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float top = fmaxf(s[j], s[2 + j]);
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          const float m_new = fmaxf(m[j], top), ref = m_new == -INFINITY ? 0.f : m_new;
-          fix[j] = ex2(m[j] - ref);
-          m[j] = m_new;
-          pr[j] = ex2(s[j] - ref);
-          pr[2 + j] = ex2(s[2 + j] - ref);
-          l[j] = l[j] * fix[j] + pr[j] + pr[2 + j];
-        }
-        if (__any_sync(0xffffffffu, fix[0] != 1.0f || fix[1] != 1.0f)) {
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) { o[i][0] *= fix[0]; o[i][1] *= fix[1]; o[i][2] *= fix[0]; o[i][3] *= fix[1]; }
-        }
-        // p in two parts of 16 bits, transposed: column g, tokens 2t, 2t + 1 (part [0]) and 2t + 8, 2t + 9 (part [1])
-        uint32_t hi[2], lo[2];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t hw, lw;
-          if (BF) {
-            const __nv_bfloat162 hb = __floats2bfloat162_rn(pr[2 * half], pr[2 * half + 1]);
-            const float2 hf = __bfloat1622float2(hb);
-            const __nv_bfloat162 lb = __floats2bfloat162_rn(pr[2 * half] - hf.x, pr[2 * half + 1] - hf.y);
-            hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
-          } else {
-            const __half2 hb = __floats2half2_rn(pr[2 * half], pr[2 * half + 1]);
-            const float2 hf = __half22float2(hb);
-            const __half2 lb = __floats2half2_rn(pr[2 * half] - hf.x, pr[2 * half + 1] - hf.y);
-            hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
-          }
-          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(hi[half]) : "r"(hw));
-          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(lo[half]) : "r"(lw));
-        }
-        // A token that is not there, or that only later queries see, must not bring a NaN to a product with p = 0: what is not there is read as zero, and
-        // where a tile has tokens that only some of the queries see, each of the queries' tokens takes its turn with what it sees
-        const int l_first = r0 / p.group, l_last = min(r0 + NR, p.qrows) - 1;
-        const int see0 = len - p.q_len - packed;               // token l sees those up to see0 + l
-        const bool apart = i0 + 15 > see0 + l_first && l_last / p.group > l_first;
-        const int turns = apart ? l_last / p.group - l_first + 1 : 1;
-        for (int turn = 0; turn < turns; ++turn) {
-          const int see = apart ? min(see0 + l_first + turn, tokens - 1) : tokens - 1;
-          const bool mine = !apart || (r0 + g) / p.group == l_first + turn;
-          const uint32_t h0 = mine ? hi[0] : 0u, h1 = mine ? hi[1] : 0u, e0 = mine ? lo[0] : 0u, e1 = mine ? lo[1] : 0u;
-#pragma unroll
-          for (int grp = 0; grp < D / 64; ++grp) {
-            uint4 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int i = i0 + 2 * t + (k & 1) + 8 * (k >> 1);
-              v[k] = make_uint4(0, 0, 0, 0);
-              if (i <= see) v[k] = *(const uint4*)(ring_v + (long long)place(i) * D + grp * 64 + 8 * g);
-            }
-            const uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
-            const uint32_t w2[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              // rows g / g + 8 = channels 8g + 2k / 8g + 2k + 1
-              const uint32_t a0 = prmt(w0[k], w1[k], 0x5410u), a1 = prmt(w0[k], w1[k], 0x7632u);
-              const uint32_t a2 = prmt(w2[k], w3[k], 0x5410u), a3 = prmt(w2[k], w3[k], 0x7632u);
-              mma16<BF>(o[grp * 4 + k], a0, a1, a2, a3, e0, e1);
-              mma16<BF>(o[grp * 4 + k], a0, a1, a2, a3, h0, h1);
-            }
-          }
-        }
-      }
-      // ---- the eight warps' parts -> one record
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], off);
-        if (g == 0 && 2 * t + j < NR) { x.ring_m[warp][2 * t + j] = m[j]; x.ring_l[warp][2 * t + j] = l[j]; }
-      }
-      __syncthreads();
-      float* part = (float*)smem;                // [warp][NR][D]
-      if (2 * t < NR) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float top = x.ring_m[0][2 * t + j];
-#pragma unroll
-          for (int w = 1; w < 8; ++w) top = fmaxf(top, x.ring_m[w][2 * t + j]);
-          const float f = m[j] == -INFINITY ? 0.f : ex2(m[j] - top);
-          float* dst = part + (warp * NR + 2 * t + j) * D + 8 * g;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) *(float2*)(dst + (i >> 2) * 64 + 2 * (i & 3)) = make_float2(o[i][j] * f, o[i][2 + j] * f);
-        }
-      }
-      __syncthreads();
-      const long long slot = ring_slots + unit;
-      for (int i = tid; i < NR * D; i += THREADS) {
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) sum += part[w * NR * D + i];
-        p.acc[slot * NR * D + i] = sum;
-      }
-      if (tid < NR) {
-        float top = x.ring_m[0][tid], sum = 0.f;
-#pragma unroll
-        for (int w = 1; w < 8; ++w) top = fmaxf(top, x.ring_m[w][tid]);
-#pragma unroll
-        for (int w = 0; w < 8; ++w) sum += x.ring_m[w][tid] == -INFINITY ? 0.f : x.ring_l[w][tid] * ex2(x.ring_m[w][tid] - top);
-        p.ml[slot * NR + tid] = make_float2(top, sum);
-      }
-      __syncthreads();
-    }
-    return;
-  }
-
-  // ================= steps
-  const int cta = (int)blockIdx.x - n_ring;
-  if (cta >= W) return;
-  const long long f0 = T * cta / W, f1 = T * (cta + 1) / W;
+  const int G = gridDim.x, cta = blockIdx.x;
+  const int W = (int)min((long long)G, T);       // CTAs that share the steps: none of them is left without one
+  if (cta == 0 && tid == 0) { p.head[0] = W; *(long long*)(p.head + 2) = T; }
+  const long long f0 = cta < W ? T * cta / W : 0, f1 = cta < W ? T * (cta + 1) / W : 0;
   const int n = (int)(f1 - f0);
-  if (n <= 0) return;
-  if (warp == 0) {
+  if (n > 0 && warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&x.tmem)), "n"(S::TM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     tm_before();
   }
   __syncthreads();
   tm_after();
-  const uint32_t tmem = x.tmem;
-  bool failed = false;
-  Cursor cur;
-  {
-    int lo = 0, hi = p.batch;                    // prefix[lo] * kp_all <= f0 < prefix[lo + 1] * kp_all
-    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if ((long long)x.prefix[mid] * kp_all <= f0) lo = mid; else hi = mid; }
-    cur.b = lo;
-    cur.steps = x.prefix[lo + 1] - x.prefix[lo];
-    const int rem = (int)(f0 - (long long)x.prefix[lo] * kp_all);
-    cur.kp = rem / cur.steps;
-    cur.step = rem % cur.steps;
-  }
-  auto advance = [&](Cursor& q) {
-    if (++q.step < q.steps) return;
-    q.step = 0;
-    if (++q.kp < kp_all) return;
-    q.kp = 0;
-    do { ++q.b; } while (q.b < p.batch && x.prefix[q.b + 1] == x.prefix[q.b]);
-    q.steps = q.b < p.batch ? x.prefix[q.b + 1] - x.prefix[q.b] : 1;
-  };
+  if (cta == 0) for (int b = tid; b <= p.batch; b += THREADS) p.head[4 + b] = x.prefix[b];
+  const uint32_t tmem = n > 0 ? x.tmem : 0u;
+  const int team = warp >> 2;
   const int r = tid & 127;                       // key channel or token of this thread
-  // the page of this thread's rows: both pages (keys, D = 128) or the one that position r lies in
-  auto page_at = [&](const Cursor& q, int which) -> const uint8_t* {
-    if (q.b >= p.batch) return nullptr;
-    const int row = p.rows ? p.rows[q.b] : q.b;
-    const int pages = mzp_packed(length_of(q.b), c.residual) / MZP_PAGE, k = 2 * q.step + which;
-    if (k >= pages) return nullptr;
-    const int id = k < c.width ? __ldg(c.block_table + (long long)row * c.width + k) : -1;
-    if (id < 0 || id >= c.pages) { atomicOr(c.status, MZ_PAGED_BAD_INDEX); return nullptr; }
-    return (const uint8_t*)c.store + (long long)p.layer * c.store_stride_layer + (long long)id * c.store_stride_page + (long long)(q.kp / p.passes) * PB;
-  };
-  uint4 code[RPT][2];
-  uint32_t word[RPT];
-  // a row's codes and word; a page that is not there has T = 0
-  auto load_row = [&](int j, const uint8_t* codes, const uint8_t* words) {
-    code[j][0] = code[j][1] = make_uint4(0, 0, 0, 0);
-    word[j] = 0;
-    if (codes) {
-      code[j][0] = ldg128(codes);
-      code[j][1] = ldg128(codes + 16);
-      word[j] = __ldg((const uint32_t*)words);
-    }
-  };
 
-  if (warp < 4) {
+  if (team == 0) {
     // ================= keys: thread = channel
     const int ch = D == 128 ? r : r & 63;
-    auto load_keys = [&](const Cursor& q) {
-#pragma unroll
-      for (int j = 0; j < RPT; ++j) {
-        const uint8_t* base = page_at(q, D == 128 ? j : r >> 6);
-        load_row(j, base ? base + ch * 32 : nullptr, base + 32 * D + 4 * ch);
-      }
-    };
     float q[NR];
-    int pair = -1, seg = -1;
-    load_keys(cur);
+    int seg = -1;
     for (int it = 0; it < n; ++it) {
-      const int this_pair = cur.b * kp_all + cur.kp;
-      const bool fresh = this_pair != pair;
-      MzpRow row[RPT];
-      uint32_t tb = 0;
-#pragma unroll
-      for (int j = 0; j < RPT; ++j) { row[j] = mzp_row(word[j]); tb = max(tb, word[j] & 0xffffu); }
-      tb = warp_max_u32(tb);
-      if (lane == 0) x.kt[it & 3][warp] = tb;
-      if (fresh) {
-        pair = this_pair; ++seg;
-        const int head = cur.kp / p.passes, r0 = cur.kp % p.passes * NR;
+      const int stage = it % K_STAGES;
+      const uint32_t phase = it / K_STAGES & 1;
+      bar_wait(k_full + 8 * stage, phase, &x.failed);
+      const StepInfo info = x.info[it & 3];
+      if (info.fresh) {
+        ++seg;
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
           q[i] = 0.f;
-          if (r0 + i < p.qrows) {
-            const int l = (r0 + i) / p.group, h = head * p.group + (r0 + i) % p.group;
-            q[i] = MzType<DT>::load(p.query, (long long)cur.b * p.qsb + l * p.qsl + h * p.qsh + ch);
+          if (info.r0 + i < p.qrows) {
+            const int l = (info.r0 + i) / p.group, h = info.head * p.group + (info.r0 + i) % p.group;
+            q[i] = MzType<DT>::load(p.query, (long long)info.b * p.qsb + l * p.qsl + h * p.qsh + ch);
           }
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
           // as bits, so that a NaN is the largest
           const uint32_t top = warp_max_u32(__float_as_uint(fabsf(q[i])));
-          if (lane == 0) x.qmax[seg & 3][warp][i] = __uint_as_float(top);
+          if (lane == 0) x.qmax[seg & 1][warp][i] = __uint_as_float(top);
         }
-      }
-      team_barrier(0);
-      if (fresh) {
+        team_barrier(0);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
           uint32_t top = 0;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) top = max(top, __float_as_uint(x.qmax[seg & 3][w][i]));
+          for (int w = 0; w < 4; ++w) top = max(top, __float_as_uint(x.qmax[seg & 1][w][i]));
           const int e = max((int)(top >> 23) - 126, -60), e1 = e >> 1, e2 = e - e1;        // |q| < 2^e, taken off in two factors
           const bool wild = top >= 0x7f800000u;                        // infinity or NaN: the row's logits are NaN
           q[i] = wild ? 0.f : q[i] * pow2(-e1) * pow2(-e2);
           if (tid == 0) x.qs[seg & 3][i] = wild ? __int_as_float(0x7fffffff) : pow2(e1) * p.scaling * pow2(e2);
         }
       }
-      const uint32_t top = max(max(x.kt[it & 3][0], x.kt[it & 3][1]), max(x.kt[it & 3][2], x.kt[it & 3][3]));
-      const float up = pow2(30 - ((int)(top >> 10) - 14));             // T < 2^(exponent field - 14)
+      bar_wait(k_scaled + 8 * stage, phase, &x.failed);
+      const float up = pow2(30 - ((int)(x.kt[it & 3] >> 10) - 14));    // T < 2^(exponent field - 14)
+      MzpRow row[RPT];
       uint32_t fold[RPT][NR];
       {
         float base[RPT * NR];
 #pragma unroll
         for (int j = 0; j < RPT; ++j) {
+          const int pg = D == 128 ? j : r >> 6;
+          const uint32_t word = info.valid >> pg & 1 ? lds32(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + 32 * D + 4 * ch) : 0u;
+          row[j] = mzp_row(word);
           const float ts = row[j].t * up, cz = fmaf(row[j].t, (float)row[j].z * -0.03125f, row[j].a);
 #pragma unroll
           for (int i = 0; i < NR; ++i) { fold[j][i] = digits_of(q[i] * ts); base[j * NR + i] = q[i] * cz; }
@@ -580,59 +392,39 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
         const float sum = warp_sums<RPT * NR>(base, lane, index);
         if ((lane & (32 / (RPT * NR) - 1)) == 0) x.base[it & 3][warp][index] = sum;
       }
-      if (it > 0) bar_wait(k_done + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, &x.failed, failed);      // the operand is free
+      if (it > 0) bar_wait(k_done + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, &x.failed);      // the operand is free
 #pragma unroll
       for (int j = 0; j < RPT; ++j) {
-        const int blk = D == 128 ? j : r >> 6;
+        const int pg = D == 128 ? j : r >> 6;
 #pragma unroll
         for (int i = 0; i < NR; i += 4)
-          sts128(sbase + S::K_B + (blk * (NR / 4) + i / 4) * S::CHUNK + ch * 16, fold[j][i], fold[j][i + 1], fold[j][i + 2], fold[j][i + 3]);
-        expand_row(code[j][0], code[j][1], book128(sbook + row[j].z * 16), sbase + S::K_A + blk * 4 * S::CHUNK + ch * 16, S::CHUNK);
+          sts128(sbase + S::K_B + (pg * (NR / 4) + i / 4) * S::CHUNK + ch * 16, fold[j][i], fold[j][i + 1], fold[j][i + 2], fold[j][i + 3]);
+        expand_row(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + ch * 32, book128(sbook + row[j].z * 16), sbase + S::K_A + pg * 4 * S::CHUNK + ch * 16,
+                   S::CHUNK, lane);
       }
-      Cursor nxt = cur;
-      advance(nxt);
-      if (it + 1 < n) load_keys(nxt);
-      cur = nxt;
       fence_operands();
-      team_barrier(0);
-      if (tid == 0) {
-        if (it >= 2) bar_wait(k_free + 8 * (it & 1), ((it - 2) >> 1) & 1, &x.failed, failed);
-        bar_arrive(k_done + 8 * (it & 1));
-        if (!x.failed) {
-          tm_after();
-          const uint64_t a = descriptor(sbase + S::K_A, S::CHUNK), b = descriptor(sbase + S::K_B, S::CHUNK);
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_S + (it & 1) * S::N, a + k * (512 >> 4), b + k * (512 >> 4), k > 0);
-          umma_commit(k_done + 8 * (it & 1));
-        }
-      }
+      __syncwarp();
+      if (lane == 0) { bar_arrive(k_ready); bar_arrive(k_used + 8 * stage); }
     }
-  } else {
+  } else if (team == 1) {
     // ================= softmax and values: thread = token, and position of the output
+    more_registers<Regs<NR>::VALUES>();
     const int tw = warp - 4, blk = r >> 6;
     const uint32_t lanes = tmem + ((uint32_t)(tw * 32) << 16);
-    auto load_values = [&](const Cursor& q) {
-      const uint8_t* base = page_at(q, r >> 6);
-#pragma unroll
-      for (int j = 0; j < RPT; ++j) {
-        const int vr = (r & 63) * RPT + j;
-        load_row(j, base ? base + 36 * D + vr * 32 : nullptr, base + 68 * D + 4 * vr);
-      }
-    };
     float m[NR], l[NR], o[NR], base_v[RPT][NR], qs[NR];
     float vunit = 0.f;
-    int pair = -1, seg = -1, limit0 = 0, packed = 0;
-    bool masked = false;
-    int r0 = 0;
+    int pair = -1, seg = -1;
+    auto reset = [&]() {
 #pragma unroll
-    for (int i = 0; i < NR; ++i) { m[i] = -INFINITY; l[i] = 0.f; o[i] = 0.f; qs[i] = 0.f; }
+      for (int i = 0; i < NR; ++i) { m[i] = -INFINITY; l[i] = 0.f; o[i] = 0.f; }
 #pragma unroll
-    for (int j = 0; j < RPT; ++j)
+      for (int j = 0; j < RPT; ++j)
 #pragma unroll
-      for (int i = 0; i < NR; ++i) base_v[j][i] = 0.f;
-    // the products of the step before, which is number `done`
+        for (int i = 0; i < NR; ++i) base_v[j][i] = 0.f;
+    };
+    // the products of step `done`
     auto take_output = [&](int done) {
-      bar_wait(v_done, done & 1, &x.failed, failed);
+      bar_wait(v_done, done & 1, &x.failed);
       tm_after();
 #pragma unroll
       for (int i = 0; i < NR; i += 4) {
@@ -682,43 +474,39 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
       }
       team_barrier(1);                                       // fin and halves are free again
     };
-    load_values(cur);
+    reset();
     for (int it = 0; it < n; ++it) {
-      const int this_pair = cur.b * kp_all + cur.kp;
-      const bool fresh = this_pair != pair;
-      if (fresh) {
+      const int stage = it % V_STAGES;
+      const uint32_t phase = it / V_STAGES & 1;
+      bar_wait(v_full + 8 * stage, phase, &x.failed);
+      const StepInfo info = x.info[it & 3];
+      if (info.fresh) {
         if (pair >= 0) {
           take_output(it - 1);
           write_record();
+          reset();
         }
-        pair = this_pair; ++seg;
-        r0 = cur.kp % p.passes * NR;
-        const int len = length_of(cur.b);
-        packed = mzp_packed(len, c.residual);
-        limit0 = len - p.q_len;
-        masked = packed > limit0 + 1;
-#pragma unroll
-        for (int i = 0; i < NR; ++i) { m[i] = -INFINITY; l[i] = 0.f; o[i] = 0.f; }
-#pragma unroll
-        for (int j = 0; j < RPT; ++j)
-#pragma unroll
-          for (int i = 0; i < NR; ++i) base_v[j][i] = 0.f;
+        pair = info.pair; ++seg;
       }
-      MzpRow row[RPT];
-      uint32_t tb = 0;
-#pragma unroll
-      for (int j = 0; j < RPT; ++j) { row[j] = mzp_row(word[j]); tb = max(tb, word[j] & 0xffffu); }
-      tb = warp_max_u32(tb);
       // ---- logits
-      bar_wait(k_done + 8 * (it & 1), (it >> 1) & 1, &x.failed, failed);
+      bar_wait(k_done + 8 * (it & 1), (it >> 1) & 1, &x.failed);
       tm_after();
-      if (fresh) {
+      if (info.fresh) load_floats(qs, x.qs[seg & 3]);
+      const float kunit = pow2((int)(x.kt[it & 3] >> 10) - 14 - 35);
+      float s[NR], base[NR];
+      if (D == 128) {
+        float b[4][NR];
 #pragma unroll
-        for (int i = 0; i < NR; ++i) qs[i] = x.qs[seg & 3][i];
+        for (int w = 0; w < 4; ++w) load_floats(b[w], x.base[it & 3][w] + blk * NR);
+#pragma unroll
+        for (int i = 0; i < NR; ++i) base[i] = (b[0][i] + b[1][i]) + (b[2][i] + b[3][i]);
+      } else {
+        float b[2][NR];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) load_floats(b[w], x.base[it & 3][2 * blk + w]);
+#pragma unroll
+        for (int i = 0; i < NR; ++i) base[i] = b[0][i] + b[1][i];
       }
-      const uint32_t ktop = max(max(x.kt[it & 3][0], x.kt[it & 3][1]), max(x.kt[it & 3][2], x.kt[it & 3][3]));
-      const float kunit = pow2((int)(ktop >> 10) - 14 - 35);
-      float s[NR];
 #pragma unroll
       for (int i = 0; i < NR; i += 4) {
         int a[16];
@@ -726,49 +514,47 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
 #pragma unroll
         for (int k = 0; k < 4; ++k) s[i + k] = number_of(a + 4 * k) * kunit;
       }
-      const int pos = cur.step * STEP + r;
+      tm_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(k_free + 8 * (it & 1));
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        float base;
-        if (D == 128) {
-          const int at = blk * NR + i;
-          base = (x.base[it & 3][0][at] + x.base[it & 3][1][at]) + (x.base[it & 3][2][at] + x.base[it & 3][3][at]);
-        } else {
-          base = x.base[it & 3][2 * blk][i] + x.base[it & 3][2 * blk + 1][i];
-        }
-        s[i] = (s[i] + base) * qs[i];
-        if (pos >= packed) s[i] = -INFINITY;
+        s[i] = (s[i] + base[i]) * qs[i];
+        if (r >= info.count) s[i] = -INFINITY;
       }
-      if (masked) {
+      if (info.see < info.count - 1) {                       // not every query sees all of the step
 #pragma unroll
-        for (int i = 0; i < NR; ++i) if (pos > limit0 + (r0 + i) / p.group) s[i] = -INFINITY;
+        for (int i = 0; i < NR; ++i) if (r > info.see + (info.r0 + i) / p.group - info.r0 / p.group) s[i] = -INFINITY;
       }
-      tm_before();
-      bar_arrive(k_free + 8 * (it & 1));
       // ---- running maximum
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
         const float top = warp_max(s[i]);
         if (lane == 0) x.vmax[it & 1][tw][i] = top;
       }
-      if (lane == 0) x.vt[it & 1][tw] = tb;
       team_barrier(1);
       float fix[NR];
       bool moved = false;
+      {
+        float v[4][NR];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) load_floats(v[w], x.vmax[it & 1][w]);
+#pragma unroll
+        for (int i = 0; i < NR; ++i) fix[i] = fmaxf(fmaxf(v[0][i], v[1][i]), fmaxf(v[2][i], v[3][i]));
+      }
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        const float top = fmaxf(fmaxf(x.vmax[it & 1][0][i], x.vmax[it & 1][1][i]), fmaxf(x.vmax[it & 1][2][i], x.vmax[it & 1][3][i]));
-        const float m_new = fmaxf(m[i], top), ref = m_new == -INFINITY ? 0.f : m_new;
+        const float m_new = fmaxf(m[i], fix[i]), ref = m_new == -INFINITY ? 0.f : m_new;
         fix[i] = ex2(m[i] - ref);
         moved |= m_new != m[i];
         m[i] = m_new;
         s[i] = ex2(s[i] - ref);
       }
-      const uint32_t vtop = max(max(x.vt[it & 1][0], x.vt[it & 1][1]), max(x.vt[it & 1][2], x.vt[it & 1][3]));
-      const int ev = (int)(vtop >> 10) - 14;
+      bar_wait(v_scaled + 8 * stage, phase, &x.failed);
+      const int ev = (int)(x.vt[it & 3] >> 10) - 14;
       const float up = pow2(30 - ev);
       // ---- the output so far; then the operand is free
-      if (it > 0 && !fresh) take_output(it - 1);
+      if (it > 0 && !info.fresh) take_output(it - 1);
       if (moved) {                                           // the same for all threads
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
@@ -782,7 +568,10 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
       for (int i = 0; i < NR; ++i) l[i] += s[i];
 #pragma unroll
       for (int j = 0; j < RPT; ++j) {
-        const float ts = row[j].t * up, cz = fmaf(row[j].t, (float)row[j].z * -0.03125f, row[j].a);
+        const int vr = (r & 63) * RPT + j;
+        const uint32_t in = sbase + S::V_IN + (2 * stage + blk) * S::SIDE;
+        const MzpRow row = mzp_row(info.valid >> blk & 1 ? lds32(in + 32 * D + 4 * vr) : 0u);
+        const float ts = row.t * up, cz = fmaf(row.t, (float)row.z * -0.03125f, row.a);
         const int b2 = D == 128 ? j : blk, at = D == 128 ? r : r & 63;
 #pragma unroll
         for (int i = 0; i < NR; ++i) base_v[j][i] = fmaf(s[i], cz, base_v[j][i]);
@@ -790,30 +579,272 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
         for (int i = 0; i < NR; i += 4)
           sts128(sbase + S::V_B + (b2 * (NR / 4) + i / 4) * S::CHUNK + at * 16, digits_of(s[i] * ts), digits_of(s[i + 1] * ts),
                  digits_of(s[i + 2] * ts), digits_of(s[i + 3] * ts));
-        expand_row(code[j][0], code[j][1], book128(sbook + row[j].z * 16), sbase + S::V_A + b2 * 4 * S::CHUNK + at * 16, S::CHUNK);
+        expand_row(in + vr * 32, book128(sbook + row.z * 16), sbase + S::V_A + b2 * 4 * S::CHUNK + at * 16, S::CHUNK, lane);
       }
-      Cursor nxt = cur;
-      advance(nxt);
-      if (it + 1 < n) load_values(nxt);
-      cur = nxt;
       fence_operands();
       tm_before();
-      team_barrier(1);
-      if (r == 0 && !*(volatile int*)&x.failed) {
-        tm_after();
-        const uint64_t a = descriptor(sbase + S::V_A, S::CHUNK), b = descriptor(sbase + S::V_B, S::CHUNK);
+      __syncwarp();
+      if (lane == 0) { bar_arrive(v_ready); bar_arrive(v_used + 8 * stage); }
+    }
+    if (n > 0) {
+      take_output(n - 1);
+      write_record();
+    }
+  } else if (team == 2) {
+    // ================= rings: a warp takes 16 tokens at a time, and (D = 128) 64 of the channels of the output.  A = keys [token][channel], B =
+    // queries; A = values [channel][token], B = p in two parts of 16 bits
+    if (Regs<NR>::RINGS > 64) more_registers<Regs<NR>::RINGS>();
+    const int g = lane >> 2, t = lane & 3, rw = warp - 8;
+    const int half = D == 128 ? rw & 1 : 0, stream = D == 128 ? rw >> 1 : rw;
+    const long long units = p.pairs * p.parts, first_slot = (long long)G + p.pairs;
+    for (long long unit = G - 1 - cta; unit < units; unit += G) {        // CTAs without steps come first
+      const int part = (int)(unit % p.parts);
+      const long long pair = unit / p.parts;
+      const int b = (int)(pair / kp_all), kp = (int)(pair % kp_all), head = kp / p.passes, r0 = kp % p.passes * NR;
+      int row;
+      const int len = length_of(b, row), packed = mzp_packed(len, c.residual), tokens = len - packed;
+      if (tokens == 0) continue;
+      const int tiles = (tokens + 15) / 16, end = tiles * (part + 1) / p.parts;
+      const uint16_t* ring_k = (const uint16_t*)c.tail + (long long)p.layer * c.tail_stride_layer + (long long)row * c.tail_stride_row + (long long)head * c.ring * D;
+      const uint16_t* ring_v = ring_k + (long long)c.kv_heads * c.ring * D + half * 64;
+      const int ring0 = packed % c.ring;
+      auto place = [&](int i) { const int at = ring0 + i; return (at >= c.ring ? at - c.ring : at) * D; };      // i < tokens <= ring
+      // queries into shared memory; rows that are not there are zero
+      team_barrier(2);
+      for (int i = r; i < 8 * D; i += 128) {
+        const int qi = i / D, d = i % D, qr = r0 + qi;
+        uint16_t v = 0;
+        if (qi < NR && qr < p.qrows) v = p.query[(long long)b * p.qsb + qr / p.group * p.qsl + (head * p.group + qr % p.group) * p.qsh + d];
+        *(uint16_t*)(smem + S::QUERY + qi * S::Q_ROW + 2 * d) = v;
+      }
+      team_barrier(2);
+      const int see0 = len - p.q_len - packed;               // query token l sees the ring's tokens up to see0 + l
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4][4];
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_O, a + k * (512 >> 4), b + k * (512 >> 4), k > 0);
-        umma_commit(v_done);
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+      for (int tile = tiles * part / p.parts + stream; tile < end; tile += STREAMS) {
+        const int i0 = tile * 16;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        {
+          const uint16_t* ka = ring_k + place(min(i0 + g, tokens - 1)) + 8 * t;
+          const uint16_t* kb = ring_k + place(min(i0 + g + 8, tokens - 1)) + 8 * t;
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) {
+            const uint4 va = *(const uint4*)(ka + 32 * k), vb = *(const uint4*)(kb + 32 * k);
+            const uint4 qf = lds128(sbase + S::QUERY + g * S::Q_ROW + (32 * k + 8 * t) * 2);
+            mma16<BF>(s, va.x, vb.x, va.y, vb.y, qf.x, qf.y);
+            mma16<BF>(s, va.z, vb.z, va.w, vb.w, qf.z, qf.w);
+          }
+        }
+        // s[0], s[1]: token g, columns (query rows) 2t, 2t + 1; s[2], s[3]: token g + 8
+        float fix[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int last = min(see0 + (r0 + 2 * t + j) / p.group, tokens - 1);
+          s[j] = i0 + g <= last ? s[j] * p.scaling : -INFINITY;
+          s[2 + j] = i0 + g + 8 <= last ? s[2 + j] * p.scaling : -INFINITY;
+          float top = fmaxf(s[j], s[2 + j]);
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          const float m_new = fmaxf(m[j], top), ref = m_new == -INFINITY ? 0.f : m_new;
+          fix[j] = ex2(m[j] - ref);
+          m[j] = m_new;
+          s[j] = ex2(s[j] - ref);
+          s[2 + j] = ex2(s[2 + j] - ref);
+          l[j] = l[j] * fix[j] + s[j] + s[2 + j];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { o[i][0] *= fix[0]; o[i][1] *= fix[1]; o[i][2] *= fix[0]; o[i][3] *= fix[1]; }
+        // p in two parts, transposed: column g, tokens 2t, 2t + 1 ([0]) and 2t + 8, 2t + 9 ([1])
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t hw, lw;
+          if (BF) {
+            const __nv_bfloat162 hb = __floats2bfloat162_rn(s[2 * h], s[2 * h + 1]);
+            const float2 hf = __bfloat1622float2(hb);
+            const __nv_bfloat162 lb = __floats2bfloat162_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
+            hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
+          } else {
+            const __half2 hb = __floats2half2_rn(s[2 * h], s[2 * h + 1]);
+            const float2 hf = __half22float2(hb);
+            const __half2 lb = __floats2half2_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
+            hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
+          }
+          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(hi[h]) : "r"(hw));
+          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(lo[h]) : "r"(lw));
+        }
+        // A token that is not there, or that only later queries see, must not bring a NaN to a product with p = 0: what is not there is read as zero, and
+        // where a tile has tokens that only some of the queries see, each of the queries' tokens takes its turn with what it sees
+        const int l_first = r0 / p.group, l_last = (min(r0 + NR, p.qrows) - 1) / p.group;
+        const bool apart = i0 + 15 > see0 + l_first && l_last > l_first;
+        for (int turn = 0; turn <= (apart ? l_last - l_first : 0); ++turn) {
+          const int see = apart ? min(see0 + l_first + turn, tokens - 1) : tokens - 1;
+          const bool mine = !apart || (r0 + g) / p.group == l_first + turn;
+          uint4 v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int i = i0 + 2 * t + (k & 1) + 8 * (k >> 1);
+            v[k] = make_uint4(0, 0, 0, 0);
+            if (i <= see) v[k] = *(const uint4*)(ring_v + place(i) + 8 * g);
+          }
+          const uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+          const uint32_t w2[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // rows g / g + 8 = channels 8g + 2k / 8g + 2k + 1
+            const uint32_t a0 = prmt(w0[k], w1[k], 0x5410u), a1 = prmt(w0[k], w1[k], 0x7632u);
+            const uint32_t a2 = prmt(w2[k], w3[k], 0x5410u), a3 = prmt(w2[k], w3[k], 0x7632u);
+            mma16<BF>(o[k], a0, a1, a2, a3, mine ? lo[0] : 0u, mine ? lo[1] : 0u);
+            mma16<BF>(o[k], a0, a1, a2, a3, mine ? hi[0] : 0u, mine ? hi[1] : 0u);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], off);
+        if (2 * t + j < NR) {
+          const long long slot = (first_slot + unit * STREAMS + stream) * NR + 2 * t + j;
+          float* dst = p.acc + slot * D + half * 64 + 8 * g;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) *(float2*)(dst + 2 * k) = make_float2(o[k][j], o[k][2 + j]);
+          if (g == 0 && half == 0) p.ml[slot] = make_float2(m[j], l[j]);
+        }
       }
     }
-    take_output(n - 1);
-    write_record();
+  } else {
+    fewer_registers<Regs<NR>::SERVICE>();
+    if (warp == 12) {
+      // ================= the line: page numbers, copies
+      int b = 0, head = 0, pass = 0, step = 0, steps = 1, row = 0, len = 0;
+      bool fresh = true;
+      if (n > 0) {
+        int hi = p.batch;                        // prefix[b] * kp_all <= f0 < prefix[b + 1] * kp_all
+        while (hi - b > 1) { const int mid = (b + hi) >> 1; if ((long long)x.prefix[mid] * kp_all <= f0) b = mid; else hi = mid; }
+        steps = x.prefix[b + 1] - x.prefix[b];
+        const int rem = (int)(f0 - (long long)x.prefix[b] * kp_all), kp = rem / steps;
+        head = kp / p.passes;
+        pass = kp % p.passes;
+        step = rem % steps;
+        len = length_of(b, row);
+      }
+      int ids = -1, ids_at = -64;                // page numbers ids_at .. ids_at + 31 of the row, one per lane
+      for (int it = 0; it < n; ++it) {
+        const int pages = mzp_packed(len, c.residual) / MZP_PAGE, k0 = 2 * step;
+        if (k0 < ids_at || k0 >= ids_at + 32) {
+          ids_at = k0;
+          ids = -1;
+          if (k0 + lane < pages) {
+            ids = k0 + lane < c.width ? c.block_table[(long long)row * c.width + k0 + lane] : -1;
+            if (ids < 0 || ids >= c.pages) { ids = -1; atomicOr(c.status, MZ_PAGED_BAD_INDEX); }
+          }
+        }
+        const int page0 = __shfl_sync(0xffffffffu, ids, k0 - ids_at), page1 = __shfl_sync(0xffffffffu, ids, k0 + 1 - ids_at);
+        const int ks = it % K_STAGES, vs = it % V_STAGES;
+        if (it >= K_STAGES) bar_wait(k_used + 8 * ks, (it / K_STAGES - 1) & 1, &x.failed);
+        if (lane == 0) {
+          StepInfo info;
+          info.pair = (b * c.kv_heads + head) * p.passes + pass;
+          info.fresh = fresh;
+          info.count = min(STEP, pages * MZP_PAGE - step * STEP);
+          info.r0 = pass * NR;
+          info.see = len - p.q_len + info.r0 / p.group - step * STEP;
+          info.b = b;
+          info.head = head;
+          info.valid = (page0 >= 0 ? 1 : 0) | (page1 >= 0 ? 2 : 0);
+          x.info[it & 3] = info;
+          const uint32_t bytes = S::SIDE * ((page0 >= 0) + (page1 >= 0));
+          const uint8_t* store = (const uint8_t*)c.store + (long long)p.layer * c.store_stride_layer + head * PB;
+          const uint8_t *src0 = store + (long long)page0 * c.store_stride_page, *src1 = store + (long long)page1 * c.store_stride_page;
+          const uint32_t kin = sbase + S::K_IN + 2 * ks * S::SIDE, vin = sbase + S::V_IN + 2 * vs * S::SIDE;
+          bar_expect(k_full + 8 * ks, bytes);
+          if (page0 >= 0) bulk_copy(kin, src0, S::SIDE, k_full + 8 * ks);
+          if (page1 >= 0) bulk_copy(kin + S::SIDE, src1, S::SIDE, k_full + 8 * ks);
+          if (it >= V_STAGES) bar_wait(v_used + 8 * vs, (it / V_STAGES - 1) & 1, &x.failed);
+          bar_expect(v_full + 8 * vs, bytes);
+          if (page0 >= 0) bulk_copy(vin, src0 + S::SIDE, S::SIDE, v_full + 8 * vs);
+          if (page1 >= 0) bulk_copy(vin + S::SIDE, src1 + S::SIDE, S::SIDE, v_full + 8 * vs);
+        }
+        __syncwarp();
+        fresh = false;
+        if (++step == steps) {
+          step = 0; fresh = true; ids_at = -64;
+          if (++pass == p.passes) {
+            pass = 0;
+            if (++head == c.kv_heads) {
+              head = 0;
+              do { ++b; } while (b < p.batch && x.prefix[b + 1] == x.prefix[b]);
+              if (b < p.batch) { steps = x.prefix[b + 1] - x.prefix[b]; len = length_of(b, row); }
+            }
+          }
+        }
+      }
+      // copies in flight end before the CTA does (the teams have waited for all of them unless a wait ran out)
+      for (int it = max(0, n - K_STAGES); it < n; ++it)
+        for (int k = 0; k < SPIN_LIMIT && !bar_test(k_full + 8 * (it % K_STAGES), it / K_STAGES & 1); ++k) {}
+      for (int it = max(0, n - V_STAGES); it < n; ++it)
+        for (int k = 0; k < SPIN_LIMIT && !bar_test(v_full + 8 * (it % V_STAGES), it / V_STAGES & 1); ++k) {}
+    } else if (warp == 13) {
+      // ================= a step's largest T, as the bits of an f16
+      auto largest = [&](uint32_t in, int valid) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg)
+          if (valid >> pg & 1) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) top = max(top, lds32(in + pg * S::SIDE + 32 * D + 4 * (lane + 32 * i)) & 0xffffu);
+          }
+        return warp_max_u32(top);
+      };
+      for (int it = 0; it < n; ++it) {
+        const int ks = it % K_STAGES, vs = it % V_STAGES;
+        bar_wait(k_full + 8 * ks, it / K_STAGES & 1, &x.failed);
+        const int valid = x.info[it & 3].valid;
+        const uint32_t kt = largest(sbase + S::K_IN + 2 * ks * S::SIDE, valid);
+        if (lane == 0) { x.kt[it & 3] = kt; bar_arrive(k_scaled + 8 * ks); }
+        bar_wait(v_full + 8 * vs, it / V_STAGES & 1, &x.failed);
+        const uint32_t vt = largest(sbase + S::V_IN + 2 * vs * S::SIDE, valid);
+        if (lane == 0) { x.vt[it & 3] = vt; bar_arrive(v_scaled + 8 * vs); }
+      }
+    } else if (warp == 14) {
+      // ================= products of the keys
+      if (lane == 0) {
+        const uint64_t a = descriptor(sbase + S::K_A, S::CHUNK), bd = descriptor(sbase + S::K_B, S::CHUNK);
+        for (int it = 0; it < n; ++it) {
+          bar_wait(k_ready, it & 1, &x.failed);
+          if (it >= 2) bar_wait(k_free + 8 * (it & 1), ((it - 2) >> 1) & 1, &x.failed);
+          bar_arrive(k_done + 8 * (it & 1));     // hands on what the keys' threads wrote beside the operand
+          if (*(volatile int*)&x.failed) break;
+          tm_after();
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_S + (it & 1) * S::N, a + k * (512 >> 4), bd + k * (512 >> 4), k > 0);
+          umma_commit(k_done + 8 * (it & 1));
+        }
+      }
+    } else {
+      // ================= products of the values
+      if (lane == 0) {
+        const uint64_t a = descriptor(sbase + S::V_A, S::CHUNK), bd = descriptor(sbase + S::V_B, S::CHUNK);
+        for (int it = 0; it < n; ++it) {
+          bar_wait(v_ready, it & 1, &x.failed);
+          if (*(volatile int*)&x.failed) break;
+          tm_after();
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_O, a + k * (512 >> 4), bd + k * (512 >> 4), k > 0);
+          umma_commit(v_done);
+        }
+      }
+    }
+    __syncwarp();
   }
   __syncthreads();
-  if (x.failed && tid == 0) {                    // products in flight end before their memory goes back
+  if (n == 0) return;
+  if (x.failed && (tid & ~32) == 14 * 32) {      // products in flight end before their memory goes back
     umma_commit(b_end);
-    bar_wait(b_end, 0, &x.failed, failed = false);
+    for (int k = 0; k < SPIN_LIMIT && !bar_test(b_end, 0); ++k) {}
   }
   tm_before();
   __syncthreads();
@@ -826,7 +857,6 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
 // merges the records of one query row of a pair: a thread per channel, records in their order
 template <int D, bool BF, int NR>
 __global__ void __launch_bounds__(D) merge_kernel(const Args p, int G) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int i = blockIdx.x % NR, d = threadIdx.x;
   const long long pair = blockIdx.x / NR;
   const int kp_all = p.c.kv_heads * p.passes, b = (int)(pair / kp_all), kp = (int)(pair % kp_all), head = kp / p.passes, qr = kp % p.passes * NR + i;
@@ -837,6 +867,7 @@ __global__ void __launch_bounds__(D) merge_kernel(const Args p, int G) {
   if (!known && d == 0) atomicOr(p.c.status, MZ_PAGED_BAD_INDEX);
   const int len = known ? max(0, min(p.c.lengths[row], 0x7fffffff - STEP)) : 0;
   const bool ring = len > mzp_packed(len, p.c.residual);
+  constexpr int STREAMS = D == 128 ? 2 : 4;
   const long long W = p.head[0], T = *(const long long*)(p.head + 2);
   const long long steps = p.head[4 + b + 1] - p.head[4 + b], s0 = (long long)p.head[4 + b] * kp_all + kp * steps;
   float m = -INFINITY, l = 0.f, a = 0.f;
@@ -864,8 +895,19 @@ __global__ void __launch_bounds__(D) merge_kernel(const Args p, int G) {
     }
   }
   if (ring) {
-    const long long slot = (G + p.pairs + pair) * NR + i;
-    take(p.ml[slot], p.acc[slot * D + d]);
+    const long long first = G + p.pairs + pair * p.parts * STREAMS;
+    for (int k0 = 0; k0 < p.parts * STREAMS; k0 += 4) {
+      float2 ml[4];
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const long long slot = (first + min(k0 + k, p.parts * STREAMS - 1)) * NR + i;
+        ml[k] = p.ml[slot];
+        v[k] = p.acc[slot * D + d];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) if (k0 + k < p.parts * STREAMS) take(ml[k], v[k]);
+    }
   }
   const float out = l == 0.f ? 0.f : a / l;
   const int ql = qr / p.group, h = head * p.group + qr % p.group;
@@ -877,6 +919,10 @@ int launch(const Args& p, const uint8_t* book, int G, cudaStream_t st) {
   auto kern = attention_kernel<D, BF, NR>;
   using S = Smem<D, NR>;
   MZ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL));
+  kern<<<G, THREADS, S::TOTAL, st>>>(p, book);
+  MZ_LAUNCH_CHECK("paged attention");
+  // The merge kernel's launch overlaps the first kernel's end.  (Not so the first kernel's with the merge before it: an SM does not change its split of
+  // L1 and shared memory while a CTA runs on it, and two of these CTAs then do not fit.)
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -884,20 +930,14 @@ int launch(const Args& p, const uint8_t* book, int G, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.stream = st;
-  cfg.gridDim = dim3((unsigned)G);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = S::TOTAL;
-  MZ_CUDA(cudaLaunchKernelEx(&cfg, kern, p, book));
-  MZ_LAUNCH_CHECK("paged attention");
   cfg.gridDim = dim3((unsigned)(p.pairs * NR));
   cfg.blockDim = dim3(D);
-  cfg.dynamicSmemBytes = 0;
   MZ_CUDA(cudaLaunchKernelEx(&cfg, merge_kernel<D, BF, NR>, p, G));
   MZ_LAUNCH_CHECK("paged attention merge");
   return MZ_OK;
 }
 
-struct Shape { int nr, passes, G; long long pairs; size_t head_bytes, slots, bytes; };
+struct Shape { int nr, passes, parts, G; long long pairs; size_t head_bytes, slots, bytes; };
 int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* s) {
   MZ_REQUIRE(batch >= 0 && batch <= MAX_BATCH, "batch %d (at most %d)", batch, MAX_BATCH);
   MZ_REQUIRE(q_len >= 1 && q_heads >= 1 && q_heads % c->kv_heads == 0, "q_len %d, q_heads %d of %d kv heads", q_len, q_heads, c->kv_heads);
@@ -910,9 +950,13 @@ int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* 
   s->passes = (int)((qrows + s->nr - 1) / s->nr);
   s->pairs = (long long)batch * c->kv_heads * s->passes;
   MZ_REQUIRE(s->pairs * s->nr < (1ll << 31), "too many query rows for one call");
-  s->G = sms * (s->nr == 4 ? 3 : 2);
+  s->G = sms * CTAS_PER_SM;
+  // few pairs: their rings are cut until a warp has one tile of 16 tokens or the CTAs are taken
+  const int streams = c->head_dim == 128 ? 2 : 4, most = ((c->residual + MZP_PAGE - 1 + 15) / 16 + streams - 1) / streams;
+  const long long share = s->pairs > 0 ? s->G / s->pairs : 1;
+  s->parts = (int)(share < 1 ? 1 : share > most ? most : share);
   s->head_bytes = ((4 + (size_t)batch + 1) * sizeof(int) + 127) / 128 * 128;
-  s->slots = (size_t)s->G + 2 * (size_t)s->pairs;
+  s->slots = (size_t)s->G + (size_t)s->pairs * (1 + s->parts * streams);
   s->bytes = s->head_bytes + s->slots * s->nr * (sizeof(float2) + (size_t)c->head_dim * sizeof(float));
   return MZ_OK;
 }
@@ -952,6 +996,7 @@ extern "C" int mz_paged_attention(const mz_paged_cache* cache, int layer, const 
   p.group = args->q_heads / cache->kv_heads;
   p.qrows = p.group * args->q_len;
   p.passes = s.passes;
+  p.parts = s.parts;
   p.scaling = args->scaling * mzp::LOG2E;
   p.head = (int*)args->workspace;
   p.acc = (float*)((uint8_t*)args->workspace + s.head_bytes);
