@@ -15,24 +15,26 @@
 // finds there; a CTA leaves a record (m, l, out) per pair that it met, slot = CTA + pair.  The 16-bit tokens of the rings are shared out over the CTAs
 // as well; their records follow.  A second kernel merges a pair's records.
 //
-// A CTA is four groups of four warps, two CTAs to an SM:
-//   keys     expand the keys' codes and scale the queries, up to two steps ahead of
-//   values   logits, softmax, expansion of the values, running output (thread = token, then channel)
-//   rings    16-bit tokens on mma.sync, from memory; they fill the gaps of the others
-//   service  a warp that walks the line, looks pages up and has them copied to shared memory (bulk copies: keys two steps ahead, values three),
-//            one that finds a step's largest T, and one each that issues the MMAs of the keys and of the values
+// A CTA is five groups of four warps, two CTAs to an SM; what a group does in a step is short, and the groups are up to two steps apart:
+//   key levels     expand the keys' codes                                   (thread = channel)
+//   key folds      scale the queries to fixed point, sum the constant terms (thread = channel)
+//   value levels   expand the values' codes                                 (thread = token)
+//   softmax        logits, probabilities to fixed point, running output     (thread = token, then channel)
+//   service        a warp that walks the line, looks pages up and has them copied to shared memory (bulk copies: keys two steps ahead, values three), one
+//                  that issues MMAs, two that take the rings' 16-bit tokens from memory on mma.sync, in the gaps of the others
 // mbarriers tie them together.  Every wait is bounded; one that runs out makes the CTA's records NaN and ends its MMAs.
 #include "mz_paged.cuh"
 
 namespace mzp {
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int THREADS = 512, MAX_BATCH = 1024, CTAS_PER_SM = 2;
+constexpr int THREADS = 640, MAX_BATCH = 1024, CTAS_PER_SM = 2;
 constexpr int SPIN_LIMIT = 1000000;              // looks of a wait before it gives up; afterwards one look each
-// registers: 4 x 32 threads each of keys (as launched), values, rings and service share 512 x 64
+// registers of the groups: they share what the 640 threads are launched with, 48 each
 template <int NR>
 struct Regs {
-  static constexpr int VALUES = NR == 4 ? 88 : 104, RINGS = NR == 4 ? 72 : 64, SERVICE = NR == 4 ? 32 : 24;
-  static_assert(64 + VALUES + RINGS + SERVICE <= 4 * 64, "register split");
+  static constexpr int KEY_LEVELS = NR == 4 ? 40 : 32, KEY_FOLDS = NR == 4 ? 48 : 56, VALUE_LEVELS = NR == 4 ? 40 : 32, SOFTMAX = NR == 4 ? 72 : 88,
+                       SERVICE = NR == 4 ? 40 : 32;
+  static_assert(KEY_LEVELS + KEY_FOLDS + VALUE_LEVELS + SOFTMAX + SERVICE <= 5 * 48, "register split");
 };
 constexpr int STEP = 2 * MZP_PAGE;
 
@@ -107,14 +109,15 @@ __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile int* s_failed) {
   for (int it = 0; it < SPIN_LIMIT; ++it) {
     if (bar_test(bar, parity)) return;
-    if ((it & 255) == 255 && *s_failed) return;
+    if ((it & 63) == 63 && *s_failed) return;
   }
   *s_failed = 1;
 }
 template <int N>
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ void registers() {    // launched with 48
+  if constexpr (N > 48) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+  if constexpr (N < 48) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 // shared-memory operand, not swizzled, major along the kept dimension: cores of 8 rows x 16 bytes, 128 bytes apart along the reduction,
 // `chunk` bytes apart along the kept dimension
 __device__ __forceinline__ uint64_t descriptor(uint32_t sa, uint32_t chunk) {
@@ -238,15 +241,19 @@ struct Exchange {
   alignas(16) float vmax[2][4][NR];         // largest logit, by step parity and warp
   alignas(16) StepInfo info[4];             // by step
   float qmax[2][4][NR];                     // largest |q|, by pair and warp
-  uint32_t kt[4], vt[4];                    // largest T (bits) of the step's keys, values
-  // copied [stage], scaled [stage] and used [stage] of keys and values; operand written, products done [2], sums read [2] of the keys; operand
-  // written, products done of the values; end
-  unsigned long long bar[3 * (K_STAGES + V_STAGES) + 8];
-  int warp_sum[16];
+  alignas(16) uint32_t kt[4][4], vt[4][4];  // largest T (bits) of the step's keys, values, by step and warp
+  // copied [stage] and used [stage] of keys and values; largest T found [2], operand written, products done [2], sums read [2] of the keys; largest T
+  // found [2], operand written, products done of the values; end
+  unsigned long long bar[2 * (K_STAGES + V_STAGES) + 12];
+  int warp_sum[THREADS / 32];
   uint32_t tmem;
   int failed;
   int prefix[MAX_BATCH + 1];                // steps of the entries before
 };
+__device__ __forceinline__ uint32_t max4(const uint32_t* s) {
+  const uint4 v = *(const uint4*)s;
+  return max(max(v.x, v.y), max(v.z, v.w));
+}
 template <int N>
 __device__ __forceinline__ void load_floats(float (&v)[N], const float* s) {
 #pragma unroll
@@ -262,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
   constexpr int DT = BF ? MZ_BF16 : MZ_F16;
   constexpr int PB = 72 * D;                     // page bytes per kv head
   constexpr int RPT = D / 64;                    // rows of codes per thread, side and step
-  constexpr int STREAMS = D == 128 ? 2 : 4;      // records of a ring's part
+  constexpr int STREAMS = D == 128 ? 1 : 2;      // records of a ring's part
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Exchange<NR> x;
   const mz_paged_cache& c = p.c;
@@ -270,16 +277,16 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
   const uint32_t sbase = smem_u32(smem), sbook = sbase + S::BOOK;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t bars = smem_u32(x.bar);
-  const uint32_t k_full = bars, k_scaled = k_full + 8 * K_STAGES, k_used = k_scaled + 8 * K_STAGES;
-  const uint32_t v_full = k_used + 8 * K_STAGES, v_scaled = v_full + 8 * V_STAGES, v_used = v_scaled + 8 * V_STAGES;
-  const uint32_t k_ready = v_used + 8 * V_STAGES, k_done = k_ready + 8, k_free = k_done + 16, v_ready = k_free + 16, v_done = v_ready + 8, b_end = v_done + 8;
+  const uint32_t k_full = bars, k_used = k_full + 8 * K_STAGES, v_full = k_used + 8 * K_STAGES, v_used = v_full + 8 * V_STAGES;
+  const uint32_t k_scaled = v_used + 8 * V_STAGES, k_ready = k_scaled + 16, k_done = k_ready + 8, k_free = k_done + 16;
+  const uint32_t v_scaled = k_free + 16, v_ready = v_scaled + 16, v_done = v_ready + 8, b_end = v_done + 8;
   if (tid == 0) {
     x.failed = 0;
-    for (int i = 0; i < K_STAGES; ++i) { bar_init(k_full + 8 * i, 1); bar_init(k_scaled + 8 * i, 1); bar_init(k_used + 8 * i, 4); }
-    for (int i = 0; i < V_STAGES; ++i) { bar_init(v_full + 8 * i, 1); bar_init(v_scaled + 8 * i, 1); bar_init(v_used + 8 * i, 4); }
-    bar_init(k_ready, 4); bar_init(v_ready, 4);
-    for (int i = 0; i < 2; ++i) { bar_init(k_done + 8 * i, 2); bar_init(k_free + 8 * i, 4); }
-    bar_init(v_done, 1); bar_init(b_end, 2);
+    for (int i = 0; i < K_STAGES; ++i) { bar_init(k_full + 8 * i, 1); bar_init(k_used + 8 * i, 8); }
+    for (int i = 0; i < V_STAGES; ++i) { bar_init(v_full + 8 * i, 1); bar_init(v_used + 8 * i, 8); }
+    for (int i = 0; i < 2; ++i) { bar_init(k_scaled + 8 * i, 4); bar_init(k_done + 8 * i, 2); bar_init(k_free + 8 * i, 4); bar_init(v_scaled + 8 * i, 4); }
+    bar_init(k_ready, 8); bar_init(v_ready, 8);
+    bar_init(v_done, 1); bar_init(b_end, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (tid < MZP_BOOKS * MZP_LEVELS / 16) ((uint4*)(smem + S::BOOK))[tid] = ((const uint4*)book_table)[tid];
@@ -292,7 +299,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
   const int kp_all = c.kv_heads * p.passes;
   int total_steps = 0;
   {
-    constexpr int PER = MAX_BATCH / THREADS;
+    constexpr int PER = (MAX_BATCH + THREADS) / THREADS;      // one more entry than the batch has: the end
     int st[PER], sum = 0;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
@@ -308,14 +315,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
     __syncthreads();
     int before = scan - sum;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) { const int t = x.warp_sum[w]; if (w < warp) before += t; total_steps += t; }
+    for (int w = 0; w < THREADS / 32; ++w) { const int t = x.warp_sum[w]; if (w < warp) before += t; total_steps += t; }
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       const int b = tid * PER + k;
       if (b <= p.batch) x.prefix[b] = before;
       before += st[k];
     }
-    if (tid == THREADS - 1 && p.batch == MAX_BATCH) x.prefix[MAX_BATCH] = before;
   }
   const long long T = (long long)total_steps * kp_all;
   const int G = gridDim.x, cta = blockIdx.x;
@@ -335,17 +341,53 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
   const int team = warp >> 2;
   const int r = tid & 127;                       // key channel or token of this thread
 
+  // the largest T of a team's rows, found before anyone scales by it
+  auto publish_largest = [&](const uint32_t (&word)[RPT], uint32_t* slot, uint32_t bar) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < RPT; ++j) top = max(top, word[j] & 0xffffu);
+    top = warp_max_u32(top);
+    if (lane == 0) { slot[warp & 3] = top; bar_arrive(bar); }
+  };
+
   if (team == 0) {
-    // ================= keys: thread = channel
+    // ================= key levels: thread = channel
+    registers<Regs<NR>::KEY_LEVELS>();
     const int ch = D == 128 ? r : r & 63;
+    for (int it = 0; it < n; ++it) {
+      const int stage = it % K_STAGES;
+      bar_wait(k_full + 8 * stage, it / K_STAGES & 1, &x.failed);
+      const int valid = x.info[it & 3].valid;
+      uint32_t word[RPT];
+#pragma unroll
+      for (int j = 0; j < RPT; ++j) {
+        const int pg = D == 128 ? j : r >> 6;
+        word[j] = valid >> pg & 1 ? lds32(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + 32 * D + 4 * ch) : 0u;
+      }
+      publish_largest(word, x.kt[it & 3], k_scaled + 8 * (it & 1));
+      if (it > 0) bar_wait(k_done + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, &x.failed);      // the operand is free
+#pragma unroll
+      for (int j = 0; j < RPT; ++j) {
+        const int pg = D == 128 ? j : r >> 6;
+        expand_row(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + ch * 32, book128(sbook + mzp_row(word[j]).z * 16),
+                   sbase + S::K_A + pg * 4 * S::CHUNK + ch * 16, S::CHUNK, lane);
+      }
+      fence_operands();
+      __syncwarp();
+      if (lane == 0) { bar_arrive(k_ready); bar_arrive(k_used + 8 * stage); }
+    }
+  } else if (team == 1) {
+    // ================= key folds: thread = channel
+    registers<Regs<NR>::KEY_FOLDS>();
+    const int ch = D == 128 ? r : r & 63, tw = warp & 3;
     float q[NR];
     int seg = -1;
     for (int it = 0; it < n; ++it) {
       const int stage = it % K_STAGES;
-      const uint32_t phase = it / K_STAGES & 1;
-      bar_wait(k_full + 8 * stage, phase, &x.failed);
-      const StepInfo info = x.info[it & 3];
-      if (info.fresh) {
+      bar_wait(k_full + 8 * stage, it / K_STAGES & 1, &x.failed);
+      const int valid = x.info[it & 3].valid;
+      if (x.info[it & 3].fresh) {
+        const StepInfo info = x.info[it & 3];
         ++seg;
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
@@ -359,9 +401,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         for (int i = 0; i < NR; ++i) {
           // as bits, so that a NaN is the largest
           const uint32_t top = warp_max_u32(__float_as_uint(fabsf(q[i])));
-          if (lane == 0) x.qmax[seg & 1][warp][i] = __uint_as_float(top);
+          if (lane == 0) x.qmax[seg & 1][tw][i] = __uint_as_float(top);
         }
-        team_barrier(0);
+        team_barrier(1);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
           uint32_t top = 0;
@@ -370,46 +412,69 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
           const int e = max((int)(top >> 23) - 126, -60), e1 = e >> 1, e2 = e - e1;        // |q| < 2^e, taken off in two factors
           const bool wild = top >= 0x7f800000u;                        // infinity or NaN: the row's logits are NaN
           q[i] = wild ? 0.f : q[i] * pow2(-e1) * pow2(-e2);
-          if (tid == 0) x.qs[seg & 3][i] = wild ? __int_as_float(0x7fffffff) : pow2(e1) * p.scaling * pow2(e2);
+          if (r == 0) x.qs[seg & 3][i] = wild ? __int_as_float(0x7fffffff) : pow2(e1) * p.scaling * pow2(e2);
         }
       }
-      bar_wait(k_scaled + 8 * stage, phase, &x.failed);
-      const float up = pow2(30 - ((int)(x.kt[it & 3] >> 10) - 14));    // T < 2^(exponent field - 14)
       MzpRow row[RPT];
-      uint32_t fold[RPT][NR];
+#pragma unroll
+      for (int j = 0; j < RPT; ++j) {
+        const int pg = D == 128 ? j : r >> 6;
+        row[j] = mzp_row(valid >> pg & 1 ? lds32(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + 32 * D + 4 * ch) : 0u);
+      }
       {
         float base[RPT * NR];
 #pragma unroll
         for (int j = 0; j < RPT; ++j) {
-          const int pg = D == 128 ? j : r >> 6;
-          const uint32_t word = info.valid >> pg & 1 ? lds32(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + 32 * D + 4 * ch) : 0u;
-          row[j] = mzp_row(word);
-          const float ts = row[j].t * up, cz = fmaf(row[j].t, (float)row[j].z * -0.03125f, row[j].a);
+          const float cz = fmaf(row[j].t, (float)row[j].z * -0.03125f, row[j].a);
 #pragma unroll
-          for (int i = 0; i < NR; ++i) { fold[j][i] = digits_of(q[i] * ts); base[j * NR + i] = q[i] * cz; }
+          for (int i = 0; i < NR; ++i) base[j * NR + i] = q[i] * cz;
         }
         int index;
         const float sum = warp_sums<RPT * NR>(base, lane, index);
-        if ((lane & (32 / (RPT * NR) - 1)) == 0) x.base[it & 3][warp][index] = sum;
+        if ((lane & (32 / (RPT * NR) - 1)) == 0) x.base[it & 3][tw][index] = sum;
       }
-      if (it > 0) bar_wait(k_done + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, &x.failed);      // the operand is free
+      bar_wait(k_scaled + 8 * (it & 1), it >> 1 & 1, &x.failed);
+      const float up = pow2(30 - ((int)(max4(x.kt[it & 3]) >> 10) - 14));      // T < 2^(exponent field - 14)
+      if (it > 0) bar_wait(k_done + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, &x.failed);
 #pragma unroll
       for (int j = 0; j < RPT; ++j) {
         const int pg = D == 128 ? j : r >> 6;
+        const float ts = row[j].t * up;
 #pragma unroll
         for (int i = 0; i < NR; i += 4)
-          sts128(sbase + S::K_B + (pg * (NR / 4) + i / 4) * S::CHUNK + ch * 16, fold[j][i], fold[j][i + 1], fold[j][i + 2], fold[j][i + 3]);
-        expand_row(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + ch * 32, book128(sbook + row[j].z * 16), sbase + S::K_A + pg * 4 * S::CHUNK + ch * 16,
-                   S::CHUNK, lane);
+          sts128(sbase + S::K_B + (pg * (NR / 4) + i / 4) * S::CHUNK + ch * 16, digits_of(q[i] * ts), digits_of(q[i + 1] * ts), digits_of(q[i + 2] * ts),
+                 digits_of(q[i + 3] * ts));
       }
       fence_operands();
       __syncwarp();
       if (lane == 0) { bar_arrive(k_ready); bar_arrive(k_used + 8 * stage); }
     }
-  } else if (team == 1) {
-    // ================= softmax and values: thread = token, and position of the output
-    more_registers<Regs<NR>::VALUES>();
-    const int tw = warp - 4, blk = r >> 6;
+  } else if (team == 2) {
+    // ================= value levels: thread = token
+    registers<Regs<NR>::VALUE_LEVELS>();
+    const int blk = r >> 6;
+    for (int it = 0; it < n; ++it) {
+      const int stage = it % V_STAGES;
+      bar_wait(v_full + 8 * stage, it / V_STAGES & 1, &x.failed);
+      const bool valid = x.info[it & 3].valid >> blk & 1;
+      const uint32_t in = sbase + S::V_IN + (2 * stage + blk) * S::SIDE;
+      uint32_t word[RPT];
+#pragma unroll
+      for (int j = 0; j < RPT; ++j) word[j] = valid ? lds32(in + 32 * D + 4 * ((r & 63) * RPT + j)) : 0u;
+      publish_largest(word, x.vt[it & 3], v_scaled + 8 * (it & 1));
+      if (it > 0) bar_wait(v_done, (it - 1) & 1, &x.failed);                   // the operand is free
+#pragma unroll
+      for (int j = 0; j < RPT; ++j)
+        expand_row(in + ((r & 63) * RPT + j) * 32, book128(sbook + mzp_row(word[j]).z * 16),
+                   sbase + S::V_A + (D == 128 ? j : blk) * 4 * S::CHUNK + (D == 128 ? r : r & 63) * 16, S::CHUNK, lane);
+      fence_operands();
+      __syncwarp();
+      if (lane == 0) { bar_arrive(v_ready); bar_arrive(v_used + 8 * stage); }
+    }
+  } else if (team == 3) {
+    // ================= softmax: thread = token, and position of the output
+    registers<Regs<NR>::SOFTMAX>();
+    const int tw = warp & 3, blk = r >> 6;
     const uint32_t lanes = tmem + ((uint32_t)(tw * 32) << 16);
     float m[NR], l[NR], o[NR], base_v[RPT][NR], qs[NR];
     float vunit = 0.f;
@@ -453,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
 #pragma unroll
         for (int i = 0; i < NR; ++i) halves[(r - 64) * NR + i] = o[i];
       }
-      team_barrier(1);
+      team_barrier(3);
       const long long slot = (long long)cta + pair;
       const bool bad = *(volatile int*)&x.failed != 0;
       if (D == 128 || r < 64) {
@@ -472,13 +537,12 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         for (int i = 1; i < NR; ++i) top = r == i ? m[i] : top;
         p.ml[slot * NR + r] = bad ? make_float2(INFINITY, __int_as_float(0x7fffffff)) : make_float2(top, sum_l);
       }
-      team_barrier(1);                                       // fin and halves are free again
+      team_barrier(3);                                       // fin and halves are free again
     };
     reset();
     for (int it = 0; it < n; ++it) {
       const int stage = it % V_STAGES;
-      const uint32_t phase = it / V_STAGES & 1;
-      bar_wait(v_full + 8 * stage, phase, &x.failed);
+      bar_wait(v_full + 8 * stage, it / V_STAGES & 1, &x.failed);
       const StepInfo info = x.info[it & 3];
       if (info.fresh) {
         if (pair >= 0) {
@@ -492,7 +556,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
       bar_wait(k_done + 8 * (it & 1), (it >> 1) & 1, &x.failed);
       tm_after();
       if (info.fresh) load_floats(qs, x.qs[seg & 3]);
-      const float kunit = pow2((int)(x.kt[it & 3] >> 10) - 14 - 35);
+      const float kunit = pow2((int)(max4(x.kt[it & 3]) >> 10) - 14 - 35);
       float s[NR], base[NR];
       if (D == 128) {
         float b[4][NR];
@@ -532,7 +596,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         const float top = warp_max(s[i]);
         if (lane == 0) x.vmax[it & 1][tw][i] = top;
       }
-      team_barrier(1);
+      team_barrier(3);
       float fix[NR];
       bool moved = false;
       {
@@ -550,8 +614,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         m[i] = m_new;
         s[i] = ex2(s[i] - ref);
       }
-      bar_wait(v_scaled + 8 * stage, phase, &x.failed);
-      const int ev = (int)(x.vt[it & 3] >> 10) - 14;
+      bar_wait(v_scaled + 8 * (it & 1), it >> 1 & 1, &x.failed);
+      const int ev = (int)(max4(x.vt[it & 3]) >> 10) - 14;
       const float up = pow2(30 - ev);
       // ---- the output so far; then the operand is free
       if (it > 0 && !info.fresh) take_output(it - 1);
@@ -579,7 +643,6 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         for (int i = 0; i < NR; i += 4)
           sts128(sbase + S::V_B + (b2 * (NR / 4) + i / 4) * S::CHUNK + at * 16, digits_of(s[i] * ts), digits_of(s[i + 1] * ts),
                  digits_of(s[i + 2] * ts), digits_of(s[i + 3] * ts));
-        expand_row(in + vr * 32, book128(sbook + row.z * 16), sbase + S::V_A + b2 * 4 * S::CHUNK + at * 16, S::CHUNK, lane);
       }
       fence_operands();
       tm_before();
@@ -590,134 +653,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
       take_output(n - 1);
       write_record();
     }
-  } else if (team == 2) {
-    // ================= rings: a warp takes 16 tokens at a time, and (D = 128) 64 of the channels of the output.  A = keys [token][channel], B =
-    // queries; A = values [channel][token], B = p in two parts of 16 bits
-    if (Regs<NR>::RINGS > 64) more_registers<Regs<NR>::RINGS>();
-    const int g = lane >> 2, t = lane & 3, rw = warp - 8;
-    const int half = D == 128 ? rw & 1 : 0, stream = D == 128 ? rw >> 1 : rw;
-    const long long units = p.pairs * p.parts, first_slot = (long long)G + p.pairs;
-    for (long long unit = G - 1 - cta; unit < units; unit += G) {        // CTAs without steps come first
-      const int part = (int)(unit % p.parts);
-      const long long pair = unit / p.parts;
-      const int b = (int)(pair / kp_all), kp = (int)(pair % kp_all), head = kp / p.passes, r0 = kp % p.passes * NR;
-      int row;
-      const int len = length_of(b, row), packed = mzp_packed(len, c.residual), tokens = len - packed;
-      if (tokens == 0) continue;
-      const int tiles = (tokens + 15) / 16, end = tiles * (part + 1) / p.parts;
-      const uint16_t* ring_k = (const uint16_t*)c.tail + (long long)p.layer * c.tail_stride_layer + (long long)row * c.tail_stride_row + (long long)head * c.ring * D;
-      const uint16_t* ring_v = ring_k + (long long)c.kv_heads * c.ring * D + half * 64;
-      const int ring0 = packed % c.ring;
-      auto place = [&](int i) { const int at = ring0 + i; return (at >= c.ring ? at - c.ring : at) * D; };      // i < tokens <= ring
-      // queries into shared memory; rows that are not there are zero
-      team_barrier(2);
-      for (int i = r; i < 8 * D; i += 128) {
-        const int qi = i / D, d = i % D, qr = r0 + qi;
-        uint16_t v = 0;
-        if (qi < NR && qr < p.qrows) v = p.query[(long long)b * p.qsb + qr / p.group * p.qsl + (head * p.group + qr % p.group) * p.qsh + d];
-        *(uint16_t*)(smem + S::QUERY + qi * S::Q_ROW + 2 * d) = v;
-      }
-      team_barrier(2);
-      const int see0 = len - p.q_len - packed;               // query token l sees the ring's tokens up to see0 + l
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
-      for (int tile = tiles * part / p.parts + stream; tile < end; tile += STREAMS) {
-        const int i0 = tile * 16;
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-        {
-          const uint16_t* ka = ring_k + place(min(i0 + g, tokens - 1)) + 8 * t;
-          const uint16_t* kb = ring_k + place(min(i0 + g + 8, tokens - 1)) + 8 * t;
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) {
-            const uint4 va = *(const uint4*)(ka + 32 * k), vb = *(const uint4*)(kb + 32 * k);
-            const uint4 qf = lds128(sbase + S::QUERY + g * S::Q_ROW + (32 * k + 8 * t) * 2);
-            mma16<BF>(s, va.x, vb.x, va.y, vb.y, qf.x, qf.y);
-            mma16<BF>(s, va.z, vb.z, va.w, vb.w, qf.z, qf.w);
-          }
-        }
-        // s[0], s[1]: token g, columns (query rows) 2t, 2t + 1; s[2], s[3]: token g + 8
-        float fix[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int last = min(see0 + (r0 + 2 * t + j) / p.group, tokens - 1);
-          s[j] = i0 + g <= last ? s[j] * p.scaling : -INFINITY;
-          s[2 + j] = i0 + g + 8 <= last ? s[2 + j] * p.scaling : -INFINITY;
-          float top = fmaxf(s[j], s[2 + j]);
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          const float m_new = fmaxf(m[j], top), ref = m_new == -INFINITY ? 0.f : m_new;
-          fix[j] = ex2(m[j] - ref);
-          m[j] = m_new;
-          s[j] = ex2(s[j] - ref);
-          s[2 + j] = ex2(s[2 + j] - ref);
-          l[j] = l[j] * fix[j] + s[j] + s[2 + j];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { o[i][0] *= fix[0]; o[i][1] *= fix[1]; o[i][2] *= fix[0]; o[i][3] *= fix[1]; }
-        // p in two parts, transposed: column g, tokens 2t, 2t + 1 ([0]) and 2t + 8, 2t + 9 ([1])
-        uint32_t hi[2], lo[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t hw, lw;
-          if (BF) {
-            const __nv_bfloat162 hb = __floats2bfloat162_rn(s[2 * h], s[2 * h + 1]);
-            const float2 hf = __bfloat1622float2(hb);
-            const __nv_bfloat162 lb = __floats2bfloat162_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
-            hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
-          } else {
-            const __half2 hb = __floats2half2_rn(s[2 * h], s[2 * h + 1]);
-            const float2 hf = __half22float2(hb);
-            const __half2 lb = __floats2half2_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
-            hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
-          }
-          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(hi[h]) : "r"(hw));
-          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(lo[h]) : "r"(lw));
-        }
-        // A token that is not there, or that only later queries see, must not bring a NaN to a product with p = 0: what is not there is read as zero, and
-        // where a tile has tokens that only some of the queries see, each of the queries' tokens takes its turn with what it sees
-        const int l_first = r0 / p.group, l_last = (min(r0 + NR, p.qrows) - 1) / p.group;
-        const bool apart = i0 + 15 > see0 + l_first && l_last > l_first;
-        for (int turn = 0; turn <= (apart ? l_last - l_first : 0); ++turn) {
-          const int see = apart ? min(see0 + l_first + turn, tokens - 1) : tokens - 1;
-          const bool mine = !apart || (r0 + g) / p.group == l_first + turn;
-          uint4 v[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int i = i0 + 2 * t + (k & 1) + 8 * (k >> 1);
-            v[k] = make_uint4(0, 0, 0, 0);
-            if (i <= see) v[k] = *(const uint4*)(ring_v + place(i) + 8 * g);
-          }
-          const uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
-          const uint32_t w2[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // rows g / g + 8 = channels 8g + 2k / 8g + 2k + 1
-            const uint32_t a0 = prmt(w0[k], w1[k], 0x5410u), a1 = prmt(w0[k], w1[k], 0x7632u);
-            const uint32_t a2 = prmt(w2[k], w3[k], 0x5410u), a3 = prmt(w2[k], w3[k], 0x7632u);
-            mma16<BF>(o[k], a0, a1, a2, a3, mine ? lo[0] : 0u, mine ? lo[1] : 0u);
-            mma16<BF>(o[k], a0, a1, a2, a3, mine ? hi[0] : 0u, mine ? hi[1] : 0u);
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], off);
-        if (2 * t + j < NR) {
-          const long long slot = (first_slot + unit * STREAMS + stream) * NR + 2 * t + j;
-          float* dst = p.acc + slot * D + half * 64 + 8 * g;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) *(float2*)(dst + 2 * k) = make_float2(o[k][j], o[k][2 + j]);
-          if (g == 0 && half == 0) p.ml[slot] = make_float2(m[j], l[j]);
-        }
-      }
-    }
   } else {
-    fewer_registers<Regs<NR>::SERVICE>();
-    if (warp == 12) {
+    registers<Regs<NR>::SERVICE>();
+    if (warp == 16) {
       // ================= the line: page numbers, copies
       int b = 0, head = 0, pass = 0, step = 0, steps = 1, row = 0, len = 0;
       bool fresh = true;
@@ -787,54 +725,154 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         for (int k = 0; k < SPIN_LIMIT && !bar_test(k_full + 8 * (it % K_STAGES), it / K_STAGES & 1); ++k) {}
       for (int it = max(0, n - V_STAGES); it < n; ++it)
         for (int k = 0; k < SPIN_LIMIT && !bar_test(v_full + 8 * (it % V_STAGES), it / V_STAGES & 1); ++k) {}
-    } else if (warp == 13) {
-      // ================= a step's largest T, as the bits of an f16
-      auto largest = [&](uint32_t in, int valid) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int pg = 0; pg < 2; ++pg)
-          if (valid >> pg & 1) {
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) top = max(top, lds32(in + pg * S::SIDE + 32 * D + 4 * (lane + 32 * i)) & 0xffffu);
-          }
-        return warp_max_u32(top);
-      };
-      for (int it = 0; it < n; ++it) {
-        const int ks = it % K_STAGES, vs = it % V_STAGES;
-        bar_wait(k_full + 8 * ks, it / K_STAGES & 1, &x.failed);
-        const int valid = x.info[it & 3].valid;
-        const uint32_t kt = largest(sbase + S::K_IN + 2 * ks * S::SIDE, valid);
-        if (lane == 0) { x.kt[it & 3] = kt; bar_arrive(k_scaled + 8 * ks); }
-        bar_wait(v_full + 8 * vs, it / V_STAGES & 1, &x.failed);
-        const uint32_t vt = largest(sbase + S::V_IN + 2 * vs * S::SIDE, valid);
-        if (lane == 0) { x.vt[it & 3] = vt; bar_arrive(v_scaled + 8 * vs); }
-      }
-    } else if (warp == 14) {
-      // ================= products of the keys
+    } else if (warp == 17) {
+      // ================= MMAs, of the keys and of the values as each are ready
       if (lane == 0) {
-        const uint64_t a = descriptor(sbase + S::K_A, S::CHUNK), bd = descriptor(sbase + S::K_B, S::CHUNK);
-        for (int it = 0; it < n; ++it) {
-          bar_wait(k_ready, it & 1, &x.failed);
-          if (it >= 2) bar_wait(k_free + 8 * (it & 1), ((it - 2) >> 1) & 1, &x.failed);
-          bar_arrive(k_done + 8 * (it & 1));     // hands on what the keys' threads wrote beside the operand
-          if (*(volatile int*)&x.failed) break;
-          tm_after();
+        const uint64_t ka = descriptor(sbase + S::K_A, S::CHUNK), kb = descriptor(sbase + S::K_B, S::CHUNK);
+        const uint64_t va = descriptor(sbase + S::V_A, S::CHUNK), vb = descriptor(sbase + S::V_B, S::CHUNK);
+        int ki = 0, vi = 0;
+        for (int idle = 0; vi < n && idle < SPIN_LIMIT; ++idle) {
+          if (ki < n && bar_test(k_ready, ki & 1) && (ki < 2 || bar_test(k_free + 8 * (ki & 1), (ki >> 1 & 1) ^ 1))) {
+            bar_arrive(k_done + 8 * (ki & 1));   // hands on what the keys' threads wrote beside the operand
+            tm_after();
 #pragma unroll
-          for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_S + (it & 1) * S::N, a + k * (512 >> 4), bd + k * (512 >> 4), k > 0);
-          umma_commit(k_done + 8 * (it & 1));
+            for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_S + (ki & 1) * S::N, ka + k * (512 >> 4), kb + k * (512 >> 4), k > 0);
+            umma_commit(k_done + 8 * (ki & 1));
+            ++ki; idle = 0;
+          }
+          if (bar_test(v_ready, vi & 1)) {
+            tm_after();
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_O, va + k * (512 >> 4), vb + k * (512 >> 4), k > 0);
+            umma_commit(v_done);
+            ++vi; idle = 0;
+          }
+          if (*(volatile int*)&x.failed) break;
         }
+        if (vi < n) *(volatile int*)&x.failed = 1;
       }
     } else {
-      // ================= products of the values
-      if (lane == 0) {
-        const uint64_t a = descriptor(sbase + S::V_A, S::CHUNK), bd = descriptor(sbase + S::V_B, S::CHUNK);
-        for (int it = 0; it < n; ++it) {
-          bar_wait(v_ready, it & 1, &x.failed);
-          if (*(volatile int*)&x.failed) break;
-          tm_after();
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_O, a + k * (512 >> 4), bd + k * (512 >> 4), k > 0);
-          umma_commit(v_done);
+      // ================= rings: a warp takes 16 tokens at a time, and (D = 128) 64 of the channels of the output.  A = keys [token][channel], B =
+      // queries; A = values [channel][token], B = p in two parts of 16 bits
+      const int g = lane >> 2, t = lane & 3, rw = warp - 18;
+      const int half = D == 128 ? rw : 0, stream = D == 128 ? 0 : rw;
+      const long long units = p.pairs * p.parts, first_slot = (long long)G + p.pairs;
+      for (long long unit = G - 1 - cta; unit < units; unit += G) {        // CTAs without steps come first
+        const int part = (int)(unit % p.parts);
+        const long long pair = unit / p.parts;
+        const int b = (int)(pair / kp_all), kp = (int)(pair % kp_all), head = kp / p.passes, r0 = kp % p.passes * NR;
+        int row;
+        const int len = length_of(b, row), packed = mzp_packed(len, c.residual), tokens = len - packed;
+        if (tokens == 0) continue;
+        const int tiles = (tokens + 15) / 16, end = tiles * (part + 1) / p.parts;
+        const uint16_t* ring_k = (const uint16_t*)c.tail + (long long)p.layer * c.tail_stride_layer + (long long)row * c.tail_stride_row + (long long)head * c.ring * D;
+        const uint16_t* ring_v = ring_k + (long long)c.kv_heads * c.ring * D + half * 64;
+        const int ring0 = packed % c.ring;
+        auto place = [&](int i) { const int at = ring0 + i; return (at >= c.ring ? at - c.ring : at) * D; };      // i < tokens <= ring
+        // queries into shared memory; rows that are not there are zero
+        asm volatile("bar.sync 6, 64;" ::: "memory");
+        for (int i = tid & 63; i < 8 * D; i += 64) {
+          const int qi = i / D, d = i % D, qr = r0 + qi;
+          uint16_t v = 0;
+          if (qi < NR && qr < p.qrows) v = p.query[(long long)b * p.qsb + qr / p.group * p.qsl + (head * p.group + qr % p.group) * p.qsh + d];
+          *(uint16_t*)(smem + S::QUERY + qi * S::Q_ROW + 2 * d) = v;
+        }
+        asm volatile("bar.sync 6, 64;" ::: "memory");
+        const int see0 = len - p.q_len - packed;               // query token l sees the ring's tokens up to see0 + l
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4][4];
+  #pragma unroll
+        for (int i = 0; i < 4; ++i)
+  #pragma unroll
+          for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+        for (int tile = tiles * part / p.parts + stream; tile < end; tile += STREAMS) {
+          const int i0 = tile * 16;
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
+          {
+            const uint16_t* ka = ring_k + place(min(i0 + g, tokens - 1)) + 8 * t;
+            const uint16_t* kb = ring_k + place(min(i0 + g + 8, tokens - 1)) + 8 * t;
+  #pragma unroll
+            for (int k = 0; k < D / 32; ++k) {
+              const uint4 va = *(const uint4*)(ka + 32 * k), vb = *(const uint4*)(kb + 32 * k);
+              const uint4 qf = lds128(sbase + S::QUERY + g * S::Q_ROW + (32 * k + 8 * t) * 2);
+              mma16<BF>(s, va.x, vb.x, va.y, vb.y, qf.x, qf.y);
+              mma16<BF>(s, va.z, vb.z, va.w, vb.w, qf.z, qf.w);
+            }
+          }
+          // s[0], s[1]: token g, columns (query rows) 2t, 2t + 1; s[2], s[3]: token g + 8
+          float fix[2];
+  #pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int last = min(see0 + (r0 + 2 * t + j) / p.group, tokens - 1);
+            s[j] = i0 + g <= last ? s[j] * p.scaling : -INFINITY;
+            s[2 + j] = i0 + g + 8 <= last ? s[2 + j] * p.scaling : -INFINITY;
+            float top = fmaxf(s[j], s[2 + j]);
+  #pragma unroll
+            for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            const float m_new = fmaxf(m[j], top), ref = m_new == -INFINITY ? 0.f : m_new;
+            fix[j] = ex2(m[j] - ref);
+            m[j] = m_new;
+            s[j] = ex2(s[j] - ref);
+            s[2 + j] = ex2(s[2 + j] - ref);
+            l[j] = l[j] * fix[j] + s[j] + s[2 + j];
+          }
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) { o[i][0] *= fix[0]; o[i][1] *= fix[1]; o[i][2] *= fix[0]; o[i][3] *= fix[1]; }
+          // p in two parts, transposed: column g, tokens 2t, 2t + 1 ([0]) and 2t + 8, 2t + 9 ([1])
+          uint32_t hi[2], lo[2];
+  #pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t hw, lw;
+            if (BF) {
+              const __nv_bfloat162 hb = __floats2bfloat162_rn(s[2 * h], s[2 * h + 1]);
+              const float2 hf = __bfloat1622float2(hb);
+              const __nv_bfloat162 lb = __floats2bfloat162_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
+              hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
+            } else {
+              const __half2 hb = __floats2half2_rn(s[2 * h], s[2 * h + 1]);
+              const float2 hf = __half22float2(hb);
+              const __half2 lb = __floats2half2_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
+              hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
+            }
+            asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(hi[h]) : "r"(hw));
+            asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(lo[h]) : "r"(lw));
+          }
+          // A token that is not there, or that only later queries see, must not bring a NaN to a product with p = 0: what is not there is read as zero, and
+          // where a tile has tokens that only some of the queries see, each of the queries' tokens takes its turn with what it sees
+          const int l_first = r0 / p.group, l_last = (min(r0 + NR, p.qrows) - 1) / p.group;
+          const bool apart = i0 + 15 > see0 + l_first && l_last > l_first;
+          for (int turn = 0; turn <= (apart ? l_last - l_first : 0); ++turn) {
+            const int see = apart ? min(see0 + l_first + turn, tokens - 1) : tokens - 1;
+            const bool mine = !apart || (r0 + g) / p.group == l_first + turn;
+            uint4 v[4];
+  #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int i = i0 + 2 * t + (k & 1) + 8 * (k >> 1);
+              v[k] = make_uint4(0, 0, 0, 0);
+              if (i <= see) v[k] = *(const uint4*)(ring_v + place(i) + 8 * g);
+            }
+            const uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+            const uint32_t w2[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
+  #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              // rows g / g + 8 = channels 8g + 2k / 8g + 2k + 1
+              const uint32_t a0 = prmt(w0[k], w1[k], 0x5410u), a1 = prmt(w0[k], w1[k], 0x7632u);
+              const uint32_t a2 = prmt(w2[k], w3[k], 0x5410u), a3 = prmt(w2[k], w3[k], 0x7632u);
+              mma16<BF>(o[k], a0, a1, a2, a3, mine ? lo[0] : 0u, mine ? lo[1] : 0u);
+              mma16<BF>(o[k], a0, a1, a2, a3, mine ? hi[0] : 0u, mine ? hi[1] : 0u);
+            }
+          }
+        }
+  #pragma unroll
+        for (int j = 0; j < 2; ++j) {
+  #pragma unroll
+          for (int off = 4; off < 32; off <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], off);
+          if (2 * t + j < NR) {
+            const long long slot = (first_slot + unit * STREAMS + stream) * NR + 2 * t + j;
+            float* dst = p.acc + slot * D + half * 64 + 8 * g;
+  #pragma unroll
+            for (int k = 0; k < 4; ++k) *(float2*)(dst + 2 * k) = make_float2(o[k][j], o[k][2 + j]);
+            if (g == 0 && half == 0) p.ml[slot] = make_float2(m[j], l[j]);
+          }
         }
       }
     }
@@ -842,7 +880,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
   }
   __syncthreads();
   if (n == 0) return;
-  if (x.failed && (tid & ~32) == 14 * 32) {      // products in flight end before their memory goes back
+  if (x.failed && tid == 17 * 32) {      // products in flight end before their memory goes back
     umma_commit(b_end);
     for (int k = 0; k < SPIN_LIMIT && !bar_test(b_end, 0); ++k) {}
   }
@@ -867,7 +905,7 @@ __global__ void __launch_bounds__(D) merge_kernel(const Args p, int G) {
   if (!known && d == 0) atomicOr(p.c.status, MZ_PAGED_BAD_INDEX);
   const int len = known ? max(0, min(p.c.lengths[row], 0x7fffffff - STEP)) : 0;
   const bool ring = len > mzp_packed(len, p.c.residual);
-  constexpr int STREAMS = D == 128 ? 2 : 4;
+  constexpr int STREAMS = D == 128 ? 1 : 2;
   const long long W = p.head[0], T = *(const long long*)(p.head + 2);
   const long long steps = p.head[4 + b + 1] - p.head[4 + b], s0 = (long long)p.head[4 + b] * kp_all + kp * steps;
   float m = -INFINITY, l = 0.f, a = 0.f;
@@ -952,7 +990,7 @@ int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* 
   MZ_REQUIRE(s->pairs * s->nr < (1ll << 31), "too many query rows for one call");
   s->G = sms * CTAS_PER_SM;
   // few pairs: their rings are cut until a warp has one tile of 16 tokens or the CTAs are taken
-  const int streams = c->head_dim == 128 ? 2 : 4, most = ((c->residual + MZP_PAGE - 1 + 15) / 16 + streams - 1) / streams;
+  const int streams = c->head_dim == 128 ? 1 : 2, most = ((c->residual + MZP_PAGE - 1 + 15) / 16 + streams - 1) / streams;
   const long long share = s->pairs > 0 ? s->G / s->pairs : 1;
   s->parts = (int)(share < 1 ? 1 : share > most ? most : share);
   s->head_bytes = ((4 + (size_t)batch + 1) * sizeof(int) + 127) / 128 * 128;
