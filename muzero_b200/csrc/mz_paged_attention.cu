@@ -152,6 +152,21 @@ __device__ __forceinline__ float number_of(const int* c) { return fmaf((float)(c
 __device__ __forceinline__ uint32_t digits_of(float x) { return ((uint32_t)__float2int_rn(x) + 0x808080u) ^ 0x808080u; }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
 
+// pairs of fp32 operations
+__device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void fma2(float& c0, float& c1, float a0, float a1, float f) {      // c += a * f
+  asm("{\n\t.reg .b64 a, c, f;\n\tmov.b64 c, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\tmov.b64 f, {%4, %4};\n\tfma.rn.f32x2 c, a, f, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "+f"(c0), "+f"(c1) : "f"(a0), "f"(a1), "f"(f));
+}
+// r = (a * f + b) * c
+__device__ __forceinline__ void mul_add2(float& r0, float& r1, float a0, float a1, float b0, float b1, float c0, float c1, float f) {
+  asm("{\n\t.reg .b64 a, b, c, f;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tmov.b64 f, {%8, %8};\n\t"
+      "fma.rn.f32x2 a, a, f, b;\n\tmul.rn.f32x2 a, a, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(r0), "=f"(r1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1), "f"(f));
+}
+
 // Sums of N values over a warp, N values at a time: after it lane l has the sum of value index_of(l).  N a power of two, at most 32
 template <int N>
 __device__ __forceinline__ float warp_sums(float (&v)[N], int lane, int& index) {
@@ -202,12 +217,12 @@ __device__ __forceinline__ void expand_half(const uint4& codes, const uint4& boo
   }
 }
 // A row's 32 bytes of codes at `src` -> its 64 levels.  Of eight neighbouring threads the upper four take the second half first: then the
-// eight read from different banks.
+// eight read from different banks.  A loop, as are those around it: what a group does in a step is straight code otherwise, and an SM that runs five such
+// pieces waits for instructions
 __device__ __forceinline__ void expand_row(uint32_t src, const uint4& book, uint32_t dst, uint32_t chunk, int lane) {
-  const uint32_t half = (lane >> 2) & 1;
-  const uint4 first = lds128(src + 16 * half), second = lds128(src + 16 - 16 * half);
-  expand_half(first, book, dst + 2 * half * chunk, chunk);
-  expand_half(second, book, dst + 2 * (1 - half) * chunk, chunk);
+  uint32_t half = (lane >> 2) & 1;
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k, half ^= 1) expand_half(lds128(src + 16 * half), book, dst + 2 * half * chunk, chunk);
 }
 
 // shared memory of a CTA
@@ -366,10 +381,10 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
       }
       publish_largest(word, x.kt[it & 3], k_scaled + 8 * (it & 1));
       if (it > 0) bar_wait(k_done + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, &x.failed);      // the operand is free
-#pragma unroll
+#pragma unroll 1
       for (int j = 0; j < RPT; ++j) {
         const int pg = D == 128 ? j : r >> 6;
-        expand_row(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + ch * 32, book128(sbook + mzp_row(word[j]).z * 16),
+        expand_row(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + ch * 32, book128(sbook + mzp_row(j ? word[RPT - 1] : word[0]).z * 16),
                    sbase + S::K_A + pg * 4 * S::CHUNK + ch * 16, S::CHUNK, lane);
       }
       fence_operands();
@@ -427,7 +442,10 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         for (int j = 0; j < RPT; ++j) {
           const float cz = fmaf(row[j].t, (float)row[j].z * -0.03125f, row[j].a);
 #pragma unroll
-          for (int i = 0; i < NR; ++i) base[j * NR + i] = q[i] * cz;
+          for (int i = 0; i < NR; i += 2) {
+            base[j * NR + i] = base[j * NR + i + 1] = 0.f;
+            fma2(base[j * NR + i], base[j * NR + i + 1], q[i], q[i + 1], cz);
+          }
         }
         int index;
         const float sum = warp_sums<RPT * NR>(base, lane, index);
@@ -441,9 +459,12 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         const int pg = D == 128 ? j : r >> 6;
         const float ts = row[j].t * up;
 #pragma unroll
-        for (int i = 0; i < NR; i += 4)
-          sts128(sbase + S::K_B + (pg * (NR / 4) + i / 4) * S::CHUNK + ch * 16, digits_of(q[i] * ts), digits_of(q[i + 1] * ts), digits_of(q[i + 2] * ts),
-                 digits_of(q[i + 3] * ts));
+        for (int i = 0; i < NR; i += 4) {
+          float f[4] = {0.f, 0.f, 0.f, 0.f};
+          fma2(f[0], f[1], q[i], q[i + 1], ts);
+          fma2(f[2], f[3], q[i + 2], q[i + 3], ts);
+          sts128(sbase + S::K_B + (pg * (NR / 4) + i / 4) * S::CHUNK + ch * 16, digits_of(f[0]), digits_of(f[1]), digits_of(f[2]), digits_of(f[3]));
+        }
       }
       fence_operands();
       __syncwarp();
@@ -463,9 +484,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
       for (int j = 0; j < RPT; ++j) word[j] = valid ? lds32(in + 32 * D + 4 * ((r & 63) * RPT + j)) : 0u;
       publish_largest(word, x.vt[it & 3], v_scaled + 8 * (it & 1));
       if (it > 0) bar_wait(v_done, (it - 1) & 1, &x.failed);                   // the operand is free
-#pragma unroll
+#pragma unroll 1
       for (int j = 0; j < RPT; ++j)
-        expand_row(in + ((r & 63) * RPT + j) * 32, book128(sbook + mzp_row(word[j]).z * 16),
+        expand_row(in + ((r & 63) * RPT + j) * 32, book128(sbook + mzp_row(j ? word[RPT - 1] : word[0]).z * 16),
                    sbase + S::V_A + (D == 128 ? j : blk) * 4 * S::CHUNK + (D == 128 ? r : r & 63) * 16, S::CHUNK, lane);
       fence_operands();
       __syncwarp();
@@ -563,7 +584,12 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
 #pragma unroll
         for (int w = 0; w < 4; ++w) load_floats(b[w], x.base[it & 3][w] + blk * NR);
 #pragma unroll
-        for (int i = 0; i < NR; ++i) base[i] = (b[0][i] + b[1][i]) + (b[2][i] + b[3][i]);
+        for (int i = 0; i < NR; i += 2) {
+          add2(b[0][i], b[0][i + 1], b[1][i], b[1][i + 1]);
+          add2(b[2][i], b[2][i + 1], b[3][i], b[3][i + 1]);
+          add2(b[0][i], b[0][i + 1], b[2][i], b[2][i + 1]);
+          base[i] = b[0][i]; base[i + 1] = b[0][i + 1];
+        }
       } else {
         float b[2][NR];
 #pragma unroll
@@ -576,28 +602,30 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         int a[16];
         tm_ld16(lanes + S::TM_S + (it & 1) * S::N + blk * (4 * NR) + 4 * i, a);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[i + k] = number_of(a + 4 * k) * kunit;
+        for (int k = 0; k < 4; ++k) s[i + k] = number_of(a + 4 * k);
       }
       tm_before();
       __syncwarp();
       if (lane == 0) bar_arrive(k_free + 8 * (it & 1));
 #pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        s[i] = (s[i] + base[i]) * qs[i];
-        if (r >= info.count) s[i] = -INFINITY;
+      for (int i = 0; i < NR; i += 2) mul_add2(s[i], s[i + 1], s[i], s[i + 1], base[i], base[i + 1], qs[i], qs[i + 1], kunit);
+      if (info.count < STEP) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i) if (r >= info.count) s[i] = -INFINITY;
       }
       if (info.see < info.count - 1) {                       // not every query sees all of the step
 #pragma unroll
         for (int i = 0; i < NR; ++i) if (r > info.see + (info.r0 + i) / p.group - info.r0 / p.group) s[i] = -INFINITY;
       }
       // ---- running maximum
+      float fix[NR];
 #pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        const float top = warp_max(s[i]);
-        if (lane == 0) x.vmax[it & 1][tw][i] = top;
+      for (int i = 0; i < NR; ++i) fix[i] = warp_max(s[i]);
+      if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < NR; i += 4) *(float4*)&x.vmax[it & 1][tw][i] = make_float4(fix[i], fix[i + 1], fix[i + 2], fix[i + 3]);
       }
       team_barrier(3);
-      float fix[NR];
       bool moved = false;
       {
         float v[4][NR];
@@ -608,11 +636,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
       }
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        const float m_new = fmaxf(m[i], fix[i]), ref = m_new == -INFINITY ? 0.f : m_new;
-        fix[i] = ex2(m[i] - ref);
-        moved |= m_new != m[i];
-        m[i] = m_new;
-        s[i] = ex2(s[i] - ref);
+        moved |= fix[i] > m[i];
+        fix[i] = fmaxf(m[i], fix[i]);
+        s[i] = ex2(s[i] - (fix[i] == -INFINITY ? 0.f : fix[i]));
       }
       bar_wait(v_scaled + 8 * (it & 1), it >> 1 & 1, &x.failed);
       const int ev = (int)(max4(x.vt[it & 3]) >> 10) - 14;
@@ -622,14 +648,16 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
       if (moved) {                                           // the same for all threads
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-          o[i] *= fix[i]; l[i] *= fix[i];
+          const float f = ex2(m[i] - (fix[i] == -INFINITY ? 0.f : fix[i]));
+          m[i] = fix[i];
+          o[i] *= f; l[i] *= f;
 #pragma unroll
-          for (int j = 0; j < RPT; ++j) base_v[j][i] *= fix[i];
+          for (int j = 0; j < RPT; ++j) base_v[j][i] *= f;
         }
       }
       vunit = pow2(ev - 35);
 #pragma unroll
-      for (int i = 0; i < NR; ++i) l[i] += s[i];
+      for (int i = 0; i < NR; i += 2) add2(l[i], l[i + 1], s[i], s[i + 1]);
 #pragma unroll
       for (int j = 0; j < RPT; ++j) {
         const int vr = (r & 63) * RPT + j;
@@ -638,11 +666,14 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         const float ts = row.t * up, cz = fmaf(row.t, (float)row.z * -0.03125f, row.a);
         const int b2 = D == 128 ? j : blk, at = D == 128 ? r : r & 63;
 #pragma unroll
-        for (int i = 0; i < NR; ++i) base_v[j][i] = fmaf(s[i], cz, base_v[j][i]);
+        for (int i = 0; i < NR; i += 2) fma2(base_v[j][i], base_v[j][i + 1], s[i], s[i + 1], cz);
 #pragma unroll
-        for (int i = 0; i < NR; i += 4)
-          sts128(sbase + S::V_B + (b2 * (NR / 4) + i / 4) * S::CHUNK + at * 16, digits_of(s[i] * ts), digits_of(s[i + 1] * ts),
-                 digits_of(s[i + 2] * ts), digits_of(s[i + 3] * ts));
+        for (int i = 0; i < NR; i += 4) {
+          float f[4] = {0.f, 0.f, 0.f, 0.f};
+          fma2(f[0], f[1], s[i], s[i + 1], ts);
+          fma2(f[2], f[3], s[i + 2], s[i + 3], ts);
+          sts128(sbase + S::V_B + (b2 * (NR / 4) + i / 4) * S::CHUNK + at * 16, digits_of(f[0]), digits_of(f[1]), digits_of(f[2]), digits_of(f[3]));
+        }
       }
       fence_operands();
       tm_before();
@@ -683,6 +714,10 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         const int page0 = __shfl_sync(0xffffffffu, ids, k0 - ids_at), page1 = __shfl_sync(0xffffffffu, ids, k0 + 1 - ids_at);
         const int ks = it % K_STAGES, vs = it % V_STAGES;
         if (it >= K_STAGES) bar_wait(k_used + 8 * ks, (it / K_STAGES - 1) & 1, &x.failed);
+        const uint32_t bytes = S::SIDE * ((page0 >= 0) + (page1 >= 0));
+        const uint8_t* store = (const uint8_t*)c.store + (long long)p.layer * c.store_stride_layer + head * PB;
+        const uint8_t *src0 = store + (long long)page0 * c.store_stride_page, *src1 = store + (long long)page1 * c.store_stride_page;
+        const uint32_t kin = sbase + S::K_IN + 2 * ks * S::SIDE, vin = sbase + S::V_IN + 2 * vs * S::SIDE;
         if (lane == 0) {
           StepInfo info;
           info.pair = (b * c.kv_heads + head) * p.passes + pass;
@@ -694,14 +729,12 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
           info.head = head;
           info.valid = (page0 >= 0 ? 1 : 0) | (page1 >= 0 ? 2 : 0);
           x.info[it & 3] = info;
-          const uint32_t bytes = S::SIDE * ((page0 >= 0) + (page1 >= 0));
-          const uint8_t* store = (const uint8_t*)c.store + (long long)p.layer * c.store_stride_layer + head * PB;
-          const uint8_t *src0 = store + (long long)page0 * c.store_stride_page, *src1 = store + (long long)page1 * c.store_stride_page;
-          const uint32_t kin = sbase + S::K_IN + 2 * ks * S::SIDE, vin = sbase + S::V_IN + 2 * vs * S::SIDE;
           bar_expect(k_full + 8 * ks, bytes);
           if (page0 >= 0) bulk_copy(kin, src0, S::SIDE, k_full + 8 * ks);
           if (page1 >= 0) bulk_copy(kin + S::SIDE, src1, S::SIDE, k_full + 8 * ks);
-          if (it >= V_STAGES) bar_wait(v_used + 8 * vs, (it / V_STAGES - 1) & 1, &x.failed);
+        }
+        if (it >= V_STAGES) bar_wait(v_used + 8 * vs, (it / V_STAGES - 1) & 1, &x.failed);
+        if (lane == 0) {
           bar_expect(v_full + 8 * vs, bytes);
           if (page0 >= 0) bulk_copy(vin, src0 + S::SIDE, S::SIDE, v_full + 8 * vs);
           if (page1 >= 0) bulk_copy(vin + S::SIDE, src1 + S::SIDE, S::SIDE, v_full + 8 * vs);
@@ -726,30 +759,34 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
       for (int it = max(0, n - V_STAGES); it < n; ++it)
         for (int k = 0; k < SPIN_LIMIT && !bar_test(v_full + 8 * (it % V_STAGES), it / V_STAGES & 1); ++k) {}
     } else if (warp == 17) {
-      // ================= MMAs, of the keys and of the values as each are ready
-      if (lane == 0) {
-        const uint64_t ka = descriptor(sbase + S::K_A, S::CHUNK), kb = descriptor(sbase + S::K_B, S::CHUNK);
-        const uint64_t va = descriptor(sbase + S::V_A, S::CHUNK), vb = descriptor(sbase + S::V_B, S::CHUNK);
-        int ki = 0, vi = 0;
-        for (int idle = 0; vi < n && idle < SPIN_LIMIT; ++idle) {
-          if (ki < n && bar_test(k_ready, ki & 1) && (ki < 2 || bar_test(k_free + 8 * (ki & 1), (ki >> 1 & 1) ^ 1))) {
-            bar_arrive(k_done + 8 * (ki & 1));   // hands on what the keys' threads wrote beside the operand
+      // ================= MMAs, in the order keys 0, keys 1, values 0, keys 2, values 1, ...  (The whole warp waits: a diverged one would poll.)
+      const uint64_t ka = descriptor(sbase + S::K_A, S::CHUNK), kb = descriptor(sbase + S::K_B, S::CHUNK);
+      const uint64_t va = descriptor(sbase + S::V_A, S::CHUNK), vb = descriptor(sbase + S::V_B, S::CHUNK);
+      auto keys = [&](int it) {
+        bar_wait(k_ready, it & 1, &x.failed);
+        if (it >= 2) bar_wait(k_free + 8 * (it & 1), (it >> 1 & 1) ^ 1, &x.failed);
+        if (lane == 0) {
+          bar_arrive(k_done + 8 * (it & 1));     // hands on what the keys' threads wrote beside the operand
+          if (!*(volatile int*)&x.failed) {
             tm_after();
 #pragma unroll
-            for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_S + (ki & 1) * S::N, ka + k * (512 >> 4), kb + k * (512 >> 4), k > 0);
-            umma_commit(k_done + 8 * (ki & 1));
-            ++ki; idle = 0;
+            for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_S + (it & 1) * S::N, ka + k * (512 >> 4), kb + k * (512 >> 4), k > 0);
+            umma_commit(k_done + 8 * (it & 1));
           }
-          if (bar_test(v_ready, vi & 1)) {
-            tm_after();
-#pragma unroll
-            for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_O, va + k * (512 >> 4), vb + k * (512 >> 4), k > 0);
-            umma_commit(v_done);
-            ++vi; idle = 0;
-          }
-          if (*(volatile int*)&x.failed) break;
         }
-        if (vi < n) *(volatile int*)&x.failed = 1;
+        __syncwarp();
+      };
+      if (n > 0) keys(0);
+      for (int it = 0; it < n; ++it) {
+        if (it + 1 < n) keys(it + 1);
+        bar_wait(v_ready, it & 1, &x.failed);
+        if (lane == 0 && !*(volatile int*)&x.failed) {
+          tm_after();
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_O, va + k * (512 >> 4), vb + k * (512 >> 4), k > 0);
+          umma_commit(v_done);
+        }
+        __syncwarp();
       }
     } else {
       // ================= rings: a warp takes 16 tokens at a time, and (D = 128) 64 of the channels of the output.  A = keys [token][channel], B =
