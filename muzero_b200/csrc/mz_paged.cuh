@@ -32,6 +32,11 @@ __device__ __forceinline__ MzpRow mzp_row(uint32_t word) {
   r.z = off ? ((field & 0x8000u) ? 127 : 0) : (int)field;
   return r;
 }
+// its zero level alone
+__device__ __forceinline__ int mzp_zero(uint32_t word) {
+  const uint32_t field = word >> 16;
+  return (field & 0x7FFFu) < 128u ? (int)field : (field & 0x8000u) ? 127 : 0;
+}
 
 // The other way: smallest and largest value of the row (NaN taken as 0, clamped to f16's range) -> constants of the quantizer and the word.  One IEEE
 // operation per step, none contracted: the codes are a definition, not an approximation.

@@ -32,9 +32,8 @@ constexpr int SPIN_LIMIT = 1000000;              // looks of a wait before it gi
 // registers of the groups: they share what the 640 threads are launched with, 48 each
 template <int NR>
 struct Regs {
-  static constexpr int KEY_LEVELS = NR == 4 ? 40 : 32, KEY_FOLDS = NR == 4 ? 48 : 56, VALUE_LEVELS = NR == 4 ? 40 : 32, SOFTMAX = NR == 4 ? 72 : 88,
-                       SERVICE = NR == 4 ? 40 : 32;
-  static_assert(KEY_LEVELS + KEY_FOLDS + VALUE_LEVELS + SOFTMAX + SERVICE <= 5 * 48, "register split");
+  static constexpr int LEVELS = 32, KEY_FOLDS = NR == 4 ? 48 : 56, SOFTMAX = NR == 4 ? 72 : 88, SERVICE = NR == 4 ? 56 : 32;
+  static_assert(2 * LEVELS + KEY_FOLDS + SOFTMAX + SERVICE <= 5 * 48, "register split");
 };
 constexpr int STEP = 2 * MZP_PAGE;
 
@@ -123,10 +122,10 @@ __device__ __forceinline__ void registers() {    // launched with 48
 __device__ __forceinline__ uint64_t descriptor(uint32_t sa, uint32_t chunk) {
   return (uint64_t)((sa >> 4) & 0x3FFF) | (128ull >> 4) << 16 | (uint64_t)(chunk >> 4) << 32 | 1ull << 46;
 }
-// D[128 x N] (+)= A[128 x 32] * B[32 x N], unsigned times signed bytes into 32 bits
-template <int N>
+// D[128 x N] (+)= A[128 x 32] * B[32 x N], unsigned times signed or unsigned bytes into 32 bits
+template <int N, bool SIGNED_B>
 __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t accumulate) {
-  const uint32_t idesc = (2u << 4) | (1u << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(N / 8) << 17) | (8u << 24);
+  const uint32_t idesc = (2u << 4) | ((SIGNED_B ? 1u : 0u) << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(N / 8) << 17) | (8u << 24);
   const uint32_t zero = 0;
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -148,7 +147,7 @@ __device__ __forceinline__ void tm_ld16(uint32_t taddr, int* c) {
 }
 // four bytes' accumulators -> their number
 __device__ __forceinline__ float number_of(const int* c) { return fmaf((float)(c[2] + (c[3] << 8)), 65536.0f, (float)(c[0] + (c[1] << 8))); }
-// 31-bit fixed point -> four signed bytes
+// 31-bit fixed point -> four signed bytes.  (A number that is not negative stands for its four unsigned bytes as it is.)
 __device__ __forceinline__ uint32_t digits_of(float x) { return ((uint32_t)__float2int_rn(x) + 0x808080u) ^ 0x808080u; }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
 
@@ -216,11 +215,9 @@ __device__ __forceinline__ void expand_half(const uint4& codes, const uint4& boo
     sts128(dst + q * chunk, o[0], o[1], o[2], o[3]);
   }
 }
-// A row's 32 bytes of codes at `src` -> its 64 levels.  Of eight neighbouring threads the upper four take the second half first: then the
-// eight read from different banks.  A loop, as are those around it: what a group does in a step is straight code otherwise, and an SM that runs five such
-// pieces waits for instructions
-__device__ __forceinline__ void expand_row(uint32_t src, const uint4& book, uint32_t dst, uint32_t chunk, int lane) {
-  uint32_t half = (lane >> 2) & 1;
+// A row's 32 bytes of codes at `src` -> its 64 levels.  Of eight neighbouring threads the upper four (half = 1) take the second half first: then the
+// eight read from different banks.  (Callers loop over rows without unrolling: an SM that runs five straight pieces of code waits for instructions.)
+__device__ __forceinline__ void expand_row(uint32_t src, const uint4& book, uint32_t dst, uint32_t chunk, uint32_t half) {
 #pragma unroll 1
   for (int k = 0; k < 2; ++k, half ^= 1) expand_half(lds128(src + 16 * half), book, dst + 2 * half * chunk, chunk);
 }
@@ -254,12 +251,11 @@ struct Exchange {
   alignas(16) float fin[4][4 * NR];         // end of a pair: sums of p, constant terms of the output
   alignas(16) float qs[4][NR];              // logit per unit of the scaled query, by pair
   alignas(16) float vmax[2][4][NR];         // largest logit, by step parity and warp
-  alignas(16) StepInfo info[4];             // by step
+  alignas(16) StepInfo info[8];             // by step (the line is up to five ahead of the softmax)
   float qmax[2][4][NR];                     // largest |q|, by pair and warp
-  alignas(16) uint32_t kt[4][4], vt[4][4];  // largest T (bits) of the step's keys, values, by step and warp
-  // copied [stage] and used [stage] of keys and values; largest T found [2], operand written, products done [2], sums read [2] of the keys; largest T
-  // found [2], operand written, products done of the values; end
-  unsigned long long bar[2 * (K_STAGES + V_STAGES) + 12];
+  float2 row[2][2][2][128];                 // scale and constant term of the rows, by side, step parity, row of a thread, thread
+  alignas(16) uint32_t top[2][4][4];        // largest T (bits) of the rows, by side, step and warp
+  unsigned long long bar[2 * 11 + 3];
   int warp_sum[THREADS / 32];
   uint32_t tmem;
   int failed;
@@ -292,16 +288,20 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
   const uint32_t sbase = smem_u32(smem), sbook = sbase + S::BOOK;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t bars = smem_u32(x.bar);
-  const uint32_t k_full = bars, k_used = k_full + 8 * K_STAGES, v_full = k_used + 8 * K_STAGES, v_used = v_full + 8 * V_STAGES;
-  const uint32_t k_scaled = v_used + 8 * V_STAGES, k_ready = k_scaled + 16, k_done = k_ready + 8, k_free = k_done + 16;
-  const uint32_t v_scaled = k_free + 16, v_ready = v_scaled + 16, v_done = v_ready + 8, b_end = v_done + 8;
+  // of a side (keys, values): copied [stage], used [stage], scaled [2], operand written, products done [2]; sums of the keys read [2]; end
+  constexpr uint32_t FULL = 0, USED = 24, SCALED = 48, READY = 64, DONE = 72, SIDE_BARS = 88;
+  const uint32_t k_scaled = bars + SCALED, k_ready = bars + READY, k_done = bars + DONE, v_scaled = k_scaled + SIDE_BARS, v_ready = k_ready + SIDE_BARS,
+                 v_done = k_done + SIDE_BARS, k_free = bars + 2 * SIDE_BARS, b_end = k_free + 16;
   if (tid == 0) {
     x.failed = 0;
-    for (int i = 0; i < K_STAGES; ++i) { bar_init(k_full + 8 * i, 1); bar_init(k_used + 8 * i, 8); }
-    for (int i = 0; i < V_STAGES; ++i) { bar_init(v_full + 8 * i, 1); bar_init(v_used + 8 * i, 8); }
-    for (int i = 0; i < 2; ++i) { bar_init(k_scaled + 8 * i, 4); bar_init(k_done + 8 * i, 2); bar_init(k_free + 8 * i, 4); bar_init(v_scaled + 8 * i, 4); }
-    bar_init(k_ready, 8); bar_init(v_ready, 8);
-    bar_init(v_done, 1); bar_init(b_end, 1);
+    for (int side = 0; side < 2; ++side) {
+      const uint32_t b = bars + side * SIDE_BARS;
+      for (int i = 0; i < 3; ++i) { bar_init(b + FULL + 8 * i, 1); bar_init(b + USED + 8 * i, 4); }
+      for (int i = 0; i < 2; ++i) { bar_init(b + SCALED + 8 * i, 4); bar_init(b + DONE + 8 * i, side ? 1 : 2); }
+      bar_init(b + READY, 8);
+    }
+    for (int i = 0; i < 2; ++i) bar_init(k_free + 8 * i, 4);
+    bar_init(b_end, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (tid < MZP_BOOKS * MZP_LEVELS / 16) ((uint4*)(smem + S::BOOK))[tid] = ((const uint4*)book_table)[tid];
@@ -356,40 +356,42 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
   const int team = warp >> 2;
   const int r = tid & 127;                       // key channel or token of this thread
 
-  // the largest T of a team's rows, found before anyone scales by it
-  auto publish_largest = [&](const uint32_t (&word)[RPT], uint32_t* slot, uint32_t bar) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < RPT; ++j) top = max(top, word[j] & 0xffffu);
-    top = warp_max_u32(top);
-    if (lane == 0) { slot[warp & 3] = top; bar_arrive(bar); }
-  };
-
-  if (team == 0) {
-    // ================= key levels: thread = channel
-    registers<Regs<NR>::KEY_LEVELS>();
-    const int ch = D == 128 ? r : r & 63;
-    for (int it = 0; it < n; ++it) {
-      const int stage = it % K_STAGES;
-      bar_wait(k_full + 8 * stage, it / K_STAGES & 1, &x.failed);
-      const int valid = x.info[it & 3].valid;
-      uint32_t word[RPT];
+  if (team == 0 || team == 2) {
+    // ================= levels, of keys (thread = channel) or values (thread = token): one piece of code, for an SM that runs many short of instructions
+    registers<Regs<NR>::LEVELS>();
+    const int side = team >> 1, blk = r >> 6, in_page = r & 63;
+    const uint32_t half = (lane >> 2) & 1, b = bars + side * SIDE_BARS;
+    // a thread's first row; keys of D = 128 have the channel's rows of both pages, values the token's two groups
+    const int key_page = D == 128 ? 0 : blk, row0 = side ? in_page * RPT : D == 128 ? r : in_page;
+    const uint32_t stages = side ? V_STAGES : K_STAGES, next_row = side ? 32 : S::SIDE, next_word = side ? 4 : S::SIDE;
+    uint32_t in = sbase + (side ? S::V_IN + blk * S::SIDE : S::K_IN + key_page * S::SIDE), phase = 0;
+    const uint32_t out = sbase + (side ? S::V_A + (D == 128 ? 0 : blk * 4 * S::CHUNK) : S::K_A + key_page * 4 * S::CHUNK) + (D == 128 ? r : in_page) * 16;
+    const int valid0 = side ? blk : key_page, valid1 = side ? blk : key_page + 1;
+    for (uint32_t it = 0, stage = 0; it < (uint32_t)n; ++it) {
+      bar_wait(b + FULL + 8 * stage, phase, &x.failed);
+      const int valid = x.info[it & 7].valid;
+      uint32_t zeros[RPT], top = 0;
 #pragma unroll
       for (int j = 0; j < RPT; ++j) {
-        const int pg = D == 128 ? j : r >> 6;
-        word[j] = valid >> pg & 1 ? lds32(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + 32 * D + 4 * ch) : 0u;
+        uint32_t word = lds32(in + 32 * D + 4 * row0 + j * next_word);
+        if (!(valid >> (j ? valid1 : valid0) & 1)) word = 0u;
+        top = max(top, word & 0xffffu);
+        const MzpRow row = mzp_row(word);
+        x.row[side][it & 1][j][r] = make_float2(row.t, fmaf(row.t, (float)row.z * -0.03125f, row.a));
+        zeros[j] = sbook + row.z * 16;
       }
-      publish_largest(word, x.kt[it & 3], k_scaled + 8 * (it & 1));
-      if (it > 0) bar_wait(k_done + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, &x.failed);      // the operand is free
+      // the step's largest T scales it; what the other lanes wrote goes with it
+      top = warp_max_u32(top);
+      __syncwarp();
+      if (lane == 0) { x.top[side][it & 3][warp & 3] = top; bar_arrive(b + SCALED + 8 * (it & 1)); }
+      if (it > 0) bar_wait(b + DONE + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, &x.failed);    // the operand is free
 #pragma unroll 1
-      for (int j = 0; j < RPT; ++j) {
-        const int pg = D == 128 ? j : r >> 6;
-        expand_row(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + ch * 32, book128(sbook + mzp_row(j ? word[RPT - 1] : word[0]).z * 16),
-                   sbase + S::K_A + pg * 4 * S::CHUNK + ch * 16, S::CHUNK, lane);
-      }
+      for (int j = 0; j < RPT; ++j) expand_row(in + row0 * 32 + j * next_row, book128(zeros[j ? RPT - 1 : 0]), out + j * 4 * S::CHUNK, S::CHUNK, half);
       fence_operands();
       __syncwarp();
-      if (lane == 0) { bar_arrive(k_ready); bar_arrive(k_used + 8 * stage); }
+      if (lane == 0) { bar_arrive(b + READY); bar_arrive(b + USED + 8 * stage); }
+      in += 2 * S::SIDE;
+      if (++stage == stages) { stage = 0; phase ^= 1; in -= stages * 2 * S::SIDE; }
     }
   } else if (team == 1) {
     // ================= key folds: thread = channel
@@ -397,12 +399,11 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
     const int ch = D == 128 ? r : r & 63, tw = warp & 3;
     float q[NR];
     int seg = -1;
+    const uint32_t out = sbase + S::K_B + (D == 128 ? 0 : r >> 6) * (NR / 4) * S::CHUNK + ch * 16;
     for (int it = 0; it < n; ++it) {
-      const int stage = it % K_STAGES;
-      bar_wait(k_full + 8 * stage, it / K_STAGES & 1, &x.failed);
-      const int valid = x.info[it & 3].valid;
-      if (x.info[it & 3].fresh) {
-        const StepInfo info = x.info[it & 3];
+      bar_wait(k_scaled + 8 * (it & 1), it >> 1 & 1, &x.failed);
+      if (x.info[it & 7].fresh) {
+        const StepInfo info = x.info[it & 7];
         ++seg;
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
@@ -430,67 +431,39 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
           if (r == 0) x.qs[seg & 3][i] = wild ? __int_as_float(0x7fffffff) : pow2(e1) * p.scaling * pow2(e2);
         }
       }
-      MzpRow row[RPT];
+      float2 row[RPT];
 #pragma unroll
-      for (int j = 0; j < RPT; ++j) {
-        const int pg = D == 128 ? j : r >> 6;
-        row[j] = mzp_row(valid >> pg & 1 ? lds32(sbase + S::K_IN + (2 * stage + pg) * S::SIDE + 32 * D + 4 * ch) : 0u);
-      }
+      for (int j = 0; j < RPT; ++j) row[j] = x.row[0][it & 1][j][r];
       {
         float base[RPT * NR];
 #pragma unroll
         for (int j = 0; j < RPT; ++j) {
-          const float cz = fmaf(row[j].t, (float)row[j].z * -0.03125f, row[j].a);
 #pragma unroll
           for (int i = 0; i < NR; i += 2) {
             base[j * NR + i] = base[j * NR + i + 1] = 0.f;
-            fma2(base[j * NR + i], base[j * NR + i + 1], q[i], q[i + 1], cz);
+            fma2(base[j * NR + i], base[j * NR + i + 1], q[i], q[i + 1], row[j].y);
           }
         }
         int index;
         const float sum = warp_sums<RPT * NR>(base, lane, index);
         if ((lane & (32 / (RPT * NR) - 1)) == 0) x.base[it & 3][tw][index] = sum;
       }
-      bar_wait(k_scaled + 8 * (it & 1), it >> 1 & 1, &x.failed);
-      const float up = pow2(30 - ((int)(max4(x.kt[it & 3]) >> 10) - 14));      // T < 2^(exponent field - 14)
+      const float up = pow2(30 - ((int)(max4(x.top[0][it & 3]) >> 10) - 14));      // T < 2^(exponent field - 14)
       if (it > 0) bar_wait(k_done + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, &x.failed);
 #pragma unroll
       for (int j = 0; j < RPT; ++j) {
-        const int pg = D == 128 ? j : r >> 6;
-        const float ts = row[j].t * up;
+        const float ts = row[j].x * up;
 #pragma unroll
         for (int i = 0; i < NR; i += 4) {
           float f[4] = {0.f, 0.f, 0.f, 0.f};
           fma2(f[0], f[1], q[i], q[i + 1], ts);
           fma2(f[2], f[3], q[i + 2], q[i + 3], ts);
-          sts128(sbase + S::K_B + (pg * (NR / 4) + i / 4) * S::CHUNK + ch * 16, digits_of(f[0]), digits_of(f[1]), digits_of(f[2]), digits_of(f[3]));
+          sts128(out + (j * (NR / 4) + i / 4) * S::CHUNK, digits_of(f[0]), digits_of(f[1]), digits_of(f[2]), digits_of(f[3]));
         }
       }
       fence_operands();
       __syncwarp();
-      if (lane == 0) { bar_arrive(k_ready); bar_arrive(k_used + 8 * stage); }
-    }
-  } else if (team == 2) {
-    // ================= value levels: thread = token
-    registers<Regs<NR>::VALUE_LEVELS>();
-    const int blk = r >> 6;
-    for (int it = 0; it < n; ++it) {
-      const int stage = it % V_STAGES;
-      bar_wait(v_full + 8 * stage, it / V_STAGES & 1, &x.failed);
-      const bool valid = x.info[it & 3].valid >> blk & 1;
-      const uint32_t in = sbase + S::V_IN + (2 * stage + blk) * S::SIDE;
-      uint32_t word[RPT];
-#pragma unroll
-      for (int j = 0; j < RPT; ++j) word[j] = valid ? lds32(in + 32 * D + 4 * ((r & 63) * RPT + j)) : 0u;
-      publish_largest(word, x.vt[it & 3], v_scaled + 8 * (it & 1));
-      if (it > 0) bar_wait(v_done, (it - 1) & 1, &x.failed);                   // the operand is free
-#pragma unroll 1
-      for (int j = 0; j < RPT; ++j)
-        expand_row(in + ((r & 63) * RPT + j) * 32, book128(sbook + mzp_row(j ? word[RPT - 1] : word[0]).z * 16),
-                   sbase + S::V_A + (D == 128 ? j : blk) * 4 * S::CHUNK + (D == 128 ? r : r & 63) * 16, S::CHUNK, lane);
-      fence_operands();
-      __syncwarp();
-      if (lane == 0) { bar_arrive(v_ready); bar_arrive(v_used + 8 * stage); }
+      if (lane == 0) bar_arrive(k_ready);
     }
   } else if (team == 3) {
     // ================= softmax: thread = token, and position of the output
@@ -510,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
     };
     // the products of step `done`
     auto take_output = [&](int done) {
-      bar_wait(v_done, done & 1, &x.failed);
+      bar_wait(v_done + 8 * (done & 1), done >> 1 & 1, &x.failed);
       tm_after();
 #pragma unroll
       for (int i = 0; i < NR; i += 4) {
@@ -562,9 +535,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
     };
     reset();
     for (int it = 0; it < n; ++it) {
-      const int stage = it % V_STAGES;
-      bar_wait(v_full + 8 * stage, it / V_STAGES & 1, &x.failed);
-      const StepInfo info = x.info[it & 3];
+      bar_wait(k_done + 8 * (it & 1), (it >> 1) & 1, &x.failed);
+      tm_after();
+      const StepInfo info = x.info[it & 7];
       if (info.fresh) {
         if (pair >= 0) {
           take_output(it - 1);
@@ -574,10 +547,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         pair = info.pair; ++seg;
       }
       // ---- logits
-      bar_wait(k_done + 8 * (it & 1), (it >> 1) & 1, &x.failed);
-      tm_after();
       if (info.fresh) load_floats(qs, x.qs[seg & 3]);
-      const float kunit = pow2((int)(max4(x.kt[it & 3]) >> 10) - 14 - 35);
+      const float kunit = pow2((int)(max4(x.top[0][it & 3]) >> 10) - 14 - 35);
       float s[NR], base[NR];
       if (D == 128) {
         float b[4][NR];
@@ -641,7 +612,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         s[i] = ex2(s[i] - (fix[i] == -INFINITY ? 0.f : fix[i]));
       }
       bar_wait(v_scaled + 8 * (it & 1), it >> 1 & 1, &x.failed);
-      const int ev = (int)(max4(x.vt[it & 3]) >> 10) - 14;
+      const int ev = (int)(max4(x.top[1][it & 3]) >> 10) - 14;
       const float up = pow2(30 - ev);
       // ---- the output so far; then the operand is free
       if (it > 0 && !info.fresh) take_output(it - 1);
@@ -660,10 +631,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
       for (int i = 0; i < NR; i += 2) add2(l[i], l[i + 1], s[i], s[i + 1]);
 #pragma unroll
       for (int j = 0; j < RPT; ++j) {
-        const int vr = (r & 63) * RPT + j;
-        const uint32_t in = sbase + S::V_IN + (2 * stage + blk) * S::SIDE;
-        const MzpRow row = mzp_row(info.valid >> blk & 1 ? lds32(in + 32 * D + 4 * vr) : 0u);
-        const float ts = row.t * up, cz = fmaf(row.t, (float)row.z * -0.03125f, row.a);
+        const float2 row = x.row[1][it & 1][j][r];
+        const float ts = row.x * up, cz = row.y;
         const int b2 = D == 128 ? j : blk, at = D == 128 ? r : r & 63;
 #pragma unroll
         for (int i = 0; i < NR; i += 2) fma2(base_v[j][i], base_v[j][i + 1], s[i], s[i + 1], cz);
@@ -672,13 +641,14 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
           float f[4] = {0.f, 0.f, 0.f, 0.f};
           fma2(f[0], f[1], s[i], s[i + 1], ts);
           fma2(f[2], f[3], s[i + 2], s[i + 3], ts);
-          sts128(sbase + S::V_B + (b2 * (NR / 4) + i / 4) * S::CHUNK + at * 16, digits_of(f[0]), digits_of(f[1]), digits_of(f[2]), digits_of(f[3]));
+          sts128(sbase + S::V_B + (b2 * (NR / 4) + i / 4) * S::CHUNK + at * 16, __float2int_rn(f[0]), __float2int_rn(f[1]), __float2int_rn(f[2]),
+                 __float2int_rn(f[3]));
         }
       }
       fence_operands();
       tm_before();
       __syncwarp();
-      if (lane == 0) { bar_arrive(v_ready); bar_arrive(v_used + 8 * stage); }
+      if (lane == 0) bar_arrive(v_ready);
     }
     if (n > 0) {
       take_output(n - 1);
@@ -713,7 +683,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         }
         const int page0 = __shfl_sync(0xffffffffu, ids, k0 - ids_at), page1 = __shfl_sync(0xffffffffu, ids, k0 + 1 - ids_at);
         const int ks = it % K_STAGES, vs = it % V_STAGES;
-        if (it >= K_STAGES) bar_wait(k_used + 8 * ks, (it / K_STAGES - 1) & 1, &x.failed);
+        if (it >= K_STAGES) bar_wait(bars + USED + 8 * ks, (it / K_STAGES - 1) & 1, &x.failed);
         const uint32_t bytes = S::SIDE * ((page0 >= 0) + (page1 >= 0));
         const uint8_t* store = (const uint8_t*)c.store + (long long)p.layer * c.store_stride_layer + head * PB;
         const uint8_t *src0 = store + (long long)page0 * c.store_stride_page, *src1 = store + (long long)page1 * c.store_stride_page;
@@ -728,16 +698,16 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
           info.b = b;
           info.head = head;
           info.valid = (page0 >= 0 ? 1 : 0) | (page1 >= 0 ? 2 : 0);
-          x.info[it & 3] = info;
-          bar_expect(k_full + 8 * ks, bytes);
-          if (page0 >= 0) bulk_copy(kin, src0, S::SIDE, k_full + 8 * ks);
-          if (page1 >= 0) bulk_copy(kin + S::SIDE, src1, S::SIDE, k_full + 8 * ks);
+          x.info[it & 7] = info;
+          bar_expect(bars + FULL + 8 * ks, bytes);
+          if (page0 >= 0) bulk_copy(kin, src0, S::SIDE, bars + FULL + 8 * ks);
+          if (page1 >= 0) bulk_copy(kin + S::SIDE, src1, S::SIDE, bars + FULL + 8 * ks);
         }
-        if (it >= V_STAGES) bar_wait(v_used + 8 * vs, (it / V_STAGES - 1) & 1, &x.failed);
+        if (it >= V_STAGES) bar_wait(bars + SIDE_BARS + USED + 8 * vs, (it / V_STAGES - 1) & 1, &x.failed);
         if (lane == 0) {
-          bar_expect(v_full + 8 * vs, bytes);
-          if (page0 >= 0) bulk_copy(vin, src0 + S::SIDE, S::SIDE, v_full + 8 * vs);
-          if (page1 >= 0) bulk_copy(vin + S::SIDE, src1 + S::SIDE, S::SIDE, v_full + 8 * vs);
+          bar_expect(bars + SIDE_BARS + FULL + 8 * vs, bytes);
+          if (page0 >= 0) bulk_copy(vin, src0 + S::SIDE, S::SIDE, bars + SIDE_BARS + FULL + 8 * vs);
+          if (page1 >= 0) bulk_copy(vin + S::SIDE, src1 + S::SIDE, S::SIDE, bars + SIDE_BARS + FULL + 8 * vs);
         }
         __syncwarp();
         fresh = false;
@@ -755,9 +725,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
       }
       // copies in flight end before the CTA does (the teams have waited for all of them unless a wait ran out)
       for (int it = max(0, n - K_STAGES); it < n; ++it)
-        for (int k = 0; k < SPIN_LIMIT && !bar_test(k_full + 8 * (it % K_STAGES), it / K_STAGES & 1); ++k) {}
+        for (int k = 0; k < SPIN_LIMIT && !bar_test(bars + FULL + 8 * (it % K_STAGES), it / K_STAGES & 1); ++k) {}
       for (int it = max(0, n - V_STAGES); it < n; ++it)
-        for (int k = 0; k < SPIN_LIMIT && !bar_test(v_full + 8 * (it % V_STAGES), it / V_STAGES & 1); ++k) {}
+        for (int k = 0; k < SPIN_LIMIT && !bar_test(bars + SIDE_BARS + FULL + 8 * (it % V_STAGES), it / V_STAGES & 1); ++k) {}
     } else if (warp == 17) {
       // ================= MMAs, in the order keys 0, keys 1, values 0, keys 2, values 1, ...  (The whole warp waits: a diverged one would poll.)
       const uint64_t ka = descriptor(sbase + S::K_A, S::CHUNK), kb = descriptor(sbase + S::K_B, S::CHUNK);
@@ -770,7 +740,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
           if (!*(volatile int*)&x.failed) {
             tm_after();
 #pragma unroll
-            for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_S + (it & 1) * S::N, ka + k * (512 >> 4), kb + k * (512 >> 4), k > 0);
+            for (int k = 0; k < D / 32; ++k) umma<S::N, true>(tmem + S::TM_S + (it & 1) * S::N, ka + k * (512 >> 4), kb + k * (512 >> 4), k > 0);
             umma_commit(k_done + 8 * (it & 1));
           }
         }
@@ -783,8 +753,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) attention_kernel(const A
         if (lane == 0 && !*(volatile int*)&x.failed) {
           tm_after();
 #pragma unroll
-          for (int k = 0; k < D / 32; ++k) umma<S::N>(tmem + S::TM_O, va + k * (512 >> 4), vb + k * (512 >> 4), k > 0);
-          umma_commit(v_done);
+          for (int k = 0; k < D / 32; ++k) umma<S::N, false>(tmem + S::TM_O, va + k * (512 >> 4), vb + k * (512 >> 4), k > 0);
+          umma_commit(v_done + 8 * (it & 1));
         }
         __syncwarp();
       }
