@@ -421,7 +421,7 @@ int mz_paged_append(const mz_paged_cache* cache, int layer, const void* key, lon
  */
 typedef struct {
   const void* query;
-  long long q_stride_b, q_stride_l, q_stride_h;      /* elements */
+  long long q_stride_b, q_stride_l, q_stride_h;      /* elements, multiples of 8; query is 16-byte aligned */
   int batch, q_len, q_heads;
   const int* rows;                                   /* NULL: row b is b */
   float scaling;

@@ -169,7 +169,8 @@ class MuZeroPagedCache:
         if q.dim() != 4 or q.shape[3] != self.head_dim or q.dtype != self.dtype or q.device != self.device:
             raise ValueError(f"`query` must be {self.dtype} [batch, (q_len,) q_heads, {self.head_dim}] on {self.device}, got {query.dtype} "
                              f"{tuple(query.shape)} on {query.device}")
-        if q.stride(3) != 1:
+        # rows of whole 16-byte pieces; anything else is laid out once
+        if q.stride(3) != 1 or (q.stride(0) | q.stride(1) | q.stride(2)) & 7 or q.data_ptr() & 15:
             q = q.contiguous()
         b, lq, hq, _ = q.shape
         if out is None:
