@@ -11,13 +11,14 @@
 //   pages at 64), N = 2 blocks x NR query rows x 4 bytes, of which a position reads its block's; K = the rows that are summed over
 //
 // Work.  A query row is one (token, head) that shares a kv head; NR of them (4, or 8 above 4) go through a step together, more take several
-// passes.  The steps of all (list entry, kv head, pass) pairs stand in one line that is cut evenly over CTAs on the device, from the lengths it
-// finds there; a CTA leaves a record (m, l, out) per pair that it met, slot = CTA + pair.  The 16-bit tokens of the rings go to CTAs of their own in
-// the same launch (mma.sync), by cost.  A second kernel merges a pair's records.
+// passes.  The steps of all (list entry, kv head, pass) pairs stand in one line that is cut evenly over the CTAs on the device, from the lengths it
+// finds there; a CTA leaves a record (m, l, out) per pair that it met, slot = CTA + pair.  A CTA is four warps, four CTAs to an SM (three for 8 query
+// rows), and every thread does all of a step: keys as channel r, values as token r, output as channel r.  What a step needs from memory was asked for
+// a step earlier; the products of the keys run while the values' levels are written, those of the values while the next step's keys are.  Every
+// wait for products is bounded; one that runs out makes the CTA's records NaN and ends its MMAs.
 //
-// A CTA is four warps, four CTAs to an SM (three for 8 query rows), and every thread does all of a step: keys as channel r, values as token r, output as
-// channel r.  What a step needs from memory was asked for a step earlier; the products of the keys run while the values' levels are written, those
-// of the values while the next step's keys are.  Every wait for products is bounded; one that runs out makes the CTA's records NaN and ends its MMAs.
+// A second kernel has a CTA per pair.  It takes the 16-bit tokens of the pair's ring (mma.sync) while the first kernel ends, waits for it, and merges its
+// records with that.
 #include "mz_paged.cuh"
 
 namespace mzp {
@@ -25,10 +26,6 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int THREADS = 128, MAX_BATCH = 1024;
 constexpr int SPIN_LIMIT = 1000000;              // looks of a wait before it gives up
 constexpr int STEP = 2 * MZP_PAGE;
-// CTA time of a step, of a ring and of a ring's token, in ns (measured with the SMs full)
-constexpr float STEP_COST = 3000.0f, RING_COST = 2500.0f, TOKEN_COST = 25.0f;
-
-
 struct Args {
   mz_paged_cache c;
   const uint16_t* query;
@@ -37,9 +34,8 @@ struct Args {
   void* out;
   int out_dtype, layer, batch, q_len, q_heads, group;      // group: query heads per kv head
   int qrows, passes;                             // query rows per kv head, and how many passes of NR they take
-  int parts;                                     // that a ring's tiles are cut in
   float scaling;                                 // times log2(e)
-  // workspace: header {CTAs with steps, pad, steps (64 bits)}, steps before each entry [batch + 1], records
+  // workspace: header {CTAs with steps, steps before each entry [batch + 1]}, records
   int* head;
   float2* ml;                                    // [slot][NR] maximum (base 2) and sum
   float* acc;                                    // [slot][NR][D]
@@ -199,7 +195,6 @@ struct Smem {
   static constexpr int B_BYTES = 2 * NR * 4 / 16 * CHUNK;  // 2 blocks x NR x 4 bytes
   static constexpr int K_A = 0, V_A = A_BYTES, K_B = 2 * A_BYTES, V_B = K_B + B_BYTES, BOOK = V_B + B_BYTES;
   static constexpr int TOTAL = BOOK + MZP_BOOKS * MZP_LEVELS;
-  static constexpr int ENTRIES = 0;                        // a ring CTA's rows and lengths of the list's entries, int2 [MAX_BATCH]
   static constexpr int N = 8 * NR, TM_S = 0, TM_O = N, TM_COLS = 2 * N;
   static constexpr int CTAS = NR == 4 ? 4 : 3;             // per SM
 };
@@ -208,17 +203,17 @@ struct Step { int page0, page1, pair, head, b, r0, count, see; };
 // exchange between the warps of a CTA
 template <int NR>
 struct Exchange {
-  alignas(16) Step step[64];                // two blocks of 32 of the CTA's steps; one warp fills a block while the other is worked on
+  alignas(16) Step step[32];                // two blocks of 16 of the CTA's steps; one warp fills a block while the other is worked on
   alignas(16) float base[4][2 * NR];        // constant terms of the logits, by warp
   alignas(16) float fin[4][4 * NR];         // end of a pair: sums of p, constant terms of the output
   alignas(16) float vmax[4][NR];            // largest logit, by warp
   alignas(16) uint32_t top[2][2][4];        // largest T (bits) of the rows, by step parity, side (keys, values) and warp
   float qmax[4][NR];                        // largest |q|, by warp
   unsigned long long bar[3];                // products of the keys, of the values done; end
-  int warp_sum[4][2];
+  int warp_sum[4];
+  int first, before;                        // list entry of the CTA's first step, steps of the entries before it
   uint32_t tmem;
   int failed;
-  int prefix[MAX_BATCH + 1];                // steps of the entries before
 };
 __device__ __forceinline__ uint32_t max4(const uint32_t* s) {
   const uint4 v = *(const uint4*)s;
@@ -233,13 +228,18 @@ __device__ __forceinline__ void load_floats(float (&v)[N], const float* s) {
   }
 }
 
+// row and length of a list entry; a row that is not there is empty
+__device__ __forceinline__ int length_of(const Args& p, int b, int& row) {
+  row = p.rows ? p.rows[b] : b;
+  return row < 0 || row >= p.c.rows ? 0 : max(0, min(p.c.lengths[row], 0x7fffffff - STEP));
+}
+
 template <int D, bool BF, int NR>
 __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel(const Args p, const uint8_t* __restrict__ book_table) {
   using S = Smem<D, NR>;
   constexpr int DT = BF ? MZ_BF16 : MZ_F16;
   constexpr int PB = 72 * D;                     // page bytes per kv head
   constexpr int RPT = D / 64;                    // rows of codes per thread, side and step
-  constexpr int STREAMS = D == 128 ? 2 : 4;      // records of a ring's part
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Exchange<NR> x;
   const mz_paged_cache& c = p.c;
@@ -255,267 +255,100 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   ((uint4*)(smem + S::BOOK))[tid] = ((const uint4*)book_table)[tid];
   static_assert(THREADS == MZP_BOOKS * MZP_LEVELS / 16, "one piece of the books per thread");
 
-  // ---- the line of steps, and how many CTAs take rings
-  auto length_of = [&](int b, int& row) {
-    row = p.rows ? p.rows[b] : b;
-    return row < 0 || row >= c.rows ? 0 : max(0, min(c.lengths[row], 0x7fffffff - STEP));
+  // ---- the line of steps
+  const int kp_all = c.kv_heads * p.passes, G = gridDim.x, cta = blockIdx.x;
+  auto steps_of = [&](int b, int& row, int& len) {
+    len = length_of(p, b, row);
+    return (mzp_packed(len, c.residual) + STEP - 1) / STEP;
   };
-  const int kp_all = c.kv_heads * p.passes;
-  int total_steps = 0;
-  long long ring_tokens = 0;
-  {
-    for (int b0 = 0; b0 <= p.batch; b0 += THREADS) {
-      const int b = b0 + tid;
-      int row;
-      const int len = b < p.batch ? length_of(b, row) : 0, packed = mzp_packed(len, c.residual);
-      if (b < p.batch) ((int2*)(smem + S::ENTRIES))[b] = make_int2(row, len);
-      const int st = (packed + STEP - 1) / STEP;
-      int scan = st, rt = len - packed;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, scan, o);
-        if (lane >= o) scan += y;
-        rt += __shfl_xor_sync(0xffffffffu, rt, o);
-      }
-      __syncthreads();
-      if (lane == 31) { x.warp_sum[warp][0] = scan; x.warp_sum[warp][1] = rt; }
-      __syncthreads();
-      int at = total_steps + scan - st;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        if (w < warp) at += x.warp_sum[w][0];
-        total_steps += x.warp_sum[w][0];
-        ring_tokens += x.warp_sum[w][1];
-      }
-      if (b <= p.batch) x.prefix[b] = at;
-    }
+  int total = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
+    int row, len;
+    const int st = b0 + tid < p.batch ? steps_of(b0 + tid, row, len) : 0;
+    total += st;
   }
-  const long long T = (long long)total_steps * kp_all;
-  const int G = gridDim.x;
-  // CTAs 0 .. W-1 share the steps, the others the rings.  Where the steps leave CTAs over, rings are cut in parts
-  int n_ring = 0;
-  if (ring_tokens > 0) {
-    const float cr = (float)kp_all * (RING_COST * (float)p.batch + TOKEN_COST * (float)ring_tokens), cs = STEP_COST * (float)T;
-    n_ring = max(1, min((int)((float)G * cr / (cr + cs) + 0.5f), T > 0 ? G - 1 : G));
-  }
-  const int W = (int)min((long long)(G - n_ring), T);      // no CTA is left without a step
-  n_ring = G - W;
-  const int parts = (long long)n_ring >= 2 * p.pairs ? p.parts : 1;
-  if (blockIdx.x == 0) {
-    if (tid == 0) { p.head[0] = W; p.head[1] = parts; *(long long*)(p.head + 2) = T; }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) x.warp_sum[warp] = total;
+  __syncthreads();
+  total = (x.warp_sum[0] + x.warp_sum[1]) + (x.warp_sum[2] + x.warp_sum[3]);
+  const long long T = (long long)total * kp_all;
+  const int W = (int)min((long long)G, T);       // CTAs that share the steps: none of them is left without one
+  const long long f0 = cta < W ? T * cta / W : 0;
+  const int n = cta < W ? (int)(T * (cta + 1) / W - f0) : 0;
+  if (cta == 0 && tid == 0) p.head[0] = W;
+  // the list entry of the first step (CTA 0 writes down all of them)
+  for (int b0 = 0, before = 0; b0 < p.batch; b0 += THREADS) {
+    int row, len;
+    const int b = b0 + tid, st = b < p.batch ? steps_of(b, row, len) : 0;
+    int scan = st;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, scan, o); if (lane >= o) scan += y; }
     __syncthreads();
-    for (int b = tid; b <= p.batch; b += THREADS) p.head[4 + b] = x.prefix[b];
-  }
-
-  if ((int)blockIdx.x >= W) {
-    // ================= rings: a warp takes 16 tokens at a time, and (D = 128) 64 of the channels of the output.  A = keys [token][channel], B =
-    // queries; A = values [channel][token], B = p in two parts of 16 bits
-    const int g = lane >> 2, t = lane & 3;
-    const int half = D == 128 ? warp & 1 : 0, stream = D == 128 ? warp >> 1 : warp;
-    const long long units = p.pairs * parts, first_slot = (long long)G + p.pairs;
+    if (lane == 31) x.warp_sum[warp] = scan;
     __syncthreads();
-    // A warp goes through its tiles of all its units; what a tile needs is asked for a tile ahead, in the next unit, too.  The state of the tile that is
-    // asked for:
-    long long unit = (int)blockIdx.x - W;
-    int tile = 0, end = 0, tokens = 0, len = 0, ring0 = 0, r0 = 0;
-    const uint16_t *ring_k = nullptr, *ring_v = nullptr, *query = nullptr;
-    auto open_unit = [&]() {                     // the unit's first tile for this warp; false: it has none
-      const long long pair = unit / parts;
-      const int part = (int)(unit - pair * parts), b = (int)(pair / kp_all), kp = (int)(pair - (long long)b * kp_all), head = kp / p.passes;
-      const int2 e = ((const int2*)(smem + S::ENTRIES))[b];
-      len = e.y;
-      const int packed = mzp_packed(len, c.residual);
-      tokens = len - packed;
-      const int tiles = (tokens + 15) / 16;
-      tile = tiles * part / parts + stream;
-      end = tiles * (part + 1) / parts;
-      r0 = kp % p.passes * NR;
-      ring_k = (const uint16_t*)c.tail + (long long)p.layer * c.tail_stride_layer + (long long)e.x * c.tail_stride_row + (long long)head * c.ring * D;
-      ring_v = ring_k + (long long)c.kv_heads * c.ring * D + half * 64;
-      ring0 = packed % c.ring;
-      query = p.query + (long long)b * p.qsb + (long long)(head * p.group) * p.qsh;
-    };
-    auto place = [&](int i) { const int at = ring0 + i; return (at >= c.ring ? at - c.ring : at) * D; };      // i < tokens <= ring
-    uint4 ka[D / 32], kb[D / 32], qf[D / 32];
-    auto load_tile = [&]() {
-      const uint16_t* a = ring_k + place(min(tile * 16 + g, tokens - 1)) + 8 * t;
-      const uint16_t* b = ring_k + place(min(tile * 16 + g + 8, tokens - 1)) + 8 * t;
+    int at = before + scan - st;
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) { ka[k] = *(const uint4*)(a + 32 * k); kb[k] = *(const uint4*)(b + 32 * k); }
-    };
-    auto load_query = [&]() {                    // rows that are not there are zero
-      const int qr = r0 + g;
-      const uint16_t* from = query + (long long)(qr / p.group) * p.qsl + (long long)(qr % p.group) * p.qsh + 8 * t;
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        qf[k] = make_uint4(0, 0, 0, 0);
-        if (g < NR && qr < p.qrows) qf[k] = *(const uint4*)(from + 32 * k);
-      }
-    };
-    if (unit < units) {
-      open_unit();
-      if (tile < end) { load_query(); load_tile(); }
-    }
-    for (; unit < units;) {
-      const long long this_unit = unit;
-      const int see0 = tokens - p.q_len;               // query token l sees the ring's tokens up to see0 + l
-      const int this_tokens = tokens, this_r0 = r0;
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
-      bool opened = false;                       // the next unit's first tile has been asked for
-      while (!opened) {
-        if (tile >= end) {                       // a unit without a tile for this warp
-          unit += n_ring;
-          if (unit < units) { open_unit(); if (tile < end) { load_query(); load_tile(); } }
-          break;
-        }
-        const int i0 = tile * 16;
-        uint4 v[4];
-        // what is not there is read as zero
-        const uint16_t* this_v = ring_v;
-        const int this_ring0 = ring0;
-        auto load_values = [&](int see) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int i = i0 + 2 * t + (k & 1) + 8 * (k >> 1), at = this_ring0 + i;
-            v[k] = make_uint4(0, 0, 0, 0);
-            if (i <= see) v[k] = *(const uint4*)(this_v + (at >= c.ring ? at - c.ring : at) * D + 8 * g);
-          }
-        };
-        load_values(this_tokens - 1);
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          mma16<BF>(s, ka[k].x, kb[k].x, ka[k].y, kb[k].y, qf[k].x, qf[k].y);
-          mma16<BF>(s, ka[k].z, kb[k].z, ka[k].w, kb[k].w, qf[k].z, qf[k].w);
-        }
-        if (tile + STREAMS < end) {
-          tile += STREAMS;
-          load_tile();
-        } else {
-          opened = true;
-          unit += n_ring;
-          if (unit < units) { open_unit(); if (tile < end) { load_query(); load_tile(); } }
-        }
-        // s[0], s[1]: token g, columns (query rows) 2t, 2t + 1; s[2], s[3]: token g + 8
-        float fix[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int last = min(see0 + (this_r0 + 2 * t + j) / p.group, this_tokens - 1);
-          s[j] = i0 + g <= last ? s[j] * p.scaling : -INFINITY;
-          s[2 + j] = i0 + g + 8 <= last ? s[2 + j] * p.scaling : -INFINITY;
-          float top = fmaxf(s[j], s[2 + j]);
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          const float m_new = fmaxf(m[j], top), ref = m_new == -INFINITY ? 0.f : m_new;
-          fix[j] = ex2(m[j] - ref);
-          m[j] = m_new;
-          s[j] = ex2(s[j] - ref);
-          s[2 + j] = ex2(s[2 + j] - ref);
-          l[j] = l[j] * fix[j] + s[j] + s[2 + j];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { o[i][0] *= fix[0]; o[i][1] *= fix[1]; o[i][2] *= fix[0]; o[i][3] *= fix[1]; }
-        // p in two parts, transposed: column g, tokens 2t, 2t + 1 ([0]) and 2t + 8, 2t + 9 ([1])
-        uint32_t hi[2], lo[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t hw, lw;
-          if (BF) {
-            const __nv_bfloat162 hb = __floats2bfloat162_rn(s[2 * h], s[2 * h + 1]);
-            const float2 hf = __bfloat1622float2(hb);
-            const __nv_bfloat162 lb = __floats2bfloat162_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
-            hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
-          } else {
-            const __half2 hb = __floats2half2_rn(s[2 * h], s[2 * h + 1]);
-            const float2 hf = __half22float2(hb);
-            const __half2 lb = __floats2half2_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
-            hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
-          }
-          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(hi[h]) : "r"(hw));
-          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(lo[h]) : "r"(lw));
-        }
-        // A token that only later queries see must not bring a NaN to a product with p = 0: where a tile has tokens that only some of the queries see, each
-        // of the queries' tokens takes its turn with what it sees
-        const int l_first = this_r0 / p.group, l_last = (min(this_r0 + NR, p.qrows) - 1) / p.group;
-        const bool apart = i0 + 15 > see0 + l_first && l_last > l_first;
-        for (int turn = 0; turn <= (apart ? l_last - l_first : 0); ++turn) {
-          const bool mine = !apart || (this_r0 + g) / p.group == l_first + turn;
-          if (apart) load_values(min(see0 + l_first + turn, this_tokens - 1));
-          const uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
-          const uint32_t w2[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // rows g / g + 8 = channels 8g + 2k / 8g + 2k + 1
-            const uint32_t a0 = prmt(w0[k], w1[k], 0x5410u), a1 = prmt(w0[k], w1[k], 0x7632u);
-            const uint32_t a2 = prmt(w2[k], w3[k], 0x5410u), a3 = prmt(w2[k], w3[k], 0x7632u);
-            mma16<BF>(o[k], a0, a1, a2, a3, mine ? lo[0] : 0u, mine ? lo[1] : 0u);
-            mma16<BF>(o[k], a0, a1, a2, a3, mine ? hi[0] : 0u, mine ? hi[1] : 0u);
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], off);
-        if (2 * t + j < NR) {
-          const long long slot = (first_slot + this_unit * STREAMS + stream) * NR + 2 * t + j;
-          float* dst = p.acc + slot * D + half * 64 + 8 * g;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) *(float2*)(dst + 2 * k) = make_float2(o[k][j], o[k][2 + j]);
-          if (g == 0 && half == 0) p.ml[slot] = make_float2(m[j], l[j]);
-        }
-      }
-    }
-    return;
+    for (int w = 0; w < 4; ++w) { const int t = x.warp_sum[w]; if (w < warp) at += t; before += t; }
+    if (n > 0 && (long long)at * kp_all <= f0 && f0 < (long long)(at + st) * kp_all) { x.first = b; x.before = at; }
+    if (cta == 0 && b < p.batch) p.head[2 + b] = at + st;
+    if (before * (long long)kp_all > f0 && cta != 0) break;          // the same for all threads
   }
+  if (cta == 0 && tid == 0) p.head[1] = 0;
+  if (n == 0) return;
 
-  // ================= steps
-  const int cta = blockIdx.x;
-  const long long f0 = T * cta / W;
-  const int n = (int)(T * (cta + 1) / W - f0);
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&x.tmem)), "n"(S::TM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     tm_before();
   }
-  __syncthreads();                               // (the line's prefix is complete, too)
+  __syncthreads();
   tm_after();
   const uint32_t tmem = x.tmem;
-  // what the CTA's steps first .. first + 31 are, one per lane
-  auto plan = [&](int first) {
-    const int it = first + lane;
+  // What the CTA's steps at .. at + 15 are, one per lane: the entries from the CTA's first one on are looked through, 32 at a time
+  auto plan = [&](int at) {
+    const int it = at + lane;
+    const long long f = f0 + it;
+    bool open = lane < 16 && it < n;
     Step s = {-1, -1, 0, 0, 0, 0, 0, 0};
-    if (it < n) {
-      const long long f = f0 + it;
-      int b = 0, hi = p.batch;                   // prefix[b] * kp_all <= f < prefix[b + 1] * kp_all
-      while (hi - b > 1) { const int mid = (b + hi) >> 1; if ((long long)x.prefix[mid] * kp_all <= f) b = mid; else hi = mid; }
-      const int steps = x.prefix[b + 1] - x.prefix[b], rem = (int)(f - (long long)x.prefix[b] * kp_all), kp = rem / steps, step = rem - kp * steps;
-      int row;
-      const int len = length_of(b, row), pages = mzp_packed(len, c.residual) / MZP_PAGE;
-      s.pair = b * kp_all + kp;
-      s.b = b;
-      s.head = kp / p.passes;
-      s.r0 = kp % p.passes * NR;
-      s.count = min(STEP, pages * MZP_PAGE - step * STEP);
-      s.see = len - p.q_len + s.r0 / p.group - step * STEP;
-      int id[2];
+    int before = x.before;
+    for (int b0 = x.first; b0 < p.batch && __any_sync(0xffffffffu, open); b0 += 32) {
+      int row = 0, len = 0;
+      const int st = b0 + lane < p.batch ? steps_of(b0 + lane, row, len) : 0;
+      int scan = st;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        id[k] = -1;
-        if (2 * step + k < pages) {
-          id[k] = 2 * step + k < c.width ? c.block_table[(long long)row * c.width + 2 * step + k] : -1;
-          if (id[k] < 0 || id[k] >= c.pages) { id[k] = -1; atomicOr(c.status, MZ_PAGED_BAD_INDEX); }
+      for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, scan, o); if (lane >= o) scan += y; }
+      const int start = before + scan - st;      // of entry b0 + lane
+      before += __shfl_sync(0xffffffffu, scan, 31);
+      int k = 0;                                 // the last entry that starts at or before f
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) if ((long long)__shfl_sync(0xffffffffu, start, k + o) * kp_all <= f) k += o;
+      const int steps = __shfl_sync(0xffffffffu, st, k), first = __shfl_sync(0xffffffffu, start, k), its_row = __shfl_sync(0xffffffffu, row, k);
+      const int its_len = __shfl_sync(0xffffffffu, len, k);
+      if (open && f < (long long)before * kp_all) {
+        open = false;
+        const int rem = (int)(f - (long long)first * kp_all), kp = rem / steps, step = rem - kp * steps, pages = mzp_packed(its_len, c.residual) / MZP_PAGE;
+        s.b = b0 + k;
+        s.pair = s.b * kp_all + kp;
+        s.head = kp / p.passes;
+        s.r0 = (kp - s.head * p.passes) * NR;
+        s.count = min(STEP, pages * MZP_PAGE - step * STEP);
+        s.see = its_len - p.q_len + s.r0 / p.group - step * STEP;
+        int id[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          id[w] = -1;
+          if (2 * step + w < pages) {
+            id[w] = 2 * step + w < c.width ? c.block_table[(long long)its_row * c.width + 2 * step + w] : -1;
+            if (id[w] < 0 || id[w] >= c.pages) { id[w] = -1; atomicOr(c.status, MZ_PAGED_BAD_INDEX); }
+          }
         }
+        s.page0 = id[0]; s.page1 = id[1];
       }
-      s.page0 = id[0]; s.page1 = id[1];
     }
-    x.step[it & 63] = s;
+    if (lane < 16) x.step[it & 31] = s;
   };
-  if (warp < 2) plan(32 * warp);
+  if (warp < 2) plan(16 * warp);
   __syncthreads();
 
   const int r = tid, blk = r >> 6, in_page = r & 63;         // key channel, token, output channel
@@ -630,7 +463,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   publish(0);
   __syncthreads();
   for (int it = 0; it < n; ++it) {
-    const Step s = x.step[it & 63];
+    const Step s = x.step[it & 31];
     const bool fresh = s.pair != pair;
     if (fresh) {
       if (pair >= 0) {
@@ -699,8 +532,8 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
       for (int k = 0; k < D / 32; ++k) umma<S::N, true>(tmem + S::TM_S, ka + k * (512 >> 4), kb + k * (512 >> 4), k > 0);
       umma_commit(k_done);
     }
-    if (warp == 3 && (it & 31) == 0 && it > 0) plan(it + 32);
-    const Step next = x.step[(it + 1) & 63];     // beyond the CTA's last step: pages that are not there, or a step that nobody takes
+    if (warp == 3 && (it & 15) == 0 && it > 0) plan(it + 16);
+    const Step next = x.step[(it + 1) & 31];     // beyond the CTA's last step: pages that are not there, or a step that nobody takes
     if (it + 1 < n) load_keys(next, true, true);
     // ---- values: the output so far, then levels while the products of the keys run
     if (it > 0 && !fresh) take_output(it - 1);
@@ -825,65 +658,188 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   }
 }
 
-// merges the records of one query row of a pair: a thread per channel, records in their order
+// One pair per CTA of eight warps.  Rings: a warp takes 16 tokens at a time, and (D = 128) 64 of the channels of the output; A = keys [token][channel],
+// B = queries; A = values [channel][token], B = p in two parts of 16 bits.  Then a thread has a channel, and every second query row.
+constexpr int END_THREADS = 256;
 template <int D, bool BF, int NR>
-__global__ void __launch_bounds__(D) merge_kernel(const Args p, int G) {
-  const int i = blockIdx.x % NR, d = threadIdx.x;
-  const long long pair = blockIdx.x / NR;
-  const int kp_all = p.c.kv_heads * p.passes, b = (int)(pair / kp_all), kp = (int)(pair % kp_all), head = kp / p.passes, qr = kp % p.passes * NR + i;
-  if (qr >= p.qrows) return;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int row = p.rows ? p.rows[b] : b;
-  const bool known = row >= 0 && row < p.c.rows;
-  if (!known && d == 0) atomicOr(p.c.status, MZ_PAGED_BAD_INDEX);
-  const int len = known ? max(0, min(p.c.lengths[row], 0x7fffffff - STEP)) : 0;
-  const bool ring = len > mzp_packed(len, p.c.residual);
-  constexpr int STREAMS = D == 128 ? 2 : 4;
-  const int parts = p.head[1];
-  const long long W = p.head[0], T = *(const long long*)(p.head + 2);
-  const long long steps = p.head[4 + b + 1] - p.head[4 + b], s0 = (long long)p.head[4 + b] * kp_all + kp * steps;
-  float m = -INFINITY, l = 0.f, a = 0.f;
-  auto take = [&](float2 ml, float v) {
-    const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top;
-    const float f = ex2(m - ref), g = ex2(ml.x - ref);
-    l = l * f + ml.y * g;
-    a = a * f + v * g;
-    m = top;
+__global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
+  constexpr int HALVES = D / 64, STREAMS = 8 / HALVES, GROUPS = END_THREADS / D, ROWS = NR / GROUPS;      // D = 64: four groups
+  __shared__ float s_part[STREAMS][NR][D], s_m[STREAMS][NR], s_l[STREAMS][NR];
+  const mz_paged_cache& c = p.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const long long pair = blockIdx.x;
+  const int kp_all = c.kv_heads * p.passes, b = (int)(pair / kp_all), kp = (int)(pair - (long long)b * kp_all), head = kp / p.passes;
+  const int r0 = (kp - head * p.passes) * NR;
+  int row;
+  const int len = length_of(p, b, row), packed = mzp_packed(len, c.residual), tokens = len - packed;
+  if ((row < 0 || row >= c.rows) && tid == 0) atomicOr(c.status, MZ_PAGED_BAD_INDEX);
+  const int half = warp % HALVES, stream = warp / HALVES;
+  if (tokens > 0) {
+    const int see0 = tokens - p.q_len;           // query token l sees the ring's tokens up to see0 + l
+    const uint16_t* ring_k = (const uint16_t*)c.tail + (long long)p.layer * c.tail_stride_layer + (long long)row * c.tail_stride_row + (long long)head * c.ring * D;
+    const uint16_t* ring_v = ring_k + (long long)c.kv_heads * c.ring * D + half * 64;
+    const int ring0 = packed % c.ring;
+    auto place = [&](int i) { const int at = ring0 + i; return (at >= c.ring ? at - c.ring : at) * D; };      // i < tokens <= ring
+    // query row r0 + g; rows that are not there are zero
+    const int qr = r0 + g;
+    const bool on = g < NR && qr < p.qrows;
+    const uint16_t* query = p.query + (long long)b * p.qsb + (long long)(qr / p.group) * p.qsl + (long long)(head * p.group + qr % p.group) * p.qsh + 8 * t;
+    uint4 qf[D / 32];
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      qf[k] = make_uint4(0, 0, 0, 0);
+      if (on) qf[k] = *(const uint4*)(query + 32 * k);
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+    for (int i0 = stream * 16; i0 < tokens; i0 += STREAMS * 16) {
+      uint4 v[4];
+      // what is not there is read as zero
+      auto load_values = [&](int see) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = i0 + 2 * t + (k & 1) + 8 * (k >> 1);
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (i <= see) v[k] = *(const uint4*)(ring_v + place(i) + 8 * g);
+        }
+      };
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      {
+        const uint16_t* ka = ring_k + place(min(i0 + g, tokens - 1)) + 8 * t;
+        const uint16_t* kb = ring_k + place(min(i0 + g + 8, tokens - 1)) + 8 * t;
+        uint4 va[D / 32], vb[D / 32];
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) { va[k] = *(const uint4*)(ka + 32 * k); vb[k] = *(const uint4*)(kb + 32 * k); }
+        load_values(tokens - 1);
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          mma16<BF>(s, va[k].x, vb[k].x, va[k].y, vb[k].y, qf[k].x, qf[k].y);
+          mma16<BF>(s, va[k].z, vb[k].z, va[k].w, vb[k].w, qf[k].z, qf[k].w);
+        }
+      }
+      // s[0], s[1]: token g, columns (query rows) 2t, 2t + 1; s[2], s[3]: token g + 8
+      float fix[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int last = min(see0 + (r0 + 2 * t + j) / p.group, tokens - 1);
+        s[j] = i0 + g <= last ? s[j] * p.scaling : -INFINITY;
+        s[2 + j] = i0 + g + 8 <= last ? s[2 + j] * p.scaling : -INFINITY;
+        float top = fmaxf(s[j], s[2 + j]);
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float m_new = fmaxf(m[j], top), ref = m_new == -INFINITY ? 0.f : m_new;
+        fix[j] = ex2(m[j] - ref);
+        m[j] = m_new;
+        s[j] = ex2(s[j] - ref);
+        s[2 + j] = ex2(s[2 + j] - ref);
+        l[j] = l[j] * fix[j] + s[j] + s[2 + j];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { o[i][0] *= fix[0]; o[i][1] *= fix[1]; o[i][2] *= fix[0]; o[i][3] *= fix[1]; }
+      // p in two parts, transposed: column g, tokens 2t, 2t + 1 ([0]) and 2t + 8, 2t + 9 ([1])
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t hw, lw;
+        if (BF) {
+          const __nv_bfloat162 hb = __floats2bfloat162_rn(s[2 * h], s[2 * h + 1]);
+          const float2 hf = __bfloat1622float2(hb);
+          const __nv_bfloat162 lb = __floats2bfloat162_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
+          hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
+        } else {
+          const __half2 hb = __floats2half2_rn(s[2 * h], s[2 * h + 1]);
+          const float2 hf = __half22float2(hb);
+          const __half2 lb = __floats2half2_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
+          hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
+        }
+        asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(hi[h]) : "r"(hw));
+        asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(lo[h]) : "r"(lw));
+      }
+      // A token that only later queries see must not bring a NaN to a product with p = 0: where a tile has tokens that only some of the queries see, each
+      // of the queries' tokens takes its turn with what it sees
+      const int l_first = r0 / p.group, l_last = (min(r0 + NR, p.qrows) - 1) / p.group;
+      const bool apart = i0 + 15 > see0 + l_first && l_last > l_first;
+      for (int turn = 0; turn <= (apart ? l_last - l_first : 0); ++turn) {
+        const bool mine = !apart || qr / p.group == l_first + turn;
+        if (apart) load_values(min(see0 + l_first + turn, tokens - 1));
+        const uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+        const uint32_t w2[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // rows g / g + 8 = channels 8g + 2k / 8g + 2k + 1
+          const uint32_t a0 = prmt(w0[k], w1[k], 0x5410u), a1 = prmt(w0[k], w1[k], 0x7632u);
+          const uint32_t a2 = prmt(w2[k], w3[k], 0x5410u), a3 = prmt(w2[k], w3[k], 0x7632u);
+          mma16<BF>(o[k], a0, a1, a2, a3, mine ? lo[0] : 0u, mine ? lo[1] : 0u);
+          mma16<BF>(o[k], a0, a1, a2, a3, mine ? hi[0] : 0u, mine ? hi[1] : 0u);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], off);
+      if (2 * t + j < NR) {
+        float* dst = &s_part[stream][2 * t + j][half * 64 + 8 * g];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *(float2*)(dst + 2 * k) = make_float2(o[k][j], o[k][2 + j]);
+        if (g == 0 && half == 0) { s_m[stream][2 * t + j] = m[j]; s_l[stream][2 * t + j] = l[j]; }
+      }
+    }
+  }
+  __syncthreads();
+  // ---- this thread: channel d of query rows i0, i0 + GROUPS, ...
+  const int d = tid % D, i0 = tid / D;
+  float m[ROWS], l[ROWS], a[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) { m[i] = -INFINITY; l[i] = 0.f; a[i] = 0.f; }
+  auto take = [&](int i, float2 ml, float v) {
+    const float top = fmaxf(m[i], ml.x), ref = top == -INFINITY ? 0.f : top;
+    const float f = ex2(m[i] - ref), h = ex2(ml.x - ref);
+    l[i] = l[i] * f + ml.y * h;
+    a[i] = a[i] * f + v * h;
+    m[i] = top;
   };
+  asm volatile("griddepcontrol.wait;" ::: "memory");         // the first kernel's records are written
+  const long long W = p.head[0], before = p.head[1 + b], steps = p.head[2 + b] - before;
   if (steps > 0) {
+    const long long T = (long long)p.head[1 + p.batch] * kp_all, s0 = before * kp_all + kp * steps;
     // CTA c has the steps from T c / W on: the one with step f is ((f + 1) W - 1) / T
     const long long first = ((s0 + 1) * W - 1) / T, last = ((s0 + steps) * W - 1) / T;
     for (long long c0 = first; c0 <= last; c0 += 4) {
-      float2 ml[4];
-      float v[4];
+      float2 ml[4][ROWS];
+      float v[4][ROWS];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const long long slot = (min(c0 + k, last) + pair) * NR + i;
-        ml[k] = p.ml[slot];
-        v[k] = p.acc[slot * D + d];
-      }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) if (c0 + k <= last) take(ml[k], v[k]);
-    }
-  }
-  if (ring) {
-    const long long first = G + p.pairs + pair * parts * STREAMS;
-    for (int k0 = 0; k0 < parts * STREAMS; k0 += 4) {
-      float2 ml[4];
-      float v[4];
+        for (int i = 0; i < ROWS; ++i) {
+          const long long slot = (min(c0 + k, last) + pair) * NR + i0 + i * GROUPS;
+          ml[k][i] = p.ml[slot];
+          v[k][i] = p.acc[slot * D + d];
+        }
+      }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const long long slot = (first + min(k0 + k, parts * STREAMS - 1)) * NR + i;
-        ml[k] = p.ml[slot];
-        v[k] = p.acc[slot * D + d];
-      }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) if (k0 + k < parts * STREAMS) take(ml[k], v[k]);
+        for (int i = 0; i < ROWS; ++i) if (c0 + k <= last) take(i, ml[k][i], v[k][i]);
+      }
     }
   }
-  const float out = l == 0.f ? 0.f : a / l;
-  const int ql = qr / p.group, h = head * p.group + qr % p.group;
-  mz_store_from_float(p.out, (((long long)b * p.q_len + ql) * p.q_heads + h) * D + d, out, p.out_dtype);
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int at = i0 + i * GROUPS, qr = r0 + at;
+    if (tokens > 0) {
+#pragma unroll
+      for (int k = 0; k < STREAMS; ++k) take(i, make_float2(s_m[k][at], s_l[k][at]), s_part[k][at][d]);
+    }
+    if (qr < p.qrows) {
+      const float out = l[i] == 0.f ? 0.f : a[i] / l[i];
+      const int ql = qr / p.group, h = head * p.group + qr % p.group;
+      mz_store_from_float(p.out, (((long long)b * p.q_len + ql) * p.q_heads + h) * D + d, out, p.out_dtype);
+    }
+  }
 }
 
 template <int D, bool BF, int NR>
@@ -894,8 +850,8 @@ int launch(const Args& p, const uint8_t* book, int G, cudaStream_t st) {
   MZ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
   kern<<<G, THREADS, S::TOTAL, st>>>(p, book);
   MZ_LAUNCH_CHECK("paged attention");
-  // The merge kernel's launch overlaps the first kernel's end.  (Not so the first kernel's with the merge before it: an SM does not change its split of
-  // L1 and shared memory while a CTA runs on it, and two of these CTAs then do not fit.)
+  // The second kernel starts while the first one ends.  (Not so the first one while the second of the call before ends: an SM does not change its split
+  // of L1 and shared memory while a CTA runs on it, and four of these CTAs then do not fit.)
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -903,14 +859,14 @@ int launch(const Args& p, const uint8_t* book, int G, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.stream = st;
-  cfg.gridDim = dim3((unsigned)(p.pairs * NR));
-  cfg.blockDim = dim3(D);
-  MZ_CUDA(cudaLaunchKernelEx(&cfg, merge_kernel<D, BF, NR>, p, G));
-  MZ_LAUNCH_CHECK("paged attention merge");
+  cfg.gridDim = dim3((unsigned)p.pairs);
+  cfg.blockDim = dim3(END_THREADS);
+  MZ_CUDA(cudaLaunchKernelEx(&cfg, finish_kernel<D, BF, NR>, p));
+  MZ_LAUNCH_CHECK("paged attention end");
   return MZ_OK;
 }
 
-struct Shape { int nr, passes, parts, G; long long pairs; size_t head_bytes, slots, bytes; };
+struct Shape { int nr, passes, G; long long pairs; size_t head_bytes, slots, bytes; };
 int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* s) {
   MZ_REQUIRE(batch >= 0 && batch <= MAX_BATCH, "batch %d (at most %d)", batch, MAX_BATCH);
   MZ_REQUIRE(q_len >= 1 && q_heads >= 1 && q_heads % c->kv_heads == 0, "q_len %d, q_heads %d of %d kv heads", q_len, q_heads, c->kv_heads);
@@ -922,14 +878,10 @@ int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* 
   s->nr = qrows <= 4 ? 4 : 8;
   s->passes = (int)((qrows + s->nr - 1) / s->nr);
   s->pairs = (long long)batch * c->kv_heads * s->passes;
-  MZ_REQUIRE(s->pairs * s->nr < (1ll << 31), "too many query rows for one call");
+  MZ_REQUIRE(s->pairs < (1ll << 31) - s->nr * 2048, "too many query rows for one call");
   s->G = sms * (s->nr == 4 ? 4 : 3);
-  // few pairs: their rings are cut until a warp has one tile of 16 tokens or the CTAs are taken
-  const int streams = c->head_dim == 128 ? 2 : 4, most = ((c->residual + MZP_PAGE - 1 + 15) / 16 + streams - 1) / streams;
-  const long long share = s->pairs > 0 ? s->G / s->pairs : 1;
-  s->parts = (int)(share < 1 ? 1 : share > most ? most : share);
-  s->head_bytes = ((4 + (size_t)batch + 1) * sizeof(int) + 127) / 128 * 128;
-  s->slots = (size_t)s->G + (size_t)s->pairs * (1 + s->parts * streams);
+  s->head_bytes = ((2 + (size_t)batch) * sizeof(int) + 127) / 128 * 128;
+  s->slots = (size_t)s->G + (size_t)s->pairs;
   s->bytes = s->head_bytes + s->slots * s->nr * (sizeof(float2) + (size_t)c->head_dim * sizeof(float));
   return MZ_OK;
 }
@@ -971,7 +923,6 @@ extern "C" int mz_paged_attention(const mz_paged_cache* cache, int layer, const 
   p.group = args->q_heads / cache->kv_heads;
   p.qrows = p.group * args->q_len;
   p.passes = s.passes;
-  p.parts = s.parts;
   p.scaling = args->scaling * mzp::LOG2E;
   p.head = (int*)args->workspace;
   p.acc = (float*)((uint8_t*)args->workspace + s.head_bytes);
