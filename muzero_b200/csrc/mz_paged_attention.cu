@@ -34,8 +34,9 @@ struct Args {
   void* out;
   int out_dtype, layer, batch, q_len, q_heads, group;      // group: query heads per kv head
   int qrows, passes;                             // query rows per kv head, and how many passes of NR they take
+  int sms, per_sm;                               // the grid, if the machine is full
   float scaling;                                 // times log2(e)
-  // workspace: header {CTAs with steps, steps before each entry [batch + 1]}, records
+  // workspace: header {CTAs, steps before each entry [batch + 1]}, records
   int* head;
   float2* ml;                                    // [slot][NR] maximum (base 2) and sum
   float* acc;                                    // [slot][NR][D]
@@ -228,6 +229,30 @@ __device__ __forceinline__ void load_floats(float (&v)[N], const float* s) {
   }
 }
 
+// How the line of T steps is cut over the CTAs.  The warps that have been on an SM for longest come first at its schedulers: with equal parts an SM's four CTAs
+// ended after 80, 88, 99 and 111 us (two rows of 131072 and 100003 tokens).  CTAs start in their order, one on each SM before the next ones, so where there
+// is enough to share out the k-th on an SM gets 16 + per_sm - 1 - 2 k sixteenths of an equal part.  Otherwise parts are equal, and no CTA is empty.
+struct Cut {
+  long long T, W;
+  int sms, per_sm;                               // per_sm 0: equal parts
+  __device__ __forceinline__ Cut(const Args& p, long long steps, int grid) : T(steps), sms(p.sms), per_sm(0) {
+    W = min((long long)grid, T);
+    if (grid == p.sms * p.per_sm && T >= 2 * W) per_sm = p.per_sm;
+  }
+  __device__ __forceinline__ long long start(int cta) const {          // the first step of a CTA
+    if (per_sm == 0) return T * cta / W;
+    const int k = cta / sms;
+    return T * ((long long)sms * (k * (16 + per_sm - k)) + (long long)(cta - k * sms) * (15 + per_sm - 2 * k)) / (16ll * per_sm * sms);
+  }
+  __device__ __forceinline__ int owner(long long step) const {         // the CTA that has a step
+    if (per_sm == 0) return (int)(((step + 1) * W - 1) / T);
+    const long long v = ((step + 1) * (16ll * per_sm * sms) - 1) / T;
+    int k = 0;
+    while (k + 1 < per_sm && v >= (long long)sms * ((k + 1) * (16 + per_sm - (k + 1)))) ++k;
+    return k * sms + (int)((v - (long long)sms * (k * (16 + per_sm - k))) / (15 + per_sm - 2 * k));
+  }
+};
+
 // row and length of a list entry; a row that is not there is empty
 __device__ __forceinline__ int length_of(const Args& p, int b, int& row) {
   row = p.rows ? p.rows[b] : b;
@@ -273,10 +298,10 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   __syncthreads();
   total = (x.warp_sum[0] + x.warp_sum[1]) + (x.warp_sum[2] + x.warp_sum[3]);
   const long long T = (long long)total * kp_all;
-  const int W = (int)min((long long)G, T);       // CTAs that share the steps: none of them is left without one
-  const long long f0 = cta < W ? T * cta / W : 0;
-  const int n = cta < W ? (int)(T * (cta + 1) / W - f0) : 0;
-  if (cta == 0 && tid == 0) p.head[0] = W;
+  const Cut cut(p, T, G);
+  const long long f0 = cta < cut.W ? cut.start(cta) : 0;
+  const int n = cta < cut.W ? (int)(cut.start(cta + 1) - f0) : 0;
+  if (cta == 0 && tid == 0) p.head[0] = G;
   // the list entry of the first step (CTA 0 writes down all of them)
   for (int b0 = 0, before = 0; b0 < p.batch; b0 += THREADS) {
     int row, len;
@@ -803,11 +828,10 @@ __global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
     m[i] = top;
   };
   asm volatile("griddepcontrol.wait;" ::: "memory");         // the first kernel's records are written
-  const long long W = p.head[0], before = p.head[1 + b], steps = p.head[2 + b] - before;
+  const long long before = p.head[1 + b], steps = p.head[2 + b] - before;
   if (steps > 0) {
-    const long long T = (long long)p.head[1 + p.batch] * kp_all, s0 = before * kp_all + kp * steps;
-    // CTA c has the steps from T c / W on: the one with step f is ((f + 1) W - 1) / T
-    const long long first = ((s0 + 1) * W - 1) / T, last = ((s0 + steps) * W - 1) / T;
+    const Cut cut(p, (long long)p.head[1 + p.batch] * kp_all, p.head[0]);
+    const long long s0 = before * kp_all + kp * steps, first = cut.owner(s0), last = cut.owner(s0 + steps - 1);
     for (long long c0 = first; c0 <= last; c0 += 4) {
       float2 ml[4][ROWS];
       float v[4][ROWS];
@@ -866,7 +890,7 @@ int launch(const Args& p, const uint8_t* book, int G, cudaStream_t st) {
   return MZ_OK;
 }
 
-struct Shape { int nr, passes, G; long long pairs; size_t head_bytes, slots, bytes; };
+struct Shape { int nr, passes, sms, per_sm, G; long long pairs; size_t head_bytes, slots, bytes; };
 int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* s) {
   MZ_REQUIRE(batch >= 0 && batch <= MAX_BATCH, "batch %d (at most %d)", batch, MAX_BATCH);
   MZ_REQUIRE(q_len >= 1 && q_heads >= 1 && q_heads % c->kv_heads == 0, "q_len %d, q_heads %d of %d kv heads", q_len, q_heads, c->kv_heads);
@@ -879,7 +903,12 @@ int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* 
   s->passes = (int)((qrows + s->nr - 1) / s->nr);
   s->pairs = (long long)batch * c->kv_heads * s->passes;
   MZ_REQUIRE(s->pairs < (1ll << 31) - s->nr * 2048, "too many query rows for one call");
-  s->G = sms * (s->nr == 4 ? 4 : 3);
+  s->sms = sms;
+  s->per_sm = s->nr == 4 ? 4 : 3;
+  s->G = sms * s->per_sm;
+  // a CTA costs its start (592 of them 6 us): no more than there can be steps
+  const long long most = s->pairs * ((c->width + 1) / 2);
+  if (s->G > most) s->G = most < 1 ? 1 : (int)most;
   s->head_bytes = ((2 + (size_t)batch) * sizeof(int) + 127) / 128 * 128;
   s->slots = (size_t)s->G + (size_t)s->pairs;
   s->bytes = s->head_bytes + s->slots * s->nr * (sizeof(float2) + (size_t)c->head_dim * sizeof(float));
@@ -923,6 +952,7 @@ extern "C" int mz_paged_attention(const mz_paged_cache* cache, int layer, const 
   p.group = args->q_heads / cache->kv_heads;
   p.qrows = p.group * args->q_len;
   p.passes = s.passes;
+  p.sms = s.sms; p.per_sm = s.per_sm;
   p.scaling = args->scaling * mzp::LOG2E;
   p.head = (int*)args->workspace;
   p.acc = (float*)((uint8_t*)args->workspace + s.head_bytes);
