@@ -2,6 +2,9 @@
 // by rows (a thread owns half of a token's 64 channels), smallest and largest value first, then the codes through the table of nearest levels in shared
 // memory.  Tokens that stay are copied to the ring by the same grid, or by a second launch where a new token could take the place of an old
 // one that is still to be quantized.
+//
+// What bounds it is the instructions of a value: two to find the range (pairs of 16 bits), eight to its code, of which one is the table's load.  What is
+// rare is kept out of them: a row with a NaN, an infinity, a value beyond f16 or a scale below f16's normal numbers is done again by the general form.
 #include "mz_paged.cuh"
 
 namespace {
@@ -23,17 +26,64 @@ __device__ __forceinline__ float2 widen(uint32_t w) {
   return __half22float2(*reinterpret_cast<__half2*>(&w));
 }
 
+// Table of nearest levels in shared memory: row z from NEAR_ROW * z on, entries -1 .. 128 of it (a value may round to a level beyond the ends)
+constexpr int NEAR_ROW = 132;
+constexpr float MAGIC = 12582912.0f;            // 1.5 * 2^23: adding it rounds to an integer, which stands in the low bits
+
+// smallest and largest of 16-bit pairs, as pairs; `odd` becomes NaN where a value is not finite
+template <bool BF>
+struct Range {
+  uint32_t lo, hi, odd;
+  __device__ __forceinline__ void start(uint32_t w) {
+    lo = hi = w;
+    odd = 0;
+    note(w);
+  }
+  __device__ __forceinline__ void note(uint32_t w) {
+    if (BF) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(odd) : "r"(w), "r"(0u));
+    else asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(odd) : "r"(w), "r"(0u));
+  }
+  __device__ __forceinline__ void add(uint32_t w) {
+    if (BF) {
+      asm("min.bf16x2 %0, %0, %1;" : "+r"(lo) : "r"(w));
+      asm("max.bf16x2 %0, %0, %1;" : "+r"(hi) : "r"(w));
+    } else {
+      asm("min.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(w));
+      asm("max.f16x2 %0, %0, %1;" : "+r"(hi) : "r"(w));
+    }
+    note(w);
+  }
+};
+// what a thread needs for the codes of a row
+struct Coder { float a, inv, z; int near; };    // near: address of the row's entry 0 in the table, less the bits of MAGIC
+__device__ __forceinline__ uint32_t code_of(const Coder& q, float x) {
+  const float y = __fadd_rn(__fmul_rn(__fsub_rn(x, q.a), q.inv), q.z);
+  uint32_t v;
+  asm("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(q.near + __float_as_int(__fadd_rn(y, MAGIC))));
+  return v;
+}
+// the general form: any value, any scale
+__device__ __forceinline__ uint32_t code_of_any(const Coder& q, float x) {
+  const float y = __fadd_rn(__fmul_rn(__fsub_rn(mzp_finite(x), q.a), q.inv), q.z);
+  uint32_t v;
+  asm("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(q.near + __float_as_int(__fadd_rn(fminf(fmaxf(y, 0.0f), 127.0f), MAGIC))));
+  return v;
+}
+// whether a row is one for the general form: something in it was not finite, or its scale is below f16's normal numbers (then it is coarse)
+__device__ __forceinline__ bool needs_care(bool odd, uint32_t word) { return odd || (word & 0x7C00u) == 0u; }
+
 template <int D, bool BF>
-__global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs a, const uint8_t* __restrict__ nearest) {
+__global__ void __launch_bounds__(THREADS, 4) append_kernel(const AppendArgs a, const uint8_t* __restrict__ nearest) {
   constexpr int QUARTERS = THREADS / (D / 2);   // parts of the 64 tokens that a pair of channels is shared out in: 4 (D = 128) or 8
   constexpr int KT = MZP_PAGE / QUARTERS;       // key tokens per thread
   constexpr int VPARTS = THREADS / (MZP_PAGE * D / 64), VN = 64 / VPARTS;     // threads per row of 64 values, and values per thread: 2 x 32 or 4 x 16
-  __shared__ __align__(16) uint8_t s_near[MZP_BOOKS * 128];
+  __shared__ __align__(16) uint8_t s_near[MZP_BOOKS * NEAR_ROW];
   __shared__ float2 s_range[QUARTERS][D];
-  __shared__ float4 s_row[D];                   // quantizer constants of the keys' rows
+  __shared__ float4 s_row[D];                   // quantizer constants of the keys' rows; the last is not 0 for the general form
   __shared__ __align__(16) uint8_t s_out[D * 32];
   const mz_paged_cache& c = a.c;
   if (*c.status & (MZ_PAGED_NO_PAGES | MZ_PAGED_TOO_LONG)) return;      // the extension failed: there is no room for these tokens
+  const int near0 = (int)__cvta_generic_to_shared(s_near) + 1 - __float_as_int(MAGIC);
   bool have_table = false;
   const long long units = (long long)a.batch * a.slots * c.kv_heads;
   for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
@@ -49,47 +99,74 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs a, con
     const int packed = mzp_packed(after, c.residual);
     uint16_t* ring_k = (uint16_t*)c.tail + (long long)a.layer * c.tail_stride_layer + (long long)row * c.tail_stride_row + (long long)head * c.ring * D;
     uint16_t* ring_v = ring_k + (long long)c.kv_heads * c.ring * D;
-    const uint16_t *new_k = a.key + (long long)head * a.ksh, *new_v = a.value + (long long)head * a.vsh;
+    const uint16_t *new_k = a.key + (long long)first * a.kst + (long long)head * a.ksh, *new_v = a.value + (long long)first * a.vst + (long long)head * a.vsh;
     if (a.keep) {
       // 64 of the tokens that stay
       const int start = max(packed, before) + slot * MZP_PAGE, count = min(MZP_PAGE, after - start);
       constexpr int PIECES = D / 8;
       for (int x = threadIdx.x; x < count * PIECES; x += THREADS) {
         const int pos = start + x / PIECES, piece = x % PIECES * 8;
-        const long long from = first + (pos - before);
         const int to = pos % c.ring * D + piece;
-        *(uint4*)(ring_k + to) = *(const uint4*)(new_k + from * a.kst + piece);
-        *(uint4*)(ring_v + to) = *(const uint4*)(new_v + from * a.vst + piece);
+        *(uint4*)(ring_k + to) = *(const uint4*)(new_k + (pos - before) * a.kst + piece);
+        *(uint4*)(ring_v + to) = *(const uint4*)(new_v + (pos - before) * a.vst + piece);
       }
     }
     const int page = mzp_packed(before, c.residual) / MZP_PAGE + slot;
     if (!a.quantize || page >= packed / MZP_PAGE || page >= c.width) continue;
     const int id = c.block_table[(long long)row * c.width + page];
     if (id < 0 || id >= c.pages) { if (threadIdx.x == 0) atomicOr(c.status, MZ_PAGED_BAD_INDEX); continue; }
+    // ---- all loads first
+    const int tok0 = page * MZP_PAGE, ring0 = tok0 % c.ring;
+    const int pair = threadIdx.x % (D / 2), quarter = threadIdx.x / (D / 2);
+    uint32_t x[KT];
+    if (tok0 >= before) {                       // the page is all new tokens
+      const uint16_t* from = new_k + (tok0 - before + quarter * KT) * a.kst + 2 * pair;
+#pragma unroll
+      for (int t = 0; t < KT; ++t) x[t] = *(const uint32_t*)(from + t * a.kst);
+    } else {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const int tok = quarter * KT + t, pos = tok0 + tok, place = ring0 + tok - (ring0 + tok >= c.ring ? c.ring : 0);
+        x[t] = *(const uint32_t*)((pos < before ? ring_k + place * D : new_k + (pos - before) * a.kst) + 2 * pair);
+      }
+    }
+    const int vrow = threadIdx.x / VPARTS, part = threadIdx.x % VPARTS;
+    uint4 v[VN / 8];
+    {
+      const int tok = vrow / (D / 64), pos = tok0 + tok, place = ring0 + tok - (ring0 + tok >= c.ring ? c.ring : 0);
+      const uint16_t* src = (pos < before ? ring_v + place * D : new_v + (pos - before) * a.vst) + vrow % (D / 64) * 64 + part * VN;
+#pragma unroll
+      for (int k = 0; k < VN / 8; ++k) v[k] = *(const uint4*)(src + 8 * k);
+    }
     if (!have_table) {
-      for (int x = threadIdx.x; x < MZP_BOOKS * 128 / 16; x += THREADS) ((uint4*)s_near)[x] = ((const uint4*)nearest)[x];
+      for (int k = threadIdx.x; k < MZP_BOOKS * 130; k += THREADS) {
+        const int z = k / 130, r = k % 130 - 1;
+        s_near[z * NEAR_ROW + r + 1] = nearest[z * 128 + min(max(r, 0), 127)];
+      }
       have_table = true;                        // (the barriers below come before its first use)
     }
     uint8_t* out = (uint8_t*)c.store + (long long)a.layer * c.store_stride_layer + (long long)id * c.store_stride_page + (long long)head * mzp_page_bytes(D);
-    const int tok0 = page * MZP_PAGE;
-    auto key_of = [&](int t) { const int pos = tok0 + t; return pos < before ? ring_k + pos % c.ring * D : new_k + (long long)(first + pos - before) * a.kst; };
-    auto value_of = [&](int t) { const int pos = tok0 + t; return pos < before ? ring_v + pos % c.ring * D : new_v + (long long)(first + pos - before) * a.vst; };
     // ---- keys
-    const int pair = threadIdx.x % (D / 2), quarter = threadIdx.x / (D / 2);
-    uint32_t x[KT];
-#pragma unroll
-    for (int t = 0; t < KT; ++t) x[t] = *(const uint32_t*)(key_of(quarter * KT + t) + 2 * pair);
+    bool odd_pair;
     {
-      float lo0 = INFINITY, hi0 = -INFINITY, lo1 = INFINITY, hi1 = -INFINITY;
+      Range<BF> rg;
+      rg.start(x[0]);
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        float2 f = widen<BF>(x[t]);
-        f.x = mzp_finite(f.x); f.y = mzp_finite(f.y);
-        lo0 = fminf(lo0, f.x); hi0 = fmaxf(hi0, f.x);
-        lo1 = fminf(lo1, f.y); hi1 = fmaxf(hi1, f.y);
+      for (int t = 1; t < KT; ++t) rg.add(x[t]);
+      float2 lo = widen<BF>(rg.lo), hi = widen<BF>(rg.hi);
+      const float2 odd = widen<BF>(rg.odd);
+      odd_pair = odd.x != 0.f || odd.y != 0.f || fmaxf(fmaxf(hi.x, hi.y), -fminf(lo.x, lo.y)) > 65504.0f;      // (NaN is not 0 either)
+      if (odd_pair) {
+        lo = make_float2(INFINITY, INFINITY); hi = make_float2(-INFINITY, -INFINITY);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          float2 f = widen<BF>(x[t]);
+          f.x = mzp_finite(f.x); f.y = mzp_finite(f.y);
+          lo.x = fminf(lo.x, f.x); hi.x = fmaxf(hi.x, f.x);
+          lo.y = fminf(lo.y, f.y); hi.y = fmaxf(hi.y, f.y);
+        }
       }
-      s_range[quarter][2 * pair] = make_float2(lo0, hi0);
-      s_range[quarter][2 * pair + 1] = make_float2(lo1, hi1);
+      *(float4*)&s_range[quarter][2 * pair] = make_float4(lo.x, hi.x, lo.y, hi.y);
     }
     __syncthreads();
     if (threadIdx.x < D) {
@@ -97,72 +174,109 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs a, con
 #pragma unroll
       for (int k = 1; k < QUARTERS; ++k) { const float2 s = s_range[k][threadIdx.x]; r.x = fminf(r.x, s.x); r.y = fmaxf(r.y, s.y); }
       const MzpQuant q = mzp_quant(r.x, r.y);
-      s_row[threadIdx.x] = make_float4(q.a, q.inv, q.z, 0.f);
+      s_row[threadIdx.x] = make_float4(q.a, q.inv, q.z, needs_care(false, q.word) ? 1.f : 0.f);
       ((uint32_t*)(out + 32 * D))[threadIdx.x] = q.word;
+    }
+    // ---- values' ranges meanwhile
+    Range<BF> rg;
+    rg.start(v[0].x);
+#pragma unroll
+    for (int k = 0; k < VN / 8; ++k) {
+      if (k > 0) rg.add(v[k].x);
+      rg.add(v[k].y); rg.add(v[k].z); rg.add(v[k].w);
+    }
+    float vlo, vhi;
+    bool odd_row;
+    {
+      const float2 lo = widen<BF>(rg.lo), hi = widen<BF>(rg.hi), odd = widen<BF>(rg.odd);
+      vlo = fminf(lo.x, lo.y);
+      vhi = fmaxf(hi.x, hi.y);
+      odd_row = odd.x != 0.f || odd.y != 0.f || fmaxf(vhi, -vlo) > 65504.0f;
+      if (odd_row) {
+        vlo = INFINITY; vhi = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < VN / 8; ++k) {
+          const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = widen<BF>(w[j]);
+            const float f0 = mzp_finite(f.x), f1 = mzp_finite(f.y);
+            vlo = fminf(vlo, fminf(f0, f1));
+            vhi = fmaxf(vhi, fmaxf(f0, f1));
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < VPARTS; o <<= 1) {
+        vlo = fminf(vlo, __shfl_xor_sync(0xffffffffu, vlo, o));
+        vhi = fmaxf(vhi, __shfl_xor_sync(0xffffffffu, vhi, o));
+      }
     }
     __syncthreads();
     {
       const float4 r0 = s_row[2 * pair], r1 = s_row[2 * pair + 1];
-      const MzpQuant q0 = {r0.x, r0.y, r0.z, 0}, q1 = {r1.x, r1.y, r1.z, 0};
-      const uint8_t *n0 = s_near + (int)r0.z * 128, *n1 = s_near + (int)r1.z * 128;
+      const Coder q0 = {r0.x, r0.y, r0.z, near0 + (int)r0.z * NEAR_ROW}, q1 = {r1.x, r1.y, r1.z, near0 + (int)r1.z * NEAR_ROW};
+      const bool care = odd_pair || r0.w != 0.f || r1.w != 0.f;
+      uint32_t c0[KT / 8], c1[KT / 8];
+#pragma unroll
+      for (int w = 0; w < KT / 8; ++w) c0[w] = c1[w] = 0;
+      if (!care) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          const float2 f = widen<BF>(x[t]);
+          c0[t / 8] += code_of(q0, f.x) * (1u << 4 * (t % 8));
+          c1[t / 8] += code_of(q1, f.y) * (1u << 4 * (t % 8));
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          const float2 f = widen<BF>(x[t]);
+          c0[t / 8] += code_of_any(q0, f.x) << 4 * (t % 8);
+          c1[t / 8] += code_of_any(q1, f.y) << 4 * (t % 8);
+        }
+      }
 #pragma unroll
       for (int w = 0; w < KT / 8; ++w) {
-        uint32_t c0 = 0, c1 = 0;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          const float2 f = widen<BF>(x[8 * w + t]);
-          c0 |= (uint32_t)n0[mzp_level(q0, mzp_finite(f.x))] << (4 * t);
-          c1 |= (uint32_t)n1[mzp_level(q1, mzp_finite(f.y))] << (4 * t);
-        }
-        *(uint32_t*)(s_out + (2 * pair) * 32 + quarter * (KT / 2) + 4 * w) = c0;
-        *(uint32_t*)(s_out + (2 * pair + 1) * 32 + quarter * (KT / 2) + 4 * w) = c1;
+        *(uint32_t*)(s_out + (2 * pair) * 32 + quarter * (KT / 2) + 4 * w) = c0[w];
+        *(uint32_t*)(s_out + (2 * pair + 1) * 32 + quarter * (KT / 2) + 4 * w) = c1[w];
       }
     }
     // ---- values
-    const int vrow = threadIdx.x / VPARTS, part = threadIdx.x % VPARTS;
-    uint4 v[VN / 8];
     {
-      const uint16_t* src = value_of(vrow / (D / 64)) + vrow % (D / 64) * 64 + part * VN;
+      const MzpQuant qq = mzp_quant(vlo, vhi);
+      const Coder q = {qq.a, qq.inv, qq.z, near0 + (int)qq.z * NEAR_ROW};
+      uint32_t code[VN / 8];
+      if (!needs_care(odd_row, qq.word)) {
 #pragma unroll
-      for (int k = 0; k < VN / 8; ++k) v[k] = *(const uint4*)(src + 8 * k);
+        for (int k = 0; k < VN / 8; ++k) {
+          const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          code[k] = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = widen<BF>(w[j]);
+            code[k] += code_of(q, f.x) * (1u << 8 * j) + code_of(q, f.y) * (1u << (8 * j + 4));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < VN / 8; ++k) {
+          const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          code[k] = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = widen<BF>(w[j]);
+            code[k] += (code_of_any(q, f.x) << 8 * j) + (code_of_any(q, f.y) << (8 * j + 4));
+          }
+        }
+      }
+      uint32_t* vout = (uint32_t*)(out + 36 * D + vrow * 32 + part * (VN / 2));
+      if constexpr (VN == 32) *(uint4*)vout = make_uint4(code[0], code[1], code[2], code[3]);
+      else *(uint2*)vout = make_uint2(code[0], code[1]);
+      if (part == 0) ((uint32_t*)(out + 68 * D))[vrow] = qq.word;
     }
     __syncthreads();
     for (int k = threadIdx.x; k < D * 2; k += THREADS) ((uint4*)out)[k] = ((const uint4*)s_out)[k];
-    float lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < VN / 8; ++k) {
-      const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = widen<BF>(w[j]);
-        const float f0 = mzp_finite(f.x), f1 = mzp_finite(f.y);
-        lo = fminf(lo, fminf(f0, f1));
-        hi = fmaxf(hi, fmaxf(f0, f1));
-      }
-    }
-#pragma unroll
-    for (int o = 1; o < VPARTS; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const MzpQuant q = mzp_quant(lo, hi);
-    const uint8_t* near_row = s_near + (int)q.z * 128;
-    uint32_t code[VN / 8];
-#pragma unroll
-    for (int k = 0; k < VN / 8; ++k) {
-      const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-      code[k] = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = widen<BF>(w[j]);
-        code[k] |= (uint32_t)near_row[mzp_level(q, mzp_finite(f.x))] << (8 * j) | (uint32_t)near_row[mzp_level(q, mzp_finite(f.y))] << (8 * j + 4);
-      }
-    }
-    uint32_t* vout = (uint32_t*)(out + 36 * D + vrow * 32 + part * (VN / 2));
-#pragma unroll
-    for (int k = 0; k < VN / 8; ++k) vout[k] = code[k];
-    if (part == 0) ((uint32_t*)(out + 68 * D))[vrow] = q.word;
-    __syncthreads();                            // s_out, s_range and s_row are written again
+    // (s_out is written again after the next unit's two barriers, s_range and s_row have been read)
   }
 }
 
