@@ -44,7 +44,7 @@ def packed_tokens(length: int, residual_length: int) -> int:
 def _index(t: Optional[torch.Tensor], what: str, device: torch.device, n: Optional[int] = None) -> int:
     if t is None:
         return 0
-    if t.dtype != torch.int32 or t.dim() != 1 or t.device != device or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.dim() != 1 or t.device != device or t.stride(0) != 1:
         raise ValueError(f"`{what}` must be a contiguous int32 vector on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     if n is not None and t.shape[0] != n:
         raise ValueError(f"`{what}` has {t.shape[0]} entries, expected {n}")
@@ -105,8 +105,11 @@ class MuZeroPagedCache:
         self._c = PagedCache(layers, rows, pages, block_table.shape[1], kv_heads, head_dim, residual_length, ring, dtype_code(tail.dtype),
                              store.data_ptr(), store.stride(0), store.stride(1), tail.data_ptr(), tail.stride(0), tail.stride(1),
                              block_table.data_ptr(), lengths.data_ptr(), page_refs.data_ptr(), status.data_ptr())
+        self._ref = ctypes.byref(self._c)
         self._args = PagedAttentionArgs()
+        self._args_ref = ctypes.byref(self._args)
         self._workspaces: dict = {}
+        self._needs: dict = {}
 
     @classmethod
     def allocate(cls, *, layers: int, kv_heads: int, head_dim: int, pages: int, rows: int, max_length: int, residual_length: int = 128,
@@ -131,7 +134,7 @@ class MuZeroPagedCache:
         ``rows``).  Lengths grow and the pages that they need are taken, for all layers at once, or nothing changes and ``check`` raises."""
         n = self._entries(rows, offsets)
         r, o = _index(rows, "rows", self.device), _index(offsets, "offsets", self.device, n + 1)
-        check(on_device(self.device, self._lib.mz_paged_extend, self._c, r, o, n, stream_ptr(self.device)), "mz_paged_extend")
+        check(on_device(self.device, self._lib.mz_paged_extend, self._ref, r, o, n, stream_ptr(self.device)), "mz_paged_extend")
 
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, *, rows: Optional[torch.Tensor] = None,
                offsets: Optional[torch.Tensor] = None, max_new: Optional[int] = None) -> None:
@@ -151,14 +154,17 @@ class MuZeroPagedCache:
             raise ValueError(f"{shape[0]} tokens for {n} rows: without `offsets` each row brings one")
         if max_new is None:
             max_new = 1 if offsets is None else shape[0]
-        check(on_device(self.device, self._lib.mz_paged_append, self._c, layer, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+        check(on_device(self.device, self._lib.mz_paged_append, self._ref, layer, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
                         v.stride(1), r, o, n, shape[0], max_new, stream_ptr(self.device)), "mz_paged_append")
 
-    def _workspace(self, nbytes: int, stream: int) -> torch.Tensor:
+    def _workspace(self, nbytes: int, stream: int) -> tuple:
         # one per stream, grown by replacement.  An outgrown one is kept: a captured graph may hold its address
-        held = self._workspaces.setdefault(stream, [])
-        if not held or held[-1].numel() < nbytes:
-            held.append(torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device))
+        held = self._workspaces.get(stream)
+        if held is None or held[-1][1] < nbytes:
+            size = max(nbytes, 1 << 20)
+            t = torch.empty(size, dtype=torch.uint8, device=self.device)
+            held = self._workspaces.setdefault(stream, [])
+            held.append((t.data_ptr(), size, t))
         return held[-1]
 
     def attend(self, layer: int, query: torch.Tensor, *, rows: Optional[torch.Tensor] = None, scaling: Optional[float] = None,
@@ -178,13 +184,15 @@ class MuZeroPagedCache:
         elif out.shape != query.shape or not out.is_contiguous() or out.device != self.device or (out_dtype or out.dtype) != out.dtype:
             raise ValueError("`out` must be a contiguous tensor of the query's shape on the cache's device")
         a, st = self._args, stream_ptr(self.device)
-        need = self._lib.mz_paged_attention_workspace_bytes(self._c, b, lq, hq)
+        need = self._needs.get((b, lq, hq))
+        if need is None:                                  # 0: a shape that the call below refuses with its reason
+            need = self._needs[b, lq, hq] = on_device(self.device, self._lib.mz_paged_attention_workspace_bytes, self._ref, b, lq, hq)
         ws = self._workspace(need, st)
         a.query, a.q_stride_b, a.q_stride_l, a.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1), q.stride(2)
         a.batch, a.q_len, a.q_heads, a.rows = b, lq, hq, _index(rows, "rows", self.device, b)
         a.scaling = self.head_dim ** -0.5 if scaling is None else scaling
-        a.out, a.out_dtype, a.workspace, a.workspace_bytes = out.data_ptr(), dtype_code(out.dtype), ws.data_ptr(), ws.numel()
-        check(on_device(self.device, self._lib.mz_paged_attention, self._c, layer, a, st), "mz_paged_attention")
+        a.out, a.out_dtype, a.workspace, a.workspace_bytes = out.data_ptr(), dtype_code(out.dtype), ws[0], ws[1]
+        check(on_device(self.device, self._lib.mz_paged_attention, self._ref, layer, self._args_ref, st), "mz_paged_attention")
         return out
 
     # ---- rows and pages
@@ -192,24 +200,24 @@ class MuZeroPagedCache:
         """Row ``target[i]`` becomes a copy of row ``source[i]`` in all layers: pages are shared, the ring is copied, what the target held is released.
         Targets are distinct, and none is a source."""
         n = target.shape[0]
-        check(on_device(self.device, self._lib.mz_paged_fork, self._c, _index(source, "source", self.device, n),
+        check(on_device(self.device, self._lib.mz_paged_fork, self._ref, _index(source, "source", self.device, n),
                         _index(target, "target", self.device), n, stream_ptr(self.device)), "mz_paged_fork")
 
     def free(self, rows: torch.Tensor) -> None:
         """Empties rows; pages that no other row holds are free again."""
-        check(on_device(self.device, self._lib.mz_paged_free, self._c, _index(rows, "rows", self.device), rows.shape[0],
+        check(on_device(self.device, self._lib.mz_paged_free, self._ref, _index(rows, "rows", self.device), rows.shape[0],
                         stream_ptr(self.device)), "mz_paged_free")
 
     def compact(self) -> None:
         """Moves the live pages into the lowest places of the pool, so that what lies above them is free in one piece."""
         st = stream_ptr(self.device)
-        ws = self._workspace(self._lib.mz_paged_compact_workspace_bytes(self._c), st)
-        check(on_device(self.device, self._lib.mz_paged_compact, self._c, ws.data_ptr(), ws.numel(), st), "mz_paged_compact")
+        ws = self._workspace(self._lib.mz_paged_compact_workspace_bytes(self._ref), st)
+        check(on_device(self.device, self._lib.mz_paged_compact, self._ref, ws[0], ws[1], st), "mz_paged_compact")
 
     def copy_pages(self, source: torch.Tensor, target: torch.Tensor) -> None:
         """Copies page ``source[i]`` onto page ``target[i]`` in all layers; tables and counts stay as they are."""
         n = target.shape[0]
-        check(on_device(self.device, self._lib.mz_paged_copy_pages, self._c, _index(source, "source", self.device, n),
+        check(on_device(self.device, self._lib.mz_paged_copy_pages, self._ref, _index(source, "source", self.device, n),
                         _index(target, "target", self.device), n, stream_ptr(self.device)), "mz_paged_copy_pages")
 
     def check(self) -> None:

@@ -19,6 +19,8 @@
 //
 // A second kernel has a CTA per pair.  It takes the 16-bit tokens of the pair's ring (mma.sync) while the first kernel ends, waits for it, and merges its
 // records with that.
+#include <atomic>
+
 #include "mz_paged.cuh"
 
 namespace mzp {
@@ -870,8 +872,15 @@ template <int D, bool BF, int NR>
 int launch(const Args& p, const uint8_t* book, int G, cudaStream_t st) {
   auto kern = attention_kernel<D, BF, NR>;
   using S = Smem<D, NR>;
-  MZ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL));
-  MZ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  static std::atomic<unsigned> ready[8];         // a bit per device: its limits are set
+  int dev = 0;
+  MZ_CUDA(cudaGetDevice(&dev));
+  const bool known = dev < 256 && (ready[dev >> 5].load(std::memory_order_relaxed) >> (dev & 31) & 1u);
+  if (!known) {
+    MZ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL));
+    MZ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    if (dev < 256) ready[dev >> 5].fetch_or(1u << (dev & 31), std::memory_order_relaxed);
+  }
   kern<<<G, THREADS, S::TOTAL, st>>>(p, book);
   MZ_LAUNCH_CHECK("paged attention");
   // The second kernel starts while the first one ends.  (Not so the first one while the second of the call before ends: an SM does not change its split
@@ -896,9 +905,8 @@ int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* 
   MZ_REQUIRE(q_len >= 1 && q_heads >= 1 && q_heads % c->kv_heads == 0, "q_len %d, q_heads %d of %d kv heads", q_len, q_heads, c->kv_heads);
   const long long qrows = (long long)q_heads / c->kv_heads * q_len;
   MZ_REQUIRE(qrows <= 1 << 20, "%lld query rows per kv head", qrows);
-  int dev = 0, sms = 0;
-  MZ_CUDA(cudaGetDevice(&dev));
-  MZ_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  int sms = 0, rc = mz_paged_sms(&sms);
+  if (rc != MZ_OK) return rc;
   s->nr = qrows <= 4 ? 4 : 8;
   s->passes = (int)((qrows + s->nr - 1) / s->nr);
   s->pairs = (long long)batch * c->kv_heads * s->passes;

@@ -1,4 +1,5 @@
 // Paged cache: tables, argument checks, and what moves whole pages or rows (extend, fork, free, compact, copy).
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <mutex>
@@ -6,10 +7,10 @@
 #include "mz_paged.cuh"
 
 namespace {
-__device__ uint8_t g_book[MZP_BOOKS * MZP_LEVELS];
-__device__ uint8_t g_nearest[MZP_BOOKS * 128];
+__device__ __align__(16) uint8_t g_book[MZP_BOOKS * MZP_LEVELS];
+__device__ __align__(16) uint8_t g_nearest[MZP_BOOKS * MZP_NEAR_ROW];
 std::mutex g_mu;
-unsigned long long g_filled[4] = {0, 0, 0, 0};      // devices whose tables are in place
+struct Tables { const uint8_t *book, *nearest; } g_tables[256];     // by device; NULL until they are in place
 
 // Levels of book z: z' = round(15 z / 127) codes lie below the zero level and 15 - z' above it, spaced by the law (3^t - 1) / 2.  No entry
 // is near a rounding boundary (the closest by 0.001), so any correctly working pow gives the same table.
@@ -37,20 +38,40 @@ extern "C" int mz_paged_books(unsigned char* book, unsigned char* nearest) {
   return MZ_OK;
 }
 
+int mz_paged_sms(int* sms) {
+  static std::atomic<int> known[256];
+  int dev = 0;
+  MZ_CUDA(cudaGetDevice(&dev));
+  MZ_REQUIRE(dev >= 0 && dev < 256, "device %d", dev);
+  *sms = known[dev].load(std::memory_order_relaxed);
+  if (*sms == 0) {
+    MZ_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+    known[dev].store(*sms, std::memory_order_relaxed);
+  }
+  return MZ_OK;
+}
+
 int mz_paged_tables(const uint8_t** book, const uint8_t** nearest) {
   int dev = 0;
   MZ_CUDA(cudaGetDevice(&dev));
   MZ_REQUIRE(dev >= 0 && dev < 256, "device %d", dev);
   std::lock_guard<std::mutex> lk(g_mu);
-  if (!(g_filled[dev >> 6] >> (dev & 63) & 1ull)) {
-    uint8_t b[sizeof(g_book)], n[sizeof(g_nearest)];
+  Tables& t = g_tables[dev];
+  if (t.nearest == nullptr) {
+    uint8_t b[sizeof(g_book)], n[MZP_BOOKS * 128], padded[sizeof(g_nearest)] = {};
     fill_books(b, n);
+    for (int z = 0; z < MZP_BOOKS; ++z)
+      for (int r = -1; r <= 128; ++r) padded[z * MZP_NEAR_ROW + r + 1] = n[z * 128 + (r < 0 ? 0 : r > 127 ? 127 : r)];
     MZ_CUDA(cudaMemcpyToSymbol(g_book, b, sizeof(b)));
-    MZ_CUDA(cudaMemcpyToSymbol(g_nearest, n, sizeof(n)));
-    g_filled[dev >> 6] |= 1ull << (dev & 63);
+    MZ_CUDA(cudaMemcpyToSymbol(g_nearest, padded, sizeof(padded)));
+    void *book_at = nullptr, *nearest_at = nullptr;
+    MZ_CUDA(cudaGetSymbolAddress(&book_at, g_book));
+    MZ_CUDA(cudaGetSymbolAddress(&nearest_at, g_nearest));
+    t.book = (const uint8_t*)book_at;
+    t.nearest = (const uint8_t*)nearest_at;
   }
-  if (book) MZ_CUDA(cudaGetSymbolAddress((void**)book, g_book));
-  if (nearest) MZ_CUDA(cudaGetSymbolAddress((void**)nearest, g_nearest));
+  if (book) *book = t.book;
+  if (nearest) *nearest = t.nearest;
   return MZ_OK;
 }
 
@@ -267,12 +288,6 @@ __global__ void __launch_bounds__(256) move_pages_kernel(const mz_paged_cache c,
   }
 }
 
-int sm_count(int* n) {
-  int dev = 0;
-  MZ_CUDA(cudaGetDevice(&dev));
-  MZ_CUDA(cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev));
-  return MZ_OK;
-}
 }  // namespace
 
 extern "C" int mz_paged_extend(const mz_paged_cache* cache, const int* rows, const int* offsets, int batch, void* stream) {
@@ -324,7 +339,7 @@ extern "C" int mz_paged_compact(const mz_paged_cache* cache, void* workspace, si
   if (!workspace || (uintptr_t)workspace % 16 != 0 || workspace_bytes < mz_paged_compact_workspace_bytes(cache))
     return mz_fail(MZ_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, mz_paged_compact_workspace_bytes(cache));
   int sms = 0;
-  if ((rc = sm_count(&sms)) != MZ_OK) return rc;
+  if ((rc = mz_paged_sms(&sms)) != MZ_OK) return rc;
   int* ws = (int*)workspace;
   compact_plan_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(*cache, ws);
   MZ_LAUNCH_CHECK("compact_plan");
@@ -341,7 +356,7 @@ extern "C" int mz_paged_copy_pages(const mz_paged_cache* cache, const int* sourc
   if (n == 0) return MZ_OK;
   MZ_REQUIRE(source != nullptr && target != nullptr, "a list is NULL");
   int sms = 0;
-  if ((rc = sm_count(&sms)) != MZ_OK) return rc;
+  if ((rc = mz_paged_sms(&sms)) != MZ_OK) return rc;
   const long long units = (long long)n * cache->layers * cache->kv_heads;
   move_pages_kernel<<<(unsigned)(units < sms * 8 ? units : sms * 8), 256, 0, (cudaStream_t)stream>>>(*cache, source, target, nullptr, n, nullptr);
   MZ_LAUNCH_CHECK("move_pages");
