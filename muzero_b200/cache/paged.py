@@ -148,7 +148,7 @@ class MuZeroPagedCache:
             if t.dtype != self.dtype or t.device != self.device or tuple(t.shape) != shape:
                 raise ValueError(f"`{name}` must be {self.dtype} {shape} on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
             # rows of whole 16-byte pieces; anything else is laid out once
-            tensors.append(t if t.stride(2) == 1 and not (t.stride(0) | t.stride(1)) & 7 and not t.data_ptr() & 15 else t.contiguous())
+            tensors.append(t if t.stride(2) == 1 and not (t.stride(0) | t.stride(1)) & 7 and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format))
         k, v = tensors
         if offsets is None and shape[0] != n:
             raise ValueError(f"{shape[0]} tokens for {n} rows: without `offsets` each row brings one")
@@ -177,10 +177,10 @@ class MuZeroPagedCache:
                              f"{tuple(query.shape)} on {query.device}")
         # rows of whole 16-byte pieces; anything else is laid out once
         if q.stride(3) != 1 or (q.stride(0) | q.stride(1) | q.stride(2)) & 7 or q.data_ptr() & 15:
-            q = q.contiguous()
+            q = q.clone(memory_format=torch.contiguous_format)
         b, lq, hq, _ = q.shape
         if out is None:
-            out = torch.empty(query.shape, dtype=out_dtype or self.dtype, device=self.device)
+            out = query.new_empty(query.shape) if out_dtype is None else torch.empty(query.shape, dtype=out_dtype, device=self.device)
         elif out.shape != query.shape or not out.is_contiguous() or out.device != self.device or (out_dtype or out.dtype) != out.dtype:
             raise ValueError("`out` must be a contiguous tensor of the query's shape on the cache's device")
         a, st = self._args, stream_ptr(self.device)

@@ -1015,6 +1015,8 @@ int mz_launch_decode_umma(const MzDecodeParams& p, cudaStream_t st) {
   return mz_fail(MZ_ERR_UNSUPPORTED, "bits %d, %d planes", p.s.bits, p.planes);
 }
 
+int mz_waits_fail() { return mzu::g_fail_waits.load(std::memory_order_relaxed); }
+
 extern "C" int mz_debug_fail_waits(int on) {
 #ifdef MZ_BOUNDS
   return mzu::g_fail_waits.exchange(on != 0);

@@ -16,6 +16,8 @@ constexpr int MZP_NEAR_ROW = 132;
 int mz_paged_tables(const uint8_t** book, const uint8_t** nearest);
 // multiprocessors of the current device (asked once)
 int mz_paged_sms(int* sms);
+// whether mz_debug_fail_waits is on (checked build)
+int mz_waits_fail();
 // argument checks that every entry point shares
 int mz_paged_check(const mz_paged_cache* c);
 

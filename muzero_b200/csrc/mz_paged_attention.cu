@@ -42,7 +42,8 @@ struct Args {
   int* head;
   float2* ml;                                    // [slot][NR] maximum (base 2) and sum
   float* acc;                                    // [slot][NR][D]
-  long long pairs;
+  long long pairs, slots;
+  int fail_waits;                                // checked build: not 0 = waits run out at once
 };
 
 // ---- small wrappers
@@ -85,6 +86,9 @@ __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
 }
 // Waits for the phase of this parity.  Who gives up says so before it goes on; the others notice.
 __device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile int* s_failed) {
+#ifdef MZ_BOUNDS
+  if (*s_failed) return;                         // a test makes every wait run out
+#endif
   for (int it = 0; it < SPIN_LIMIT; ++it) {
     if (bar_test(bar, parity)) return;
     if ((it & 63) == 63 && *s_failed) return;
@@ -197,7 +201,7 @@ struct Smem {
   static constexpr int A_BYTES = 8 * CHUNK;                // 128 positions
   static constexpr int B_BYTES = 2 * NR * 4 / 16 * CHUNK;  // 2 blocks x NR x 4 bytes
   static constexpr int K_A = 0, V_A = A_BYTES, K_B = 2 * A_BYTES, V_B = K_B + B_BYTES, BOOK = V_B + B_BYTES;
-  static constexpr int TOTAL = BOOK + MZP_BOOKS * MZP_LEVELS;
+  static constexpr int ALIGN = 1024, TOTAL = BOOK + MZP_BOOKS * MZP_LEVELS + ALIGN;      // (a linker of device code may give the window less)
   static constexpr int N = 8 * NR, TM_S = 0, TM_O = N, TM_COLS = 2 * N;
   static constexpr int CTAS = NR == 4 ? 4 : 3;             // per SM
 };
@@ -267,7 +271,8 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   constexpr int DT = BF ? MZ_BF16 : MZ_F16;
   constexpr int PB = 72 * D;                     // page bytes per kv head
   constexpr int RPT = D / 64;                    // rows of codes per thread, side and step
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ uint8_t window[];
+  uint8_t* smem = window + (S::ALIGN - smem_u32(window) % S::ALIGN) % S::ALIGN;
   __shared__ Exchange<NR> x;
   const mz_paged_cache& c = p.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -275,7 +280,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t k_done = smem_u32(x.bar), v_done = k_done + 8, b_end = k_done + 16;
   if (tid == 0) {
-    x.failed = 0;
+    x.failed = p.fail_waits;
     bar_init(k_done, 1); bar_init(v_done, 1); bar_init(b_end, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -468,8 +473,8 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
     }
     __syncthreads();
     const long long slot = (long long)cta + pair;
-    const bool bad = *(volatile int*)&x.failed != 0;
-    if (D == 128 || r < 64) {
+    const bool bad = *(volatile int*)&x.failed != 0, inside = MZ_IN_BOUNDS(slot, p.slots, 20);
+    if (inside && (D == 128 || r < 64)) {
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
         const int at = (1 + (D == 128 ? blk : 0)) * NR + i;
@@ -478,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
         p.acc[(slot * NR + i) * D + r] = out;
       }
     }
-    if (r < NR) {
+    if (inside && r < NR) {
       const float sum_l = (x.fin[0][r] + x.fin[1][r]) + (x.fin[2][r] + x.fin[3][r]);
       float top = m[0];
 #pragma unroll
@@ -966,6 +971,8 @@ extern "C" int mz_paged_attention(const mz_paged_cache* cache, int layer, const 
   p.acc = (float*)((uint8_t*)args->workspace + s.head_bytes);
   p.ml = (float2*)(p.acc + s.slots * s.nr * cache->head_dim);
   p.pairs = s.pairs;
+  p.slots = (long long)s.slots;
+  p.fail_waits = mz_waits_fail();
   cudaStream_t st = (cudaStream_t)stream;
   const bool bf = cache->kv_dtype == MZ_BF16;
 #define MZP_GO(D, NR) return bf ? mzp::launch<D, true, NR>(p, book, s.G, st) : mzp::launch<D, false, NR>(p, book, s.G, st)
