@@ -506,3 +506,14 @@ def test_checked_build_and_waits_that_run_out():
     env = dict(os.environ, MUZERO_B200_LIB=lib)
     res = subprocess.run([sys.executable, "-c", CHILD.format(root=root)], env=env, capture_output=True, text=True, timeout=300)
     assert res.returncode == 0 and "paged checked build ok" in res.stdout, res.stdout + res.stderr
+
+
+def test_the_example_runs(capsys):
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_serving.py")
+    spec = importlib.util.spec_from_file_location("paged_serving", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    out = m.main(["--layers", "2", "--rows", "6", "--prefix", "300", "--requests", "15", "--new-tokens", "40"])
+    assert out["requests"] >= 15 and out["error"] <= 2.0 ** -8          # bf16 output
