@@ -19,6 +19,7 @@
 //
 // A second kernel has a CTA per pair.  It takes the 16-bit tokens of the pair's ring (mma.sync) while the first kernel ends, waits for it, and merges its
 // records with that.
+#include <algorithm>
 #include <atomic>
 
 #include "mz_paged.cuh"
@@ -37,6 +38,7 @@ struct Args {
   int out_dtype, layer, batch, q_len, q_heads, group;      // group: query heads per kv head
   int qrows, passes;                             // query rows per kv head, and how many passes of NR they take
   int sms, per_sm;                               // the grid, if the machine is full
+  int longest;                                   // a row is not taken for longer than its table has room for (and a page, which is then reported)
   float scaling;                                 // times log2(e)
   // workspace: header {CTAs, steps before each entry [batch + 1]}, records
   int* head;
@@ -262,7 +264,7 @@ struct Cut {
 // row and length of a list entry; a row that is not there is empty
 __device__ __forceinline__ int length_of(const Args& p, int b, int& row) {
   row = p.rows ? p.rows[b] : b;
-  return row < 0 || row >= p.c.rows ? 0 : max(0, min(p.c.lengths[row], 0x7fffffff - STEP));
+  return row < 0 || row >= p.c.rows ? 0 : max(0, min(p.c.lengths[row], p.longest));
 }
 
 template <int D, bool BF, int NR>
@@ -558,13 +560,13 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
     fence_operands();
     tm_before();
     __syncthreads();
-    if (tid == 0 && !*(volatile int*)&x.failed) {
+    if (tid == 96 && !*(volatile int*)&x.failed) {
       tm_after();
 #pragma unroll
       for (int k = 0; k < D / 32; ++k) umma<S::N, true>(tmem + S::TM_S, ka + k * (512 >> 4), kb + k * (512 >> 4), k > 0);
       umma_commit(k_done);
     }
-    if (warp == 3 && (it & 15) == 0 && it > 0) plan(it + 16);
+    if (warp == 0 && (it & 15) == 0 && it > 0) plan(it + 16);
     const Step next = x.step[(it + 1) & 31];     // beyond the CTA's last step: pages that are not there, or a step that nobody takes
     if (it + 1 < n) load_keys(next, true, true);
     // ---- values: the output so far, then levels while the products of the keys run
@@ -669,7 +671,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
     fence_operands();
     tm_before();
     __syncthreads();
-    if (tid == 64 && !*(volatile int*)&x.failed) {
+    if (tid == 32 && !*(volatile int*)&x.failed) {
       tm_after();
 #pragma unroll
       for (int k = 0; k < D / 32; ++k) umma<S::N, false>(tmem + S::TM_O, va + k * (512 >> 4), vb + k * (512 >> 4), k > 0);
@@ -678,7 +680,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   }
   take_output(n - 1);
   write_record();
-  if (x.failed && (tid & 63) == 0) {             // products in flight end before their memory goes back
+  if (x.failed && (tid & 63) == 32) {             // products in flight end before their memory goes back
     umma_commit(b_end);
     for (int k = 0; k < SPIN_LIMIT && !bar_test(b_end, 0); ++k) {}
   }
@@ -919,6 +921,7 @@ int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* 
   s->sms = sms;
   s->per_sm = s->nr == 4 ? 4 : 3;
   s->G = sms * s->per_sm;
+  MZ_REQUIRE((long long)batch * (c->width + 2) <= 1ll << 31, "%d rows of %d pages are too many for one call", batch, c->width);
   // a CTA costs its start (592 of them 6 us): no more than there can be steps
   const long long most = s->pairs * ((c->width + 1) / 2);
   if (s->G > most) s->G = most < 1 ? 1 : (int)most;
@@ -966,6 +969,7 @@ extern "C" int mz_paged_attention(const mz_paged_cache* cache, int layer, const 
   p.qrows = p.group * args->q_len;
   p.passes = s.passes;
   p.sms = s.sms; p.per_sm = s.per_sm;
+  p.longest = (int)std::min<long long>(0x7fffffff - mzp::STEP, cache->residual + (cache->width + 2ll) * MZP_PAGE - 1);
   p.scaling = args->scaling * mzp::LOG2E;
   p.head = (int*)args->workspace;
   p.acc = (float*)((uint8_t*)args->workspace + s.head_bytes);

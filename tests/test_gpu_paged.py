@@ -349,6 +349,24 @@ def test_what_the_device_finds_wrong():
     del kv
 
 
+def test_lengths_that_the_table_has_no_room_for():
+    """Spoilt lengths, whose steps added up would pass 32 bits, are reported; the rows beside them keep their results."""
+    from muzero_b200.kernels import MuZeroKernelError
+    n, d = 160, 64
+    cache = make(n, 1, d, "bf16", 0, max_length=640, pages=16)
+    fill(cache, [200, 70] + [0] * (n - 2), 1)
+    q = torch.randn(n, 1, 2, d, device="cuda", dtype=torch.bfloat16)
+    want = cache.attend(0, q, out_dtype=torch.float32)
+    cache.lengths[2:] = 0x7fffffff
+    got = cache.attend(0, q, out_dtype=torch.float32)
+    assert torch.allclose(got[:2], want[:2], rtol=0, atol=1e-5) and torch.isfinite(got).all()
+    with pytest.raises(MuZeroKernelError, match="outside"):
+        cache.check()
+    cache.lengths[2:] = -5
+    assert (cache.attend(0, q)[2:] == 0).all()
+    cache.check()
+
+
 def test_refusals():
     import muzero_b200 as mz
     cache = make(2, 2, 64, "bf16", 0)
