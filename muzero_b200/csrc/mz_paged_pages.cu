@@ -226,25 +226,40 @@ __global__ void __launch_bounds__(256) free_kernel(const mz_paged_cache c, const
   if (threadIdx.x == 0) c.lengths[row] = 0;
 }
 
-// workspace of a compaction: {pages to move, pad, pad, pad}, map[pages], from[pages], to[pages]
+// workspace of a compaction: {pages to move, pad, pad, pad}, map[pages], from[pages], to[pages].  One CTA, four neighbouring pages per thread: the places
+// in both lists come from one scan of two 16-bit counts.
 __global__ void __launch_bounds__(1024) compact_plan_kernel(const mz_paged_cache c, int* __restrict__ ws) {
   __shared__ int s_warp[32];
   int *map = ws + 4, *from = map + c.pages, *to = from + c.pages;
   int live = 0;
-  for (int p0 = 0; p0 < c.pages; p0 += 1024) {
-    const int p = p0 + threadIdx.x;
-    live += __syncthreads_count(p < c.pages && c.page_refs[p] > 0);
+  for (int p0 = 0; p0 < c.pages; p0 += 4096) {
+    int mine = 0, total;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { const int p = p0 + 4 * (int)threadIdx.x + j; mine += p < c.pages && c.page_refs[p] > 0; }
+    block_scan_exclusive(mine, &total, s_warp);
+    live += total;
   }
   int movers = 0, holes = 0;
-  for (int p0 = 0; p0 < c.pages; p0 += 1024) {
-    const int p = p0 + threadIdx.x;
-    const bool in = p < c.pages, used = in && c.page_refs[p] > 0;
-    const bool mover = used && p >= live, hole = in && !used && p < live;
-    int total;
-    const int both = block_scan_exclusive((int)mover | (int)hole << 16, &total, s_warp);       // at most 1024 of each
-    if (mover) from[movers + (both & 0xffff)] = p;
-    if (hole) to[holes + (both >> 16)] = p;
-    if (in) map[p] = p;
+  for (int p0 = 0; p0 < c.pages; p0 += 4096) {
+    bool mover[4], hole[4];
+    int mine = 0, total;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int p = p0 + 4 * (int)threadIdx.x + j;
+      const bool in = p < c.pages, used = in && c.page_refs[p] > 0;
+      mover[j] = used && p >= live;
+      hole[j] = in && !used && p < live;
+      mine += (int)mover[j] | (int)hole[j] << 16;
+      if (in) map[p] = p;
+    }
+    const int both = block_scan_exclusive(mine, &total, s_warp);       // at most 4096 of each
+    int m = movers + (both & 0xffff), h = holes + (both >> 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int p = p0 + 4 * (int)threadIdx.x + j;
+      if (mover[j]) from[m++] = p;
+      if (hole[j]) to[h++] = p;
+    }
     movers += total & 0xffff;
     holes += total >> 16;
   }
