@@ -4,7 +4,8 @@
 // one that is still to be quantized.
 //
 // What bounds it is the instructions of a value: two to find the range (pairs of 16 bits), eight to its code, of which one is the table's load.  What is
-// rare is kept out of them: a row with a NaN, an infinity, a value beyond f16 or a scale below f16's normal numbers is done again by the general form.
+// rare is kept out of them (prompts of 1777 to 4096 tokens x 8 kv heads, head_dim 128, 265 MB read and written: 102.6 us, 2.6 TB/s; issue slots 61 % used,
+// shared-memory wavefronts 64 %, most of them the lookups, which meet the same banks; 170 us with the range and the code of every value in the general form): a row with a NaN, an infinity, a value beyond f16 or a scale below f16's normal numbers is done again by the general form.
 #include "mz_paged.cuh"
 
 namespace {
