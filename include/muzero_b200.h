@@ -383,7 +383,12 @@ int mz_av_output(const mz_kv_store* store, const void* weights, int w_dtype, int
  */
 #define MZ_PAGED_NO_PAGES 1  /* extend: more pages needed than are free; nothing was changed */
 #define MZ_PAGED_TOO_LONG 2  /* extend: a row would outgrow its table row; nothing was changed */
-#define MZ_PAGED_BAD_INDEX 4 /* a row or page index outside the cache, or a row that is both source and target; skipped */
+#define MZ_PAGED_BAD_INDEX 4 /* a row or page index outside the cache, or a row that is both source and target; skipped (extend: nothing was changed) */
+/*
+ * No error of its own, and not the host's to clear: the newest mz_paged_extend was refused, for one of the reasons above.  mz_paged_append writes nothing
+ * as long as it stands; the next extension that succeeds takes it away.  Who clears errors leaves it as it is.
+ */
+#define MZ_PAGED_REFUSED 8
 
 typedef struct {
   int layers, rows, pages, width;        /* width: entries of a row of the table */
@@ -402,7 +407,8 @@ int mz_paged_books(unsigned char* book, unsigned char* nearest);
 
 /*
  * Lengthens the rows rows[0..batch) (NULL: row i is i; distinct) by offsets[i+1] - offsets[i] tokens (NULL: one each) and gives them the pages that
- * their new lengths need, the lowest free ones first, in the order of the list.  All or nothing.  batch <= 4096.
+ * their new lengths need, the lowest free ones first, in the order of the list.  All or nothing: an extension that is refused keeps the appends
+ * that go with it from writing (MZ_PAGED_REFUSED).  batch <= 4096.
  */
 int mz_paged_extend(const mz_paged_cache* cache, const int* rows, const int* offsets, int batch, void* stream);
 

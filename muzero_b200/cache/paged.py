@@ -29,6 +29,7 @@ from ..kernels._cabi import (MuZeroKernelError, PagedAttentionArgs, PagedCache, 
 PAGE_TOKENS = 64
 _MAX_ROWS_PER_CALL = 1024
 _STATUS = {1: "the pool has too few free pages", 2: "a sequence outgrew its row of the block table", 4: "a row or page index is outside the cache"}
+_ERRORS = sum(_STATUS)                               # the fourth bit says that the newest extension was refused; the device sets and clears it
 
 
 def page_bytes(head_dim: int) -> int:
@@ -131,7 +132,8 @@ class MuZeroPagedCache:
 
     def extend(self, *, rows: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None) -> None:
         """Announces new tokens: entry i brings ``offsets[i+1] - offsets[i]`` of them (one each without ``offsets``) for row ``rows[i]`` (row i without
-        ``rows``).  Lengths grow and the pages that they need are taken, for all layers at once, or nothing changes and ``check`` raises."""
+        ``rows``).  Lengths grow and the pages that they need are taken, for all layers at once, or nothing changes and ``check`` raises.  After
+        an extension that was refused ``append`` writes nothing, until another one succeeds.  The rows of a call are distinct."""
         n = self._entries(rows, offsets)
         r, o = _index(rows, "rows", self.device), _index(offsets, "offsets", self.device, n + 1)
         check(on_device(self.device, self._lib.mz_paged_extend, self._ref, r, o, n, stream_ptr(self.device)), "mz_paged_extend")
@@ -222,9 +224,9 @@ class MuZeroPagedCache:
 
     def check(self) -> None:
         """Raises what a call on this cache found wrong on the device since the last check, and forgets it.  Synchronises."""
-        seen = int(self.status.item())
+        seen = int(self.status.item()) & _ERRORS
         if seen:
-            self.status.zero_()
+            self.status.bitwise_and_(~seen)
             raise MuZeroKernelError("paged cache: " + "; ".join(text for bit, text in _STATUS.items() if seen & bit))
 
     def free_pages(self) -> int:

@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) append_kernel(const Appe
   __shared__ float4 s_row[D];                   // quantizer constants of the keys' rows; the last is not 0 for the general form
   __shared__ __align__(16) uint8_t s_out[D * 32];
   const mz_paged_cache& c = a.c;
-  if (*c.status & (MZ_PAGED_NO_PAGES | MZ_PAGED_TOO_LONG)) return;      // the extension failed: there is no room for these tokens
+  const bool refused = *c.status & MZ_PAGED_REFUSED;      // nothing has been announced: the lists are looked over, and nothing is written
   const int near0 = (int)__cvta_generic_to_shared(s_near) + 1 - __float_as_int(MAGIC);
   bool have_table = false;
   const long long units = (long long)a.batch * a.slots * c.kv_heads;
@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) append_kernel(const Appe
       if (threadIdx.x == 0) atomicOr(c.status, MZ_PAGED_BAD_INDEX);
       continue;
     }
+    if (refused) continue;
     const int after = c.lengths[row], before = after - n;
     if (before < 0) { if (threadIdx.x == 0) atomicOr(c.status, MZ_PAGED_BAD_INDEX); continue; }
     const int packed = mzp_packed(after, c.residual);

@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(1024) extend_kernel(const mz_paged_cache c, co
   if (bad) atomicOr(&s_bad, bad);
   if (threadIdx.x == 0) s_first[batch] = need_all;
   __syncthreads();
-  if (s_bad) { if (threadIdx.x == 0) atomicOr(c.status, s_bad); return; }
+  if (s_bad) { if (threadIdx.x == 0) atomicOr(c.status, s_bad | MZ_PAGED_REFUSED); return; }
   if (need_all > 0) {
     // are there enough?
     int found = 0;
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(1024) extend_kernel(const mz_paged_cache c, co
       const int p = p0 + threadIdx.x;
       found += __syncthreads_count(p < c.pages && c.page_refs[p] == 0);
     }
-    if (found < need_all) { if (threadIdx.x == 0) atomicOr(c.status, MZ_PAGED_NO_PAGES); return; }
+    if (found < need_all) { if (threadIdx.x == 0) atomicOr(c.status, MZ_PAGED_NO_PAGES | MZ_PAGED_REFUSED); return; }
     int dealt = 0;
     for (int p0 = 0; dealt < need_all; p0 += 1024) {
       const int p = p0 + threadIdx.x;
@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(1024) extend_kernel(const mz_paged_cache c, co
     __syncthreads();
   }
   for (int i = threadIdx.x; i < batch; i += 1024) c.lengths[rows ? rows[i] : i] += offsets ? offsets[i + 1] - offsets[i] : 1;
+  if (threadIdx.x == 0) atomicAnd(c.status, ~MZ_PAGED_REFUSED);       // what is appended next has been announced
 }
 
 __device__ __forceinline__ void release(const mz_paged_cache& c, int page) {
