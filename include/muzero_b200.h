@@ -395,9 +395,9 @@ typedef struct {
   int kv_heads, head_dim;                /* head_dim 64 or 128 */
   int residual, ring;                    /* residual: a multiple of 64; ring >= residual + 64 */
   int kv_dtype;                          /* MZ_F16 or MZ_BF16 */
-  void* store;                           /* [layers][pages][kv_heads][72 * head_dim] bytes */
-  long long store_stride_layer, store_stride_page;   /* bytes, multiples of 16 */
-  void* tail;                            /* [layers][rows][2 (key, value)][kv_heads][ring][head_dim] */
+  void* store;                           /* [layers][pages][kv_heads][72 * head_dim] bytes, 32-byte aligned */
+  long long store_stride_layer, store_stride_page;   /* bytes, multiples of 32 */
+  void* tail;                            /* [layers][rows][2 (key, value)][kv_heads][ring][head_dim], 16-byte aligned */
   long long tail_stride_layer, tail_stride_row;      /* elements, multiples of 8 */
   int *block_table, *lengths, *page_refs, *status;   /* [rows][width], [rows], [pages], [1] */
 } mz_paged_cache;

@@ -96,6 +96,8 @@ class MuZeroPagedCache:
                 problems.append(f"`{name}` must be contiguous int32")
         if store.stride(3) != 1 or store.stride(2) != pb or tail.stride()[2:] != (kv_heads * ring * head_dim, ring * head_dim, head_dim, 1):
             problems.append("a page and a row's ring must be contiguous")
+        if (store.data_ptr() | store.stride(0) | store.stride(1)) & 31 or tail.data_ptr() & 15 or (tail.stride(0) | tail.stride(1)) & 7:
+            problems.append("pages must begin on 32-byte boundaries, rings on 16-byte boundaries")
         if problems:
             raise ValueError("; ".join(problems))
         self.store, self.tail, self.block_table, self.lengths, self.page_refs, self.status = store, tail, block_table, lengths, page_refs, status

@@ -85,10 +85,11 @@ int mz_paged_check(const mz_paged_cache* c) {
   MZ_REQUIRE(c->residual >= 0 && c->residual % MZP_PAGE == 0, "residual %d is not a multiple of %d", c->residual, MZP_PAGE);
   MZ_REQUIRE(c->ring >= c->residual + MZP_PAGE && c->ring <= (1 << 20), "ring %d: at least residual + %d", c->ring, MZP_PAGE);
   MZ_REQUIRE(c->store && c->tail && c->block_table && c->lengths && c->page_refs && c->status, "a cache pointer is NULL");
-  MZ_REQUIRE((uintptr_t)c->store % 16 == 0 && (uintptr_t)c->tail % 16 == 0, "store and tail must be 16-byte aligned");
-  MZ_REQUIRE(c->store_stride_page % 16 == 0 && c->store_stride_layer % 16 == 0 &&
+  // attention reads the 32 bytes of a row of codes with one load (a page's size and the places of its rows are multiples of 32)
+  MZ_REQUIRE((uintptr_t)c->store % 32 == 0 && (uintptr_t)c->tail % 16 == 0, "store must be 32-byte aligned and tail 16-byte");
+  MZ_REQUIRE(c->store_stride_page % 32 == 0 && c->store_stride_layer % 32 == 0 &&
                  c->store_stride_page >= (long long)c->kv_heads * mzp_page_bytes(c->head_dim),
-             "page stride %lld bytes", c->store_stride_page);
+             "page stride %lld bytes, layer stride %lld: multiples of 32, and a page's bytes at least", c->store_stride_page, c->store_stride_layer);
   MZ_REQUIRE(c->tail_stride_row % 8 == 0 && c->tail_stride_layer % 8 == 0 &&
                  c->tail_stride_row >= 2ll * c->kv_heads * c->ring * c->head_dim,
              "ring stride %lld elements", c->tail_stride_row);
