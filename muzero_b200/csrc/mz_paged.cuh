@@ -27,7 +27,7 @@ __host__ __device__ inline int mzp_packed(int length, int residual) {       // t
   return n > 0 ? n / MZP_PAGE * MZP_PAGE : 0;
 }
 
-// a row's word -> anchor, scale, zero level
+// a row's word -> anchor, scale, zero level (0..127 whatever the word: it picks a book in shared memory)
 struct MzpRow { float a, t; int z; };
 __device__ __forceinline__ MzpRow mzp_row(uint32_t word) {
   MzpRow r;
@@ -35,7 +35,7 @@ __device__ __forceinline__ MzpRow mzp_row(uint32_t word) {
   const bool off = (field & 0x7FFFu) >= 128u;
   r.t = __half2float(__ushort_as_half((unsigned short)(word & 0xFFFFu)));
   r.a = off ? __half2float(__ushort_as_half((unsigned short)field)) : 0.0f;
-  r.z = off ? ((field & 0x8000u) ? 127 : 0) : (int)field;
+  r.z = off ? ((field & 0x8000u) ? 127 : 0) : (int)(field & 0x7Fu);
   return r;
 }
 // its zero level alone
