@@ -716,6 +716,7 @@ __global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
   const int half = warp % HALVES, stream = warp / HALVES;
   if (tokens > 0) {
     const int see0 = tokens - p.q_len;           // query token l sees the ring's tokens up to see0 + l
+    const int l_first = r0 / p.group, l_last = (min(r0 + NR, p.qrows) - 1) / p.group;      // the pass's query tokens
     const uint16_t* ring_k = (const uint16_t*)c.tail + (long long)p.layer * c.tail_stride_layer + (long long)row * c.tail_stride_row + (long long)head * c.ring * D;
     const uint16_t* ring_v = ring_k + (long long)c.kv_heads * c.ring * D + half * 64;
     const int ring0 = packed % c.ring;
@@ -753,7 +754,7 @@ __global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
         uint4 va[D / 32], vb[D / 32];
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) { va[k] = *(const uint4*)(ka + 32 * k); vb[k] = *(const uint4*)(kb + 32 * k); }
-        load_values(tokens - 1);
+        load_values(min(see0 + l_last, tokens - 1));
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
           mma16<BF>(s, va[k].x, vb[k].x, va[k].y, vb[k].y, qf[k].x, qf[k].y);
@@ -798,13 +799,12 @@ __global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
         asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(hi[h]) : "r"(hw));
         asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(lo[h]) : "r"(lw));
       }
-      // A token that only later queries see must not bring a NaN to a product with p = 0: where a tile has tokens that only some of the queries see, each
-      // of the queries' tokens takes its turn with what it sees
-      const int l_first = r0 / p.group, l_last = (min(r0 + NR, p.qrows) - 1) / p.group;
+      // A token that only later queries see must not bring a NaN to a product with p = 0: what no query of the pass sees is not loaded, and where a tile has
+      // tokens that only some of the queries see, each of the queries' tokens takes its turn with what it sees, and only its columns are added
       const bool apart = i0 + 15 > see0 + l_first && l_last > l_first;
       for (int turn = 0; turn <= (apart ? l_last - l_first : 0); ++turn) {
-        const bool mine = !apart || qr / p.group == l_first + turn;
         if (apart) load_values(min(see0 + l_first + turn, tokens - 1));
+        const bool mine0 = !apart || (r0 + 2 * t) / p.group == l_first + turn, mine1 = !apart || (r0 + 2 * t + 1) / p.group == l_first + turn;
         const uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
         const uint32_t w2[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
 #pragma unroll
@@ -812,8 +812,11 @@ __global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
           // rows g / g + 8 = channels 8g + 2k / 8g + 2k + 1
           const uint32_t a0 = prmt(w0[k], w1[k], 0x5410u), a1 = prmt(w0[k], w1[k], 0x7632u);
           const uint32_t a2 = prmt(w2[k], w3[k], 0x5410u), a3 = prmt(w2[k], w3[k], 0x7632u);
-          mma16<BF>(o[k], a0, a1, a2, a3, mine ? lo[0] : 0u, mine ? lo[1] : 0u);
-          mma16<BF>(o[k], a0, a1, a2, a3, mine ? hi[0] : 0u, mine ? hi[1] : 0u);
+          float c4[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16<BF>(c4, a0, a1, a2, a3, lo[0], lo[1]);
+          mma16<BF>(c4, a0, a1, a2, a3, hi[0], hi[1]);
+          if (mine0) { o[k][0] += c4[0]; o[k][2] += c4[2]; }
+          if (mine1) { o[k][1] += c4[1]; o[k][3] += c4[3]; }
         }
       }
     }
