@@ -699,7 +699,8 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
 }
 
 // One pair per CTA of eight warps; 26 us alone for 512 pairs of 128 ring tokens (36 MB; it waits for loads), of which 13 us show behind the first kernel.  Rings: a warp takes 16 tokens at a time, and (D = 128) 64 of the channels of the output; A = keys [token][channel],
-// B = queries; A = values [channel][token], B = p in two parts of 16 bits.  Then a thread has a channel, and every second query row.
+// B = queries; A = values [channel][token], B = p in parts of 16 bits, as many as fp32 has bits.  Products go to fresh accumulators that are added in round-to-nearest:
+// the tensor cores truncate their running sums.  Then a thread has a channel, and every second query row.
 constexpr int END_THREADS = 256;
 template <int D, bool BF, int NR>
 __global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
@@ -757,8 +758,11 @@ __global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
         load_values(min(see0 + l_last, tokens - 1));
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
-          mma16<BF>(s, va[k].x, vb[k].x, va[k].y, vb[k].y, qf[k].x, qf[k].y);
-          mma16<BF>(s, va[k].z, vb[k].z, va[k].w, vb[k].w, qf[k].z, qf[k].w);
+          float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16<BF>(c0, va[k].x, vb[k].x, va[k].y, vb[k].y, qf[k].x, qf[k].y);
+          mma16<BF>(c1, va[k].z, vb[k].z, va[k].w, vb[k].w, qf[k].z, qf[k].w);
+          add2(c0[0], c0[1], c1[0], c1[1]); add2(c0[2], c0[3], c1[2], c1[3]);
+          add2(s[0], s[1], c0[0], c0[1]); add2(s[2], s[3], c0[2], c0[3]);
         }
       }
       // s[0], s[1]: token g, columns (query rows) 2t, 2t + 1; s[2], s[3]: token g + 8
@@ -780,24 +784,31 @@ __global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) { o[i][0] *= fix[0]; o[i][1] *= fix[1]; o[i][2] *= fix[0]; o[i][3] *= fix[1]; }
-      // p in two parts, transposed: column g, tokens 2t, 2t + 1 ([0]) and 2t + 8, 2t + 9 ([1])
-      uint32_t hi[2], lo[2];
+      // p in parts, transposed: column g, tokens 2t, 2t + 1 ([0]) and 2t + 8, 2t + 9 ([1]).  Three of 8 bits or two of 11 leave less than fp32's own
+      // rounding; f16 has p times 2^15, so that a second part does not end at its smallest numbers
+      constexpr int PARTS = BF ? 3 : 2;
+      constexpr float P_SCALE = BF ? 1.0f : 32768.0f, P_UNIT = 1.0f / P_SCALE;
+      uint32_t part[PARTS][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t hw, lw;
-        if (BF) {
-          const __nv_bfloat162 hb = __floats2bfloat162_rn(s[2 * h], s[2 * h + 1]);
-          const float2 hf = __bfloat1622float2(hb);
-          const __nv_bfloat162 lb = __floats2bfloat162_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
-          hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
-        } else {
-          const __half2 hb = __floats2half2_rn(s[2 * h], s[2 * h + 1]);
-          const float2 hf = __half22float2(hb);
-          const __half2 lb = __floats2half2_rn(s[2 * h] - hf.x, s[2 * h + 1] - hf.y);
-          hw = *reinterpret_cast<const uint32_t*>(&hb); lw = *reinterpret_cast<const uint32_t*>(&lb);
+        float p0 = s[2 * h] * P_SCALE, p1 = s[2 * h + 1] * P_SCALE;
+#pragma unroll
+        for (int x = 0; x < PARTS; ++x) {
+          uint32_t w;
+          float2 f;
+          if (BF) {
+            const __nv_bfloat162 b2 = __floats2bfloat162_rn(p0, p1);
+            w = *reinterpret_cast<const uint32_t*>(&b2);
+            f = __bfloat1622float2(b2);
+          } else {
+            const __half2 h2 = __floats2half2_rn(p0, p1);
+            w = *reinterpret_cast<const uint32_t*>(&h2);
+            f = __half22float2(h2);
+          }
+          p0 -= f.x;
+          p1 -= f.y;
+          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(part[x][h]) : "r"(w));
         }
-        asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(hi[h]) : "r"(hw));
-        asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(lo[h]) : "r"(lw));
       }
       // A token that only later queries see must not bring a NaN to a product with p = 0: what no query of the pass sees is not loaded, and where a tile has
       // tokens that only some of the queries see, each of the queries' tokens takes its turn with what it sees, and only its columns are added
@@ -813,10 +824,10 @@ __global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
           const uint32_t a0 = prmt(w0[k], w1[k], 0x5410u), a1 = prmt(w0[k], w1[k], 0x7632u);
           const uint32_t a2 = prmt(w2[k], w3[k], 0x5410u), a3 = prmt(w2[k], w3[k], 0x7632u);
           float c4[4] = {0.f, 0.f, 0.f, 0.f};
-          mma16<BF>(c4, a0, a1, a2, a3, lo[0], lo[1]);
-          mma16<BF>(c4, a0, a1, a2, a3, hi[0], hi[1]);
-          if (mine0) { o[k][0] += c4[0]; o[k][2] += c4[2]; }
-          if (mine1) { o[k][1] += c4[1]; o[k][3] += c4[3]; }
+#pragma unroll
+          for (int x = PARTS - 1; x >= 0; --x) mma16<BF>(c4, a0, a1, a2, a3, part[x][0], part[x][1]);
+          if (mine0) { o[k][0] = fmaf(c4[0], P_UNIT, o[k][0]); o[k][2] = fmaf(c4[2], P_UNIT, o[k][2]); }
+          if (mine1) { o[k][1] = fmaf(c4[1], P_UNIT, o[k][1]); o[k][3] = fmaf(c4[3], P_UNIT, o[k][3]); }
         }
       }
     }

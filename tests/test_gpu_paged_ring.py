@@ -1,10 +1,10 @@
-"""GPU: the 16-bit window of the paged cache: what a query does not see."""
+"""GPU: the 16-bit window of the paged cache: what a query does not see, and its precision."""
 import numpy as np
 import pytest
 import torch
 
 import paged_plain as plain
-from test_gpu_paged import f32, ints, make, tokens
+from test_gpu_paged import DT, f32, ints, make, tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +36,31 @@ def test_later_tokens_do_not_reach_earlier_queries(d, group, lq, bad_from, bad):
         for h in range(group):
             assert np.linalg.norm(got[j, h] - want[j, h]) <= 3e-5 * np.linalg.norm(want[j, h]), (j, h)
     assert not np.isfinite(got[bad_from:]).any()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_probabilities_have_the_precision_of_fp32(dt, d):
+    """One token has the largest logit and no value, 90 others have the same smaller logit and the value 1: the output is 90 p / (1 + 90 p), so an error of p is not averaged
+    away.  128 queries give 128 different p from 1/2 to 2^-16.  The logit is one exact product times the scale: at most 2^-24 of 11.1 in the product and in the factor to
+    base 2, together 1.4e-6 (natural log units; the largest logit's own error is as large only where its size is, and it is chosen as zero here); the exponential 2^-22, sums
+    and the quotient 2^-22: 1.9e-6 of the output in the worst case, 3e-6 is asked for."""
+    n = 91
+    cache = make(1, 1, d, dt, 128)
+    k, v = torch.zeros(n, 1, d), torch.ones(n, 1, d)
+    k[1:, 0, 0] = -1.0
+    v[0] = 0.0
+    put(cache, k.to(DT[dt]), v.to(DT[dt]))
+    size = torch.linspace(0.6, 11.0, 128)
+    errors = []
+    for i in range(0, 128, 8):
+        q = torch.zeros(1, 1, 8, d)
+        q[0, 0, :, 0] = size[i:i + 8]
+        q = q.to(DT[dt])
+        got = cache.attend(0, q.cuda(), out_dtype=torch.float32, scaling=1.0)[0, 0].double().cpu().numpy()
+        p = np.exp(-q[0, 0, :, 0].double().numpy())
+        want = 90 * p / (1 + 90 * p)
+        errors.append(got / want[:, None] - 1)
+        assert np.abs(errors[-1]).max() <= 3e-6, (i, np.abs(errors[-1]).max())
+    # in the mean square: a logit of up to 15.9 (base 2) rounds by up to 2^-21, 1.9e-7 of the exponential; the factor to base 2 adds 1.5e-7 and the exponential 1e-7
+    assert np.square(errors).mean() ** 0.5 <= 5e-7, np.square(errors).mean() ** 0.5
