@@ -185,6 +185,22 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Pairs of 16-bit values: `odd` becomes not zero where one is not finite
+template <bool BF>
+__device__ __forceinline__ void note_odd(uint32_t& odd, uint32_t w) {
+  // x * 0 is a zero, of either sign, or NaN; adding +0 leaves +0 or NaN
+  if (BF) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(odd) : "r"(w), "r"(0u));
+  else asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(odd) : "r"(w), "r"(0u));
+}
+// takes what is not finite out of a pair
+template <bool BF>
+__device__ __forceinline__ uint32_t take_odd(uint32_t& w) {
+  constexpr uint32_t TOP = BF ? 0x7F80u : 0x7C00u;
+  const uint32_t mask = ((w & TOP) == TOP ? 0xFFFFu : 0u) | (((w >> 16) & TOP) == TOP ? 0xFFFF0000u : 0u), taken = w & mask;
+  w &= ~mask;
+  return taken;
+}
+
 // A row's 64 codes -> 64 bytes, four pieces of 16, `chunk` bytes apart.  A selector's top bit asks for the sign of a level, which is zero: so the two
 // permutes of a nibble are zero exactly where they are not meant, and their results are or-ed.
 __device__ __forceinline__ void expand_row(const uint32_t (&w)[8], const uint4& book, uint32_t dst, uint32_t chunk) {
@@ -787,6 +803,7 @@ __global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
       // p in parts, transposed: column g, tokens 2t, 2t + 1 ([0]) and 2t + 8, 2t + 9 ([1]).  Three of 8 bits or two of 11 leave less than fp32's own
       // rounding; f16 has p times 2^15, so that a second part does not end at its smallest numbers
       constexpr int PARTS = BF ? 3 : 2;
+      constexpr uint32_t ONE16 = BF ? 0x3F80u : 0x3C00u;
       constexpr float P_SCALE = BF ? 1.0f : 32768.0f, P_UNIT = 1.0f / P_SCALE;
       uint32_t part[PARTS][2];
 #pragma unroll
@@ -816,8 +833,29 @@ __global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
       for (int turn = 0; turn <= (apart ? l_last - l_first : 0); ++turn) {
         if (apart) load_values(min(see0 + l_first + turn, tokens - 1));
         const bool mine0 = !apart || (r0 + 2 * t) / p.group == l_first + turn, mine1 = !apart || (r0 + 2 * t + 1) / p.group == l_first + turn;
-        const uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
-        const uint32_t w2[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
+        uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+        uint32_t w2[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
+        // An infinite value is not a matter of p's parts (a lower one may be zero or negative): values that are not finite are taken out and meet a 1 where
+        // p is not zero, in a product of their own
+        uint32_t odd = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { note_odd<BF>(odd, w0[k]); note_odd<BF>(odd, w1[k]); note_odd<BF>(odd, w2[k]); note_odd<BF>(odd, w3[k]); }
+        if (__any_sync(0xffffffffu, odd != 0)) {
+          uint32_t one[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t w = (s[2 * h] > 0.f ? ONE16 : 0u) | (s[2 * h + 1] > 0.f ? ONE16 << 16 : 0u);
+            asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(one[h]) : "r"(w));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t x0 = take_odd<BF>(w0[k]), x1 = take_odd<BF>(w1[k]), x2 = take_odd<BF>(w2[k]), x3 = take_odd<BF>(w3[k]);
+            float c4[4] = {0.f, 0.f, 0.f, 0.f};
+            mma16<BF>(c4, prmt(x0, x1, 0x5410u), prmt(x0, x1, 0x7632u), prmt(x2, x3, 0x5410u), prmt(x2, x3, 0x7632u), one[0], one[1]);
+            if (mine0) { o[k][0] += c4[0]; o[k][2] += c4[2]; }
+            if (mine1) { o[k][1] += c4[1]; o[k][3] += c4[3]; }
+          }
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           // rows g / g + 8 = channels 8g + 2k / 8g + 2k + 1

@@ -1,4 +1,4 @@
-"""GPU: the 16-bit window of the paged cache: what a query does not see, and its precision."""
+"""GPU: the 16-bit window of the paged cache: what a query does not see, what is not finite, and its precision."""
 import numpy as np
 import pytest
 import torch
@@ -36,6 +36,38 @@ def test_later_tokens_do_not_reach_earlier_queries(d, group, lq, bad_from, bad):
         for h in range(group):
             assert np.linalg.norm(got[j, h] - want[j, h]) <= 3e-5 * np.linalg.norm(want[j, h]), (j, h)
     assert not np.isfinite(got[bad_from:]).any()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n, lq, group", [(20, 1, 4), (150, 1, 8), (150, 3, 2), (40, 2, 8), (330, 1, 5)])
+def test_infinite_values(dt, d, n, lq, group):
+    """Values that are infinite in the window: a sum of positive multiples of them is that infinity, of both signs NaN, and a NaN is NaN; channels without any are
+    what they are without them."""
+    cache = make(1, 1, d, dt, 128)
+    k, v = tokens(n, 1, d, DT[dt], 5)
+    spoilt = v.clone()
+    at = n - lq - 3                                               # every query sees it
+    spoilt[at, 0, 3], spoilt[at - 1, 0, 7] = float("inf"), float("-inf")
+    spoilt[at, 0, 9], spoilt[at - 2, 0, 9] = float("inf"), float("-inf")
+    spoilt[at, 0, 11], spoilt[at, 0, d - 1] = float("nan"), float("inf")
+    spoilt[at - 1, 0, d - 1] = float("inf")
+    spoilt[n - 1, 0, 20] = float("inf")                           # the last query only sees this one
+    put(cache, k, spoilt)
+    q = torch.randn(1, lq, group, d, generator=torch.Generator().manual_seed(group)).to(DT[dt]).cuda()
+    got = cache.attend(0, q, out_dtype=torch.float32)[0].cpu().numpy()
+    kk, vv = plain.held(f32(k), f32(v), 128)
+    want = plain.attention(f32(q[0].cpu()), kk, vv, d ** -0.5)
+    inf = np.inf
+    assert (got[..., 3] == inf).all() and (got[..., 7] == -inf).all() and (got[..., d - 1] == inf).all()
+    assert np.isnan(got[..., 9]).all() and np.isnan(got[..., 11]).all() and (got[-1, :, 20] == inf).all()
+    plain_channels = [c for c in range(d) if c not in (3, 7, 9, 11, d - 1, 20)]
+    for j in range(lq):
+        for h in range(group):
+            x, y = got[j, h, plain_channels], want[j, h, plain_channels]
+            assert np.linalg.norm(x - y) <= 3e-5 * np.linalg.norm(y), (j, h)
+    if lq > 1:
+        assert np.abs(got[:-1, :, 20] - want[:-1, :, 20]).max() <= 3e-5 * np.linalg.norm(want, axis=-1).max()
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
