@@ -406,6 +406,12 @@ typedef struct {
 int mz_paged_books(unsigned char* book, unsigned char* nearest);
 
 /*
+ * Puts the codec's tables on the current device and waits for them (the first time on a device; later calls return at once).  The calls below do it where it has
+ * not been done, but cannot inside a stream capture.
+ */
+int mz_paged_prepare(void);
+
+/*
  * Lengthens the rows rows[0..batch) (NULL: row i is i; distinct) by offsets[i+1] - offsets[i] tokens (NULL: one each) and gives them the pages that
  * their new lengths need, the lowest free ones first, in the order of the list.  All or nothing: an extension that is refused keeps the appends
  * that go with it from writing (MZ_PAGED_REFUSED).  batch <= 4096.

@@ -105,6 +105,7 @@ class MuZeroPagedCache:
         self.layers, self.pages, self.kv_heads, self.rows, self.head_dim, self.dtype = layers, pages, kv_heads, rows, head_dim, tail.dtype
         self.device = store.device
         self._lib = load_library()
+        check(on_device(self.device, self._lib.mz_paged_prepare), "mz_paged_prepare")      # so that a first call may stand in a captured graph
         self._c = PagedCache(layers, rows, pages, block_table.shape[1], kv_heads, head_dim, residual_length, ring, dtype_code(tail.dtype),
                              store.data_ptr(), store.stride(0), store.stride(1), tail.data_ptr(), tail.stride(0), tail.stride(1),
                              block_table.data_ptr(), lengths.data_ptr(), page_refs.data_ptr(), status.data_ptr())

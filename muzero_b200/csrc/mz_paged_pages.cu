@@ -64,6 +64,8 @@ int mz_paged_tables(const uint8_t** book, const uint8_t** nearest) {
       for (int r = -1; r <= 128; ++r) padded[z * MZP_NEAR_ROW + r + 1] = n[z * 128 + (r < 0 ? 0 : r > 127 ? 127 : r)];
     MZ_CUDA(cudaMemcpyToSymbol(g_book, b, sizeof(b)));
     MZ_CUDA(cudaMemcpyToSymbol(g_nearest, padded, sizeof(padded)));
+    // the copies may still be on their way from their staging memory, and a non-blocking stream does not wait for the legacy one
+    MZ_CUDA(cudaStreamSynchronize(cudaStreamLegacy));
     void *book_at = nullptr, *nearest_at = nullptr;
     MZ_CUDA(cudaGetSymbolAddress(&book_at, g_book));
     MZ_CUDA(cudaGetSymbolAddress(&nearest_at, g_nearest));
@@ -74,6 +76,8 @@ int mz_paged_tables(const uint8_t** book, const uint8_t** nearest) {
   if (nearest) *nearest = t.nearest;
   return MZ_OK;
 }
+
+extern "C" int mz_paged_prepare(void) { return mz_paged_tables(nullptr, nullptr); }
 
 int mz_paged_check(const mz_paged_cache* c) {
   MZ_REQUIRE(c != nullptr, "cache is NULL");

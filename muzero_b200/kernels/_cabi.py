@@ -24,7 +24,7 @@ EXPORTS = (
     "mz_decode_attention_partial", "mz_lse_merge", "mz_qk_logits", "mz_av_output", "mz_decode_attention_static",
     "mz_decode_step", "mz_decode_step_workspace_bytes", "mz_flush_kv_parts", "mz_decode_workspace_bound", "mz_decode_attention_partial_packed", "mz_lse_merge_packed", "mz_store_gather_batch", "mz_debug_force_kernel", "mz_debug_fail_waits", "mz_debug_decode_kernel", "mz_bounds_violations",
     "mz_alpha_stats", "mz_alpha_stats_workspace_bytes", "mz_materialize_kv", "mz_roundtrip_kv", "mz_flush_kv_move",
-    "mz_paged_books", "mz_paged_extend", "mz_paged_append", "mz_paged_attention_workspace_bytes", "mz_paged_attention", "mz_paged_fork",
+    "mz_paged_books", "mz_paged_prepare", "mz_paged_extend", "mz_paged_append", "mz_paged_attention_workspace_bytes", "mz_paged_attention", "mz_paged_fork",
     "mz_paged_free", "mz_paged_compact_workspace_bytes", "mz_paged_compact", "mz_paged_copy_pages",
 )
 
@@ -156,6 +156,7 @@ def load_library() -> ctypes.CDLL:
     lib.mz_qk_logits.argtypes = [POINTER(KVStore), c_void_p, c_longlong, c_longlong, c_int, c_float, c_void_p, c_int, c_void_p]
     lib.mz_av_output.argtypes = [POINTER(KVStore), c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p]
     lib.mz_paged_books.argtypes = [c_void_p, c_void_p]
+    lib.mz_paged_prepare.argtypes = []
     lib.mz_paged_extend.argtypes = [POINTER(PagedCache), c_void_p, c_void_p, c_int, c_void_p]
     lib.mz_paged_append.argtypes = [POINTER(PagedCache), c_int] + [c_void_p, c_longlong, c_longlong] * 2 + [c_void_p, c_void_p, c_int, c_int, c_int,
                                                                                                             c_void_p]

@@ -1,4 +1,8 @@
 """GPU: the paged cache's calls: what the host refuses, first calls, arguments at their limits."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -21,3 +25,45 @@ def test_tensors_that_the_kernels_cannot_read_are_refused(off, gap):
     tail = torch.zeros(c.tail.numel() + 4, dtype=c.dtype, device="cuda")[4:].view(c.tail.shape)
     with pytest.raises(ValueError, match="boundaries"):
         mz.MuZeroPagedCache(store=c.store, tail=tail, **rest)
+
+
+FIRST = r"""
+import sys, torch
+sys.path[:0] = [{root!r}, {root!r} + "/tests"]
+import paged_plain as plain
+from test_gpu_paged import assert_row, check_attention, ints, make, tokens
+cache = make(2, 2, 128, "bf16", 0, pages=16, max_length=640)
+k, v = tokens(330, 2, 128, torch.bfloat16, 3)
+kd, vd, q = k.cuda(), v.cuda(), torch.randn(2, 1, 8, 128, device="cuda", dtype=torch.bfloat16)
+o, rows = ints(0, 200, 330), ints(0, 1)
+torch.cuda.synchronize()
+side = torch.cuda.Stream()
+if {captured}:
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        cache.extend(offsets=o)
+        cache.append(0, kd, vd, offsets=o)
+        out = cache.attend(0, q)
+    graph.replay()
+else:
+    with torch.cuda.stream(side):
+        cache.extend(offsets=o)
+        cache.append(0, kd, vd, offsets=o)
+        out = cache.attend(0, q)
+torch.cuda.synchronize()
+cache.check()
+kv = [(k[:200], v[:200]), (k[200:], v[200:])]
+for r in range(2):
+    assert_row(cache, r, *kv[r])
+check_attention(cache, kv, q, [0, 1])
+assert torch.equal(out, cache.attend(0, q))
+print("first call ok")
+"""
+
+
+@pytest.mark.parametrize("captured", [True, False])
+def test_the_first_calls_of_a_process(captured):
+    """The first calls of all stand in a captured graph, or on a stream that does not wait for the legacy one: the codec's tables are in place."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", FIRST.format(root=root, captured=captured)], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "first call ok" in res.stdout, res.stdout + res.stderr
