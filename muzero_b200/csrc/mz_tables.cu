@@ -92,6 +92,14 @@ void build_expand_host(int bits, float alpha, std::vector<float>& t) {
   }
 }
 
+// Host memory -> a table.  The copy may still be on its way from its staging memory when it returns, and a non-blocking stream does not wait for the legacy
+// one.
+int upload(void* dev, const void* host, size_t bytes) {
+  MZ_CUDA(cudaMemcpy(dev, host, bytes, cudaMemcpyHostToDevice));
+  MZ_CUDA(cudaStreamSynchronize(cudaStreamLegacy));
+  return MZ_OK;
+}
+
 int upload_expand(int dev, int bits, float alpha, const float* host) {
   const size_t n = (size_t)1 << (2 * bits);
   auto key = std::make_tuple(dev, bits, fbits(alpha));
@@ -99,7 +107,8 @@ int upload_expand(int dev, int bits, float alpha, const float* host) {
   auto it = g_expand.find(key);
   if (it != g_expand.end()) d = it->second;
   else MZ_CUDA(cudaMalloc(&d, n * sizeof(float)));
-  MZ_CUDA(cudaMemcpy(d, host, n * sizeof(float), cudaMemcpyHostToDevice));
+  const int rc = upload(d, host, n * sizeof(float));
+  if (rc != MZ_OK) return rc;
   g_expand[key] = d;
   return MZ_OK;
 }
@@ -150,7 +159,8 @@ int mz_get_compand_table(int dtype, float alpha, const uint16_t** dev_table, int
     }
     uint16_t* d = nullptr;
     MZ_CUDA(cudaMalloc(&d, (size_t)n * sizeof(uint16_t)));
-    MZ_CUDA(cudaMemcpy(d, host.data(), (size_t)n * sizeof(uint16_t), cudaMemcpyHostToDevice));
+    const int rc = upload(d, host.data(), (size_t)n * sizeof(uint16_t));
+    if (rc != MZ_OK) return rc;
     it = g_compand.emplace(key, std::make_pair(d, n)).first;
   }
   *dev_table = it->second.first;
