@@ -163,10 +163,11 @@ class MuZeroPagedCache:
                         v.stride(1), r, o, n, shape[0], max_new, stream_ptr(self.device)), "mz_paged_append")
 
     def _workspace(self, nbytes: int, stream: int) -> tuple:
-        # one per stream, grown by replacement.  An outgrown one is kept: a captured graph may hold its address
+        # One per stream, grown by replacement.  An outgrown one is kept, as a captured graph may hold its address; one that has to grow at least
+        # doubles, so that its predecessors are smaller than it all together
         held = self._workspaces.get(stream)
         if held is None or held[-1][1] < nbytes:
-            size = max(nbytes, 1 << 20)
+            size = max(nbytes, 1 << 20, 2 * held[-1][1] if held else 0)
             t = torch.empty(size, dtype=torch.uint8, device=self.device)
             held = self._workspaces.setdefault(stream, [])
             held.append((t.data_ptr(), size, t))

@@ -22,3 +22,26 @@ def test_a_store_that_32_byte_loads_cannot_read_is_refused(change):
 def test_a_store_on_32_byte_boundaries_is_taken(change):
     from muzero_b200.kernels import _cabi
     assert _cabi.load_library().mz_paged_extend(_cache(**change), None, None, 0, None) == 0          # checked, and nothing to do
+
+
+def _host_cache():
+    """A cache's host side without a device."""
+    import torch
+    from muzero_b200.cache.paged import MuZeroPagedCache
+    c = object.__new__(MuZeroPagedCache)
+    c.device, c._workspaces = torch.device("cpu"), {}
+    return c
+
+
+@pytest.mark.parametrize("sizes", [range(1 << 20, 9 << 20, 1 << 16), range(9 << 20, 1 << 20, -(1 << 16)), [5, 1 << 22, 7, 1 << 23, (1 << 23) + 1]])
+def test_workspaces_of_growing_calls(sizes):
+    """What a stream's calls of many sizes hold together is less than four times what the largest needs: a workspace that has to grow doubles at least, and its
+    predecessors are smaller than it all together."""
+    c = _host_cache()
+    for n in sizes:
+        at, size, t = c._workspace(n, 1)
+        assert size >= n and t.numel() == size and t.data_ptr() == at
+    held = [w[1] for w in c._workspaces[1]]
+    assert sum(held) < 4 * max(max(sizes), 1 << 20) and sum(held[:-1]) < held[-1]
+    small = c._workspace(3, 2)                                     # another stream's own
+    assert small[1] == 1 << 20 and len(c._workspaces) == 2
