@@ -110,8 +110,6 @@ class MuZeroPagedCache:
                              store.data_ptr(), store.stride(0), store.stride(1), tail.data_ptr(), tail.stride(0), tail.stride(1),
                              block_table.data_ptr(), lengths.data_ptr(), page_refs.data_ptr(), status.data_ptr())
         self._ref = ctypes.byref(self._c)
-        self._args = PagedAttentionArgs()
-        self._args_ref = ctypes.byref(self._args)
         self._workspaces: dict = {}
         self._needs: dict = {}
 
@@ -189,16 +187,15 @@ class MuZeroPagedCache:
             out = query.new_empty(query.shape) if out_dtype is None else torch.empty(query.shape, dtype=out_dtype, device=self.device)
         elif out.shape != query.shape or not out.is_contiguous() or out.device != self.device or (out_dtype or out.dtype) != out.dtype:
             raise ValueError("`out` must be a contiguous tensor of the query's shape on the cache's device")
-        a, st = self._args, stream_ptr(self.device)
+        st = stream_ptr(self.device)
         need = self._needs.get((b, lq, hq))
         if need is None:                                  # 0: a shape that the call below refuses with its reason
             need = self._needs[b, lq, hq] = on_device(self.device, self._lib.mz_paged_attention_workspace_bytes, self._ref, b, lq, hq)
         ws = self._workspace(need, st)
-        a.query, a.q_stride_b, a.q_stride_l, a.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1), q.stride(2)
-        a.batch, a.q_len, a.q_heads, a.rows = b, lq, hq, _index(rows, "rows", self.device, b)
-        a.scaling = self.head_dim ** -0.5 if scaling is None else scaling
-        a.out, a.out_dtype, a.workspace, a.workspace_bytes = out.data_ptr(), dtype_code(out.dtype), ws[0], ws[1]
-        check(on_device(self.device, self._lib.mz_paged_attention, self._ref, layer, self._args_ref, st), "mz_paged_attention")
+        # a block per call: another thread may attend another layer meanwhile
+        a = PagedAttentionArgs(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), b, lq, hq, _index(rows, "rows", self.device, b),
+                               self.head_dim ** -0.5 if scaling is None else scaling, out.data_ptr(), dtype_code(out.dtype), ws[0], ws[1])
+        check(on_device(self.device, self._lib.mz_paged_attention, self._ref, layer, ctypes.byref(a), st), "mz_paged_attention")
         return out
 
     # ---- rows and pages

@@ -45,3 +45,45 @@ def test_workspaces_of_growing_calls(sizes):
     assert sum(held) < 4 * max(max(sizes), 1 << 20) and sum(held[:-1]) < held[-1]
     small = c._workspace(3, 2)                                     # another stream's own
     assert small[1] == 1 << 20 and len(c._workspaces) == 2
+
+
+def test_calls_of_two_threads_have_their_own_arguments(monkeypatch):
+    """Two threads attend at the same time, on streams of their own: what the library finds in its argument block is the caller's query, output and workspace, also when
+    the other thread has come as far as the library meanwhile."""
+    import ctypes
+    import threading
+
+    import torch
+    from muzero_b200.cache import paged
+    from muzero_b200.kernels._cabi import PagedAttentionArgs
+    c = _host_cache()
+    c.head_dim, c.dtype, c._needs, c._ref = 64, torch.bfloat16, {}, None
+    both = threading.Barrier(2, timeout=20)
+    seen = {}
+
+    class Library:
+        @staticmethod
+        def mz_paged_attention_workspace_bytes(*_):
+            return 1 << 20
+
+        @staticmethod
+        def mz_paged_attention(_, layer, ref, stream):
+            both.wait()                                            # both have filled their blocks
+            a = ctypes.cast(ref, ctypes.POINTER(PagedAttentionArgs)).contents
+            seen[layer] = a.query, a.out, a.workspace, a.batch, a.q_heads, a.scaling, stream
+            both.wait()
+            return 0
+
+    c._lib = Library
+    monkeypatch.setattr(paged, "stream_ptr", lambda device: threading.current_thread().name)
+    monkeypatch.setattr(paged, "on_device", lambda device, fn, *args: fn(*args))
+    queries = [torch.zeros(1 + i, 1, 2 + 2 * i, 64, dtype=torch.bfloat16) for i in range(2)]
+    outs = [torch.empty_like(q) for q in queries]
+    threads = [threading.Thread(target=lambda i=i: c.attend(i, queries[i], out=outs[i], scaling=float(i)), name=f"stream {i}") for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        ws = c._workspaces[f"stream {i}"][-1][0]
+        assert seen[i] == (queries[i].data_ptr(), outs[i].data_ptr(), ws, 1 + i, 2 + 2 * i, float(i), f"stream {i}")
