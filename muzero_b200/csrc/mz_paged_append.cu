@@ -312,6 +312,7 @@ extern "C" int mz_paged_append(const mz_paged_cache* cache, int layer, const voi
   MZ_REQUIRE(key != nullptr && value != nullptr, "key or value is NULL");
   MZ_REQUIRE(((uintptr_t)key | (uintptr_t)value) % 16 == 0 && (k_stride_token | k_stride_head | v_stride_token | v_stride_head) % 8 == 0,
              "key and value must be 16-byte aligned with strides in multiples of 8 elements");
+  max_new = max_new < tokens ? max_new : tokens;      // (an entry that brought more would pass the end of the tokens)
   AppendArgs a = {*cache, (const uint16_t*)key, (const uint16_t*)value, k_stride_token, k_stride_head, v_stride_token, v_stride_head, rows, offsets,
                   layer, batch, tokens, max_new, 0, 1, 1};
   const int pages = (max_new + MZP_PAGE - 1) / MZP_PAGE, window = cache->residual + MZP_PAGE - 1;       // tokens that may stay

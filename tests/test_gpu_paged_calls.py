@@ -6,7 +6,7 @@ import sys
 import pytest
 import torch
 
-from test_gpu_paged import make
+from test_gpu_paged import assert_row, ints, make, tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,16 @@ def test_the_first_calls_of_a_process(captured):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     res = subprocess.run([sys.executable, "-c", FIRST.format(root=root, captured=captured)], capture_output=True, text=True, timeout=300)
     assert res.returncode == 0 and "first call ok" in res.stdout, res.stdout + res.stderr
+
+
+@pytest.mark.parametrize("most", [300, 301, 1 << 20, (1 << 31) - 64, (1 << 31) - 63, (1 << 31) - 1])
+def test_a_bound_on_new_tokens_may_be_any(most):
+    """`max_new` is a bound: the largest there is does no more than the tokens' number."""
+    cache = make(2, 1, 64, "bf16", 64)
+    k, v = tokens(310, 1, 64, torch.bfloat16, 4)
+    o = ints(0, 300, 310)
+    cache.extend(offsets=o)
+    cache.append(0, k.cuda(), v.cuda(), offsets=o, max_new=most)
+    cache.check()
+    assert_row(cache, 0, k[:300], v[:300])
+    assert_row(cache, 1, k[300:], v[300:])
