@@ -45,7 +45,7 @@ def packed_tokens(length: int, residual_length: int) -> int:
 def _index(t: Optional[torch.Tensor], what: str, device: torch.device, n: Optional[int] = None) -> int:
     if t is None:
         return 0
-    if t.dtype != torch.int32 or t.dim() != 1 or t.device != device or t.stride(0) != 1:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.device != device or not t.is_contiguous():
         raise ValueError(f"`{what}` must be a contiguous int32 vector on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     if n is not None and t.shape[0] != n:
         raise ValueError(f"`{what}` has {t.shape[0]} entries, expected {n}")

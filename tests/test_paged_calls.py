@@ -87,3 +87,17 @@ def test_calls_of_two_threads_have_their_own_arguments(monkeypatch):
     for i in range(2):
         ws = c._workspaces[f"stream {i}"][-1][0]
         assert seen[i] == (queries[i].data_ptr(), outs[i].data_ptr(), ws, 1 + i, 2 + 2 * i, float(i), f"stream {i}")
+
+
+def test_index_vectors():
+    """A vector of one entry is contiguous whatever its stride; longer ones that are not, other types and other shapes are refused."""
+    import torch
+    from muzero_b200.cache.paged import _index
+    cpu = torch.device("cpu")
+    whole = torch.arange(6, dtype=torch.int32)
+    for one in (whole[::2][:1], whole[:1].expand(1), torch.arange(4, dtype=torch.int32).view(2, 2)[:1, 1]):
+        assert _index(one, "rows", cpu, 1) == one.data_ptr()
+    assert _index(whole[2:], "rows", cpu, 4) == whole.data_ptr() + 8
+    for bad in (whole[::2], whole[:1].expand(3), whole.long(), whole.view(2, 3)):
+        with pytest.raises(ValueError):
+            _index(bad, "rows", cpu)
