@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(1024) extend_kernel(const mz_paged_cache c, co
     }
     if (found < need_all) { if (threadIdx.x == 0) atomicOr(c.status, MZ_PAGED_NO_PAGES | MZ_PAGED_REFUSED); return; }
     int dealt = 0;
-    for (int p0 = 0; dealt < need_all; p0 += 1024) {
+    for (int p0 = 0; p0 < c.pages && dealt < need_all; p0 += 1024) {      // (ends whatever another stream does to the counts meanwhile)
       const int p = p0 + threadIdx.x;
       const bool free_page = p < c.pages && c.page_refs[p] == 0;
       int total;
