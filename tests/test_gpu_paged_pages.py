@@ -1,8 +1,10 @@
 """GPU: attention over what pages hold: bytes that no append has written, rows of very unlike scales."""
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_paged import fill, make
+import paged_plain as plain
+from test_gpu_paged import f32, fill, ints, make
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +41,67 @@ def test_pages_of_any_bytes(d, group):
     cache.store.copy_(store)
     assert torch.equal(cache.attend(0, q, out_dtype=torch.float32), want)
     cache.check()
+
+
+def scales_case(d, k, v, q):
+    """one row of k, v [n, 1, d], queries q [1, 1, heads, d] -> output and the same in 64 bits, [heads, d], and the pages' largest T on either side"""
+    k, v, q = k.bfloat16(), v.bfloat16(), q.bfloat16()
+    cache = make(1, 1, d, "bf16", 0)
+    o = ints(0, k.shape[0])
+    cache.extend(offsets=o)
+    cache.append(0, k.cuda(), v.cuda(), offsets=o)
+    got = cache.attend(0, q.cuda(), out_dtype=torch.float32)[0, 0].double().cpu().numpy()
+    want = plain.attention(f32(q[0]), *plain.held(f32(k), f32(v), 0), d ** -0.5)[0]
+    top = []
+    for words in (plain.quantize(f32(k[:, 0]).reshape(-1, 64, d).swapaxes(1, 2))[1], plain.quantize(f32(v[:, 0]).reshape(-1, 64))[1]):
+        top.append(float((words & 0xFFFF).astype(np.uint16).view(np.float16).max()))
+    return got, want, top
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("ratio", [0, 4, 7, 10, 12, 14])
+def test_channels_of_unlike_scales(d, ratio):
+    """Key channels 2^ratio times as large as the others, whose queries are as much smaller, or zero.  q T is rounded to 2^-31 of a power of two above the product of the
+    largest |q| and T (both up to twice those), levels are 64 / 32 in the mean: an error of a logit of sqrt(d) * 2^-29 * |q| T * 2 / sqrt(3) * scaling in the mean square, and
+    of the output as large in parts of it; twice that, beside the tolerance of ordinary rows."""
+    gen = torch.Generator().manual_seed(ratio)
+    k, v, q = (torch.randn(*s, generator=gen) for s in ((1024, 1, d), (1024, 1, d), (1, 1, 4, d)))
+    for c, factor in ((5, 2.0 ** -ratio), (17, 0.0)):
+        k[..., c] *= 2.0 ** ratio
+        q[..., c] *= factor
+    got, want, (top, _) = scales_case(d, k, v, q)
+    for h in range(4):
+        logit = d ** 0.5 * 2.0 ** -29 * float(q[0, 0, h].abs().max()) * top * 2 / 3 ** 0.5 * d ** -0.5
+        assert np.linalg.norm(got[h] - want[h]) <= (3e-5 + 2 * logit) * np.linalg.norm(want[h]), h
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("ratio, bits", [(0, 0), (4, 0), (10, 0), (4, 6), (7, 9), (10, 12), (13, 15)])
+def test_tokens_of_unlike_scales(d, ratio, bits):
+    """Every 64th token's value is 2^ratio times as large as the others', and its probability 2^-bits times as large.  p T is rounded to 2^-31 of a power of two above the
+    largest T (up to twice that): an error of each channel of sqrt(tokens) * 2^-30 * T * 2 / sqrt(3) in the mean square, before the division by a sum of at least 1; twice
+    that, beside the tolerance of ordinary rows."""
+    n = 1024
+    gen = torch.Generator().manual_seed(ratio + bits)
+    k, v, q = (torch.randn(*s, generator=gen) for s in ((n, 1, d), (n, 1, d), (1, 1, 4, d)))
+    v[::64] *= 2.0 ** ratio
+    q[..., 3], k[..., 3] = 4.0, 0.0
+    k[::64, :, 3] = -bits * 0.6931 * d ** 0.5 / 4
+    got, want, (_, top) = scales_case(d, k, v, q)
+    for h in range(4):
+        assert np.linalg.norm(got[h] - want[h]) <= 3e-5 * np.linalg.norm(want[h]) + 2 * (n * d) ** 0.5 * 2.0 ** -30 * top * 2 / 3 ** 0.5, h
+
+
+@pytest.mark.parametrize("bits", [4, 8, 12, 16])
+def test_a_token_that_takes_nearly_all(bits):
+    """The first token has 2^bits times the probability of the others and hardly a value: what the others carry keeps the precision that p T of 31 bits leaves it, of
+    n tokens whose p is 2^-bits (bound as above, T as for ordinary rows)."""
+    n, d = 1024, 128
+    gen = torch.Generator().manual_seed(bits)
+    k, v, q = (torch.randn(*s, generator=gen) for s in ((n, 1, d), (n, 1, d), (1, 1, 4, d)))
+    v[0] *= 1e-3
+    q[..., 3], k[..., 3] = 4.0, 0.0
+    k[0, :, 3] = bits * 0.6931 * d ** 0.5 / 4
+    got, want, (_, top) = scales_case(d, k, v, q)
+    for h in range(4):
+        assert np.linalg.norm(got[h] - want[h]) <= 3e-5 * np.linalg.norm(want[h]) + 2 * (n * d) ** 0.5 * 2.0 ** -30 * top * 2 / 3 ** 0.5, h
