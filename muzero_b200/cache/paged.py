@@ -27,7 +27,6 @@ import torch
 from ..kernels._cabi import (MuZeroKernelError, PagedAttentionArgs, PagedCache, check, dtype_code, load_library, on_device, stream_ptr)
 
 PAGE_TOKENS = 64
-_MAX_ROWS_PER_CALL = 1024
 _STATUS = {1: "the pool has too few free pages", 2: "a sequence outgrew its row of the block table", 4: "a row or page index is outside the cache"}
 _ERRORS = sum(_STATUS)                               # the fourth bit says that the newest extension was refused; the device sets and clears it
 

@@ -38,11 +38,6 @@ __device__ __forceinline__ MzpRow mzp_row(uint32_t word) {
   r.z = off ? ((field & 0x8000u) ? 127 : 0) : (int)(field & 0x7Fu);
   return r;
 }
-// its zero level alone
-__device__ __forceinline__ int mzp_zero(uint32_t word) {
-  const uint32_t field = word >> 16;
-  return (field & 0x7FFFu) < 128u ? (int)field : (field & 0x8000u) ? 127 : 0;
-}
 
 // The other way: smallest and largest value of the row (NaN taken as 0, clamped to f16's range) -> constants of the quantizer and the word.  One IEEE
 // operation per step, none contracted: the codes are a definition, not an approximation.
@@ -63,10 +58,5 @@ __device__ __forceinline__ MzpQuant mzp_quant(float lo, float hi) {
   q.inv = tf > 0.0f ? __fdiv_rn(32.0f, tf) : 0.0f;
   q.word = (uint32_t)__half_as_ushort(t) | (off ? bits : (uint32_t)q.z) << 16;
   return q;
-}
-// the level (0..127) nearest x
-__device__ __forceinline__ int mzp_level(const MzpQuant& q, float x) {
-  const float y = __fadd_rn(__fmul_rn(__fsub_rn(x, q.a), q.inv), q.z);
-  return __float2int_rn(fminf(fmaxf(y, 0.0f), 127.0f));
 }
 __device__ __forceinline__ float mzp_finite(float x) { return x != x ? 0.0f : fminf(fmaxf(x, -65504.0f), 65504.0f); }

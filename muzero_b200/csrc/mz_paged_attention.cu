@@ -71,11 +71,6 @@ __device__ __forceinline__ uint4 book128(uint32_t a) {      // constant after th
   asm("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
 // the 64 codes of a row: a whole sector by one thread, read once
 __device__ __forceinline__ void ldg256(uint32_t (&v)[8], const void* p) {
   asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -413,23 +408,23 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
   uint32_t kc[RPT][8], vc[RPT][8], kw[RPT], vw[RPT];         // codes and words of the next step to work on
   // a page that is not there has T = 0
-  auto load_keys = [&](const Step& s, bool words, bool codes) {
+  auto load_keys = [&](const Step& s) {
     const uint8_t* base = store + s.head * PB;
 #pragma unroll
     for (int j = 0; j < RPT; ++j) {
       const int page = (D == 128 ? j : blk) ? s.page1 : s.page0;
       const uint8_t* at = base + (long long)page * c.store_stride_page;
-      if (words) kw[j] = page >= 0 ? __ldg((const uint32_t*)(at + 32 * D + 4 * ch)) : 0u;
-      if (codes && page >= 0) ldg256(kc[j], at + 32 * ch);
+      kw[j] = page >= 0 ? __ldg((const uint32_t*)(at + 32 * D + 4 * ch)) : 0u;
+      if (page >= 0) ldg256(kc[j], at + 32 * ch);
     }
   };
-  auto load_values = [&](const Step& s, bool words, bool codes) {
+  auto load_values = [&](const Step& s) {
     const int page = blk ? s.page1 : s.page0;
     const uint8_t* at = store + s.head * PB + (long long)page * c.store_stride_page + 36 * D;
 #pragma unroll
     for (int j = 0; j < RPT; ++j) {
-      if (words) vw[j] = page >= 0 ? __ldg((const uint32_t*)(at + 32 * D + 4 * (in_page * RPT + j))) : 0u;
-      if (codes && page >= 0) ldg256(vc[j], at + 32 * (in_page * RPT + j));
+      vw[j] = page >= 0 ? __ldg((const uint32_t*)(at + 32 * D + 4 * (in_page * RPT + j))) : 0u;
+      if (page >= 0) ldg256(vc[j], at + 32 * (in_page * RPT + j));
     }
   };
   // the largest T of a step's rows scales its fixed point
@@ -447,8 +442,8 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
     for (int k = 0; k < 8; ++k) kc[j][k] = vc[j][k] = 0;
   {
     const Step s = x.step[0];
-    load_keys(s, true, true);
-    load_values(s, true, true);
+    load_keys(s);
+    load_values(s);
   }
   const uint64_t ka = descriptor(sbase + S::K_A, S::CHUNK), kb = descriptor(sbase + S::K_B, S::CHUNK);
   const uint64_t va = descriptor(sbase + S::V_A, S::CHUNK), vb = descriptor(sbase + S::V_B, S::CHUNK);
@@ -590,7 +585,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
     }
     if (warp == 0 && (it & 15) == 0 && it > 0) plan(it + 16);
     const Step next = x.step[(it + 1) & 31];     // beyond the CTA's last step: pages that are not there, or a step that nobody takes
-    if (it + 1 < n) load_keys(next, true, true);
+    if (it + 1 < n) load_keys(next);
     // ---- values: the output so far, then levels while the products of the keys run
     if (it > 0 && !fresh) take_output(it - 1);
     const float up = pow2(30 - ev);
@@ -602,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
       cz[j] = fmaf(row.t, (float)row.z * -0.03125f, row.a);
       expand_row(vc[j], book128(sbook + row.z * 16), sbase + S::V_A + (D == 128 ? j : blk) * 4 * S::CHUNK + (D == 128 ? r : in_page) * 16, S::CHUNK);
     }
-    if (it + 1 < n) load_values(next, true, true);
+    if (it + 1 < n) load_values(next);
     // ---- logits
     float base[NR];
     if (D == 128) {
