@@ -712,9 +712,9 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
 // One pair per CTA of eight warps; 26 us alone for 512 pairs of 128 ring tokens (36 MB; it waits for loads), of which 13 us show behind the first kernel.  Rings: a warp takes 16 tokens at a time, and (D = 128) 64 of the channels of the output; A = keys [token][channel],
 // B = queries; A = values [channel][token], B = p in parts of 16 bits, as many as fp32 has bits.  Products go to fresh accumulators that are added in round-to-nearest:
 // the tensor cores truncate their running sums.  Then a thread has a channel, and every second query row.
-constexpr int END_THREADS = 256;
+constexpr int END_THREADS = 256;                 // two CTAs to an SM; three have 80 registers, which spill: 64 x 8 x 4224 tokens 129 instead of 123 us
 template <int D, bool BF, int NR>
-__global__ void __launch_bounds__(END_THREADS, 3) finish_kernel(const Args p) {
+__global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
   constexpr int HALVES = D / 64, STREAMS = 8 / HALVES, GROUPS = END_THREADS / D, ROWS = NR / GROUPS;      // D = 64: four groups
   __shared__ float s_part[STREAMS][NR][D], s_m[STREAMS][NR], s_l[STREAMS][NR];
   const mz_paged_cache& c = p.c;
