@@ -5,7 +5,8 @@
 A stack of attention layers with random projections stands in for a model.  A common prefix is written once and forked into every request's row (pages are
 shared, only the 16-bit window is copied); requests bring prompts of their own, decode until they are done, and make room for the next ones; one
 in eight branches into two continuations half way.  A decode step (extend, then append and attend per layer) is captured once in a CUDA graph:
-lengths and pages live on the device.  At the end one sequence's attention is checked against dense attention over what its pages hold.
+lengths and pages live on the device.  The first sequence that ends, the first branch that does and the prefix are checked in every layer: their attention against dense
+attention over what their pages hold, and of the first one what its pages hold against the keys that were written.
 """
 from __future__ import annotations
 
@@ -67,7 +68,8 @@ def main(argv=None) -> dict:
     cache = MuZeroPagedCache.allocate(layers=a.layers, kv_heads=kv_heads, head_dim=dim, pages=pages, rows=a.rows + 1, max_length=longest, residual_length=residual)
     home = a.rows
     index = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
-    prefill(cache, layers, torch.randn(a.prefix, hidden, device="cuda", generator=gen).bfloat16(), index(home), [a.prefix])
+    history = [torch.randn(a.prefix, hidden, device="cuda", generator=gen).bfloat16()]      # what the first request's row is given, in the end
+    prefill(cache, layers, history[0], index(home), [a.prefix])
 
     left = [0] * a.rows                                   # tokens that a row still has to decode; 0: the row is free
     x = torch.zeros(a.rows, hidden, device="cuda", dtype=torch.bfloat16)
@@ -79,7 +81,10 @@ def main(argv=None) -> dict:
         if new:
             cache.fork(index(*[home] * len(new)), index(*new))
             lengths = [rng.randint(1, 512) for _ in new]
-            prefill(cache, layers, torch.randn(sum(lengths), hidden, device="cuda", generator=gen).bfloat16(), index(*new), lengths)
+            prompts = torch.randn(sum(lengths), hidden, device="cuda", generator=gen).bfloat16()
+            prefill(cache, layers, prompts, index(*new), lengths)
+            if len(history) == 1:
+                history.append(prompts[:lengths[0]])      # the first request has row 0
             for r in new:
                 left[r] = a.new_tokens - rng.randint(0, a.new_tokens // 2)
         return len(new)
@@ -110,10 +115,24 @@ def main(argv=None) -> dict:
     with torch.cuda.graph(graph, stream=side):
         y = step()
 
+    def dense_error(row: int) -> float:
+        """The largest error, over the layers, of a row's attention against dense attention over what its pages and ring hold."""
+        q, worst = torch.randn(1, heads, dim, device="cuda", generator=gen).bfloat16(), 0.0
+        for layer in range(a.layers):
+            got = cache.attend(layer, q, rows=index(row)).float()
+            k, v = read_row(cache, layer, row)
+            s = torch.einsum("hd,thd->ht", q[0].float(), k.repeat_interleave(heads // kv_heads, 1)) * dim ** -0.5
+            want = torch.einsum("ht,thd->hd", torch.softmax(s, -1), v.repeat_interleave(heads // kv_heads, 1))
+            worst = max(worst, float((got[0] - want).norm() / want.norm()))
+        return worst
+
+    errors, branches, held = {}, [], None
     done = branched = decoded = moved = 0
     torch.cuda.synchronize()
     began = time.perf_counter()
     while any(left):
+        if held is None:
+            history.append(x[:1].clone())
         graph.replay()
         x.copy_(torch.nn.functional.normalize(y.float(), dim=-1).mul_(hidden ** 0.5))      # the next token's embedding
         ended = []
@@ -125,6 +144,18 @@ def main(argv=None) -> dict:
                     ended.append(r)
         if ended:
             done += len(ended)
+            first, branch = held is None and 0 in ended, "branch" not in errors and set(branches) & set(ended)
+            if first or branch:
+                torch.cuda.synchronize()
+                paused = time.perf_counter()
+                if first:
+                    errors["first"] = dense_error(0)
+                    _, key, _ = layers[0].project(torch.cat(history))
+                    held = float((read_row(cache, 0, 0)[0] - key.float()).norm() / key.float().norm())
+                if branch:
+                    errors["branch"] = dense_error(min(branch))
+                began += time.perf_counter() - paused
+            branches = [r for r in branches if r not in ended]
             cache.free(index(*ended))
             waiting -= admit(waiting)
             idle = [r for r in range(a.rows) if left[r] == 0]
@@ -134,6 +165,7 @@ def main(argv=None) -> dict:
                     cache.fork(index(running[0]), index(idle[0]))
                     x[idle[0]] = x[running[0]] + 0.1 * torch.randn(hidden, device="cuda", generator=gen).bfloat16()
                     left[idle[0]] = left[running[0]]
+                    branches.append(idle[0])
                     branched += 1
                     idle = idle[1:]
                 if idle:
@@ -145,15 +177,10 @@ def main(argv=None) -> dict:
     seconds = time.perf_counter() - began
     cache.check()
 
-    # one row against dense attention over what its pages and ring hold
-    q = torch.randn(1, heads, dim, device="cuda", generator=gen).bfloat16()
-    got = cache.attend(0, q, rows=index(home)).float()
-    k, v = read_row(cache, 0, home)
-    s = torch.einsum("hd,thd->ht", q[0].float(), k.repeat_interleave(heads // kv_heads, 1)) * dim ** -0.5
-    want = torch.einsum("ht,thd->hd", torch.softmax(s, -1), v.repeat_interleave(heads // kv_heads, 1))
-    err = float((got[0] - want).norm() / want.norm())
+    errors["prefix"] = dense_error(home)
     out = {"requests": done, "branches": branched, "compactions": moved, "tokens": decoded, "seconds": round(seconds, 3),
-           "tokens_per_s": round(decoded / seconds, 1), "free_pages": cache.free_pages(), "pages": pages, "error": err}
+           "tokens_per_s": round(decoded / seconds, 1), "free_pages": cache.free_pages(), "pages": pages,
+           "error": max(errors.values()), "errors": errors, "held": held}
     print(out)
     return out
 

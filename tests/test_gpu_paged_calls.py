@@ -80,3 +80,16 @@ def test_a_bound_on_new_tokens_may_be_any(most):
     cache.check()
     assert_row(cache, 0, k[:300], v[:300])
     assert_row(cache, 1, k[300:], v[300:])
+
+
+def test_the_example_checks_rows_that_were_decoded():
+    """The serving example checks a decoded row, a branch and the prefix in every layer (bf16 output), and a row's keys against those that were written (error of
+    the 4-bit codec on normal rows: 0.085)."""
+    import importlib.util
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_serving.py")
+    spec = importlib.util.spec_from_file_location("paged_serving", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    out = m.main(["--layers", "3", "--rows", "8", "--prefix", "500", "--requests", "40", "--new-tokens", "96", "--seed", "1"])
+    assert out["branches"] > 0 and set(out["errors"]) == {"first", "branch", "prefix"}
+    assert max(out["errors"].values()) <= 2.0 ** -8 and 0.0 < out["held"] <= 0.1
