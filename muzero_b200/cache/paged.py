@@ -141,7 +141,8 @@ class MuZeroPagedCache:
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, *, rows: Optional[torch.Tensor] = None,
                offsets: Optional[torch.Tensor] = None, max_new: Optional[int] = None) -> None:
         """Writes the announced tokens of one layer: ``key`` and ``value`` [tokens, kv_heads, head_dim], entry after entry.  ``max_new``: the most
-        tokens that an entry brings, if the host knows it (else all might be one entry's)."""
+        tokens that an entry brings, if the host knows it.  Without it all might be one entry's, and the grid grows with entries times tokens: 64 prompts of 1000 tokens take
+        943 instead of 138 us, 16 of 1777 150 instead of 71, one of 4096 the same 28 (8 kv heads, head_dim 128)."""
         n = self._entries(rows, offsets)
         r, o = _index(rows, "rows", self.device), _index(offsets, "offsets", self.device, n + 1)
         shape = (key.shape[0], self.kv_heads, self.head_dim)

@@ -12,7 +12,7 @@ constexpr int MZP_BOOKS = 128, MZP_LEVELS = 16;
 // Rows of the device's table of nearest levels: entries -1 .. 128 (a value may round to a level beyond the ends), padded so that rows start at different banks
 constexpr int MZP_NEAR_ROW = 132;
 
-// device copies of the two tables of mz_paged_books, the second in rows of MZP_NEAR_ROW (static device memory, filled on the first call on a device)
+// device copies of the two tables of mz_paged_books, the second in rows of MZP_NEAR_ROW (static device memory, filled and waited for by mz_paged_prepare, or by the first call on a device)
 int mz_paged_tables(const uint8_t** book, const uint8_t** nearest);
 // multiprocessors of the current device (asked once)
 int mz_paged_sms(int* sms);

