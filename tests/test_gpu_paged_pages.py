@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import paged_plain as plain
-from test_gpu_paged import f32, fill, ints, make
+from test_gpu_paged import DT, check_attention, f32, fill, ints, make
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +105,13 @@ def test_a_token_that_takes_nearly_all(bits):
     got, want, (_, top) = scales_case(d, k, v, q)
     for h in range(4):
         assert np.linalg.norm(got[h] - want[h]) <= 3e-5 * np.linalg.norm(want[h]) + 2 * (n * d) ** 0.5 * 2.0 ** -30 * top * 2 / 3 ** 0.5, h
+
+
+@pytest.mark.parametrize("d, dt, kvh, hq, residual, lq", [(128, "bf16", 1, 3, 0, 130), (64, "fp16", 2, 4, 64, 77), (128, "bf16", 2, 8, 128, 33), (64, "bf16", 1, 8, 0, 64)])
+def test_a_block_of_new_tokens(d, dt, kvh, hq, residual, lq):
+    """As many query tokens as a short prompt has: their own tokens stand in pages and in the window, some rows are shorter than the block."""
+    lengths = [lq + 200, lq, lq - 20, 1, 0, 300]
+    cache = make(len(lengths), kvh, d, dt, residual)
+    kv = fill(cache, lengths, 1, seed=lq)
+    q = torch.randn(len(lengths), lq, hq, d, generator=torch.Generator().manual_seed(hq)).to(DT[dt]).cuda()
+    check_attention(cache, kv, q, list(range(len(lengths))))
