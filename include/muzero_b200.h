@@ -446,6 +446,39 @@ size_t mz_paged_attention_workspace_bytes(const mz_paged_cache* cache, int batch
 int mz_paged_attention(const mz_paged_cache* cache, int layer, const mz_paged_attention_args* args, void* stream);
 
 /*
+ * The same over a part of the tokens, or with what rows have in common taken once:
+ *   window > 0   a query sees its own token, the window - 1 tokens before it, and the row's first `sinks` tokens.  Pages that no query sees are not read.
+ *   n_groups > 0 the list entries groups[g] .. groups[g+1] - 1 (ascending, device memory, n_groups + 1 numbers, at most 1024 groups) are a group.  The pages that the tables of all
+ *                its rows begin with, as far as every query sees them whole, are found on the device, read once, and taken by one matrix product for all rows of
+ *                the group.  The result is that of mz_paged_attention but for rounding: keys are taken with 22 bits, probabilities and values with 11, sums with 24 (about 2e-4
+ *                of the output).  Entries that no group has, groups of one, and rows without a common page go as they do there.  Numbers that do not ascend from 0
+ *                or more to `batch` or less share nothing and set MZ_PAGED_BAD_INDEX.
+ * Not both.  workspace: mz_paged_attention_view_workspace_bytes() bytes (NULL view: those of mz_paged_attention), 32-byte aligned with groups.
+ */
+typedef struct {
+  int window, sinks;
+  const int* groups;
+  int n_groups;
+} mz_paged_view;
+size_t mz_paged_attention_view_workspace_bytes(const mz_paged_cache* cache, const mz_paged_view* view, int batch, int q_len, int q_heads);
+int mz_paged_attention_view(const mz_paged_cache* cache, int layer, const mz_paged_attention_args* args, const mz_paged_view* view, void* stream);
+
+/*
+ * Tokens back as ordinary keys and values: entry i's places offsets[i] .. offsets[i+1] - 1 of key and value get the tokens first[i], first[i] + 1, ... (NULL: from
+ * 0) of row rows[i] (NULL: row i), as their codes stand for them, rounded once and held to the type's finite range.  Tokens that a row does not have are zero; places that no
+ * entry has, or at or beyond `tokens`, are left as they are.  Rows may be repeated.  batch <= 4096.
+ * Replaces: the range dequantizer of muzero/cache/layer.py:303-345 for the paged cache.
+ */
+typedef struct {
+  void *key, *value;                                 /* [tokens][kv_heads][head_dim], 16-byte aligned */
+  int dtype;                                         /* the cache's, or fp32 */
+  long long k_stride_token, k_stride_head, v_stride_token, v_stride_head;      /* elements, multiples of 16 bytes */
+  const int *rows, *offsets, *first;
+  int batch, tokens;
+} mz_paged_read_args;
+int mz_paged_read(const mz_paged_cache* cache, int layer, const mz_paged_read_args* args, void* stream);
+
+/*
  * Row target[i] becomes a copy of row source[i], in all layers: what it held is released, the source's pages are shared (counted), its ring is
  * copied as far as it is live.  Targets are distinct and no row is both.
  */

@@ -24,7 +24,7 @@ from typing import Optional
 
 import torch
 
-from ..kernels._cabi import (MuZeroKernelError, PagedAttentionArgs, PagedCache, check, dtype_code, load_library, on_device, stream_ptr)
+from ..kernels._cabi import (MuZeroKernelError, PagedAttentionArgs, PagedCache, PagedReadArgs, PagedView, check, dtype_code, load_library, on_device, stream_ptr)
 
 PAGE_TOKENS = 64
 _STATUS = {1: "the pool has too few free pages", 2: "a sequence outgrew its row of the block table", 4: "a row or page index is outside the cache"}
@@ -172,13 +172,23 @@ class MuZeroPagedCache:
         return held[-1]
 
     def attend(self, layer: int, query: torch.Tensor, *, rows: Optional[torch.Tensor] = None, scaling: Optional[float] = None,
-               out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+               out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, window: Optional[int] = None, sinks: int = 0,
+               groups: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of the rows' newest tokens, already appended: ``query`` [batch, q_len, q_heads, head_dim] or [batch, q_heads, head_dim] (one
-        token), query l of a row being its (length - q_len + l)-th token.  Each sees the tokens up to its own.  Returns the query's shape."""
+        token), query l of a row being its (length - q_len + l)-th token.  Each sees the tokens up to its own.  Returns the query's shape.
+
+        ``window``: each sees its own token and the ``window - 1`` before it, and the row's first ``sinks`` tokens; other pages are not read.
+
+        ``groups``: int32 offsets into the batch, ``groups[g]`` to ``groups[g+1]`` being a group of entries whose rows begin with the same pages (forks of a
+        prompt, say).  What they have in common is found on the device and taken once for all of them, as one matrix product: the same result, rounded
+        otherwise (2e-4 of the output).  Entries outside all groups are attended as without.  Not together with ``window``."""
         q = query if query.dim() == 4 else query.unsqueeze(1)
         if q.dim() != 4 or q.shape[3] != self.head_dim or q.dtype != self.dtype or q.device != self.device:
             raise ValueError(f"`query` must be {self.dtype} [batch, (q_len,) q_heads, {self.head_dim}] on {self.device}, got {query.dtype} "
                              f"{tuple(query.shape)} on {query.device}")
+        view = None
+        if window is not None or groups is not None or sinks:
+            view = self._view(window, sinks, groups)
         # rows of whole 16-byte pieces; anything else is laid out once
         if q.stride(3) != 1 or (q.stride(0) | q.stride(1) | q.stride(2)) & 7 or q.data_ptr() & 15:
             q = q.clone(memory_format=torch.contiguous_format)
@@ -188,15 +198,61 @@ class MuZeroPagedCache:
         elif out.shape != query.shape or not out.is_contiguous() or out.device != self.device or (out_dtype or out.dtype) != out.dtype:
             raise ValueError("`out` must be a contiguous tensor of the query's shape on the cache's device")
         st = stream_ptr(self.device)
-        need = self._needs.get((b, lq, hq))
+        key = (b, lq, hq) if view is None else (b, lq, hq, view.window, view.sinks, view.n_groups)
+        need = self._needs.get(key)
         if need is None:                                  # 0: a shape that the call below refuses with its reason
-            need = self._needs[b, lq, hq] = on_device(self.device, self._lib.mz_paged_attention_workspace_bytes, self._ref, b, lq, hq)
+            if view is None:
+                need = on_device(self.device, self._lib.mz_paged_attention_workspace_bytes, self._ref, b, lq, hq)
+            else:
+                need = on_device(self.device, self._lib.mz_paged_attention_view_workspace_bytes, self._ref, ctypes.byref(view), b, lq, hq)
+            self._needs[key] = need
         ws = self._workspace(need, st)
         # a block per call: another thread may attend another layer meanwhile
         a = PagedAttentionArgs(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), b, lq, hq, _index(rows, "rows", self.device, b),
                                self.head_dim ** -0.5 if scaling is None else scaling, out.data_ptr(), dtype_code(out.dtype), ws[0], ws[1])
-        check(on_device(self.device, self._lib.mz_paged_attention, self._ref, layer, ctypes.byref(a), st), "mz_paged_attention")
+        if view is None:
+            check(on_device(self.device, self._lib.mz_paged_attention, self._ref, layer, ctypes.byref(a), st), "mz_paged_attention")
+        else:
+            check(on_device(self.device, self._lib.mz_paged_attention_view, self._ref, layer, ctypes.byref(a), ctypes.byref(view), st), "mz_paged_attention_view")
         return out
+
+    def _view(self, window, sinks, groups) -> PagedView:
+        if window is not None and window < 1:
+            raise ValueError(f"`window` must be at least 1 (a query sees its own token), got {window}")
+        if sinks < 0 or (sinks and window is None):
+            raise ValueError(f"`sinks` counts a row's first tokens that stay in sight beside a `window`, got {sinks} with window {window}")
+        if groups is not None and window is not None:
+            raise ValueError("`groups` is for calls without a `window`, which bounds what a row reads")
+        top = 0x7fffffff
+        at = _index(groups, "groups", self.device)
+        if groups is not None and groups.shape[0] < 1:
+            raise ValueError("`groups` holds offsets: one more than there are groups")
+        return PagedView(min(window, top) if window else 0, min(sinks, top), at, 0 if groups is None else groups.shape[0] - 1)
+
+    def read(self, layer: int, *, offsets: torch.Tensor, rows: Optional[torch.Tensor] = None, first: Optional[torch.Tensor] = None,
+             tokens: Optional[int] = None, out: Optional[tuple] = None, out_dtype: Optional[torch.dtype] = None) -> tuple:
+        """Tokens of rows as ordinary keys and values [tokens, kv_heads, head_dim], what their codes stand for: places ``offsets[i]`` to ``offsets[i+1]`` get the
+        tokens from ``first[i]`` on (from 0 without ``first``) of row ``rows[i]`` (row i without ``rows``).  Tokens that a row does not have read as zero, so equal steps
+        of ``offsets`` give a padded batch.  ``tokens``: places in all, which the host has to know; or ``out``: the two tensors to write, of any
+        strides with whole 16-byte pieces.  Places that no entry has are left as they are.  ``out_dtype``: the cache's type, or float32."""
+        n = self._entries(rows, offsets)
+        if out is None:
+            if tokens is None:
+                raise ValueError("`tokens` or `out` says how many places there are")
+            shape = (tokens, self.kv_heads, self.head_dim)
+            out = tuple(torch.empty(shape, dtype=out_dtype or self.dtype, device=self.device) for _ in range(2))
+        k, v = out
+        for name, t in (("key", k), ("value", v)):
+            whole = 16 // t.element_size() - 1
+            if (t.dim() != 3 or tuple(t.shape[1:]) != (self.kv_heads, self.head_dim) or t.shape[0] != k.shape[0] or t.dtype != k.dtype or t.device != self.device
+                    or (out_dtype or t.dtype) != t.dtype or (tokens is not None and tokens != t.shape[0])):
+                raise ValueError(f"`out` must be two tensors [tokens, {self.kv_heads}, {self.head_dim}] of one type on {self.device}, the {name}s are {t.dtype} {tuple(t.shape)} on {t.device}")
+            if t.numel() and (t.stride(2) != 1 or (t.stride(0) | t.stride(1)) & whole or t.data_ptr() & 15):
+                raise ValueError(f"`out` must have rows of whole 16-byte pieces, the {name}s' strides are {t.stride()}")
+        a = PagedReadArgs(k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _index(rows, "rows", self.device),
+                          _index(offsets, "offsets", self.device, n + 1), _index(first, "first", self.device, n), n, k.shape[0])
+        check(on_device(self.device, self._lib.mz_paged_read, self._ref, layer, ctypes.byref(a), stream_ptr(self.device)), "mz_paged_read")
+        return k, v
 
     # ---- rows and pages
     def fork(self, source: torch.Tensor, target: torch.Tensor) -> None:

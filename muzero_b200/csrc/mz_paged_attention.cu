@@ -29,12 +29,10 @@
 #include <algorithm>
 #include <atomic>
 
-#include "mz_paged.cuh"
+#include "mz_paged_prefix.cuh"
 
 namespace mzp {
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr int THREADS = 128, MAX_BATCH = 1024;
-constexpr int SPIN_LIMIT = 1000000;              // looks of a wait before it gives up
 constexpr int STEP = 2 * MZP_PAGE;
 struct Args {
   mz_paged_cache c;
@@ -53,57 +51,30 @@ struct Args {
   float* acc;                                    // [slot][NR][D]
   long long pairs, slots;
   int fail_waits;                                // checked build: not 0 = waits run out at once
+  // a view (kernels with VIEW): either a window and sinks, or what rows share is taken elsewhere and its records are merged
+  int window, sinks;
+  MzpPrefix pre;                                 // pre.skip NULL: a window
 };
 
-// ---- small wrappers
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
-  uint32_t d;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(s));
-  return d;
-}
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ uint32_t warp_max_u32(uint32_t v) { uint32_t r; asm("redux.sync.max.u32 %0, %1, 0xffffffff;" : "=r"(r) : "r"(v)); return r; }
-__device__ __forceinline__ float warp_max(float v) { float r; asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
-__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-__device__ __forceinline__ uint4 book128(uint32_t a) {      // constant after the set-up
-  uint4 v;
-  asm("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-// the 64 codes of a row: a whole sector by one thread, read once
-__device__ __forceinline__ void ldg256(uint32_t (&v)[8], const void* p) {
-  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "l"(p));
-}
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void fence_operands() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n) : "memory"); }
-__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}\n"
-               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-  return done != 0;
-}
-// Waits for the phase of this parity.  Who gives up says so before it goes on; the others notice.
-__device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile int* s_failed) {
-#ifdef MZ_BOUNDS
-  if (*s_failed) return;                         // a test makes every wait run out
-#endif
-  for (int it = 0; it < SPIN_LIMIT; ++it) {
-    if (bar_test(bar, parity)) return;
-    if ((it & 63) == 63 && *s_failed) return;
+// The pages of a list entry that a pass goes through: `heads` of its first ones (sinks), then those from `first` on
+struct Reach { int count, heads, first; };
+template <bool VIEW>
+__device__ __forceinline__ Reach reach_of(const Args& p, int b, int len) {
+  const int pages = mzp_packed(len, p.c.residual) / MZP_PAGE;
+  if (!VIEW) return {pages, 0, 0};
+  Reach x;
+  if (p.pre.skip) {
+    x.heads = 0;
+    x.first = min(p.pre.skip[b], pages);
+  } else {
+    const int lo = len - p.q_len + 1 - p.window;           // the first query's window begins here
+    x.heads = min((int)(((long long)p.sinks + MZP_PAGE - 1) / MZP_PAGE), pages);
+    x.first = min(max(max(lo, 0) / MZP_PAGE, x.heads), pages);
   }
-  *s_failed = 1;
+  x.count = x.heads + pages - x.first;
+  return x;
 }
-// shared-memory operand, not swizzled, major along the kept dimension: cores of 8 rows x 16 bytes, 128 bytes apart along the reduction,
-// `chunk` bytes apart along the kept dimension
-__device__ __forceinline__ uint64_t descriptor(uint32_t sa, uint32_t chunk) {
-  return (uint64_t)((sa >> 4) & 0x3FFF) | (128ull >> 4) << 16 | (uint64_t)(chunk >> 4) << 32 | 1ull << 46;
-}
+
 // D[128 x N] (+)= A[128 x 32] * B[32 x N], unsigned times signed or unsigned bytes into 32 bits
 template <int N, bool SIGNED_B>
 __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t accumulate) {
@@ -113,9 +84,6 @@ __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a, uint64_t b, ui
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n"
       ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(zero), "r"(zero), "r"(zero), "r"(zero) : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tm_ld16(uint32_t taddr, int* c) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -131,16 +99,7 @@ __device__ __forceinline__ void tm_ld16(uint32_t taddr, int* c) {
 __device__ __forceinline__ float number_of(const int* c) { return fmaf((float)(c[2] + (c[3] << 8)), 65536.0f, (float)(c[0] + (c[1] << 8))); }
 // 31-bit fixed point -> four signed bytes.  (A number that is not negative stands for its four unsigned bytes as it is.)
 __device__ __forceinline__ uint32_t digits_of(float x) { return ((uint32_t)__float2int_rn(x) + 0x808080u) ^ 0x808080u; }
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
 
-// pairs of fp32 operations
-__device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
-  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
-}
-__device__ __forceinline__ void fma2(float& c0, float& c1, float a0, float a1, float f) {      // c += a * f
-  asm("{\n\t.reg .b64 a, c, f;\n\tmov.b64 c, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\tmov.b64 f, {%4, %4};\n\tfma.rn.f32x2 c, a, f, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
-      : "+f"(c0), "+f"(c1) : "f"(a0), "f"(a1), "f"(f));
-}
 // r = (a * f + b) * c
 __device__ __forceinline__ void mul_add2(float& r0, float& r1, float a0, float a1, float b0, float b1, float c0, float c1, float f) {
   asm("{\n\t.reg .b64 a, b, c, f;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tmov.b64 f, {%8, %8};\n\t"
@@ -227,10 +186,15 @@ struct Smem {
 };
 // a step of the line: its pages (-1: not there), pair, list entry, kv head, first query row, tokens, last position that the first query token sees
 struct Step { int page0, page1, pair, head, b, r0, count, see; };
+// the same of a view; `see` < 0: some query of the pass does not see some token.  rel: a page's first token after the position of the row's first query token;
+// sink: how many of a page's tokens every query sees that stands behind them
+struct ViewStep : Step { int rel0, rel1, sink0, sink1; };
+template <bool VIEW> struct StepOf { using T = Step; };
+template <> struct StepOf<true> { using T = ViewStep; };
 // exchange between the warps of a CTA
-template <int NR>
+template <int NR, bool VIEW>
 struct Exchange {
-  alignas(16) Step step[32];                // two blocks of 16 of the CTA's steps; one warp fills a block while the other is worked on
+  alignas(16) typename StepOf<VIEW>::T step[32];                // two blocks of 16 of the CTA's steps; one warp fills a block while the other is worked on
   alignas(16) float base[4][2 * NR];        // constant terms of the logits, by warp
   alignas(16) float fin[4][4 * NR];         // end of a pair: sums of p, constant terms of the output
   alignas(16) float vmax[4][NR];            // largest logit, by warp
@@ -285,15 +249,16 @@ __device__ __forceinline__ int length_of(const Args& p, int b, int& row) {
   return row < 0 || row >= p.c.rows ? 0 : max(0, min(p.c.lengths[row], p.longest));
 }
 
-template <int D, bool BF, int NR>
+template <int D, bool BF, int NR, bool VIEW>
 __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel(const Args p, const uint8_t* __restrict__ book_table) {
   using S = Smem<D, NR>;
+  using StepT = typename StepOf<VIEW>::T;
   constexpr int DT = BF ? MZ_BF16 : MZ_F16;
   constexpr int PB = 72 * D;                     // page bytes per kv head
   constexpr int RPT = D / 64;                    // rows of codes per thread, side and step
   extern __shared__ uint8_t window[];
   uint8_t* smem = window + (S::ALIGN - smem_u32(window) % S::ALIGN) % S::ALIGN;
-  __shared__ Exchange<NR> x;
+  __shared__ Exchange<NR, VIEW> x;
   const mz_paged_cache& c = p.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t sbase = smem_u32(smem), sbook = sbase + S::BOOK;
@@ -311,7 +276,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   const int kp_all = c.kv_heads * p.passes, G = gridDim.x, cta = blockIdx.x;
   auto steps_of = [&](int b, int& row, int& len) {
     len = length_of(p, b, row);
-    return (mzp_packed(len, c.residual) + STEP - 1) / STEP;
+    return (reach_of<VIEW>(p, b, len).count + 1) / 2;
   };
   int total = 0;
   for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
@@ -362,7 +327,8 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
     const int it = at + lane;
     const long long f = f0 + it;
     bool open = lane < 16 && it < n;
-    Step s = {-1, -1, 0, 0, 0, 0, 0, 0};
+    StepT s = {};
+    s.page0 = s.page1 = -1;
     int before = x.before;
     for (int b0 = x.first; b0 < p.batch && __any_sync(0xffffffffu, open); b0 += 32) {
       int row = 0, len = 0;
@@ -379,19 +345,31 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
       const int its_len = __shfl_sync(0xffffffffu, len, k);
       if (open && f < (long long)before * kp_all) {
         open = false;
-        const int rem = (int)(f - (long long)first * kp_all), kp = rem / steps, step = rem - kp * steps, pages = mzp_packed(its_len, c.residual) / MZP_PAGE;
+        const int rem = (int)(f - (long long)first * kp_all), kp = rem / steps, step = rem - kp * steps;
         s.b = b0 + k;
+        const Reach reach = reach_of<VIEW>(p, s.b, its_len);
+        const int pages = reach.count;
         s.pair = s.b * kp_all + kp;
         s.head = kp / p.passes;
         s.r0 = (kp - s.head * p.passes) * NR;
         s.count = min(STEP, pages * MZP_PAGE - step * STEP);
-        s.see = its_len - p.q_len + s.r0 / p.group - step * STEP;
+        if (!VIEW) s.see = its_len - p.q_len + s.r0 / p.group - step * STEP;
         int id[2];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           id[w] = -1;
           if (2 * step + w < pages) {
-            id[w] = 2 * step + w < c.width ? c.block_table[(long long)its_row * c.width + 2 * step + w] : -1;
+            int at = 2 * step + w;               // the page's place in the table's row
+            if (VIEW && at >= reach.heads) at += reach.first - reach.heads;
+            if constexpr (VIEW) {
+              const int rel = at * MZP_PAGE - (its_len - p.q_len), sink = at < reach.heads ? min(p.sinks - at * MZP_PAGE, MZP_PAGE) : 0;
+              (w ? s.rel1 : s.rel0) = rel;
+              (w ? s.sink1 : s.sink0) = sink;
+              const int l0 = s.r0 / p.group, l1 = (min(s.r0 + NR, p.qrows) - 1) / p.group;
+              if (w == 0) s.see = 0;
+              if (rel + MZP_PAGE - 1 > l0 || (rel <= l1 - p.window && sink < MZP_PAGE)) s.see = -1;
+            }
+            id[w] = at < c.width ? c.block_table[(long long)its_row * c.width + at] : -1;
             if (id[w] < 0 || id[w] >= c.pages) { id[w] = -1; atomicOr(c.status, MZ_PAGED_BAD_INDEX); }
           }
         }
@@ -409,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
   uint32_t kc[RPT][8], vc[RPT][8], kw[RPT], vw[RPT];         // codes and words of the next step to work on
   // a page that is not there has T = 0
-  auto load_keys = [&](const Step& s) {
+  auto load_keys = [&](const StepT& s) {
     const uint8_t* base = store + s.head * PB;
 #pragma unroll
     for (int j = 0; j < RPT; ++j) {
@@ -419,7 +397,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
       if (page >= 0) ldg256(kc[j], at + 32 * ch);
     }
   };
-  auto load_values = [&](const Step& s) {
+  auto load_values = [&](const StepT& s) {
     const int page = blk ? s.page1 : s.page0;
     const uint8_t* at = store + s.head * PB + (long long)page * c.store_stride_page + 36 * D;
 #pragma unroll
@@ -442,7 +420,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
 #pragma unroll
     for (int k = 0; k < 8; ++k) kc[j][k] = vc[j][k] = 0;
   {
-    const Step s = x.step[0];
+    const StepT s = x.step[0];
     load_keys(s);
     load_values(s);
   }
@@ -515,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
   publish(0);
   __syncthreads();
   for (int it = 0; it < n; ++it) {
-    const Step s = x.step[it & 31];
+    const StepT s = x.step[it & 31];
     const bool fresh = s.pair != pair;
     if (fresh) {
       if (pair >= 0) {
@@ -585,7 +563,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
       umma_commit(k_done);
     }
     if (warp == 0 && (it & 15) == 0 && it > 0) plan(it + 16);
-    const Step next = x.step[(it + 1) & 31];     // beyond the CTA's last step: pages that are not there, or a step that nobody takes
+    const StepT next = x.step[(it + 1) & 31];     // beyond the CTA's last step: pages that are not there, or a step that nobody takes
     if (it + 1 < n) load_keys(next);
     // ---- values: the output so far, then levels while the products of the keys run
     if (it > 0 && !fresh) take_output(it - 1);
@@ -631,7 +609,17 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
 #pragma unroll
       for (int i = 0; i < NR; ++i) if (r >= s.count) w[i] = -INFINITY;
     }
-    if (s.see < s.count - 1) {                               // not every query sees all of the step
+    if constexpr (VIEW) {
+      if (s.see < 0) {
+        const int at = (blk ? s.rel1 : s.rel0) + in_page;    // behind the row's first query token
+        const bool sink = in_page < (blk ? s.sink1 : s.sink0);
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+          const int l = (s.r0 + i) / p.group;
+          if (at > l || (at <= l - p.window && !sink)) w[i] = -INFINITY;
+        }
+      }
+    } else if (s.see < s.count - 1) {                        // not every query sees all of the step
 #pragma unroll
       for (int i = 0; i < NR; ++i) if (r > s.see + (s.r0 + i) / p.group - s.r0 / p.group) w[i] = -INFINITY;
     }
@@ -714,7 +702,7 @@ __global__ void __launch_bounds__(THREADS, (Smem<D, NR>::CTAS)) attention_kernel
 // takes 16 tokens at a time, and (D = 128) 64 of the channels of the output; A = keys [token][channel], B = queries; A = values [channel][token], B = p in parts of 16 bits, as many as fp32 has bits.  Products go to fresh accumulators that are added in round-to-nearest:
 // the tensor cores truncate their running sums.  Then a thread has a channel, and every second query row.
 constexpr int END_THREADS = 256;                 // two CTAs to an SM; three have 80 registers, which spill: 64 x 8 x 4224 tokens 129 instead of 123 us
-template <int D, bool BF, int NR>
+template <int D, bool BF, int NR, bool VIEW>
 __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
   constexpr int HALVES = D / 64, STREAMS = 8 / HALVES, GROUPS = END_THREADS / D, ROWS = NR / GROUPS;      // D = 64: four groups
   __shared__ float s_part[STREAMS][NR][D], s_m[STREAMS][NR], s_l[STREAMS][NR];
@@ -729,6 +717,9 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
   const int half = warp % HALVES, stream = warp / HALVES;
   if (tokens > 0) {
     const int see0 = tokens - p.q_len;           // query token l sees the ring's tokens up to see0 + l
+    // a window: from see0 + l - window + 1 on, and the first `sinks` of them
+    const bool windowed = VIEW && !p.pre.skip;
+    const int low0 = windowed ? see0 - p.window + 1 : -(1 << 30), sinks = windowed ? max(p.sinks - packed, 0) : 0;
     const int l_first = r0 / p.group, l_last = (min(r0 + NR, p.qrows) - 1) / p.group;      // the pass's query tokens
     const uint16_t* ring_k = (const uint16_t*)c.tail + (long long)p.layer * c.tail_stride_layer + (long long)row * c.tail_stride_row + (long long)head * c.ring * D;
     const uint16_t* ring_v = ring_k + (long long)c.kv_heads * c.ring * D + half * 64;
@@ -750,14 +741,15 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
     for (int i0 = stream * 16; i0 < tokens; i0 += STREAMS * 16) {
+      if (VIEW && i0 + 15 < low0 + l_first && i0 >= sinks) continue;       // behind every query's window
       uint4 v[4];
-      // what is not there is read as zero
-      auto load_values = [&](int see) {
+      // what is not there, or not in sight, is read as zero
+      auto load_values = [&](int see, int low) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int i = i0 + 2 * t + (k & 1) + 8 * (k >> 1);
           v[k] = make_uint4(0, 0, 0, 0);
-          if (i <= see) v[k] = *(const uint4*)(ring_v + place(i) + 8 * g);
+          if (i <= see && (!VIEW || i >= low || i < sinks)) v[k] = *(const uint4*)(ring_v + place(i) + 8 * g);
         }
       };
       float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -767,7 +759,7 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
         uint4 va[D / 32], vb[D / 32];
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) { va[k] = *(const uint4*)(ka + 32 * k); vb[k] = *(const uint4*)(kb + 32 * k); }
-        load_values(min(see0 + l_last, tokens - 1));
+        load_values(min(see0 + l_last, tokens - 1), low0 + l_first);
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
           float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
@@ -781,9 +773,14 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
       float fix[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int last = min(see0 + (r0 + 2 * t + j) / p.group, tokens - 1);
-        s[j] = i0 + g <= last ? s[j] * p.scaling : -INFINITY;
-        s[2 + j] = i0 + g + 8 <= last ? s[2 + j] * p.scaling : -INFINITY;
+        const int ql = (r0 + 2 * t + j) / p.group, last = min(see0 + ql, tokens - 1);
+        bool near = i0 + g <= last, far = i0 + g + 8 <= last;
+        if (VIEW) {
+          near = near && (i0 + g >= low0 + ql || i0 + g < sinks);
+          far = far && (i0 + g + 8 >= low0 + ql || i0 + g + 8 < sinks);
+        }
+        s[j] = near ? s[j] * p.scaling : -INFINITY;
+        s[2 + j] = far ? s[2 + j] * p.scaling : -INFINITY;
         float top = fmaxf(s[j], s[2 + j]);
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
@@ -825,9 +822,9 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
       }
       // A token that only later queries see must not bring a NaN to a product with p = 0: what no query of the pass sees is not loaded, and where a tile has
       // tokens that only some of the queries see, each of the queries' tokens takes its turn with what it sees, and only its columns are added
-      const bool apart = i0 + 15 > see0 + l_first && l_last > l_first;
+      const bool apart = (i0 + 15 > see0 + l_first || (VIEW && i0 < low0 + l_last && i0 + 15 >= low0 + l_first)) && l_last > l_first;
       for (int turn = 0; turn <= (apart ? l_last - l_first : 0); ++turn) {
-        if (apart) load_values(min(see0 + l_first + turn, tokens - 1));
+        if (apart) load_values(min(see0 + l_first + turn, tokens - 1), low0 + l_first + turn);
         const bool mine0 = !apart || (r0 + 2 * t) / p.group == l_first + turn, mine1 = !apart || (r0 + 2 * t + 1) / p.group == l_first + turn;
         uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
         uint32_t w2[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
@@ -914,6 +911,39 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
       }
     }
   }
+  if (VIEW && p.pre.skip && p.pre.skip[b] > 0) {             // what the row shares with its group: records of whole tiles of query rows
+    const MzpUnits units(p.pre, b, p.qrows, c.kv_heads);
+    long long slot[ROWS], first[ROWS], last[ROWS], lo = 0x7fffffff, hi = -1;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int qr = r0 + i0 + i * GROUPS;
+      first[i] = 0; last[i] = -1; slot[i] = 0;
+      if (qr < p.qrows) {
+        slot[i] = units.record(head, units.row_of(b, qr), first[i], last[i]);
+        lo = min(lo, first[i]);
+        hi = max(hi, last[i]);
+      }
+    }
+    for (long long c0 = lo; c0 <= hi; c0 += 4) {
+      float2 ml[4][ROWS];
+      float v[4][ROWS];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+          const long long at = slot[i] + MZP_TILE_ROWS * (max(first[i], min(c0 + k, last[i])));
+          ml[k][i] = make_float2(-INFINITY, 0.f);
+          v[k][i] = 0.f;
+          if (last[i] >= 0) { ml[k][i] = p.pre.ml[at]; v[k][i] = p.pre.acc[at * D + d]; }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) if (c0 + k >= first[i] && c0 + k <= last[i]) take(i, ml[k][i], v[k][i]);
+      }
+    }
+  }
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int at = i0 + i * GROUPS, qr = r0 + at;
@@ -929,9 +959,9 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
   }
 }
 
-template <int D, bool BF, int NR>
+template <int D, bool BF, int NR, bool VIEW>
 int launch(const Args& p, const uint8_t* book, int G, cudaStream_t st) {
-  auto kern = attention_kernel<D, BF, NR>;
+  auto kern = attention_kernel<D, BF, NR, VIEW>;
   using S = Smem<D, NR>;
   static std::atomic<unsigned> ready[8];         // a bit per device: its limits are set
   int dev = 0;
@@ -955,13 +985,14 @@ int launch(const Args& p, const uint8_t* book, int G, cudaStream_t st) {
   cfg.stream = st;
   cfg.gridDim = dim3((unsigned)p.pairs);
   cfg.blockDim = dim3(END_THREADS);
-  MZ_CUDA(cudaLaunchKernelEx(&cfg, finish_kernel<D, BF, NR>, p));
+  MZ_CUDA(cudaLaunchKernelEx(&cfg, finish_kernel<D, BF, NR, VIEW>, p));
   MZ_LAUNCH_CHECK("paged attention end");
   return MZ_OK;
 }
 
-struct Shape { int nr, passes, sms, per_sm, G; long long pairs; size_t head_bytes, slots, bytes; };
-int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* s) {
+struct Shape { int nr, passes, sms, per_sm, G; long long pairs; size_t head_bytes, slots, prefix_at, bytes; };
+// pages: the most of a row that a call goes through
+int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, long long pages, Shape* s) {
   MZ_REQUIRE(batch >= 0 && batch <= MAX_BATCH, "batch %d (at most %d)", batch, MAX_BATCH);
   MZ_REQUIRE(q_len >= 1 && q_heads >= 1 && q_heads % c->kv_heads == 0, "q_len %d, q_heads %d of %d kv heads", q_len, q_heads, c->kv_heads);
   const long long qrows = (long long)q_heads / c->kv_heads * q_len;
@@ -980,7 +1011,7 @@ int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* 
   s->G = sms * s->per_sm;
   MZ_REQUIRE((long long)batch * (c->width + 2) <= 1ll << 31, "%d rows of %d pages are too many for one call", batch, c->width);
   // a CTA costs its start (592 of them 6 us): no more than there can be steps
-  const long long most = s->pairs * ((c->width + 1) / 2);
+  const long long most = s->pairs * ((pages + 1) / 2);
   if (s->G > most) s->G = most < 1 ? 1 : (int)most;
   s->head_bytes = ((2 + (size_t)batch) * sizeof(int) + 127) / 128 * 128;
   s->slots = (size_t)s->G + (size_t)s->pairs;
@@ -989,31 +1020,45 @@ int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, Shape* 
 }
 }  // namespace mzp
 
-extern "C" size_t mz_paged_attention_workspace_bytes(const mz_paged_cache* cache, int batch, int q_len, int q_heads) {
-  mzp::Shape s;
-  if (mz_paged_check(cache) != MZ_OK || mzp::shape_of(cache, batch, q_len, q_heads, &s) != MZ_OK) return 0;
-  return s.bytes;
+namespace mzp {
+int shape_of(const mz_paged_cache* c, const mz_paged_view* view, int batch, int q_len, int q_heads, Shape* s, MzpPrefixShape* ps) {
+  *ps = {};
+  if (!view) return shape_of(c, batch, q_len, q_heads, c->width, s);
+  MZ_REQUIRE(view->window >= 0 && view->sinks >= 0, "window %d, sinks %d", view->window, view->sinks);
+  MZ_REQUIRE(view->n_groups >= 0 && view->n_groups <= MAX_BATCH, "%d groups (at most %d)", view->n_groups, MAX_BATCH);
+  MZ_REQUIRE(view->window == 0 || view->n_groups == 0, "a window bounds what a row reads: groups are for calls without one");
+  MZ_REQUIRE(view->window > 0 || view->sinks == 0, "sinks without a window: every token is seen");
+  long long most = c->width;
+  if (view->window > 0) most = std::min<long long>(most, ((long long)view->window + q_len) / MZP_PAGE + 2 + ((long long)view->sinks + MZP_PAGE - 1) / MZP_PAGE);
+  const int rc = shape_of(c, batch, q_len, q_heads, most, s);
+  if (rc != MZ_OK || view->n_groups == 0) return rc;
+  s->prefix_at = (s->bytes + 127) / 128 * 128;
+  mzp_prefix_shape(c, batch, view->n_groups, q_heads / c->kv_heads * q_len, s->sms, ps);
+  s->bytes = s->prefix_at + ps->bytes;
+  return MZ_OK;
 }
 
-extern "C" int mz_paged_attention(const mz_paged_cache* cache, int layer, const mz_paged_attention_args* args, void* stream) {
-  MZ_RANGE("mz_paged_attention");
+int attend(const mz_paged_cache* cache, int layer, const mz_paged_attention_args* args, const mz_paged_view* view, void* stream) {
   int rc = mz_paged_check(cache);
   if (rc != MZ_OK) return rc;
   MZ_REQUIRE(args != nullptr, "args is NULL");
   MZ_REQUIRE(layer >= 0 && layer < cache->layers, "layer %d of %d", layer, cache->layers);
   MZ_REQUIRE(args->rows != nullptr || args->batch <= cache->rows, "batch %d of %d rows", args->batch, cache->rows);
   MZ_REQUIRE(args->out_dtype == MZ_F32 || args->out_dtype == cache->kv_dtype, "out_dtype must be fp32 or the cache's");
-  mzp::Shape s;
-  if ((rc = mzp::shape_of(cache, args->batch, args->q_len, args->q_heads, &s)) != MZ_OK) return rc;
+  Shape s;
+  MzpPrefixShape ps;
+  if ((rc = shape_of(cache, view, args->batch, args->q_len, args->q_heads, &s, &ps)) != MZ_OK) return rc;
   if (args->batch == 0) return MZ_OK;
   MZ_REQUIRE(args->query && args->out, "query or out is NULL");
   MZ_REQUIRE((uintptr_t)args->query % 16 == 0 && (args->q_stride_b | args->q_stride_l | args->q_stride_h) % 8 == 0,
              "query must be 16-byte aligned with strides in multiples of 8 elements");
-  if (!args->workspace || (uintptr_t)args->workspace % 16 != 0 || args->workspace_bytes < s.bytes)
-    return mz_fail(MZ_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed (16-byte aligned)", args->workspace_bytes, s.bytes);
+  MZ_REQUIRE(!view || view->n_groups == 0 || view->groups, "groups is NULL");
+  const int whole = view && view->n_groups > 0 ? 32 : 16;              // records of groups are written 32 bytes at a time
+  if (!args->workspace || (uintptr_t)args->workspace % whole != 0 || args->workspace_bytes < s.bytes)
+    return mz_fail(MZ_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed (%d-byte aligned)", args->workspace_bytes, s.bytes, whole);
   const uint8_t* book = nullptr;
   if ((rc = mz_paged_tables(&book, nullptr)) != MZ_OK) return rc;
-  mzp::Args p = {};
+  Args p = {};
   p.c = *cache;
   p.query = (const uint16_t*)args->query;
   p.qsb = args->q_stride_b; p.qsl = args->q_stride_l; p.qsh = args->q_stride_h;
@@ -1026,8 +1071,8 @@ extern "C" int mz_paged_attention(const mz_paged_cache* cache, int layer, const 
   p.qrows = p.group * args->q_len;
   p.passes = s.passes;
   p.sms = s.sms; p.per_sm = s.per_sm;
-  p.longest = (int)std::min<long long>(0x7fffffff - mzp::STEP, cache->residual + (cache->width + 2ll) * MZP_PAGE - 1);
-  p.scaling = args->scaling * mzp::LOG2E;
+  p.longest = (int)std::min<long long>(0x7fffffff - STEP, cache->residual + (cache->width + 2ll) * MZP_PAGE - 1);
+  p.scaling = args->scaling * LOG2E;
   p.head = (int*)args->workspace;
   p.acc = (float*)((uint8_t*)args->workspace + s.head_bytes);
   p.ml = (float2*)(p.acc + s.slots * s.nr * cache->head_dim);
@@ -1035,10 +1080,43 @@ extern "C" int mz_paged_attention(const mz_paged_cache* cache, int layer, const 
   p.slots = (long long)s.slots;
   p.fail_waits = mz_waits_fail();
   cudaStream_t st = (cudaStream_t)stream;
+  const bool viewed = view && (view->window > 0 || view->n_groups > 0);
+  p.window = 0x7fffffff - (1 << 21);             // the most: positions less this stay 32-bit numbers
+  if (viewed && view->window > 0) {
+    p.window = std::min(view->window, p.window);
+    p.sinks = view->sinks;
+  } else if (viewed) {
+    if ((rc = mzp_prefix_launch(*cache, layer, *args, *view, ps, (uint8_t*)args->workspace + s.prefix_at, p.longest, book, st, &p.pre)) != MZ_OK) return rc;
+  }
   const bool bf = cache->kv_dtype == MZ_BF16;
-#define MZP_GO(D, NR) return bf ? mzp::launch<D, true, NR>(p, book, s.G, st) : mzp::launch<D, false, NR>(p, book, s.G, st)
+#define MZP_VIEW(D, BF, NR) return viewed ? launch<D, BF, NR, true>(p, book, s.G, st) : launch<D, BF, NR, false>(p, book, s.G, st)
+#define MZP_GO(D, NR) do { if (bf) MZP_VIEW(D, true, NR); MZP_VIEW(D, false, NR); } while (0)
   if (cache->head_dim == 128) { if (s.nr == 4) MZP_GO(128, 4); MZP_GO(128, 8); }
   if (s.nr == 4) MZP_GO(64, 4);
   MZP_GO(64, 8);
 #undef MZP_GO
+#undef MZP_VIEW
+}
+}  // namespace mzp
+
+extern "C" size_t mz_paged_attention_workspace_bytes(const mz_paged_cache* cache, int batch, int q_len, int q_heads) {
+  return mz_paged_attention_view_workspace_bytes(cache, nullptr, batch, q_len, q_heads);
+}
+
+extern "C" size_t mz_paged_attention_view_workspace_bytes(const mz_paged_cache* cache, const mz_paged_view* view, int batch, int q_len, int q_heads) {
+  mzp::Shape s;
+  MzpPrefixShape ps;
+  if (mz_paged_check(cache) != MZ_OK || mzp::shape_of(cache, view, batch, q_len, q_heads, &s, &ps) != MZ_OK) return 0;
+  return s.bytes;
+}
+
+extern "C" int mz_paged_attention(const mz_paged_cache* cache, int layer, const mz_paged_attention_args* args, void* stream) {
+  MZ_RANGE("mz_paged_attention");
+  return mzp::attend(cache, layer, args, nullptr, stream);
+}
+
+extern "C" int mz_paged_attention_view(const mz_paged_cache* cache, int layer, const mz_paged_attention_args* args, const mz_paged_view* view, void* stream) {
+  MZ_RANGE("mz_paged_attention_view");
+  MZ_REQUIRE(view != nullptr, "view is NULL");
+  return mzp::attend(cache, layer, args, view, stream);
 }

@@ -1,0 +1,67 @@
+// Paged cache: what the kernel for shared prefixes (mz_paged_prefix.cu) leaves for the one that ends an attention call (mz_paged_attention.cu).
+//
+// A group is a run of list entries; the pages that all its rows' tables begin with are its prefix.  The query rows of a group that share a kv head, entry after entry, are
+// cut into tiles of at most 256; a unit is a (group, kv head, tile), a step of it one page.  The steps of all units stand in one line, weighted by 1 where a tile
+// has at most 128 rows and 2 above, and the line is cut evenly over the CTAs.  Each CTA leaves a record (m, l, out) per query row of a unit that it met: with r
+// rows in the units before, the record of row i by CTA c has place r + 256 c + i.
+#pragma once
+#include "mz_paged_device.cuh"
+
+constexpr int MZP_TILE_ROWS = 256;
+
+struct alignas(16) MzpGroup { int first, rows, pages, row; };        // first list entry, query rows per kv head, pages of the prefix (0: nothing is shared), a cache row
+struct MzpSums { long long steps, records; };                        // of the groups before
+
+struct MzpPrefix {
+  int* skip;                                     // [batch] pages of an entry that its group has taken care of
+  int* group_of;                                 // [batch]
+  MzpGroup* groups;                              // [n_groups]
+  MzpSums* sums;                                 // [n_groups + 1]
+  float2* ml;                                    // [record] maximum (base 2) and sum
+  float* acc;                                    // [record][D]
+  int n_groups, grid;
+  long long records;
+};
+
+// how a group's query rows are cut
+struct MzpTiles {
+  int count, rows, weight;
+  __host__ __device__ __forceinline__ explicit MzpTiles(int m) {
+    count = (m + MZP_TILE_ROWS - 1) / MZP_TILE_ROWS;
+    rows = ((m + count - 1) / (count > 0 ? count : 1) + 7) / 8 * 8;
+    weight = rows > MZP_TILE_ROWS / 2 ? 2 : 1;
+  }
+};
+// how the line is cut
+struct MzpLine {
+  long long total, ctas;
+  __device__ __forceinline__ MzpLine(long long steps, int grid) : total(steps), ctas(steps < grid ? steps : grid) {}
+  __device__ __forceinline__ long long start(int cta) const { return total * cta / ctas; }
+  __device__ __forceinline__ int owner(long long at) const { return (int)(((at + 1) * ctas - 1) / total); }
+};
+
+// where a list entry's records are
+struct MzpUnits {
+  MzpGroup g;
+  MzpSums before;
+  MzpTiles tiles;
+  MzpLine line;
+  int qrows, kv_heads;
+  __device__ __forceinline__ MzpUnits(const MzpPrefix& p, int b, int query_rows, int heads)
+      : g(p.groups[p.group_of[b]]), before(p.sums[p.group_of[b]]), tiles(g.rows), line(p.sums[p.n_groups].steps, p.grid), qrows(query_rows), kv_heads(heads) {}
+  __device__ __forceinline__ int row_of(int b, int query_row) const { return (b - g.first) * qrows + query_row; }
+  // record of a query row of the group without its CTA's share of 256 c, and the CTAs that have one
+  __device__ __forceinline__ long long record(int head, int row, long long& first, long long& last) const {
+    const int tile = row / tiles.rows;
+    const long long at = before.steps + (long long)(head * tiles.count + tile) * g.pages * tiles.weight;
+    first = line.owner(at);
+    last = line.owner(at + (long long)(g.pages - 1) * tiles.weight);
+    return before.records + (long long)head * g.rows + row;
+  }
+};
+
+struct MzpPrefixShape { int grid; long long records; size_t skip_at, group_of_at, groups_at, sums_at, ml_at, acc_at, bytes; };
+void mzp_prefix_shape(const mz_paged_cache* c, int batch, int n_groups, int qrows, int sms, MzpPrefixShape* s);
+// Finds the prefixes of the groups and takes the attention of their rows over them; fills `out`.  longest: no row is taken for longer.
+int mzp_prefix_launch(const mz_paged_cache& c, int layer, const mz_paged_attention_args& args, const mz_paged_view& view, const MzpPrefixShape& s, uint8_t* workspace,
+                      int longest, const uint8_t* book, cudaStream_t stream, MzpPrefix* out);

@@ -26,6 +26,7 @@ EXPORTS = (
     "mz_alpha_stats", "mz_alpha_stats_workspace_bytes", "mz_materialize_kv", "mz_roundtrip_kv", "mz_flush_kv_move",
     "mz_paged_books", "mz_paged_prepare", "mz_paged_extend", "mz_paged_append", "mz_paged_attention_workspace_bytes", "mz_paged_attention", "mz_paged_fork",
     "mz_paged_free", "mz_paged_compact_workspace_bytes", "mz_paged_compact", "mz_paged_copy_pages",
+    "mz_paged_attention_view_workspace_bytes", "mz_paged_attention_view", "mz_paged_read",
 )
 
 
@@ -91,6 +92,20 @@ class PagedAttentionArgs(Structure):
         ("out", c_void_p),
         ("out_dtype", c_int),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class PagedView(Structure):
+    _fields_ = [("window", c_int), ("sinks", c_int), ("groups", c_void_p), ("n_groups", c_int)]
+
+
+class PagedReadArgs(Structure):
+    _fields_ = [
+        ("key", c_void_p), ("value", c_void_p),
+        ("dtype", c_int),
+        ("k_stride_token", c_longlong), ("k_stride_head", c_longlong), ("v_stride_token", c_longlong), ("v_stride_head", c_longlong),
+        ("rows", c_void_p), ("offsets", c_void_p), ("first", c_void_p),
+        ("batch", c_int), ("tokens", c_int),
     ]
 
 
@@ -163,6 +178,10 @@ def load_library() -> ctypes.CDLL:
     lib.mz_paged_attention_workspace_bytes.argtypes = [POINTER(PagedCache), c_int, c_int, c_int]
     lib.mz_paged_attention_workspace_bytes.restype = c_size_t
     lib.mz_paged_attention.argtypes = [POINTER(PagedCache), c_int, POINTER(PagedAttentionArgs), c_void_p]
+    lib.mz_paged_attention_view_workspace_bytes.argtypes = [POINTER(PagedCache), POINTER(PagedView), c_int, c_int, c_int]
+    lib.mz_paged_attention_view_workspace_bytes.restype = c_size_t
+    lib.mz_paged_attention_view.argtypes = [POINTER(PagedCache), c_int, POINTER(PagedAttentionArgs), POINTER(PagedView), c_void_p]
+    lib.mz_paged_read.argtypes = [POINTER(PagedCache), c_int, POINTER(PagedReadArgs), c_void_p]
     lib.mz_paged_fork.argtypes = [POINTER(PagedCache), c_void_p, c_void_p, c_int, c_void_p]
     lib.mz_paged_free.argtypes = [POINTER(PagedCache), c_void_p, c_int, c_void_p]
     lib.mz_paged_compact_workspace_bytes.argtypes = [POINTER(PagedCache)]
