@@ -706,6 +706,8 @@ template <int D, bool BF, int NR, bool VIEW>
 __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
   constexpr int HALVES = D / 64, STREAMS = 8 / HALVES, GROUPS = END_THREADS / D, ROWS = NR / GROUPS;      // D = 64: four groups
   __shared__ float s_part[STREAMS][NR][D], s_m[STREAMS][NR], s_l[STREAMS][NR];
+  struct Share { long long slot; int first, last; };         // a query row's records of the prefix: the first CTA's place less 256 times its number, the CTAs (-1: none)
+  __shared__ Share s_share[VIEW ? NR : 1];
   const mz_paged_cache& c = p.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const long long pair = blockIdx.x;
@@ -874,6 +876,14 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
       }
     }
   }
+  if (VIEW && p.pre.skip && tid < NR && p.pre.skip[b] > 0) {
+    Share s = {0, 0, -1};
+    if (r0 + tid < p.qrows) {
+      const MzpUnits units(p.pre, b, p.qrows, c.kv_heads);
+      s.slot = units.record(head, units.row_of(b, r0 + tid), s.first, s.last);
+    }
+    s_share[tid] = s;
+  }
   __syncthreads();
   // ---- this thread: channel d of query rows i0, i0 + GROUPS, ...
   const int d = tid % D, i0 = tid / D;
@@ -887,6 +897,39 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
     a[i] = a[i] * f + v * h;
     m[i] = top;
   };
+  if (VIEW && p.pre.skip && p.pre.skip[b] > 0) {             // what the row shares with its group: records of whole tiles of query rows, there since before the first kernel
+    long long slot[ROWS];
+    int first[ROWS], last[ROWS], lo = 0x7fffffff, hi = -1;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const Share s = s_share[i0 + i * GROUPS];
+      slot[i] = s.slot; first[i] = s.first; last[i] = s.last;
+      if (last[i] >= 0) { lo = min(lo, first[i]); hi = max(hi, last[i]); }
+    }
+    constexpr int DEEP = 16 / ROWS;              // records at a time
+    for (int c0 = lo; c0 <= hi; c0 += DEEP) {
+      float2 ml[DEEP][ROWS];
+      float v[DEEP][ROWS];
+#pragma unroll
+      for (int k = 0; k < DEEP; ++k) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+          ml[k][i] = make_float2(-INFINITY, 0.f);
+          v[k][i] = 0.f;
+          if (c0 + k >= first[i] && c0 + k <= last[i]) {
+            const long long at = slot[i] + (long long)MZP_TILE_ROWS * (c0 + k);
+            ml[k][i] = p.pre.ml[at];
+            v[k][i] = p.pre.acc[at * D + d];
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < DEEP; ++k) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) take(i, ml[k][i], v[k][i]);
+      }
+    }
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");         // the first kernel's records are written
   const long long before = p.head[1 + b], steps = p.head[2 + b] - before;
   if (steps > 0) {
@@ -908,39 +951,6 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
       for (int k = 0; k < 4; ++k) {
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) if (c0 + k <= last) take(i, ml[k][i], v[k][i]);
-      }
-    }
-  }
-  if (VIEW && p.pre.skip && p.pre.skip[b] > 0) {             // what the row shares with its group: records of whole tiles of query rows
-    const MzpUnits units(p.pre, b, p.qrows, c.kv_heads);
-    long long slot[ROWS], first[ROWS], last[ROWS], lo = 0x7fffffff, hi = -1;
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const int qr = r0 + i0 + i * GROUPS;
-      first[i] = 0; last[i] = -1; slot[i] = 0;
-      if (qr < p.qrows) {
-        slot[i] = units.record(head, units.row_of(b, qr), first[i], last[i]);
-        lo = min(lo, first[i]);
-        hi = max(hi, last[i]);
-      }
-    }
-    for (long long c0 = lo; c0 <= hi; c0 += 4) {
-      float2 ml[4][ROWS];
-      float v[4][ROWS];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-          const long long at = slot[i] + MZP_TILE_ROWS * (max(first[i], min(c0 + k, last[i])));
-          ml[k][i] = make_float2(-INFINITY, 0.f);
-          v[k][i] = 0.f;
-          if (last[i] >= 0) { ml[k][i] = p.pre.ml[at]; v[k][i] = p.pre.acc[at * D + d]; }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) if (c0 + k >= first[i] && c0 + k <= last[i]) take(i, ml[k][i], v[k][i]);
       }
     }
   }

@@ -13,10 +13,11 @@
 
 namespace mzp {
 namespace {
-// Warps by duty: 0 .. 7 softmax (a group of four per stream), 8 .. 15 levels, 16 issues the products; the three beside it are there for its warpgroup's registers
-constexpr int SOFTMAX_WARPS = 8, LEVEL_WARPS = 8, ISSUER = SOFTMAX_WARPS + LEVEL_WARPS, PREFIX_THREADS = 32 * (ISSUER + 4);
-// of the 96 x 640 registers that a CTA is launched with: 2 x 128 x 112 + 2 x 128 x 96 + 128 x 56 are 60416 of 61440
-constexpr int SOFTMAX_REGS = 112, ISSUER_REGS = 56;
+// Warps by duty: 0 .. 7 softmax (a group of four per stream).  Of the others, every fourth one, which are all on one scheduler, has a duty that much waits for: 11 issues the
+// products, 15 copies pages as they are, 19 and 23 decode the words of their rows; the rest make the levels, in three teams of four with a page each.
+constexpr int SOFTMAX_WARPS = 8, WARPS = 24, ISSUER = 11, FEEDER = 15, DECODER = 19, TEAMS = 3, PREFIX_THREADS = 32 * WARPS;
+// of the 80 x 768 registers that a CTA is launched with: 256 x 112 + 512 x 64 are all
+constexpr int SOFTMAX_REGS = 112, OTHER_REGS = 64;
 template <int N, bool MORE>
 __device__ __forceinline__ void registers() {
   if (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -68,18 +69,30 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
   common = s_common;
   const int row0 = first < end ? row_at(first) : 0;
   if (common > 0) {
+    // a warp compares 128 columns of its share of the rows with the first row's, four rows' loads on their way at a time
     const int* head = c.block_table + (long long)row0 * c.width;
-    const int warp = tid >> 5, lane = tid & 31;
-    // 32 columns of a row for each warp of the cluster in turn
-    const int pieces = (common + 31) / 32;
-    const long long all = (long long)pieces * (end - first);
-    for (long long i = rank * (PLAN_THREADS / 32) + warp; i < all; i += PLAN_CTAS * (PLAN_THREADS / 32)) {
-      const int b = first + (int)(i / pieces), at = (int)(i % pieces) * 32 + lane;
-      if (at < common) {
-        const int id = head[at];
-        const bool same = id >= 0 && id < c.pages && c.block_table[(long long)row_at(b) * c.width + at] == id;
-        if (!same) atomicMin(&s_common, at);
+    const int lane = tid & 31, warps = PLAN_CTAS * (PLAN_THREADS / 32), pieces = (common + 127) / 128, shares = max(1, min(warps / pieces, end - first));
+    for (int i = rank * (PLAN_THREADS / 32) + (tid >> 5); i < pieces * shares; i += warps) {
+      const int share = i / pieces, at = (i - share * pieces) * 128 + lane;
+      int id[4], bad = 0x7fffffff;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        id[k] = at + 32 * k < common ? head[at + 32 * k] : 0;
+        if (id[k] < 0 || id[k] >= c.pages) bad = min(bad, at + 32 * k);
       }
+      for (int b0 = first + share; b0 < end; b0 += 4 * shares) {
+        int other[4][4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int* theirs = c.block_table + (long long)row_at(min(b0 + r * shares, end - 1)) * c.width;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) other[r][k] = at + 32 * k < common ? theirs[at + 32 * k] : id[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if ((other[0][k] ^ id[k]) | (other[1][k] ^ id[k]) | (other[2][k] ^ id[k]) | (other[3][k] ^ id[k])) bad = min(bad, at + 32 * k);
+      }
+      if (bad != 0x7fffffff) atomicMin(&s_common, bad);
     }
   }
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
@@ -99,33 +112,48 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
 // ---- attention over the prefixes
 template <int D>
 struct PrefixSmem {
-  static constexpr int KEY_CHUNK = D * 16, VALUE_CHUNK = MZP_PAGE * 16;          // 8 tokens of all channels; 8 channels of all tokens
   static constexpr int PLANE = MZP_PAGE * D * 2;                                 // a page's keys, or values, in 16 bits
-  static constexpr int STAGES = 4, SCALES = 8;
-  static constexpr int KEYS = 0, VALUES = STAGES * 2 * PLANE, BOOK = VALUES + STAGES * PLANE;
-  static constexpr int ALIGN = 128, TOTAL = BOOK + MZP_BOOKS * MZP_LEVELS + ALIGN;
-  // columns of tensor memory: queries of both streams (A operand, two values to a column), logits (P stands over their first half), outputs
-  static constexpr int TM_Q = 0, TM_S = D, TM_O = D + 2 * MZP_PAGE, TM_COLS = 512;
-  static_assert(TM_O + 2 * D <= TM_COLS, "tensor memory");
+  static constexpr int PAGE_BYTES = 72 * D;
+  static constexpr int STAGES = 3, RAWS = 5, SCALES = 16, ROWS = 2 * D;          // ROWS: rows of codes of a page
+  static constexpr int KEYS = 0, VALUES = STAGES * 2 * PLANE, RAW = VALUES + STAGES * PLANE, BOOK = RAW + RAWS * PAGE_BYTES, TERMS = BOOK + MZP_BOOKS * MZP_LEVELS;
+  static constexpr int ALIGN = 1024, TOTAL = TERMS + RAWS * ROWS * 16 + ALIGN;
+  // columns of tensor memory: queries (A operand, two values to a column), logits of two or three jobs (P stands over their first half), outputs of the streams.
+  // Where the streams have rows of their own there are two blocks of queries and of logits, where they share theirs one and three
+  static constexpr int TM_Q = 0, TM_O = 256, TM_COLS = 512;
+  static __host__ __device__ constexpr int tm_s(bool both) { return both ? D : D / 2; }
+  static_assert(D + 2 * MZP_PAGE <= TM_O && D / 2 + 3 * MZP_PAGE <= TM_O && TM_O + 2 * D <= TM_COLS, "tensor memory");
 };
+// Operands stand major along the kept dimension (keys: tokens, values: channels): rows of 64 values (128 bytes) along it, one per index that is summed over, the eight
+// 16-byte pieces of a row in the order of their number xor the row's (128-byte swizzle); values of head_dim 128 are two such blocks
+constexpr int OPERAND_STEP = 16 * 128 >> 4;      // 16 rows further
+
+struct alignas(16) Segment { int first, row, head, m0, rows, page, count, pad; long long record; };      // a run of steps of one unit
+constexpr int ISSUE_UNROLL = 4;
+constexpr int SEGMENTS = 64;                     // of a CTA at a time
 struct PrefixShared {
-  unsigned long long k_full[4], k_free[4], v_full[4], v_free[4], s_full[2], p_full[2], o_done[2], q_full, end;
-  int2 scale[8];                                 // (ek, ev) by page of the CTA's line
+  Segment seg[SEGMENTS];
+  unsigned long long raw_full[5], raw_free[5], scaled[16], k_full[3], k_free[3], v_full[3], v_free[3], s_full[4], p_full[4], o_done[4], q_full, end;
+  int2 scale[16];                                // (ek, ev) by page of the CTA's line; pages are scaled ten ahead of their softmax at most
+  int there[5];                                  // whether a raw page is one
   float2 ml[2][128];                             // of the two streams, where they share rows
-  long long steps, records;                      // before the group of the CTA's first step
-  long long total;
-  int group;
+  int segments, more;                            // in hand; whether others follow
   uint32_t tmem;
   int failed;
 };
-struct Segment { int first, row, head, m0, rows, page, count; long long record; };      // a run of steps of one unit
 
 // D[128 x N] (+)= A[128 x 16, tensor memory] * B[16 x N], f16 into fp32, B major along N
+// (b: the operand's address in 16 bytes; its other fields are constant)
 template <int N>
-__device__ __forceinline__ void umma16(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t accumulate) {
+__device__ __forceinline__ void umma16(uint32_t d_tmem, uint32_t a_tmem, uint32_t b, uint32_t accumulate) {
   constexpr uint32_t idesc = (1u << 4) | (1u << 16) | ((uint32_t)(N / 8) << 17) | (8u << 24);
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
-               ::"r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  constexpr uint32_t low = MZP_PAGE * 128 >> 4 << 16, high = 1024u >> 4 | 1u << 14 | 2u << 29;       // blocks 8 KB apart, eight rows 1 KB, 128-byte swizzle
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 d;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 d, {%2, %3};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], d, %4, p;\n\t}\n"
+               ::"r"(d_tmem), "r"(a_tmem), "r"(b | low), "r"(high), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ bool elect() {        // one lane of a whole warp
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
 }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 #define MZP_R8(v, i) "=r"((v)[i]), "=r"((v)[i + 1]), "=r"((v)[i + 2]), "=r"((v)[i + 3]), "=r"((v)[i + 4]), "=r"((v)[i + 5]), "=r"((v)[i + 6]), "=r"((v)[i + 7])
@@ -142,6 +170,18 @@ __device__ __forceinline__ void tm_store32(uint32_t at, const uint32_t (&v)[32])
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " MZP_REGS32 ";" ::MZP_I8(v, 0), MZP_I8(v, 8), MZP_I8(v, 16), MZP_I8(v, 24), "r"(at) : "memory");
 }
 __device__ __forceinline__ void tm_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds32(uint32_t a) { uint32_t v; asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a)); return v; }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+// two values times f plus c
+__device__ __forceinline__ void mul_add2(float& a, float& b, float f, float c) {
+  asm("{\n\t.reg .b64 x, f, c;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 f, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\tfma.rn.f32x2 x, x, f, c;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b) : "f"(f), "f"(c));
+}
 __device__ __forceinline__ uint32_t half2_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 __device__ __forceinline__ __half2 bits_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 __device__ __forceinline__ void stg256(float* p, const float* v) {
@@ -161,90 +201,34 @@ __device__ __forceinline__ void levels8(uint32_t codes, const uint4& book, uint3
   }
 }
 
-// Goes through a CTA's part of the line, a run of steps of one unit at a time.  Every role walks by itself.
-struct Walk {
-  const PrefixArgs& p;
-  long long steps, records, f0, f1;
-  int g, unit;
-  __device__ __forceinline__ Walk(const PrefixArgs& args, const PrefixShared& x, long long from, long long to)
-      : p(args), steps(x.steps), records(x.records), f0(from), f1(to), g(x.group), unit(-1) {}
-  __device__ __forceinline__ bool next(Segment& s) {
-    while (g < p.out.n_groups) {
-      const MzpGroup info = p.out.groups[g];
-      if (info.pages > 0) {
-        const MzpTiles tiles(info.rows);
-        const long long len = (long long)info.pages * tiles.weight;
-        const int units = p.c.kv_heads * tiles.count;
-        if (unit < 0) unit = f0 > steps ? (int)min((f0 - steps) / len, (long long)units) : 0;
-        for (; unit < units; ++unit) {
-          const long long at = steps + unit * len;
-          if (at >= f1) return false;
-          const int first = at >= f0 ? 0 : (int)((f0 - at + tiles.weight - 1) / tiles.weight);
-          const int end = (int)min((long long)info.pages, (f1 - at + tiles.weight - 1) / tiles.weight);
-          if (first >= end) continue;
-          const int head = unit / tiles.count, tile = unit - head * tiles.count;
-          s.first = info.first; s.row = info.row; s.head = head;
-          s.m0 = tile * tiles.rows;
-          s.rows = min(tiles.rows, info.rows - s.m0);
-          s.page = first;
-          s.count = end - first;
-          s.record = records + (long long)head * info.rows + s.m0;
-          ++unit;
-          return true;
-        }
-        steps += units * len;
-        records += (long long)p.c.kv_heads * info.rows;
-      }
-      ++g;
-      unit = 0;
-    }
-    return false;
-  }
-};
-
-template <int D, bool BF>
-__global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixArgs p, const uint8_t* __restrict__ book_table) {
-  using S = PrefixSmem<D>;
-  constexpr int PB = 72 * D, HALF = MZP_TILE_ROWS / 2;
-  extern __shared__ uint8_t window[];
-  uint8_t* smem = window + (S::ALIGN - smem_u32(window) % S::ALIGN) % S::ALIGN;
-  __shared__ PrefixShared x;
-  const mz_paged_cache& c = p.c;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
-  const uint32_t sbase = smem_u32(smem), sbook = sbase + S::BOOK;
-  auto bar = [&](unsigned long long& b) { return smem_u32(&b); };
-  if (tid == 0) {
-    x.failed = p.fail_waits;
-    for (int i = 0; i < S::STAGES; ++i) { bar_init(bar(x.k_full[i]), 4); bar_init(bar(x.k_free[i]), 1); bar_init(bar(x.v_full[i]), 4); bar_init(bar(x.v_free[i]), 1); }
-    for (int i = 0; i < 2; ++i) { bar_init(bar(x.s_full[i]), 2); bar_init(bar(x.p_full[i]), 4); bar_init(bar(x.o_done[i]), 1); }
-    bar_init(bar(x.q_full), SOFTMAX_WARPS);
-    bar_init(bar(x.end), 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (tid < MZP_BOOKS * MZP_LEVELS / 16) ((uint4*)(smem + S::BOOK))[tid] = ((const uint4*)book_table)[tid];
-  // ---- the line: its length, and the group that the CTA's part begins in
-  if (warp == 0) {
-    long long steps = 0;
-    for (int i = lane; i < p.out.n_groups; i += 32) {
-      const MzpGroup info = p.out.groups[i];
-      const MzpTiles tiles(info.rows);
-      steps += (long long)info.pages * tiles.weight * tiles.count * c.kv_heads;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) steps += __shfl_xor_sync(0xffffffffu, steps, o);
-    const long long total = steps;
-    const MzpLine line(total, gridDim.x);
-    const long long f0 = cta < line.ctas ? line.start(cta) : 0;
-    long long before_s = 0, before_r = 0;
-    for (int i0 = 0; i0 < p.out.n_groups; i0 += 32) {
-      const int i = i0 + lane;
-      long long st = 0, re = 0;
-      if (i < p.out.n_groups) {
+// Lists a CTA's part of the line, SEGMENTS runs of one unit at a time.  For a whole warp.
+struct Lister {
+  long long steps, records, f0, f1;              // before group g; the part
+  int g, unit;                                   // next
+  // finds the line's length and the group that the part begins in; CTA 0 writes down where groups begin
+  __device__ __forceinline__ bool begin(const PrefixArgs& p, int lane) {
+    const int cta = blockIdx.x, n = p.out.n_groups;
+    auto size = [&](int i, long long& st, long long& re) {
+      st = re = 0;
+      if (i < n) {
         const MzpGroup info = p.out.groups[i];
         const MzpTiles tiles(info.rows);
-        st = (long long)info.pages * tiles.weight * tiles.count * c.kv_heads;
-        re = info.pages > 0 ? (long long)info.rows * c.kv_heads : 0;
+        st = (long long)info.pages * (tiles.weight * tiles.count) * p.c.kv_heads;
+        re = info.pages > 0 ? (long long)info.rows * p.c.kv_heads : 0;
       }
+    };
+    long long st, re, total = 0;
+    for (int i = lane; i < n; i += 32) { size(i, st, re); total += st; }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const MzpLine line(total, gridDim.x);
+    const bool some = cta < line.ctas;
+    f0 = some ? line.start(cta) : 0;
+    f1 = some ? line.start(cta + 1) : 0;
+    long long before_s = 0, before_r = 0;
+    g = n;
+    for (int i0 = 0; i0 < n && (cta == 0 || g == n); i0 += 32) {
+      size(i0 + lane, st, re);
       long long ss = st, rr = re;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -252,92 +236,367 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
         if (lane >= o) { ss += a; rr += b; }
       }
       const long long my_s = before_s + ss - st, my_r = before_r + rr - re;
-      if (i < p.out.n_groups) {
-        if (my_s <= f0 && f0 < my_s + st) { x.group = i; x.steps = my_s; x.records = my_r; }
-        if (cta == 0) p.out.sums[i] = {my_s, my_r};
+      if (cta == 0 && i0 + lane < n) p.out.sums[i0 + lane] = {my_s, my_r};
+      const uint32_t mine = __ballot_sync(0xffffffffu, my_s <= f0 && f0 < my_s + st);
+      if (some && mine) {
+        const int from = __ffs(mine) - 1;
+        g = i0 + from;
+        steps = __shfl_sync(0xffffffffu, my_s, from);
+        records = __shfl_sync(0xffffffffu, my_r, from);
       }
       before_s += __shfl_sync(0xffffffffu, ss, 31);
       before_r += __shfl_sync(0xffffffffu, rr, 31);
     }
-    if (lane == 0) {
-      x.total = total;
-      if (cta == 0) p.out.sums[p.out.n_groups] = {total, before_r};
-    }
+    if (cta == 0 && lane == 0) p.out.sums[n] = {total, before_r};
+    unit = -1;
+    return some;
   }
-  __syncthreads();
-  const MzpLine line(x.total, gridDim.x);
-  if (cta >= line.ctas) return;
-  const long long f0 = line.start(cta), f1 = line.start(cta + 1);
+  __device__ __forceinline__ void list(const PrefixArgs& p, PrefixShared& x, int lane) {
+    int n = 0;
+    while (g < p.out.n_groups && steps < f1 && n < SEGMENTS) {
+      const MzpGroup info = p.out.groups[g];
+      if (info.pages > 0) {
+        const MzpTiles tiles(info.rows);
+        const long long len = (long long)info.pages * tiles.weight;
+        const int units = p.c.kv_heads * tiles.count;
+        if (unit < 0) unit = f0 > steps ? (int)min((f0 - steps) / len, (long long)units) : 0;
+        const int end = (int)min((long long)units, (f1 - steps + len - 1) / len);
+        while (unit < end && n < SEGMENTS) {
+          const int u = unit + lane;
+          const long long at = steps + u * len;
+          Segment s;
+          s.page = at >= f0 ? 0 : (int)((f0 - at + tiles.weight - 1) / tiles.weight);
+          s.count = (int)min((long long)info.pages, (f1 - at + tiles.weight - 1) / tiles.weight) - s.page;
+          s.head = u / tiles.count;
+          s.m0 = (u - s.head * tiles.count) * tiles.rows;
+          s.first = info.first; s.row = info.row;
+          s.rows = min(tiles.rows, info.rows - s.m0);
+          s.record = records + (long long)s.head * info.rows + s.m0 + (long long)MZP_TILE_ROWS * blockIdx.x;
+          s.pad = 0;
+          const bool mine = u < end && s.count > 0;
+          const uint32_t all = __ballot_sync(0xffffffffu, mine);
+          const int place = n + __popc(all & ((1u << lane) - 1));
+          if (mine && place < SEGMENTS) x.seg[place] = s;
+          // the first one that does not fit begins the next list
+          const uint32_t late = __ballot_sync(0xffffffffu, mine && place >= SEGMENTS);
+          unit += late ? __ffs(late) - 1 : 32;
+          n = min(n + __popc(all), SEGMENTS);
+        }
+        if (unit < end) break;                   // full
+        steps += units * len;
+        records += (long long)p.c.kv_heads * info.rows;
+      }
+      ++g;
+      unit = 0;
+    }
+    if (lane == 0) { x.segments = n; x.more = n == SEGMENTS; }
+  }
+};
+
+template <int D, bool BF>
+__global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixArgs p, const uint8_t* __restrict__ book_table) {
+  using S = PrefixSmem<D>;
+  constexpr int PB = S::PAGE_BYTES, HALF = MZP_TILE_ROWS / 2;
+  extern __shared__ uint8_t window[];
+  uint8_t* smem = window + (S::ALIGN - smem_u32(window) % S::ALIGN) % S::ALIGN;
+  __shared__ PrefixShared x;
+  const mz_paged_cache& c = p.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t sbase = smem_u32(smem);
+  auto bar = [&](unsigned long long& b) { return smem_u32(&b); };
+  auto everyone = [&]() { asm volatile("bar.sync 0;" ::: "memory"); };
+  if (tid == 0) {
+    x.failed = p.fail_waits;
+    for (int i = 0; i < S::RAWS; ++i) { bar_init(bar(x.raw_full[i]), 1); bar_init(bar(x.raw_free[i]), 4); }
+    for (int i = 0; i < S::SCALES; ++i) bar_init(bar(x.scaled[i]), 1);
+    for (int i = 0; i < S::STAGES; ++i) { bar_init(bar(x.k_full[i]), 4); bar_init(bar(x.k_free[i]), 1); bar_init(bar(x.v_full[i]), 4); bar_init(bar(x.v_free[i]), 1); }
+    for (int i = 0; i < 4; ++i) { bar_init(bar(x.s_full[i]), 1); bar_init(bar(x.p_full[i]), 4); bar_init(bar(x.o_done[i]), 1); }
+    bar_init(bar(x.q_full), SOFTMAX_WARPS);
+    bar_init(bar(x.end), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid < MZP_BOOKS * MZP_LEVELS / 16) ((uint4*)(smem + S::BOOK))[tid] = ((const uint4*)book_table)[tid];
   if (warp == ISSUER) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&x.tmem)), "n"(S::TM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     tm_before();
   }
-  __syncthreads();
+  Lister lister;
+  if (warp == FEEDER) {
+    lister.begin(p, lane);
+    lister.list(p, x, lane);
+  }
+  everyone();
   tm_after();
-  const uint32_t tmem = x.tmem;
+  constexpr uint32_t tmem = 0;                   // all columns: they begin at 0
+  if (tid == 0 && x.tmem != 0) x.failed = 1;
   volatile int* failed = &x.failed;
-  Walk walk(p, x, f0, f1);
-  Segment seg;
 
-  if (warp >= ISSUER) {
-    registers<ISSUER_REGS, false>();
-    // ---- products: the logits of a job as soon as the stream's last P has been used
-    if (warp == ISSUER && lane == 0) {
-      int pages = 0, segment = 0, used0 = 0, used1 = 0;      // of the CTA so far: pages, segments, jobs of each stream
-      while (walk.next(seg)) {
-        const bool both = seg.rows > HALF;                   // two tiles of rows take each page; otherwise the streams take the pages in turn
-        const int jobs = both ? 2 * seg.count : seg.count;
-        bar_wait(bar(x.q_full), segment & 1, failed);
-        tm_after();
-        const int fresh0 = used0, fresh1 = used1;
-        for (int i = 0; i < jobs + 2; ++i) {
-          if (i >= 2) {
-            const int j = i - 2, s = j & 1, page = pages + (both ? j >> 1 : j), stage = page % S::STAGES;
-            const int used = s ? used1 : used0;
-            bar_wait(bar(x.p_full[s]), used & 1, failed);
-            if (!both || s == 0) bar_wait(bar(x.v_full[stage]), page / S::STAGES & 1, failed);
+  if (warp >= SOFTMAX_WARPS) {
+    registers<OTHER_REGS, false>();
+    if (warp == ISSUER) {
+      // ---- products: a job's logits as soon as the P that stands in their place has been used.  One elected lane issues, and all that it issues with is the same for the warp and shown
+      // to be (maxima and votes over it), so that it stands in uniform registers.  A look at a barrier takes 200 cycles behind products, as it queues with them: so a job looks at
+      // all of its barriers at once, while the products before it run (20 products with one look 776 cycles, with three looks one after the other 1420)
+      auto same = [&](int v) { return (int)__reduce_max_sync(0xffffffffu, (unsigned)v); };
+      auto wait3 = [&](uint32_t b0, uint32_t parity0, uint32_t b1, uint32_t parity1, uint32_t b2, uint32_t parity2) {
+#ifdef MZ_BOUNDS
+        if (__any_sync(0xffffffffu, *failed)) return;        // a test makes every wait run out
+#endif
+        for (int it = 0; it < SPIN_LIMIT; ++it) {
+          uint32_t done;
+          asm volatile("{\n\t.reg .pred p, q, r;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tmbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+                       "mbarrier.try_wait.parity.shared::cta.b64 r, [%5], %6;\n\tand.pred p, p, q;\n\tand.pred p, p, r;\n\tselp.b32 %0, 1, 0, p;\n\t}\n"
+                       : "=r"(done) : "r"(b0), "r"(parity0), "r"(b1), "r"(parity1), "r"(b2), "r"(parity2) : "memory");
+          if (__all_sync(0xffffffffu, done != 0)) return;
+          if ((it & 63) == 63 && __any_sync(0xffffffffu, *failed)) return;
+        }
+        *failed = 1;
+      };
+      int segment = 0, ahead = 0, behind = 0, k_stage = 0, v_stage = 0;    // of the CTA so far: segments, jobs whose logits, whose outputs were issued
+      uint32_t k_phase = 0, v_phase = 0;
+      const uint32_t keys = same((int)(sbase + S::KEYS) >> 4), values = same((int)(sbase + S::VALUES) >> 4);
+      const uint32_t s_full = bar(x.s_full[0]), p_full = bar(x.p_full[0]), o_done = bar(x.o_done[0]), q_full = bar(x.q_full);
+      const uint32_t k_full = bar(x.k_full[0]), k_free = bar(x.k_free[0]), v_full = bar(x.v_full[0]), v_free = bar(x.v_free[0]);
+      for (int n = same(x.segments); n > 0; n = same(x.segments)) {
+        for (int i0 = 0; i0 < n; ++i0, ++segment) {
+          const bool both = same(x.seg[i0].rows) > HALF;     // two tiles of rows take each page; otherwise the streams take the pages in turn
+          const int jobs = same(x.seg[i0].count) << (both ? 1 : 0), lead = both ? 2 : 3;
+          for (int i = 0; i < jobs + lead; ++i) {
+            const int j = i - lead;
+            // the queries' barrier, which was passed or has to be, stands for what a job does not need
+            const uint32_t q_phase = segment & 1, k_bar = i < jobs ? k_full + 8 * k_stage : q_full, k_want = i < jobs ? k_phase : q_phase;
+            if (j >= 0) wait3(v_full + 8 * v_stage, v_phase, p_full + 8 * (behind & 3), behind >> 2 & 1, k_bar, k_want);
+            else wait3(q_full, q_phase, q_full, q_phase, k_bar, k_want);
             tm_after();
-            if (!*failed) {
-              const uint64_t vd = descriptor(sbase + S::VALUES + stage * S::PLANE, S::VALUE_CHUNK);
-#pragma unroll
-              for (int k = 0; k < MZP_PAGE / 16; ++k)
-                umma16<D>(tmem + S::TM_O + s * D, tmem + S::TM_S + s * MZP_PAGE + k * 8, vd + k * (256 >> 4), used != (s ? fresh1 : fresh0) || k > 0);
-              umma_commit(bar(x.o_done[s]));
-              if (!both || s == 1) umma_commit(bar(x.v_free[stage]));
-            }
-            used0 += s ^ 1;
-            used1 += s;
-          }
-          if (i < jobs) {
-            const int s = i & 1, page = pages + (both ? i >> 1 : i), stage = page % S::STAGES;
-            if (!both || s == 0) bar_wait(bar(x.k_full[stage]), page / S::STAGES & 1, failed);
-            tm_after();
-            if (!*failed) {
-#pragma unroll
-              for (int plane = 0; plane < 2; ++plane) {
-                const uint64_t kd = descriptor(sbase + S::KEYS + (2 * stage + plane) * S::PLANE, S::KEY_CHUNK);
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-                  umma16<MZP_PAGE>(tmem + S::TM_S + s * MZP_PAGE, tmem + S::TM_Q + s * (D / 2) + k * 8, kd + k * (256 >> 4), plane > 0 || k > 0);
+            // short loops: a scheduler's instruction cache is full of the other duties, and what is executed once a page has to be fetched each time
+            if (j >= 0) {
+              const bool last = !both || (j & 1);
+              const uint32_t vd = values + v_stage * (S::PLANE >> 4), t_o = S::TM_O + (j & 1) * D, t_s = S::tm_s(both) + (both ? j & 1 : v_stage) * MZP_PAGE;
+              if (elect()) {
+#pragma unroll ISSUE_UNROLL
+                for (int k = 0; k < MZP_PAGE / 16; ++k) umma16<D>(t_o, t_s + k * 8, vd + k * OPERAND_STEP, k > 0 || j > 1);
+                umma_commit(o_done + 8 * (behind & 3));
+                if (last) umma_commit(v_free + 8 * v_stage);
               }
-              umma_commit(bar(x.s_full[s]));
-              if (!both || s == 1) umma_commit(bar(x.k_free[stage]));
+              __syncwarp();
+              ++behind;
+              if (last && ++v_stage == S::STAGES) { v_stage = 0; v_phase ^= 1; }
             }
-            bar_arrive(bar(x.s_full[s]));                    // hands on what the keys' writers left beside them
+            if (i < jobs) {
+              const bool last = !both || (i & 1);
+              const uint32_t kd = keys + k_stage * (2 * S::PLANE >> 4), t_q = S::TM_Q + (both ? (i & 1) * (D / 2) : 0), t_s = S::tm_s(both) + (both ? i & 1 : k_stage) * MZP_PAGE;
+              if (elect()) {
+#pragma unroll ISSUE_UNROLL
+                for (int k = 0; k < 2 * D / 16; ++k)         // value, then remainder: the second plane stands behind the first
+                  umma16<MZP_PAGE>(t_s, t_q + k % (D / 16) * 8, kd + k * OPERAND_STEP, k > 0);
+                umma_commit(s_full + 8 * (ahead & 3));
+                if (last) umma_commit(k_free + 8 * k_stage);
+              }
+              __syncwarp();
+              ++ahead;
+              if (last && ++k_stage == S::STAGES) { k_stage = 0; k_phase ^= 1; }
+            }
           }
         }
-        pages += seg.count;
-        ++segment;
+        everyone();
+        everyone();
+      }
+    } else if (warp == FEEDER) {
+      // ---- pages as they are, four ahead; then the next list
+      const uint8_t* store = (const uint8_t*)c.store + (long long)p.layer * c.store_stride_layer;
+      int pages = 0, sent = 0;
+      while (x.segments > 0) {
+        for (int i0 = 0; i0 < x.segments; ++i0) {
+          const Segment seg = x.seg[i0];
+          const int* table = c.block_table + (long long)seg.row * c.width + seg.page;
+          int ids = lane < seg.count ? table[lane] : -1;
+          for (int at = 0; at < seg.count; at += 32) {
+            const int coming = at + 32 + lane < seg.count ? table[at + 32 + lane] : -1;
+            for (int k = 0; k < min(32, seg.count - at); ++k, ++pages) {
+              const int slot = pages % S::RAWS, id = __shfl_sync(0xffffffffu, ids, k);
+              const bool there = id >= 0 && id < c.pages;    // a page that is not there any more has T = 0
+              bar_wait(bar(x.raw_free[slot]), (pages / S::RAWS & 1) ^ 1, failed);
+              const bool fine = !*failed;
+              if (fine) sent = pages + 1;
+              if (fine && elect()) {
+                x.there[slot] = there;
+                if (there) {
+                  const uint8_t* src = store + (long long)id * c.store_stride_page + (long long)seg.head * PB;
+                  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar(x.raw_full[slot])), "n"(PB) : "memory");
+                  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                               ::"r"(sbase + S::RAW + slot * PB), "l"(src), "n"(PB), "r"(bar(x.raw_full[slot])) : "memory");
+                } else {
+                  bar_arrive(bar(x.raw_full[slot]));
+                }
+              }
+              __syncwarp();
+            }
+            ids = coming;
+          }
+        }
+        everyone();                              // the list has been read
+        if (x.more) lister.list(p, x, lane);
+        else if (lane == 0) x.segments = 0;
+        everyone();
+      }
+      // copies land before the CTA ends, whatever else went wrong
+      for (int j = max(0, sent - S::RAWS); j < sent; ++j)
+        for (int k = 0; k < SPIN_LIMIT && !bar_test(bar(x.raw_full[j % S::RAWS]), j / S::RAWS & 1); ++k) {}
+    } else if ((warp & 3) == 3) {
+      // ---- words: the powers of two above a page's largest key and value (f16 has them below 2^14), and of every row of codes {scale, 1024 + zero level, anchor (as pairs), place of
+      // its book}.  Here, and not where the levels are made, as this scheduler has the least to do
+      const uint32_t book = sbase + S::BOOK, terms = sbase + S::TERMS;
+      int page = warp == DECODER ? 0 : 1, pages = 0;
+      while (x.segments > 0) {
+        for (int i0 = 0; i0 < x.segments; ++i0) pages += x.seg[i0].count;
+        for (; page < pages; page += 2) {
+          const int slot = page % S::RAWS;
+          const uint32_t raw = sbase + S::RAW + slot * PB + 32 * D;
+          bar_wait(bar(x.raw_full[slot]), page / S::RAWS & 1, failed);
+          const bool there = x.there[slot];
+          int e[2];
+#pragma unroll
+          for (int side = 0; side < 2; ++side) {             // two f16 numbers (T, and A or z) at a time
+            uint32_t word[D / 32], m = 0;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+              word[i] = there ? lds32(raw + side * 36 * D + 128 * i + 4 * lane) : 0u;
+              m = __vmaxu2(m, word[i] & 0x7fff7fffu);
+            }
+            const uint32_t t_max = warp_max_u32(m & 0xffffu), a_max = warp_max_u32(m >> 16);
+            const float top = fmaf(4.f, __half2float(__ushort_as_half((unsigned short)t_max)), a_max >= 128u ? __half2float(__ushort_as_half((unsigned short)a_max)) : 0.f);
+            e[side] = min(max((int)(__float_as_uint(top) >> 23) - 126, -30), 30) - 14;
+            const float scale = pow2(-e[side]);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+              const MzpRow row = mzp_row(word[i]);
+              const float unit = row.t * scale * 0.03125f, anchor = row.a * scale;
+              sts128(terms + ((slot * 2 + side) * D + 32 * i + lane) * 16, half2_bits(__floats2half2_rn(unit, unit)), (0x6400u | row.z) * 0x10001u,
+                     half2_bits(__floats2half2_rn(anchor, anchor)), book + row.z * 16);
+            }
+          }
+          if (lane == 0) x.scale[page % S::SCALES] = make_int2(e[0], e[1]);
+          __syncwarp();
+          if (lane == 0) bar_arrive(bar(x.scaled[page % S::SCALES]));
+        }
+        everyone();
+        everyone();
+      }
+    } else {
+      // ---- levels: a thread has a row of 64 keys, then one of 64 values (head_dim 64: half of either).  Rolled loops: what all duties execute has to stay near the
+      // schedulers' instruction caches
+      const int member = (warp - SOFTMAX_WARPS) / 4 * 3 + (warp & 3), t = (member & 3) * 32 + lane;
+      constexpr int PIECES = D == 128 ? 2 : 1;               // of 32 codes
+      const int part = t / 64, token = t % 64, ch = t % D;
+      // of keys, of values: the row's number in the page, its place in the operand
+      const int k_row = ch, v_row = D == 128 ? 2 * token + part : token, piece0 = D == 128 ? 0 : part;
+      const uint32_t k_at = sbase + S::KEYS + 128 * ch, v_at = sbase + S::VALUES + (D == 128 ? part * MZP_PAGE * 128 : 0) + 128 * token;
+      const uint32_t k_turn = (ch & 7) << 4, v_turn = (token & 7) << 4, terms = sbase + S::TERMS;
+      int page = member >> 2, pages = 0, slot = page, stage = page;
+      uint32_t raw_phase = 0, phase = 1;
+      // A team that waits for a place has waited for what was in it before: its last page went into a place that was free later than that.  So the parity of a phase is enough
+      static_assert(S::RAWS > TEAMS && S::STAGES >= TEAMS, "a wait could take the phase before the last one for its own");
+      while (x.segments > 0) {
+        for (int i0 = 0; i0 < x.segments; ++i0) pages += x.seg[i0].count;
+        for (; page < pages; page += TEAMS) {
+          const uint32_t raw = sbase + S::RAW + slot * PB;
+          bar_wait(bar(x.scaled[page % S::SCALES]), page / S::SCALES & 1, failed);
+          bar_wait(bar(x.raw_full[slot]), raw_phase, failed);
+          bar_wait(bar(x.k_free[stage]), phase, failed);
+          {
+            const uint4 term = lds128(terms + (slot * 2 * D + k_row) * 16), book = book128(term.w);
+            const __half2 step = bits_half2(term.x), zero = bits_half2(term.y);
+            const uint32_t at = k_at + 2 * stage * S::PLANE;
+            if (!__any_sync(0xffffffffu, term.z)) {
+#pragma unroll 1
+              for (int piece = piece0; piece < piece0 + PIECES; ++piece) {
+                const uint4 codes = lds128(raw + 32 * k_row + 16 * piece);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {    // eight tokens
+                  uint32_t u[4], lo[4];
+                  levels8((&codes.x)[q], book, u);
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const __half2 w = __hsub2(bits_half2(u[k]), zero), h = __hmul2(w, step);
+                    u[k] = half2_bits(h);
+                    lo[k] = half2_bits(__hfma2(w, step, __hneg2(h)));      // exact
+                  }
+                  const uint32_t dst = at + ((64 * piece + 16 * q) ^ k_turn);
+                  sts128(dst, u[0], u[1], u[2], u[3]);
+                  sts128(dst + S::PLANE, lo[0], lo[1], lo[2], lo[3]);
+                }
+              }
+            } else {                             // rows that do not straddle zero: the sum has more than 22 bits' worth of terms, so in fp32
+              const float unit = __low2float(step), anchor = __low2float(bits_half2(term.z));
+#pragma unroll 1
+              for (int piece = piece0; piece < piece0 + PIECES; ++piece) {
+                const uint4 codes = lds128(raw + 32 * k_row + 16 * piece);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  uint32_t u[4], lo[4];
+                  levels8((&codes.x)[q], book, u);
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const float2 w = __half22float2(__hsub2(bits_half2(u[k]), zero));
+                    const float a = fmaf(w.x, unit, anchor), b = fmaf(w.y, unit, anchor);
+                    const __half2 h = __floats2half2_rn(a, b);
+                    const float2 f = __half22float2(h);
+                    u[k] = half2_bits(h);
+                    lo[k] = half2_bits(__floats2half2_rn(a - f.x, b - f.y));
+                  }
+                  const uint32_t dst = at + ((64 * piece + 16 * q) ^ k_turn);
+                  sts128(dst, u[0], u[1], u[2], u[3]);
+                  sts128(dst + S::PLANE, lo[0], lo[1], lo[2], lo[3]);
+                }
+              }
+            }
+          }
+          fence_operands();
+          __syncwarp();
+          if (lane == 0) bar_arrive(bar(x.k_full[stage]));
+          bar_wait(bar(x.v_free[stage]), phase, failed);
+          {
+            const uint4 term = lds128(terms + ((slot * 2 + 1) * D + v_row) * 16), book = book128(term.w);
+            const __half2 step = bits_half2(term.x), zero = bits_half2(term.y), base = bits_half2(term.z);
+            const uint32_t at = v_at + stage * S::PLANE;
+#pragma unroll 1
+            for (int piece = piece0; piece < piece0 + PIECES; ++piece) {
+              const uint4 codes = lds128(raw + 36 * D + 32 * v_row + 16 * piece);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {      // eight channels
+                uint32_t u[4];
+                levels8((&codes.x)[q], book, u);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) u[k] = half2_bits(__hfma2(__hsub2(bits_half2(u[k]), zero), step, base));
+                sts128(at + ((64 * piece + 16 * q) ^ v_turn), u[0], u[1], u[2], u[3]);
+              }
+            }
+          }
+          fence_operands();
+          __syncwarp();
+          if (lane == 0) {
+            bar_arrive(bar(x.v_full[stage]));
+            bar_arrive(bar(x.raw_free[slot]));
+          }
+          slot += TEAMS;
+          if (slot >= S::RAWS) { slot -= S::RAWS; raw_phase ^= 1; }
+          stage += TEAMS;
+          if (stage >= S::STAGES) { stage -= S::STAGES; phase ^= 1; }
+        }
+        everyone();
+        everyone();
       }
     }
-  } else if (warp < SOFTMAX_WARPS) {
+  } else {
     // ---- softmax: a thread has a query row
     registers<SOFTMAX_REGS, true>();
     const int s = warp >> 2, r = (warp & 3) * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_s = lanes + S::TM_S + s * MZP_PAGE, t_o = lanes + S::TM_O + s * D;
-    int pages = 0, segment = 0, done = 0;
-    while (walk.next(seg)) {
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_o = lanes + S::TM_O + s * D;
+    int pages = 0, first_job = 0;                            // of the CTA so far
+    while (x.segments > 0) {
+    for (int i0 = 0; i0 < x.segments; ++i0) {
+      const Segment seg = x.seg[i0];
       const bool both = seg.rows > HALF;
       const int m = (both ? s * HALF : 0) + r;               // row of the tile
       const bool here = m < seg.rows;
@@ -377,7 +636,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
             const float a = mz_u16_to_float((uint16_t)(w & 0xffffu), DT) * down1 * down2, b2 = mz_u16_to_float((uint16_t)(w >> 16), DT) * down1 * down2;
             v[i] = wild ? 0x7fff7fffu : half2_bits(__floats2half2_rn(a, b2));
           }
-          tm_store32(lanes + S::TM_Q + s * (D / 2) + 32 * h, v);
+          if (both || s == 0) tm_store32(lanes + S::TM_Q + s * (D / 2) + 32 * h, v);
         }
         tm_stored();
         tm_before();
@@ -385,70 +644,94 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
         if (lane == 0) bar_arrive(bar(x.q_full));
       }
       float M = -INFINITY, l = 0.f;
-      const int mine = both ? seg.count : (seg.count + 1 - s) / 2;         // jobs of this stream
+      const int jobs = both ? 2 * seg.count : seg.count, mine = (jobs + 1 - s) / 2;        // of the segment, of this stream
       for (int j = 0; j < mine; ++j) {
-        const int page = pages + (both ? j : 2 * j + s);
-        bar_wait(bar(x.s_full[s]), done & 1, failed);
+        const int i = 2 * j + s, job = first_job + i, page = pages + (both ? j : i);
+        const uint32_t t_s = lanes + S::tm_s(both) + (both ? s : page % S::STAGES) * MZP_PAGE;
+        bar_wait(bar(x.scaled[page % S::SCALES]), page / S::SCALES & 1, failed);
+        bar_wait(bar(x.s_full[job & 3]), job >> 2 & 1, failed);
         tm_after();
         if (some) {
           const int2 sc = x.scale[page % S::SCALES];
           const float f = rowf * pow2(sc.x), ev = (float)sc.y;
-          uint32_t v0[32], v1[32];
-          tm_load32(v0, t_s);
-          tm_load32(v1, t_s + 32);
-          tm_loaded(v0);
-          tm_loaded(v1);
-          float top = -INFINITY;
+          // P under the maximum so far, of the first pages' logits: its sum stays below 2^15 unless that is passed by 8 or so.  Then the maximum is found and P taken once more
+          uint32_t w[32];
+          float total = 0.f;
+          bool known = j > 0;
+          for (int turn = 0;; ++turn) {
+            if (known) {
+              const float add = ev + 7.f - (M == -INFINITY ? 0.f : M);
+              float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top = fmaxf(top, fmaxf(__uint_as_float(v0[i]), __uint_as_float(v1[i])));
-          const float t = fmaf(top, f, ev);
-          if (j == 0) {
-            M = t;
-          } else {
-            const bool more = t > M + 8.f;
-            if (__any_sync(0xffffffffu, more)) {
-              const float to = more ? t : M, fix = more ? ex2(M - to) : 1.f;
-              M = to;
-              l *= fix;
-              bar_wait(bar(x.o_done[s]), (done - 1) & 1, failed);        // the stream's last product is in
-              tm_after();
+              for (int h = 0; h < 2; ++h) {
+                uint32_t v[32];
+                tm_load32(v, t_s + 32 * h);
+                tm_loaded(v);
 #pragma unroll
-              for (int h = 0; h < D / 32; ++h) {
-                uint32_t o[32];
-                tm_load32(o, t_o + 32 * h);
-                tm_loaded(o);
+                for (int i = 0; i < 32; i += 4) {
+                  float a = __uint_as_float(v[i]), b = __uint_as_float(v[i + 1]), c2 = __uint_as_float(v[i + 2]), d = __uint_as_float(v[i + 3]);
+                  mul_add2(a, b, f, add);
+                  mul_add2(c2, d, f, add);
+                  a = ex2(a); b = ex2(b); c2 = ex2(c2); d = ex2(d);
+                  w[16 * h + i / 2] = half2_bits(__floats2half2_rn(a, b));
+                  w[16 * h + i / 2 + 1] = half2_bits(__floats2half2_rn(c2, d));
+                  add2(sum[0], sum[1], a, b);
+                  add2(sum[2], sum[3], c2, d);
+                }
+              }
+              total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+              if (turn > 0 || !__any_sync(0xffffffffu, !(total <= 32768.f))) break;
+            }
+            float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+              uint32_t v[32];
+              tm_load32(v, t_s + 32 * h);
+              tm_loaded(v);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
-                tm_store32(t_o + 32 * h, o);
+              for (int i = 0; i < 32; i += 4) {
+                top0 = max3(top0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                top1 = max3(top1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
               }
             }
-          }
-          const float add = ev + 7.f - (M == -INFINITY ? 0.f : M);
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t w[32];
+            const float t = fmaf(fmaxf(top0, top1), f, ev);
+            if (!known) {
+              M = t;
+              known = true;
+              continue;
+            }
+            const bool more = !(total <= 32768.f) && t > M;  // where the sum is NaN it stays
+            const float fix = more ? ex2(M - t) : 1.f;
+            if (more) M = t;
+            l *= fix;
+            bar_wait(bar(x.o_done[(job - 2) & 3]), (job - 2) >> 2 & 1, failed);          // the stream's last product is in
+            tm_after();
+#pragma unroll 1
+            for (int h = 0; h < D / 32; ++h) {
+              uint32_t o[32];
+              tm_load32(o, t_o + 32 * h);
+              tm_loaded(o);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float a = ex2(fmaf(__uint_as_float(v0[i]), f, add)), b = ex2(fmaf(__uint_as_float(v0[i + 1]), f, add));
-            const float c2 = ex2(fmaf(__uint_as_float(v1[i]), f, add)), d = ex2(fmaf(__uint_as_float(v1[i + 1]), f, add));
-            w[i / 2] = half2_bits(__floats2half2_rn(a, b));
-            w[16 + i / 2] = half2_bits(__floats2half2_rn(c2, d));
-            add2(sum[0], sum[1], a, b);
-            add2(sum[2], sum[3], c2, d);
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+              tm_store32(t_o + 32 * h, o);
+            }
           }
-          tm_store32(t_s, w);
-          l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2(-sc.y - 7), l);
+          tm_store32(t_s, w);                    // over logits that have been read
+          l = fmaf(total, pow2(-sc.y - 7), l);
           tm_stored();
         }
         tm_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(bar(x.p_full[s]));
-        ++done;
+        if (lane == 0) bar_arrive(bar(x.p_full[job & 3]));
       }
       // ---- records
-      if (mine > 0) bar_wait(bar(x.o_done[s]), (done - 1) & 1, failed);
+      if (mine > 0) {
+        const int job = first_job + 2 * (mine - 1) + s;
+        bar_wait(bar(x.o_done[job & 3]), job >> 2 & 1, failed);
+      }
       tm_after();
       const bool bad = *failed != 0;
-      const long long at = seg.record + (long long)MZP_TILE_ROWS * cta + m;
+      const long long at = seg.record + m;
       const bool inside = here && MZ_IN_BOUNDS(at, p.out.records, 21);
       float f_mine = 0.0078125f, f_other = 0.f;              // P has 2^7
       uint32_t t_other = t_o;
@@ -490,138 +773,18 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
       tm_before();
       if (!both) asm volatile("bar.sync 1, 256;" ::: "memory");          // x.ml is free again
       pages += seg.count;
-      ++segment;
+      first_job += jobs;
     }
-  } else {
-    // ---- levels: four warps have a page, the other four the next one
-    const int team = (warp - SOFTMAX_WARPS) >> 2, t = (warp & 3) * 32 + lane;
-    const uint8_t* store = (const uint8_t*)c.store + (long long)p.layer * c.store_stride_layer;
-    constexpr int WPL = D / 32;                              // words per lane: all of a side
-    struct Raw { uint32_t kc[8], vc[8], kw, vw, all[2 * WPL]; };
-    const bool keys = D == 128 || t < 64, values = D == 128 || t >= 64;
-    const int ch = t % D, token = t % MZP_PAGE, part = D == 128 ? t / MZP_PAGE : 0;
-    int at = team;                                           // page of the segment
-    bool more = walk.next(seg);
-    auto settle = [&]() {
-      while (more && at >= seg.count) { at -= seg.count; more = walk.next(seg); }
-    };
-    settle();
-    auto page_of = [&]() {                                   // of the cursor; -1: none.  What is added: its head's place
-      long long place = -1;
-      if (more) {
-        const int id = c.block_table[(long long)seg.row * c.width + seg.page + at];
-        if (id >= 0 && id < c.pages) place = (long long)id * c.store_stride_page + (long long)seg.head * PB;
-        else place = -2;                                     // not there any more: T = 0
-      }
-      at += 2;
-      settle();
-      return place;
-    };
-    auto load = [&](Raw& w, long long place) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w.kc[i] = w.vc[i] = 0;
-      w.kw = w.vw = 0;
-#pragma unroll
-      for (int i = 0; i < 2 * WPL; ++i) w.all[i] = 0;
-      if (place < 0) return;
-      const uint8_t* b = store + place;
-      const int row = token * (D / 64) + part;
-      if (keys) { ldg256(w.kc, b + 32 * ch); w.kw = __ldg((const uint32_t*)(b + 32 * D + 4 * ch)); }
-      if (values) { ldg256(w.vc, b + 36 * D + 32 * row); w.vw = __ldg((const uint32_t*)(b + 68 * D + 4 * row)); }
-#pragma unroll
-      for (int i = 0; i < WPL; i += 2) {
-        const uint2 a = __ldg((const uint2*)(b + 32 * D) + (lane * WPL + i) / 2), v = __ldg((const uint2*)(b + 68 * D) + (lane * WPL + i) / 2);
-        w.all[i] = a.x; w.all[i + 1] = a.y;
-        w.all[WPL + i] = v.x; w.all[WPL + i + 1] = v.y;
-      }
-    };
-    // the power of two above a side's largest value; f16 has its values below 2^14
-    auto exponent = [&](const uint32_t* words) {
-      float top = 0.f;
-#pragma unroll
-      for (int i = 0; i < WPL; ++i) {
-        const MzpRow row = mzp_row(words[i]);
-        top = fmaxf(top, fmaf(4.f, fabsf(row.t), fabsf(row.a)));
-      }
-      return min(max((int)(warp_max_u32(__float_as_uint(top)) >> 23) - 126, -30), 30) - 14;
-    };
-    long long place = page_of(), ahead = place == -1 ? -1 : page_of();
-    Raw now;
-    load(now, place);
-    for (int page = team; place != -1; page += 2) {
-      Raw next;
-      load(next, ahead);
-      const long long far = ahead == -1 ? -1 : page_of();
-      const int stage = page % S::STAGES;
-      const uint32_t parity = (page / S::STAGES & 1) ^ 1;
-      const int ek = exponent(now.all), ev = exponent(now.all + WPL);
-      bar_wait(bar(x.k_free[stage]), parity, failed);
-      if (t == 0) x.scale[page % S::SCALES] = make_int2(ek, ev);
-      if (keys) {
-        const MzpRow row = mzp_row(now.kw);
-        const uint4 book = book128(sbook + row.z * 16);
-        const float unit = row.t * pow2(-ek) * 0.03125f, anchor = row.a * pow2(-ek);
-        const __half2 zero = __floats2half2_rn(1024.f + row.z, 1024.f + row.z), step = __floats2half2_rn(unit, unit);
-        const uint32_t hi_at = sbase + S::KEYS + 2 * stage * S::PLANE + ch * 16, lo_at = hi_at + S::PLANE;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {            // eight tokens
-          uint32_t u[4], hi[4], lo[4];
-          levels8(now.kc[q], book, u);
-          if (row.a == 0.f) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const __half2 w = __hsub2(bits_half2(u[k]), zero), h = __hmul2(w, step);
-              hi[k] = half2_bits(h);
-              lo[k] = half2_bits(__hfma2(w, step, __hneg2(h)));            // exact
-            }
-          } else {                               // the sum has more than 22 bits' worth of terms: in fp32
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 w = __half22float2(__hsub2(bits_half2(u[k]), zero));
-              const float a = fmaf(w.x, unit, anchor), b = fmaf(w.y, unit, anchor);
-              const __half2 h = __floats2half2_rn(a, b);
-              const float2 f = __half22float2(h);
-              hi[k] = half2_bits(h);
-              lo[k] = half2_bits(__floats2half2_rn(a - f.x, b - f.y));
-            }
-          }
-          sts128(hi_at + q * S::KEY_CHUNK, hi[0], hi[1], hi[2], hi[3]);
-          sts128(lo_at + q * S::KEY_CHUNK, lo[0], lo[1], lo[2], lo[3]);
-        }
-      }
-      fence_operands();
-      __syncwarp();
-      if (lane == 0) bar_arrive(bar(x.k_full[stage]));
-      bar_wait(bar(x.v_free[stage]), parity, failed);
-      if (values) {
-        const MzpRow row = mzp_row(now.vw);
-        const uint4 book = book128(sbook + row.z * 16);
-        const float unit = row.t * pow2(-ev) * 0.03125f, anchor = row.a * pow2(-ev);
-        const __half2 zero = __floats2half2_rn(1024.f + row.z, 1024.f + row.z), step = __floats2half2_rn(unit, unit), base = __floats2half2_rn(anchor, anchor);
-        const uint32_t dst = sbase + S::VALUES + stage * S::PLANE + part * 8 * S::VALUE_CHUNK + token * 16;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {            // eight channels
-          uint32_t u[4];
-          levels8(now.vc[q], book, u);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) u[k] = half2_bits(__hfma2(__hsub2(bits_half2(u[k]), zero), step, base));
-          sts128(dst + q * S::VALUE_CHUNK, u[0], u[1], u[2], u[3]);
-        }
-      }
-      fence_operands();
-      __syncwarp();
-      if (lane == 0) bar_arrive(bar(x.v_full[stage]));
-      now = next;
-      place = ahead;
-      ahead = far;
+    everyone();
+    everyone();
     }
   }
-  if (warp == ISSUER && lane == 0) {          // the products are done, and so is what they signal
+  if (warp == ISSUER && elect()) {               // the products are done, and so is what they signal
     umma_commit(bar(x.end));
     for (int k = 0; k < SPIN_LIMIT && !bar_test(bar(x.end), 0); ++k) {}
   }
   tm_before();
-  __syncthreads();
+  everyone();
   if (warp == ISSUER) {
     tm_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::TM_COLS));

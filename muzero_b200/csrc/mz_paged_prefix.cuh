@@ -51,7 +51,7 @@ struct MzpUnits {
       : g(p.groups[p.group_of[b]]), before(p.sums[p.group_of[b]]), tiles(g.rows), line(p.sums[p.n_groups].steps, p.grid), qrows(query_rows), kv_heads(heads) {}
   __device__ __forceinline__ int row_of(int b, int query_row) const { return (b - g.first) * qrows + query_row; }
   // record of a query row of the group without its CTA's share of 256 c, and the CTAs that have one
-  __device__ __forceinline__ long long record(int head, int row, long long& first, long long& last) const {
+  __device__ __forceinline__ long long record(int head, int row, int& first, int& last) const {
     const int tile = row / tiles.rows;
     const long long at = before.steps + (long long)(head * tiles.count + tile) * g.pages * tiles.weight;
     first = line.owner(at);
