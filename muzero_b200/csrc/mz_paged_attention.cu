@@ -56,6 +56,8 @@ struct Args {
   MzpPrefix pre;                                 // pre.skip NULL: a window
 };
 
+// pages that an entry's group has taken care of; none where the call was found not worth it
+__device__ __forceinline__ int shared_pages(const Args& p, int b, int pages) { return p.pre.sums[p.pre.n_groups].steps > 0 ? min(p.pre.skip[b], pages) : 0; }
 // The pages of a list entry that a pass goes through: `heads` of its first ones (sinks), then those from `first` on
 struct Reach { int count, heads, first; };
 template <bool VIEW>
@@ -65,7 +67,7 @@ __device__ __forceinline__ Reach reach_of(const Args& p, int b, int len) {
   Reach x;
   if (p.pre.skip) {
     x.heads = 0;
-    x.first = min(p.pre.skip[b], pages);
+    x.first = shared_pages(p, b, pages);
   } else {
     const int lo = len - p.q_len + 1 - p.window;           // the first query's window begins here
     x.heads = min((int)(((long long)p.sinks + MZP_PAGE - 1) / MZP_PAGE), pages);
@@ -876,7 +878,7 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
       }
     }
   }
-  if (VIEW && p.pre.skip && tid < NR && p.pre.skip[b] > 0) {
+  if (VIEW && p.pre.skip && tid < NR && shared_pages(p, b, 1) > 0) {
     Share s = {0, 0, -1};
     if (r0 + tid < p.qrows) {
       const MzpUnits units(p.pre, b, p.qrows, c.kv_heads);
@@ -897,7 +899,7 @@ __global__ void __launch_bounds__(END_THREADS, 2) finish_kernel(const Args p) {
     a[i] = a[i] * f + v * h;
     m[i] = top;
   };
-  if (VIEW && p.pre.skip && p.pre.skip[b] > 0) {             // what the row shares with its group: records of whole tiles of query rows, there since before the first kernel
+  if (VIEW && p.pre.skip && shared_pages(p, b, 1) > 0) {             // what the row shares with its group: records of whole tiles of query rows, there since before the first kernel
     long long slot[ROWS];
     int first[ROWS], last[ROWS], lo = 0x7fffffff, hi = -1;
 #pragma unroll
@@ -1000,7 +1002,7 @@ int launch(const Args& p, const uint8_t* book, int G, cudaStream_t st) {
   return MZ_OK;
 }
 
-struct Shape { int nr, passes, sms, per_sm, G; long long pairs; size_t head_bytes, slots, prefix_at, bytes; };
+struct Shape { int nr, passes, sms, per_sm, G; bool shares; long long pairs; size_t head_bytes, slots, prefix_at, bytes; };
 // pages: the most of a row that a call goes through
 int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, long long pages, Shape* s) {
   MZ_REQUIRE(batch >= 0 && batch <= MAX_BATCH, "batch %d (at most %d)", batch, MAX_BATCH);
@@ -1012,6 +1014,7 @@ int shape_of(const mz_paged_cache* c, int batch, int q_len, int q_heads, long lo
   // 8 query rows to a step where there are more than 4: 64 x 8 x 4224 tokens, head_dim 128, with 5 / 8 of them 163 / 167 us against 235 / 239 in two passes of 4, with 12
   // 300 against 341 in three; with 1 / 4 of them 157 / 161 us against 130 / 134 in a step of 4.  The same order for two long rows (138 / 189, 134 / 112) and at head_dim 64;
   // one row of 500 tokens takes 17 to 21 us either way.
+  s->shares = false;
   s->nr = qrows <= 4 ? 4 : 8;
   s->passes = (int)((qrows + s->nr - 1) / s->nr);
   s->pairs = (long long)batch * c->kv_heads * s->passes;
@@ -1042,6 +1045,9 @@ int shape_of(const mz_paged_cache* c, const mz_paged_view* view, int batch, int 
   if (view->window > 0) most = std::min<long long>(most, ((long long)view->window + q_len) / MZP_PAGE + 2 + ((long long)view->sinks + MZP_PAGE - 1) / MZP_PAGE);
   const int rc = shape_of(c, batch, q_len, q_heads, most, s);
   if (rc != MZ_OK || view->n_groups == 0) return rc;
+  // rows whose tables cannot hold enough to share are attended as without groups
+  s->shares = mzp_gain(c->width, c->kv_heads, (long long)batch * s->passes, s->nr, 0) >= mzp_gain_needed(s->sms, c->head_dim);
+  if (!s->shares) return MZ_OK;
   s->prefix_at = (s->bytes + 127) / 128 * 128;
   mzp_prefix_shape(c, batch, view->n_groups, q_heads / c->kv_heads * q_len, s->sms, ps);
   s->bytes = s->prefix_at + ps->bytes;
@@ -1063,7 +1069,7 @@ int attend(const mz_paged_cache* cache, int layer, const mz_paged_attention_args
   MZ_REQUIRE((uintptr_t)args->query % 16 == 0 && (args->q_stride_b | args->q_stride_l | args->q_stride_h) % 8 == 0,
              "query must be 16-byte aligned with strides in multiples of 8 elements");
   MZ_REQUIRE(!view || view->n_groups == 0 || view->groups, "groups is NULL");
-  const int whole = view && view->n_groups > 0 ? 32 : 16;              // records of groups are written 32 bytes at a time
+  const int whole = s.shares ? 32 : 16;                                             // records of groups are written 32 bytes at a time
   if (!args->workspace || (uintptr_t)args->workspace % whole != 0 || args->workspace_bytes < s.bytes)
     return mz_fail(MZ_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed (%d-byte aligned)", args->workspace_bytes, s.bytes, whole);
   const uint8_t* book = nullptr;
@@ -1090,13 +1096,13 @@ int attend(const mz_paged_cache* cache, int layer, const mz_paged_attention_args
   p.slots = (long long)s.slots;
   p.fail_waits = mz_waits_fail();
   cudaStream_t st = (cudaStream_t)stream;
-  const bool viewed = view && (view->window > 0 || view->n_groups > 0);
+  const bool viewed = view && (view->window > 0 || s.shares);
   p.window = 0x7fffffff - (1 << 21);             // the most: positions less this stay 32-bit numbers
   if (viewed && view->window > 0) {
     p.window = std::min(view->window, p.window);
     p.sinks = view->sinks;
   } else if (viewed) {
-    if ((rc = mzp_prefix_launch(*cache, layer, *args, *view, ps, (uint8_t*)args->workspace + s.prefix_at, p.longest, book, st, &p.pre)) != MZ_OK) return rc;
+    if ((rc = mzp_prefix_launch(*cache, layer, *args, *view, ps, (uint8_t*)args->workspace + s.prefix_at, p.longest, s.nr, s.passes, book, st, &p.pre)) != MZ_OK) return rc;
   }
   const bool bf = cache->kv_dtype == MZ_BF16;
 #define MZP_VIEW(D, BF, NR) return viewed ? launch<D, BF, NR, true>(p, book, s.G, st) : launch<D, BF, NR, false>(p, book, s.G, st)

@@ -104,6 +104,9 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
     asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(theirs) : "memory");
     common = min(common, v);
   }
+  const int entries = end - first;
+  const MzpTiles tiles(entries * p.qrows);
+  if (mzp_gain(common, c.kv_heads, (long long)entries * p.out.passes, p.out.nr, tiles.weight * tiles.count) == 0) common = 0;
   for (int b = first + rank * PLAN_THREADS + tid; b < end; b += PLAN_CTAS * PLAN_THREADS) { p.out.skip[b] = common; p.out.group_of[b] = g; }
   if (rank == 0 && tid == 0) p.out.groups[g] = {first, (end - first) * p.qrows, end > first ? common : 0, row0};
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");      // nobody's shared memory goes while it is read
@@ -217,17 +220,27 @@ struct Lister {
         re = info.pages > 0 ? (long long)info.rows * p.c.kv_heads : 0;
       }
     };
-    long long st, re, total = 0;
-    for (int i = lane; i < n; i += 32) { size(i, st, re); total += st; }
+    long long st, re, total = 0, gain = 0;
+    for (int i = lane; i < n; i += 32) {
+      size(i, st, re);
+      total += st;
+      const MzpGroup info = p.out.groups[i];
+      const MzpTiles tiles(info.rows);
+      gain += mzp_gain(info.pages, p.c.kv_heads, (long long)(info.rows / p.qrows) * p.out.passes, p.out.nr, tiles.weight * tiles.count);
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      gain += __shfl_xor_sync(0xffffffffu, gain, o);
+    }
+    if (gain < mzp_gain_needed(p.out.sms, p.c.head_dim)) total = 0;      // then nothing is shared, and the other kernels see that
     const MzpLine line(total, gridDim.x);
     const bool some = cta < line.ctas;
     f0 = some ? line.start(cta) : 0;
     f1 = some ? line.start(cta + 1) : 0;
     long long before_s = 0, before_r = 0;
     g = n;
-    for (int i0 = 0; i0 < n && (cta == 0 || g == n); i0 += 32) {
+    for (int i0 = 0; i0 < n && total > 0 && (cta == 0 || g == n); i0 += 32) {
       size(i0 + lane, st, re);
       long long ss = st, rr = re;
 #pragma unroll
@@ -825,7 +838,7 @@ void mzp_prefix_shape(const mz_paged_cache* c, int batch, int n_groups, int qrow
 }
 
 int mzp_prefix_launch(const mz_paged_cache& c, int layer, const mz_paged_attention_args& args, const mz_paged_view& view, const MzpPrefixShape& s, uint8_t* workspace,
-                      int longest, const uint8_t* book, cudaStream_t stream, MzpPrefix* out) {
+                      int longest, int nr, int passes, const uint8_t* book, cudaStream_t stream, MzpPrefix* out) {
   mzp::PrefixArgs p = {};
   p.c = c;
   p.query = (const uint16_t*)args.query;
@@ -845,7 +858,9 @@ int mzp_prefix_launch(const mz_paged_cache& c, int layer, const mz_paged_attenti
   p.out.ml = (float2*)(workspace + s.ml_at);
   p.out.acc = (float*)(workspace + s.acc_at);
   p.out.n_groups = view.n_groups;
-  p.out.grid = s.grid;
+  p.out.grid = p.out.sms = s.grid;               // a CTA per multiprocessor
+  p.out.nr = nr;
+  p.out.passes = passes;
   p.out.records = s.records;
   p.fail_waits = mz_waits_fail();
   *out = p.out;

@@ -20,6 +20,7 @@ struct MzpPrefix {
   float2* ml;                                    // [record] maximum (base 2) and sum
   float* acc;                                    // [record][D]
   int n_groups, grid;
+  int nr, passes, sms;                           // of the call without sharing: query rows to a step, steps per page
   long long records;
 };
 
@@ -32,6 +33,14 @@ struct MzpTiles {
     weight = rows > MZP_TILE_ROWS / 2 ? 2 : 1;
   }
 };
+// Whether sharing pays.  A page of a prefix costs one kv head 3.0 ns of the machine per row and pass without sharing (4.2 with 8 query rows to a step; head_dim 64: 2.0 and 2.8) and 6.5 ns
+// per weight with it (4.4), and a call that shares takes 25 to 30 us more in the first place.  In tenths of a row's visit to a page; measured on both sides, 32 query heads on 8 kv heads,
+// without / with: 8 rows of 4096 tokens 37 / 57 us, of 16384 71 / 64, 4 rows of 16384 48 / 61, of 65536 115 / 102, 64 rows of 1024 61 / 76, of 2048 84 / 84, of 4096 129 / 88.
+__host__ __device__ __forceinline__ long long mzp_gain(long long pages, int kv_heads, long long rows_passes, int nr, int weights) {
+  const long long each = rows_passes * (nr > 4 ? 14 : 10) - 22ll * weights;
+  return each > 0 ? pages * kv_heads * each : 0;
+}
+__host__ __device__ __forceinline__ long long mzp_gain_needed(int sms, int head_dim) { return (long long)sms * (head_dim == 128 ? 740 : 900); }
 // how the line is cut
 struct MzpLine {
   long long total, ctas;
@@ -64,4 +73,4 @@ struct MzpPrefixShape { int grid; long long records; size_t skip_at, group_of_at
 void mzp_prefix_shape(const mz_paged_cache* c, int batch, int n_groups, int qrows, int sms, MzpPrefixShape* s);
 // Finds the prefixes of the groups and takes the attention of their rows over them; fills `out`.  longest: no row is taken for longer.
 int mzp_prefix_launch(const mz_paged_cache& c, int layer, const mz_paged_attention_args& args, const mz_paged_view& view, const MzpPrefixShape& s, uint8_t* workspace,
-                      int longest, const uint8_t* book, cudaStream_t stream, MzpPrefix* out);
+                      int longest, int nr, int passes, const uint8_t* book, cudaStream_t stream, MzpPrefix* out);

@@ -1,21 +1,22 @@
 // Paged cache: tokens back as ordinary keys and values (sm_100a).
 //
 // A value is A + T (level - z) / 32 (mz_paged.cuh), computed with one fp32 rounding and rounded once to the output's type.  What bounds it is memory: a token's 144
-// bytes of codes and words (head_dim 128, 16-bit output) become 512.  A CTA has a piece of an entry, the tokens of one page, for one kv head.  Keys stand
-// along tokens: a thread takes 16 tokens of four neighbouring channels, so that a warp's store is a token's whole row and nothing is transposed through shared memory.  Values stand along channels: a thread takes eight
-// of a token's, a warp's store is two tokens' rows (head_dim 128).
+// bytes of codes and words (head_dim 128, 16-bit output) become 512.  A CTA has a piece of an entry, the tokens of one page, for some of the kv heads, one after the other, the
+// next one's codes on their way meanwhile.  Keys stand along tokens: a thread of the first half takes 16 tokens of four neighbouring channels, so that a warp's store is a token's
+// whole row and nothing is transposed through shared memory.  Values stand along channels: a thread of the second half takes eight of a token's, a warp's store is two tokens' rows
+// (head_dim 128).
 #include <algorithm>
 
 #include "mz_paged_device.cuh"
 
 namespace mzp {
 namespace {
-constexpr int READ_THREADS = 128, READ_MAX_BATCH = 4096;
+constexpr int READ_THREADS = 256, SIDE_THREADS = READ_THREADS / 2, READ_MAX_BATCH = 4096, READ_CTAS = 4, CTAS_PER_SM = 8;
 
 struct ReadArgs {
   mz_paged_cache c;
   mz_paged_read_args a;
-  int layer, longest;
+  int layer, longest, heads;                     // heads: of a CTA
 };
 
 // Four codes -> their levels less z, as f16 pairs (0x6400 + level is 1024 + level)
@@ -52,15 +53,15 @@ __device__ __forceinline__ void put8(void* p, long long at, const float (&v)[8])
 
 // DT: the output's type; BF: the ring's
 template <int D, int DT, bool BF>
-__global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadArgs p, const uint8_t* __restrict__ book_table) {
+__global__ void __launch_bounds__(READ_THREADS, READ_CTAS) read_kernel(const ReadArgs p, const uint8_t* __restrict__ book_table) {
   const mz_paged_cache& c = p.c;
   const mz_paged_read_args& a = p.a;
   constexpr int PB = 72 * D;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, head = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, head0 = blockIdx.y * p.heads, head1 = min(head0 + p.heads, c.kv_heads);
   __shared__ __align__(16) uint8_t s_book[MZP_BOOKS * MZP_LEVELS];
   __shared__ int s_warp[READ_THREADS / 32], s_entry, s_piece;
-  ((uint4*)s_book)[tid] = ((const uint4*)book_table)[tid];
-  static_assert(READ_THREADS == MZP_BOOKS * MZP_LEVELS / 16, "one piece of the books per thread");
+  if (tid < MZP_BOOKS * MZP_LEVELS / 16) ((uint4*)s_book)[tid] = ((const uint4*)book_table)[tid];
+  static_assert(READ_THREADS >= MZP_BOOKS * MZP_LEVELS / 16, "one piece of the books per thread");
   // ---- the entry and its piece: pieces are the pages that an entry's tokens stand in, or would
   auto pieces_of = [&](int i) {
     const long long first = a.first ? a.first[i] : 0, n = (long long)a.offsets[i + 1] - a.offsets[i];
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadArgs p, co
   // the page's tokens lo .. hi - 1 are asked for
   const int lo = (int)max(0ll, max(first - t0, -(place0 + t0)));
   const int hi = (int)max(0ll, min((long long)MZP_PAGE, min(a.offsets[entry + 1], a.tokens) - (place0 + t0)));
-  const long long k_at = (place0 + t0) * a.k_stride_token + head * a.k_stride_head, v_at = (place0 + t0) * a.v_stride_token + head * a.v_stride_head;
+  const long long k_at = (place0 + t0) * a.k_stride_token, v_at = (place0 + t0) * a.v_stride_token;
   int id = -1;
   if (t0 < packed) {
     const long long page = t0 / MZP_PAGE;
@@ -104,15 +105,15 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadArgs p, co
     if (id < 0 || id >= c.pages) { id = -1; if (tid == 0) atomicOr(c.status, MZ_PAGED_BAD_INDEX); }
   }
   if (id < 0) {                                  // the ring's tokens; what is not there is zero
-    const uint16_t* ring = (const uint16_t*)c.tail + (long long)p.layer * c.tail_stride_layer + (long long)row * c.tail_stride_row + (long long)head * c.ring * D;
+    const uint16_t* ring = (const uint16_t*)c.tail + (long long)p.layer * c.tail_stride_layer + (long long)row * c.tail_stride_row;
     const long long side = (long long)c.kv_heads * c.ring * D;
-    for (int i = tid; i < 2 * MZP_PAGE * D / 8; i += READ_THREADS) {
-      const int value = i / (MZP_PAGE * D / 8), t = i / (D / 8) % MZP_PAGE, ch = i % (D / 8) * 8;
+    for (int i = tid; i < 2 * MZP_PAGE * D / 8 * (head1 - head0); i += READ_THREADS) {
+      const int ch = i % (D / 8) * 8, t = i / (D / 8) % MZP_PAGE, value = i / (MZP_PAGE * D / 8) & 1, head = head0 + i / (2 * MZP_PAGE * D / 8);
       if (t < lo || t >= hi) continue;
       uint4 w = make_uint4(0, 0, 0, 0);
-      if (t0 >= packed && t0 + t < len) w = *(const uint4*)(ring + (value ? side : 0) + (long long)((t0 + t) % c.ring) * D + ch);
+      if (t0 >= packed && t0 + t < len) w = *(const uint4*)(ring + (value ? side : 0) + ((long long)head * c.ring + (t0 + t) % c.ring) * D + ch);
       void* out = value ? a.value : a.key;
-      const long long at = value ? v_at + t * a.v_stride_token + ch : k_at + t * a.k_stride_token + ch;
+      const long long at = value ? v_at + head * a.v_stride_head + t * a.v_stride_token + ch : k_at + head * a.k_stride_head + t * a.k_stride_token + ch;
       if (DT == MZ_F32) {
         constexpr int RT = BF ? MZ_BF16 : MZ_F16;
         float v[8];
@@ -128,57 +129,93 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadArgs p, co
     }
     return;
   }
-  const uint8_t* page = (const uint8_t*)c.store + (long long)p.layer * c.store_stride_layer + (long long)id * c.store_stride_page + (long long)head * PB;
+  const uint8_t* page = (const uint8_t*)c.store + (long long)p.layer * c.store_stride_layer + (long long)id * c.store_stride_page + (long long)head0 * PB;
   const uint32_t sbook = smem_u32(s_book);
-  // ---- keys
-  if (tid < D) {
-    const int ch = tid % (D / 4) * 4, t1 = tid / (D / 4) * 16;         // four channels, 16 tokens
+  const bool whole = lo == 0 && hi == MZP_PAGE;
+  const int t = tid % SIDE_THREADS;
+  if (tid < SIDE_THREADS) {
+    // ---- keys: four channels, 16 tokens (head_dim 64: eight)
+    constexpr int TOKENS = MZP_PAGE * (D / 4) / SIDE_THREADS;
+    const int ch = t % (D / 4) * 4, t1 = t / (D / 4) * TOKENS;
     uint2 codes[4];
-    float t[4], anchor[4];
-    __half2 zero[4];
-    uint4 book[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) codes[k] = __ldg((const uint2*)(page + 32 * (ch + k) + t1 / 2));
-    const uint4 words = __ldg((const uint4*)(page + 32 * D + 4 * ch));
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const MzpRow r = mzp_row((&words.x)[k]);
-      t[k] = r.t * 0.03125f;
-      anchor[k] = r.a;
-      zero[k] = __float2half2_rn(1024.f + r.z);
-      book[k] = book128(sbook + r.z * 16);
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {                // four tokens
-      float v[4][4];
+    uint4 words;
+    auto load = [&](const uint8_t* at) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float2 x, y;
-        steps4((q < 2 ? codes[k].x : codes[k].y) >> (16 * (q & 1)), book[k], zero[k], x, y);
-        v[0][k] = fmaf(t[k], x.x, anchor[k]); v[1][k] = fmaf(t[k], x.y, anchor[k]);
-        v[2][k] = fmaf(t[k], y.x, anchor[k]); v[3][k] = fmaf(t[k], y.y, anchor[k]);
+        if (TOKENS == 16) codes[k] = __ldg((const uint2*)(at + 32 * (ch + k) + t1 / 2));
+        else codes[k].x = __ldg((const uint32_t*)(at + 32 * (ch + k) + t1 / 2));
       }
+      words = __ldg((const uint4*)(at + 32 * D + 4 * ch));
+    };
+    load(page);
+#pragma unroll 1
+    for (int head = head0; head < head1; ++head) {
+      float scale[4], anchor[4];
+      __half2 zero[4];
+      uint4 book[4];
+      uint2 now[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int tok = t1 + 4 * q + j;
-        if (tok >= lo && tok < hi) put4<DT>(a.key, k_at + tok * a.k_stride_token + ch, v[j][0], v[j][1], v[j][2], v[j][3]);
+      for (int k = 0; k < 4; ++k) {
+        const MzpRow r = mzp_row((&words.x)[k]);
+        scale[k] = r.t * 0.03125f;
+        anchor[k] = r.a;
+        zero[k] = __float2half2_rn(1024.f + r.z);
+        book[k] = book128(sbook + r.z * 16);
+        now[k] = codes[k];
+      }
+      if (head + 1 < head1) load(page + (head + 1 - head0) * PB);
+      const long long out = k_at + head * a.k_stride_head + ch;
+#pragma unroll
+      for (int q = 0; q < TOKENS / 4; ++q) {     // four tokens
+        float v[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float2 x, y;
+          steps4((q < 2 ? now[k].x : now[k].y) >> (16 * (q & 1)), book[k], zero[k], x, y);
+          v[0][k] = fmaf(scale[k], x.x, anchor[k]); v[1][k] = fmaf(scale[k], x.y, anchor[k]);
+          v[2][k] = fmaf(scale[k], y.x, anchor[k]); v[3][k] = fmaf(scale[k], y.y, anchor[k]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int tok = t1 + 4 * q + j;
+          if (whole || (tok >= lo && tok < hi)) put4<DT>(a.key, out + tok * a.k_stride_token, v[j][0], v[j][1], v[j][2], v[j][3]);
+        }
       }
     }
-  }
-  // ---- values
-#pragma unroll 4
-  for (int i = tid; i < MZP_PAGE * D / 8; i += READ_THREADS) {
-    const int tok = i / (D / 8), ch = i % (D / 8) * 8;
-    const uint32_t codes = __ldg((const uint32_t*)(page + 36 * D) + i);
-    const MzpRow r = mzp_row(__ldg((const uint32_t*)(page + 68 * D) + i / 8));
-    const uint4 book = book128(sbook + r.z * 16);
-    const __half2 zero = __float2half2_rn(1024.f + r.z);
-    const float t = r.t * 0.03125f;
-    float2 x, y, z, w;
-    steps4(codes, book, zero, x, y);
-    steps4(codes >> 16, book, zero, z, w);
-    const float v[8] = {fmaf(t, x.x, r.a), fmaf(t, x.y, r.a), fmaf(t, y.x, r.a), fmaf(t, y.y, r.a), fmaf(t, z.x, r.a), fmaf(t, z.y, r.a), fmaf(t, w.x, r.a), fmaf(t, w.y, r.a)};
-    if (tok >= lo && tok < hi) put8<DT>(a.value, v_at + tok * a.v_stride_token + ch, v);
+  } else {
+    // ---- values: eight channels of every eighth token (head_dim 64: every sixteenth)
+    constexpr int TURNS = MZP_PAGE * D / 8 / SIDE_THREADS, STEP_TOKENS = SIDE_THREADS * 8 / D;
+    const int tok0 = t / (D / 8), ch = t % (D / 8) * 8;
+    uint32_t codes[TURNS], words[TURNS];
+    auto load = [&](const uint8_t* at) {
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        codes[i] = __ldg((const uint32_t*)(at + 36 * D) + t + i * SIDE_THREADS);
+        words[i] = __ldg((const uint32_t*)(at + 68 * D) + (t + i * SIDE_THREADS) / 8);
+      }
+    };
+    load(page);
+#pragma unroll 1
+    for (int head = head0; head < head1; ++head) {
+      uint32_t now[TURNS], word[TURNS];
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) { now[i] = codes[i]; word[i] = words[i]; }
+      if (head + 1 < head1) load(page + (head + 1 - head0) * PB);
+      const long long out = v_at + head * a.v_stride_head + ch;
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        const MzpRow r = mzp_row(word[i]);
+        const uint4 book = book128(sbook + r.z * 16);
+        const __half2 zero = __float2half2_rn(1024.f + r.z);
+        const float s = r.t * 0.03125f;
+        float2 x, y, z, w;
+        steps4(now[i], book, zero, x, y);
+        steps4(now[i] >> 16, book, zero, z, w);
+        const float v[8] = {fmaf(s, x.x, r.a), fmaf(s, x.y, r.a), fmaf(s, y.x, r.a), fmaf(s, y.y, r.a), fmaf(s, z.x, r.a), fmaf(s, z.y, r.a), fmaf(s, w.x, r.a), fmaf(s, w.y, r.a)};
+        const int tok = tok0 + i * STEP_TOKENS;
+        if (whole || (tok >= lo && tok < hi)) put8<DT>(a.value, out + tok * a.v_stride_token, v);
+      }
+    }
   }
 }
 
@@ -186,7 +223,13 @@ template <int D, int DT, bool BF>
 int launch_read(const ReadArgs& p, const uint8_t* book, cudaStream_t st) {
   const long long pieces = p.a.tokens / MZP_PAGE + 2ll * p.a.batch;
   MZ_REQUIRE(pieces < (1ll << 31), "%d tokens of %d entries are too many for one call", p.a.tokens, p.a.batch);
-  read_kernel<D, DT, BF><<<dim3((unsigned)pieces, p.c.kv_heads), READ_THREADS, 0, st>>>(p, book);
+  // heads to a CTA: all that leave 8 CTAs to an SM
+  int sms = 0;
+  const int rc = mz_paged_sms(&sms);
+  if (rc != MZ_OK) return rc;
+  ReadArgs q = p;
+  q.heads = (int)std::max(1ll, std::min<long long>(p.c.kv_heads, pieces * p.c.kv_heads / (CTAS_PER_SM * sms)));
+  read_kernel<D, DT, BF><<<dim3((unsigned)pieces, (p.c.kv_heads + q.heads - 1) / q.heads), READ_THREADS, 0, st>>>(q, book);
   MZ_LAUNCH_CHECK("paged read");
   return MZ_OK;
 }
