@@ -459,13 +459,15 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
     } else if ((warp & 3) == 3) {
       // ---- words: the powers of two above a page's largest key and value (f16 has them below 2^14), and of every row of codes {scale, 1024 + zero level, anchor (as pairs), place of
       // its book}.  Here, and not where the levels are made, as this scheduler has the least to do
-      const uint32_t book = sbase + S::BOOK, terms = sbase + S::TERMS;
+      const uint32_t terms = sbase + S::TERMS;
       int page = warp == DECODER ? 0 : 1, pages = 0;
       while (x.segments > 0) {
         for (int i0 = 0; i0 < x.segments; ++i0) pages += x.seg[i0].count;
         for (; page < pages; page += 2) {
           const int slot = page % S::RAWS;
           const uint32_t raw = sbase + S::RAW + slot * PB + 32 * D;
+          // the place's page before this one was the other decoder's: it has been there, so the parity of the next phase is this page's
+          if (page >= S::RAWS) bar_wait(bar(x.scaled[(page - S::RAWS) % S::SCALES]), (page - S::RAWS) / S::SCALES & 1, failed);
           bar_wait(bar(x.raw_full[slot]), page / S::RAWS & 1, failed);
           const bool there = x.there[slot];
           int e[2];
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
               const MzpRow row = mzp_row(word[i]);
               const float unit = row.t * scale * 0.03125f, anchor = row.a * scale;
               sts128(terms + ((slot * 2 + side) * D + 32 * i + lane) * 16, half2_bits(__floats2half2_rn(unit, unit)), (0x6400u | row.z) * 0x10001u,
-                     half2_bits(__floats2half2_rn(anchor, anchor)), book + row.z * 16);
+                     half2_bits(__floats2half2_rn(anchor, anchor)), row.z * 16);
             }
           }
           if (lane == 0) x.scale[page % S::SCALES] = make_int2(e[0], e[1]);
@@ -506,6 +508,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
       const int k_row = ch, v_row = D == 128 ? 2 * token + part : token, piece0 = D == 128 ? 0 : part;
       const uint32_t k_at = sbase + S::KEYS + 128 * ch, v_at = sbase + S::VALUES + (D == 128 ? part * MZP_PAGE * 128 : 0) + 128 * token;
       const uint32_t k_turn = (ch & 7) << 4, v_turn = (token & 7) << 4, terms = sbase + S::TERMS;
+      const uint32_t sbook = sbase + S::BOOK;                // a place in it is masked: where waits ran out, terms are whatever stood there
       int page = member >> 2, pages = 0, slot = page, stage = page;
       uint32_t raw_phase = 0, phase = 1;
       // A team that waits for a place has waited for what was in it before: its last page went into a place that was free later than that.  So the parity of a phase is enough
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
           bar_wait(bar(x.raw_full[slot]), raw_phase, failed);
           bar_wait(bar(x.k_free[stage]), phase, failed);
           {
-            const uint4 term = lds128(terms + (slot * 2 * D + k_row) * 16), book = book128(term.w);
+            const uint4 term = lds128(terms + (slot * 2 * D + k_row) * 16), book = book128(sbook + (term.w & 0x7f0u));
             const __half2 step = bits_half2(term.x), zero = bits_half2(term.y);
             const uint32_t at = k_at + 2 * stage * S::PLANE;
             if (!__any_sync(0xffffffffu, term.z)) {
@@ -570,7 +573,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
           if (lane == 0) bar_arrive(bar(x.k_full[stage]));
           bar_wait(bar(x.v_free[stage]), phase, failed);
           {
-            const uint4 term = lds128(terms + ((slot * 2 + 1) * D + v_row) * 16), book = book128(term.w);
+            const uint4 term = lds128(terms + ((slot * 2 + 1) * D + v_row) * 16), book = book128(sbook + (term.w & 0x7f0u));
             const __half2 step = bits_half2(term.x), zero = bits_half2(term.y), base = bits_half2(term.z);
             const uint32_t at = v_at + stage * S::PLANE;
 #pragma unroll 1

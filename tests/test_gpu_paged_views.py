@@ -430,3 +430,51 @@ def test_misaligned_operands_and_small_workspaces_are_refused(common):
         assert call(**kw) != 0 and text in _cabi.last_error(), kw
     assert call(at=32) == 0
     assert torch.equal(out, cache.attend(0, q, rows=rows, groups=o))
+
+
+CHILD = r"""
+import sys, torch
+sys.path[:0] = [{root!r}, {root!r} + "/tests"]
+import muzero_b200 as mz
+from muzero_b200.kernels._cabi import load_library
+lib = load_library()
+assert lib.mz_bounds_violations(None, None, None, 0) == 0
+for d, dt, rows in ((128, torch.bfloat16, 70), (64, torch.float16, 24)):
+    n = rows + 1
+    cache = mz.MuZeroPagedCache.allocate(layers=1, kv_heads=8, head_dim=d, pages=256, rows=n, max_length=8192, dtype=dt)
+    o = torch.tensor([0, 6000], dtype=torch.int32, device="cuda")
+    home = torch.tensor([rows], dtype=torch.int32, device="cuda")
+    cache.extend(rows=home, offsets=o)
+    k, v = (torch.randn(6000, 8, d, device="cuda", dtype=dt) for _ in range(2))
+    cache.append(0, k, v, rows=home, offsets=o)
+    kids = torch.arange(rows, dtype=torch.int32, device="cuda")
+    cache.fork(home.expand(rows).contiguous(), kids)
+    q = torch.randn(rows, 1, 64 if d == 64 else 32, d, device="cuda", dtype=dt)
+    for kw in (dict(groups=torch.tensor([0, rows - 1], dtype=torch.int32, device="cuda")), dict(window=700, sinks=70)):
+        good = cache.attend(0, q, rows=kids, **kw)
+        assert torch.isfinite(good).all()
+        lib.mz_debug_fail_waits(1)
+        bad = cache.attend(0, q, rows=kids, **kw)
+        torch.cuda.synchronize()
+        lib.mz_debug_fail_waits(0)
+        assert torch.isnan(bad).all(), kw
+        assert torch.equal(cache.attend(0, q, rows=kids, **kw), good)
+    cache.read(0, offsets=torch.tensor([0, 100], dtype=torch.int32, device="cuda"), rows=home, tokens=100)
+    cache.check()
+assert lib.mz_bounds_violations(None, None, None, 0) == 0
+print("views checked build ok")
+"""
+
+
+def test_checked_build_and_waits_that_run_out():
+    """In the checked build: no guarded store out of bounds; where every wait runs out the outputs are NaN, the call ends, the next one is right."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lib = os.path.join(root, "muzero_b200", "lib", "libmuzero_b200_bounds.so")
+    if not os.path.exists(lib):
+        pytest.skip("the checked library has not been built")
+    env = dict(os.environ, MUZERO_B200_LIB=lib)
+    res = subprocess.run([sys.executable, "-c", CHILD.format(root=root)], env=env, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "views checked build ok" in res.stdout, res.stdout + res.stderr
