@@ -4,8 +4,8 @@
 
 A stack of attention layers with random projections stands in for a model.  A common prefix is written once and forked into every request's row (pages are
 shared, only the 16-bit window is copied); requests bring prompts of their own, decode until they are done, and make room for the next ones; one
-in eight branches into two continuations half way.  A decode step (extend, then append and attend per layer) is captured once in a CUDA graph:
-lengths and pages live on the device.  The first sequence that ends, the first branch that does and the prefix are checked in every layer: their attention against dense
+in eight branches into two continuations half way.  A decode step (extend, then append and attend per layer, the prefix's pages once for all rows) is captured once
+in a CUDA graph: lengths and pages live on the device.  The first sequence that ends, the first branch that does and the prefix are checked in every layer: their attention against dense
 attention over what their pages hold, and of the first one what its pages hold against the keys that were written.
 """
 from __future__ import annotations
@@ -35,10 +35,10 @@ class Layer:
         kv = (x @ self.kv).view(-1, 2, self.kv_heads, self.dim)
         return (x @ self.q).view(-1, self.heads, self.dim), kv[:, 0], kv[:, 1]
 
-    def decode(self, cache: MuZeroPagedCache, x: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
+    def decode(self, cache: MuZeroPagedCache, x: torch.Tensor, rows: torch.Tensor, groups: torch.Tensor) -> torch.Tensor:
         q, k, v = self.project(x)
         cache.append(self.index, k, v, rows=rows)
-        return x + cache.attend(self.index, q, rows=rows).flatten(1) @ self.o
+        return x + cache.attend(self.index, q, rows=rows, groups=groups).flatten(1) @ self.o
 
 
 def prefill(cache: MuZeroPagedCache, layers: list, x: torch.Tensor, rows: torch.Tensor, lengths: list) -> None:
@@ -74,6 +74,7 @@ def main(argv=None) -> dict:
     left = [0] * a.rows                                   # tokens that a row still has to decode; 0: the row is free
     x = torch.zeros(a.rows, hidden, device="cuda", dtype=torch.bfloat16)
     rows = torch.arange(a.rows, dtype=torch.int32, device="cuda")
+    groups = index(0, a.rows)                             # all rows begin with the prefix: its pages are read once for all of them
 
     def admit(waiting: int) -> int:
         """Starts requests in free rows: fork the prefix, write the prompts."""
@@ -93,7 +94,7 @@ def main(argv=None) -> dict:
         cache.extend(rows=rows)
         y = x
         for layer in layers:
-            y = layer.decode(cache, y, rows)
+            y = layer.decode(cache, y, rows, groups)
         return y
 
     waiting = a.requests - admit(a.requests)
@@ -187,29 +188,9 @@ def main(argv=None) -> dict:
 
 def read_row(cache: MuZeroPagedCache, layer: int, row: int):
     """A row's keys and values as they stand in its pages and ring, [tokens, kv_heads, head_dim] in fp32."""
-    import ctypes
-    book = (ctypes.c_ubyte * 2048)()
-    cache._lib.mz_paged_books(book, (ctypes.c_ubyte * 16384)())
-    book = torch.tensor(list(book), device=cache.device).view(128, 16)
-    n, d, h = int(cache.lengths[row]), cache.head_dim, cache.kv_heads
-    np_ = max(0, n - cache.residual_length) // 64
-    raw = cache.store[layer, cache.block_table[row, :np_].long()]
-
-    def side(codes, words):
-        w = words.contiguous().view(torch.int32)
-        t, field = (w & 0xFFFF).short().view(torch.float16).float(), (w >> 16) & 0xFFFF
-        off = (field & 0x7FFF) >= 128
-        anchor = torch.where(off, field.short().view(torch.float16).float(), torch.zeros_like(t))
-        z = torch.where(off, torch.where(anchor < 0, 127, 0), field).long()
-        e = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).long()
-        return anchor[..., None] + t[..., None] * (book[z[..., None], e] - z[..., None]) / 32
-
-    kc, kw, vc, vw = raw.split([32 * d, 4 * d, 32 * d, 4 * d], -1)
-    k = side(kc.reshape(np_, h, d, 32), kw).permute(0, 3, 1, 2).reshape(np_ * 64, h, d)
-    v = side(vc.reshape(np_, h, 64 * d // 64, 32), vw).reshape(np_, h, 64, d).transpose(1, 2).reshape(np_ * 64, h, d)
-    at = torch.arange(np_ * 64, n, device=cache.device) % cache.tail.shape[4]
-    ring = cache.tail[layer, row][:, :, at].float().transpose(1, 2)
-    return torch.cat([k, ring[0]]), torch.cat([v, ring[1]])
+    n = int(cache.lengths[row])
+    one = torch.tensor([row], dtype=torch.int32, device=cache.device)
+    return cache.read(layer, rows=one, offsets=torch.tensor([0, n], dtype=torch.int32, device=cache.device), tokens=n, out_dtype=torch.float32)
 
 
 if __name__ == "__main__":

@@ -239,16 +239,16 @@ class MuZeroPagedCache:
         if out is None:
             if tokens is None:
                 raise ValueError("`tokens` or `out` says how many places there are")
-            shape = (tokens, self.kv_heads, self.head_dim)
-            out = tuple(torch.empty(shape, dtype=out_dtype or self.dtype, device=self.device) for _ in range(2))
-        k, v = out
-        for name, t in (("key", k), ("value", v)):
-            whole = 16 // t.element_size() - 1
-            if (t.dim() != 3 or tuple(t.shape[1:]) != (self.kv_heads, self.head_dim) or t.shape[0] != k.shape[0] or t.dtype != k.dtype or t.device != self.device
-                    or (out_dtype or t.dtype) != t.dtype or (tokens is not None and tokens != t.shape[0])):
-                raise ValueError(f"`out` must be two tensors [tokens, {self.kv_heads}, {self.head_dim}] of one type on {self.device}, the {name}s are {t.dtype} {tuple(t.shape)} on {t.device}")
-            if t.numel() and (t.stride(2) != 1 or (t.stride(0) | t.stride(1)) & whole or t.data_ptr() & 15):
-                raise ValueError(f"`out` must have rows of whole 16-byte pieces, the {name}s' strides are {t.stride()}")
+            k, v = (torch.empty((tokens, self.kv_heads, self.head_dim), dtype=out_dtype or self.dtype, device=self.device) for _ in range(2))
+        else:
+            k, v = out
+            for name, t in (("key", k), ("value", v)):
+                whole = 16 // t.element_size() - 1
+                if (t.dim() != 3 or tuple(t.shape[1:]) != (self.kv_heads, self.head_dim) or t.shape[0] != k.shape[0] or t.dtype != k.dtype or t.device != self.device
+                        or (out_dtype or t.dtype) != t.dtype or (tokens is not None and tokens != t.shape[0])):
+                    raise ValueError(f"`out` must be two tensors [tokens, {self.kv_heads}, {self.head_dim}] of one type on {self.device}, the {name}s are {t.dtype} {tuple(t.shape)} on {t.device}")
+                if t.numel() and (t.stride(2) != 1 or (t.stride(0) | t.stride(1)) & whole or t.data_ptr() & 15):
+                    raise ValueError(f"`out` must have rows of whole 16-byte pieces, the {name}s' strides are {t.stride()}")
         a = PagedReadArgs(k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _index(rows, "rows", self.device),
                           _index(offsets, "offsets", self.device, n + 1), _index(first, "first", self.device, n), n, k.shape[0])
         check(on_device(self.device, self._lib.mz_paged_read, self._ref, layer, ctypes.byref(a), stream_ptr(self.device)), "mz_paged_read")

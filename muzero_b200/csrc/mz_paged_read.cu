@@ -5,6 +5,9 @@
 // next one's codes on their way meanwhile.  Keys stand along tokens: a thread of the first half takes 16 tokens of four neighbouring channels, so that a warp's store is a token's
 // whole row and nothing is transposed through shared memory.  Values stand along channels: a thread of the second half takes eight of a token's, a warp's store is two tokens' rows
 // (head_dim 128).
+//
+// Measured (B200 at 1965 MHz): 16 rows of 1777 to 4224 tokens, 8 kv heads, head_dim 128, bf16: 62 us for 259 MB, 4.2 TB/s; one head to a CTA of 128 threads 60 us, but 18 instead of 14 us for one row
+// of 1000 tokens and 100 instead of 92 for two rows' 101075 later tokens at head_dim 64.
 #include <algorithm>
 
 #include "mz_paged_device.cuh"
