@@ -130,7 +130,7 @@ struct PrefixSmem {
   static constexpr int STAGES = 3, RAWS = 5, SCALES = 16, ROWS = 2 * D;          // ROWS: rows of codes of a page
   static constexpr int KEYS = 0, VALUES = STAGES * 2 * PLANE, RAW = VALUES + STAGES * PLANE, BOOK = RAW + RAWS * PAGE_BYTES, TERMS = BOOK + MZP_BOOKS * MZP_LEVELS;
   static constexpr int ALIGN = 1024, TOTAL = TERMS + RAWS * ROWS * 16 + ALIGN;
-  // columns of tensor memory: queries (A operand, two values to a column), logits of two or three jobs (P stands over their first half), outputs of the streams.
+  // columns of tensor memory: queries (A operand, two values to a column), logits of two or three jobs (P stands over their first half, its remainder over the other), outputs of the streams.
   // Where the streams have rows of their own there are two blocks of queries and of logits, where they share theirs one and three
   static constexpr int TM_Q = 0, TM_O = 256, TM_COLS = 512;
   static __host__ __device__ constexpr int tm_s(bool both) { return both ? D : D / 2; }
