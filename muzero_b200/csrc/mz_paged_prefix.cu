@@ -51,7 +51,8 @@ struct PrefixArgs {
 __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS) plan_kernel(const PrefixArgs p) {
   const mz_paged_cache& c = p.c;
   const int tid = threadIdx.x, rank = blockIdx.x % PLAN_CTAS, g = blockIdx.x / PLAN_CTAS, n_groups = p.out.n_groups;
-  __shared__ int s_common;
+  __shared__ int s_common, s_members, s_row0;
+  __shared__ uint8_t s_member[1024];             // (a call has at most 1024 entries)
   bool fine = true;
   for (int i = tid; i < n_groups; i += PLAN_THREADS) {
     const int lo = p.offsets[i], hi = p.offsets[i + 1];
@@ -65,19 +66,26 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
   if (fine && g == 0) for (int i = rank * PLAN_THREADS + tid; i < first; i += PLAN_CTAS * PLAN_THREADS) p.out.skip[i] = 0;
   if (!fine && g == 0 && rank == 0 && tid == 0) atomicOr(c.status, MZ_PAGED_BAD_INDEX);
   auto row_at = [&](int b) { return p.rows ? p.rows[b] : b; };
-  // no further than every query of every row sees, and than every row has pages
-  int common = 0x7fffffff;
+  // no further than every query of every row sees, and than every row has pages.  A row that would share no page (it is empty, or not there) stays out and leaves the others theirs
+  if (tid == 0) { s_common = c.width; s_members = 0; s_row0 = 0x7fffffff; }
+  __syncthreads();
   for (int b = first + tid; b < end; b += PLAN_THREADS) {
     const int row = row_at(b);
     const int len = row < 0 || row >= c.rows ? 0 : max(0, min(c.lengths[row], p.longest));
-    common = min(common, min(mzp_packed(len, c.residual), max(0, len - p.q_len + 1)) / MZP_PAGE);
+    const int pages = min(mzp_packed(len, c.residual), max(0, len - p.q_len + 1)) / MZP_PAGE;
+    s_member[b - first] = pages > 0;
+    if (pages > 0) {
+      atomicMin(&s_common, pages);
+      atomicAdd(&s_members, 1);
+      atomicMin(&s_row0, b);
+    }
   }
-  if (tid == 0) s_common = min(c.width, end - first < 2 ? 0 : 0x7fffffff);
   __syncthreads();
-  atomicMin(&s_common, common);
+  int common = s_members < 2 ? 0 : s_common;
+  const int row0 = s_members > 0 ? row_at(s_row0) : 0;
   __syncthreads();
-  common = s_common;
-  const int row0 = first < end ? row_at(first) : 0;
+  if (tid == 0) s_common = common;
+  __syncthreads();
   if (common > 0) {
     // a warp compares 128 columns of its share of the rows with the first row's, four rows' loads on their way at a time
     const int* head = c.block_table + (long long)row0 * c.width;
@@ -94,7 +102,8 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         int other[4][4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int* theirs = c.block_table + (long long)row_at(min(b0 + r * shares, end - 1)) * c.width;
+          const int b = min(b0 + r * shares, end - 1);
+          const int* theirs = s_member[b - first] ? c.block_table + (long long)row_at(b) * c.width : head;
 #pragma unroll
           for (int k = 0; k < 4; ++k) other[r][k] = at + 32 * k < common ? theirs[at + 32 * k] : id[k];
         }
@@ -114,10 +123,10 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
     asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(theirs) : "memory");
     common = min(common, v);
   }
-  const int entries = end - first;
+  const int entries = end - first, members = s_members;
   const MzpTiles tiles(entries * p.qrows);
-  if (mzp_gain(common, c.kv_heads, (long long)entries * p.out.passes, p.out.nr, tiles.weight * tiles.count) == 0) common = 0;
-  for (int b = first + rank * PLAN_THREADS + tid; b < end; b += PLAN_CTAS * PLAN_THREADS) { p.out.skip[b] = common; p.out.group_of[b] = g; }
+  if (mzp_gain(common, c.kv_heads, (long long)members * p.out.passes, p.out.nr, tiles.weight * tiles.count) == 0) common = 0;
+  for (int b = first + rank * PLAN_THREADS + tid; b < end; b += PLAN_CTAS * PLAN_THREADS) { p.out.skip[b] = s_member[b - first] ? common : 0; p.out.group_of[b] = g; }
   if (rank == 0 && tid == 0) p.out.groups[g] = {first, (end - first) * p.qrows, end > first ? common : 0, row0};
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");      // nobody's shared memory goes while it is read
 }

@@ -251,14 +251,33 @@ def test_the_same_row_twice_and_rows_that_are_not_there(common):
     got = cache.attend(0, q, rows=ints(*rows), groups=ints(0, 64), out_dtype=torch.float32)
     close(got, cache.attend(0, q, rows=ints(*rows), out_dtype=torch.float32).double().cpu().numpy(), SHARED_TOL)
     cache.check()
-    rows[9], rows[30] = -1, cache.rows                             # the group then shares nothing
+    rows[0], rows[9], rows[30] = -1, -1, cache.rows                # the others share all the same
     got = cache.attend(0, q, rows=ints(*rows), groups=ints(0, 64), out_dtype=torch.float32)
+    assert [i for i, n in enumerate(shares(cache, q, rows, ints(0, 64))) if n != 44] == [0, 9, 30]
     with pytest.raises(Exception, match="outside the cache"):
         cache.check()
-    assert not got[[9, 30]].any()
-    assert torch.equal(got, cache.attend(0, q, rows=ints(*rows), out_dtype=torch.float32))
+    assert not got[[0, 9, 30]].any()
+    close(got, cache.attend(0, q, rows=ints(*rows), out_dtype=torch.float32).double().cpu().numpy(), SHARED_TOL)
     with pytest.raises(Exception, match="outside the cache"):
         cache.check()
+
+
+def test_a_padded_batch(common):
+    """Rows of the batch that are empty, or so short that they have no page: they stay out, the others share."""
+    cache, kids, _ = common
+    before = cache.lengths.clone()
+    short = {kids[0]: 0, kids[7]: 0, kids[20]: 1, kids[21]: 130, kids[63]: 0}
+    for r, n in short.items():
+        cache.lengths[r] = n
+    q = query(len(kids), 1, 32, 64, "bf16", 6)
+    want = cache.attend(0, q, rows=ints(*kids), out_dtype=torch.float32)
+    got = cache.attend(0, q, rows=ints(*kids), groups=ints(0, 64), out_dtype=torch.float32)
+    skip = shares(cache, q, kids, ints(0, 64))
+    cache.lengths.copy_(before)
+    cache.check()
+    assert [i for i, n in enumerate(skip) if n != 44] == [0, 7, 20, 21, 63]
+    assert not got[[0, 7, 63]].any()
+    close(got, want.double().cpu().numpy(), SHARED_TOL)
 
 
 @pytest.mark.parametrize("scaling", [None, 0.5, -0.3, 0.0])
