@@ -240,11 +240,13 @@ struct Lister {
       }
     };
     long long st, re, total = 0, gain = 0;
+    int heaviest = 1;
     for (int i = lane; i < n; i += 32) {
       size(i, st, re);
       total += st;
       const MzpGroup info = p.out.groups[i];
       const MzpTiles tiles(info.rows);
+      if (info.pages > 0) heaviest = max(heaviest, tiles.weight);
       gain += mzp_gain(info.pages, p.c.kv_heads, (long long)(info.rows / p.qrows) * p.out.passes, p.out.nr, tiles.weight * tiles.count);
     }
 #pragma unroll
@@ -252,8 +254,9 @@ struct Lister {
       total += __shfl_xor_sync(0xffffffffu, total, o);
       gain += __shfl_xor_sync(0xffffffffu, gain, o);
     }
+    heaviest = (int)__reduce_max_sync(0xffffffffu, (unsigned)heaviest);
     if (gain < mzp_gain_needed(p.out.sms, p.c.head_dim)) total = 0;      // then nothing is shared, and the other kernels see that
-    const MzpLine line(total, gridDim.x);
+    const MzpLine line(total, heaviest, gridDim.x);
     const bool some = cta < line.ctas;
     f0 = some ? line.start(cta) : 0;
     f1 = some ? line.start(cta + 1) : 0;
@@ -268,7 +271,7 @@ struct Lister {
         if (lane >= o) { ss += a; rr += b; }
       }
       const long long my_s = before_s + ss - st, my_r = before_r + rr - re;
-      if (cta == 0 && i0 + lane < n) p.out.sums[i0 + lane] = {my_s, my_r};
+      if (cta == 0 && i0 + lane < n) p.out.sums[i0 + lane] = {my_s, my_r, 0, 0};
       const uint32_t mine = __ballot_sync(0xffffffffu, my_s <= f0 && f0 < my_s + st);
       if (some && mine) {
         const int from = __ffs(mine) - 1;
@@ -279,7 +282,7 @@ struct Lister {
       before_s += __shfl_sync(0xffffffffu, ss, 31);
       before_r += __shfl_sync(0xffffffffu, rr, 31);
     }
-    if (cta == 0 && lane == 0) p.out.sums[n] = {total, before_r};
+    if (cta == 0 && lane == 0) p.out.sums[n] = {total, before_r, heaviest, 0};
     unit = -1;
     return some;
   }
@@ -297,8 +300,9 @@ struct Lister {
           const int u = unit + lane;
           const long long at = steps + u * len;
           Segment s;
-          s.page = at >= f0 ? 0 : (int)((f0 - at + tiles.weight - 1) / tiles.weight);
-          s.count = (int)min((long long)info.pages, (f1 - at + tiles.weight - 1) / tiles.weight) - s.page;
+          const MzpRun run(at, info.pages, tiles.weight, f0, f1);
+          s.page = run.page;
+          s.count = run.count;
           s.head = u / tiles.count;
           s.m0 = (u - s.head * tiles.count) * tiles.rows;
           s.first = info.first; s.row = info.row;

@@ -2,7 +2,8 @@
 //
 // A group is a run of list entries; the pages that all its rows' tables begin with are its prefix.  The query rows of a group that share a kv head, entry after entry, are
 // cut into tiles of at most 256; a unit is a (group, kv head, tile), a step of it one page.  The steps of all units stand in one line, weighted by 1 where a tile
-// has at most 128 rows and 2 above, and the line is cut evenly over the CTAs.  Each CTA leaves a record (m, l, out) per query row of a unit that it met: with r
+// has at most 128 rows and 2 above, and the line is cut evenly over the CTAs.  A page goes to the CTA that has its first step, and no part is shorter than the heaviest page: so
+// every CTA between those of a unit's first and last page has a page of it.  Each CTA leaves a record (m, l, out) per query row of a unit that it met: with r
 // rows in the units before, the record of row i by CTA c has place r + 256 c + i.
 #pragma once
 #include "mz_paged_device.cuh"
@@ -10,7 +11,7 @@
 constexpr int MZP_TILE_ROWS = 256;
 
 struct alignas(16) MzpGroup { int first, rows, pages, row; };        // first list entry, query rows per kv head, pages of the prefix (0: nothing is shared), a cache row
-struct MzpSums { long long steps, records; };                        // of the groups before
+struct MzpSums { long long steps, records; int heaviest, pad; };     // of the groups before; behind the last group the line's length and the weight of its heaviest page
 
 struct MzpPrefix {
   int* skip;                                     // [batch] pages of an entry that its group has taken care of
@@ -44,9 +45,18 @@ __host__ __device__ __forceinline__ long long mzp_gain_needed(int sms, int head_
 // how the line is cut
 struct MzpLine {
   long long total, ctas;
-  __device__ __forceinline__ MzpLine(long long steps, int grid) : total(steps), ctas(steps < grid ? steps : grid) {}
-  __device__ __forceinline__ long long start(int cta) const { return total * cta / ctas; }
-  __device__ __forceinline__ int owner(long long at) const { return (int)(((at + 1) * ctas - 1) / total); }
+  __host__ __device__ __forceinline__ MzpLine(long long steps, int heaviest, int grid) : total(steps), ctas(steps / heaviest < grid ? steps / heaviest : grid) {}
+  __host__ __device__ __forceinline__ long long start(int cta) const { return total * cta / ctas; }
+  __host__ __device__ __forceinline__ int owner(long long at) const { return (int)(((at + 1) * ctas - 1) / total); }
+};
+// the pages of a unit, which begins at step `at`, that belong to the part f0 .. f1 - 1
+struct MzpRun {
+  int page, count;
+  __host__ __device__ __forceinline__ MzpRun(long long at, int pages, int weight, long long f0, long long f1) {
+    page = at >= f0 ? 0 : (int)((f0 - at + weight - 1) / weight);
+    const long long end = (f1 - at + weight - 1) / weight;
+    count = (int)(end < pages ? end : pages) - page;
+  }
 };
 
 // where a list entry's records are
@@ -56,11 +66,12 @@ struct MzpUnits {
   MzpTiles tiles;
   MzpLine line;
   int qrows, kv_heads;
-  __device__ __forceinline__ MzpUnits(const MzpPrefix& p, int b, int query_rows, int heads)
-      : g(p.groups[p.group_of[b]]), before(p.sums[p.group_of[b]]), tiles(g.rows), line(p.sums[p.n_groups].steps, p.grid), qrows(query_rows), kv_heads(heads) {}
-  __device__ __forceinline__ int row_of(int b, int query_row) const { return (b - g.first) * qrows + query_row; }
+  __host__ __device__ __forceinline__ MzpUnits(const MzpPrefix& p, int b, int query_rows, int heads)
+      : g(p.groups[p.group_of[b]]), before(p.sums[p.group_of[b]]), tiles(g.rows), line(p.sums[p.n_groups].steps, p.sums[p.n_groups].heaviest, p.grid), qrows(query_rows),
+        kv_heads(heads) {}
+  __host__ __device__ __forceinline__ int row_of(int b, int query_row) const { return (b - g.first) * qrows + query_row; }
   // record of a query row of the group without its CTA's share of 256 c, and the CTAs that have one
-  __device__ __forceinline__ long long record(int head, int row, int& first, int& last) const {
+  __host__ __device__ __forceinline__ long long record(int head, int row, int& first, int& last) const {
     const int tile = row / tiles.rows;
     const long long at = before.steps + (long long)(head * tiles.count + tile) * g.pages * tiles.weight;
     first = line.owner(at);
