@@ -10,7 +10,8 @@
 
 constexpr int MZP_TILE_ROWS = 256;
 
-struct alignas(16) MzpGroup { int first, rows, pages, row; };        // first list entry, query rows per kv head, pages of the prefix (0: nothing is shared), a cache row
+// first list entry, query rows per kv head, pages of the prefix (0: nothing is shared), a cache row, entries that share
+struct alignas(16) MzpGroup { int first, rows, pages, row, members; };
 struct MzpSums { long long steps, records; int heaviest, pad; };     // of the groups before; behind the last group the line's length and the weight of its heaviest page
 
 struct MzpPrefix {

@@ -45,3 +45,18 @@ def test_wide_batches_behind_short_prefixes(rows, group, kvh, pages, d, dt):
         assert shares(cache, q, kids, o) == [pages] * rows and not torch.equal(got, want)
     close(got, want.double().cpu().numpy(), SHARED_TOL)
     assert torch.equal(cache.attend(0, q, rows=ints(*kids), groups=o, out_dtype=torch.float32), got)
+
+
+@pytest.mark.parametrize("live, pays", [(8, False), (16, False), (40, True)])
+def test_whether_sharing_pays_is_a_matter_of_the_rows_that_share(live, pays):
+    """A padded batch of 64 entries behind 101 pages: 8 or 16 live rows are attended as without groups, bit for bit; 40 share."""
+    cache, members, _ = grouped([(101 * 64 + 64, [1 + i % 50 for i in range(64)])], 8, 128, "bf16", 64)
+    kids = members[0]
+    cache.lengths[torch.tensor(kids[live:], device="cuda")] = 0
+    q = query(64, 1, 32, 128, "bf16", 12)
+    want = cache.attend(0, q, rows=ints(*kids), out_dtype=torch.float32)
+    got = cache.attend(0, q, rows=ints(*kids), groups=ints(0, 64), out_dtype=torch.float32)
+    cache.check()
+    assert torch.equal(got, want) != pays
+    assert not got[live:].any()
+    close(got, want.double().cpu().numpy(), SHARED_TOL)
