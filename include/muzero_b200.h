@@ -450,8 +450,8 @@ int mz_paged_attention(const mz_paged_cache* cache, int layer, const mz_paged_at
  *   window > 0   a query sees its own token, the window - 1 tokens before it, and the row's first `sinks` tokens.  Pages that no query sees are not read.
  *   n_groups > 0 the list entries groups[g] .. groups[g+1] - 1 (ascending, device memory, n_groups + 1 numbers, at most 1024 groups) are a group.  The pages that the tables of all
  *                its rows begin with, as far as every query sees them whole, are found on the device, read once, and taken by one matrix product for all rows of
- *                the group.  The result is that of mz_paged_attention but for rounding: keys are taken with 22 bits, values with 11, probabilities with 11 (22 in an f16 cache),
- *                sums with 24 (about 2e-4 of the output).  Entries that no group has, groups of one, rows without a common page, and rows
+ *                the group.  The result is that of mz_paged_attention but for rounding: keys, values and probabilities are taken with 22 bits, sums with 24 (about 1e-5 of the
+ *                output).  Entries that no group has, groups of one, rows without a common page, and rows
  *                that are empty or without a whole page in sight go as they do there, the latter without keeping the others from sharing.  Numbers that do not ascend from 0
  *                or more to `batch` or less share nothing and set MZ_PAGED_BAD_INDEX.
  * Not both.  workspace: mz_paged_attention_view_workspace_bytes() bytes (NULL view: those of mz_paged_attention), 32-byte aligned with groups.

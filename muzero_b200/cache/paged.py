@@ -181,7 +181,7 @@ class MuZeroPagedCache:
 
         ``groups``: int32 offsets into the batch, ``groups[g]`` to ``groups[g+1]`` being a group of entries whose rows begin with the same pages (forks of a
         prompt, say).  What they have in common is found on the device and taken once for all of them, as one matrix product: the same result, rounded
-        otherwise (2e-4 of the output).  Entries outside all groups are attended as without.  Not together with ``window``."""
+        otherwise (1e-5 of the output).  Entries outside all groups are attended as without.  Not together with ``window``."""
         q = query if query.dim() == 4 else query.unsqueeze(1)
         if q.dim() != 4 or q.shape[3] != self.head_dim or q.dtype != self.dtype or q.device != self.device:
             raise ValueError(f"`query` must be {self.dtype} [batch, (q_len,) q_heads, {self.head_dim}] on {self.device}, got {query.dtype} "

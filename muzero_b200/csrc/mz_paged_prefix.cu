@@ -2,11 +2,13 @@
 //
 // Mathematics.  A code stands for A + T (u - z) / 32 (mz_paged.cuh).  For a tile of query rows and a page of 64 tokens
 //   S = q K^T          K as two f16 numbers, value and remainder: 22 bits of every key; q (bf16 or f16) is exact in f16 once its row is scaled by a power of two
-//   P = exp2(S f + e - M),  O += P V          P and V are rounded to f16 (2^-12 of each value; P in an f16 cache is value and remainder), sums are fp32
+//   P = exp2(S f + e - M),  O += P V          V like K, P as two f16 numbers too: three products, all but that of the remainders (2^-22); sums are fp32
 // Keys and values of a page are scaled into f16's range by powers of two, ek and ev; f takes ek back.  ev is taken back by the softmax itself: M is the running
 // maximum not of the logits t but of t + ev, so P V has one scale whatever the pages' ranges and l sums P 2^-ev in fp32.  P is 2^7 under M itself; M moves when a row's sum of P over a page
 // passes 2^15 (the output in tensor memory is scaled then), so P is a f16 number, and what is lost below its smallest one is under 2^-31 of the largest.
-// With one f16 plane for the keys the output's error is 1.0e-3 instead of 2e-4 where channels differ by a factor of e^2.5 (131072 tokens, 32 rows; 10 us less).
+// Scales of rows of codes are f16 as well: one below 2^-21 of its page's largest loses bits, 2^-32 of the page's largest value.
+// Measured, the output's error against the call without sharing: 1.4e-6 (64 rows behind 4224 tokens) to 1.3e-5 (32 rows behind 131072); with one f16 number for P and V 2e-4 and 10 to 40 us less,
+// with one for K 1.0e-3 where channels differ by a factor of e^2.5.
 //
 // Work.  Groups, tiles, units, the line and its cut: mz_paged_prefix.cuh.  A CTA per SM, its warps by duty: a page is copied as it is (one bulk copy), its rows' words are decoded, its codes become
 // f16 operands (MN-major, 128-byte swizzle: a thread has a row of 64 codes and stores it as 8 pieces of 16 bytes, nothing is transposed), products, softmax.  Queries and P are operands in tensor
@@ -132,18 +134,22 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
 }
 
 // ---- attention over the prefixes
+// Pages as they are, pages as operands, blocks of logits where the streams share their rows.  The barriers of an operand stage go round RING places, so that a team, which is behind its own last
+// page by TEAMS pages and knows that what was in that one's stage before has been used, cannot take another phase of a barrier for the one that it waits for
+constexpr int RAWS = 5, STAGES = 2, BLOCKS = 3, RING = 4;
+static_assert(RAWS > TEAMS && RING >= TEAMS && (RING & (RING - 1)) == 0 && RING >= STAGES, "a wait could take another phase for its own");
 template <int D>
 struct PrefixSmem {
   static constexpr int PLANE = MZP_PAGE * D * 2;                                 // a page's keys, or values, in 16 bits
   static constexpr int PAGE_BYTES = 72 * D;
-  static constexpr int STAGES = 3, RAWS = 5, SCALES = 16, ROWS = 2 * D;          // ROWS: rows of codes of a page
-  static constexpr int KEYS = 0, VALUES = STAGES * 2 * PLANE, RAW = VALUES + STAGES * PLANE, BOOK = RAW + RAWS * PAGE_BYTES, TERMS = BOOK + MZP_BOOKS * MZP_LEVELS;
+  static constexpr int SCALES = 16, ROWS = 2 * D;                                // ROWS: rows of codes of a page
+  static constexpr int KEYS = 0, VALUES = STAGES * 2 * PLANE, RAW = 2 * VALUES, BOOK = RAW + RAWS * PAGE_BYTES, TERMS = BOOK + MZP_BOOKS * MZP_LEVELS;
   static constexpr int ALIGN = 1024, TOTAL = TERMS + RAWS * ROWS * 16 + ALIGN;
   // columns of tensor memory: queries (A operand, two values to a column), logits of two or three jobs (P stands over their first half, its remainder over the other), outputs of the streams.
   // Where the streams have rows of their own there are two blocks of queries and of logits, where they share theirs one and three
   static constexpr int TM_Q = 0, TM_O = 256, TM_COLS = 512;
   static __host__ __device__ constexpr int tm_s(bool both) { return both ? D : D / 2; }
-  static_assert(D + 2 * MZP_PAGE <= TM_O && D / 2 + 3 * MZP_PAGE <= TM_O && TM_O + 2 * D <= TM_COLS, "tensor memory");
+  static_assert(D + 2 * MZP_PAGE <= TM_O && D / 2 + BLOCKS * MZP_PAGE <= TM_O && TM_O + 2 * D <= TM_COLS, "tensor memory");
 };
 // Operands stand major along the kept dimension (keys: tokens, values: channels): rows of 64 values (128 bytes) along it, one per index that is summed over, the eight
 // 16-byte pieces of a row in the order of their number xor the row's (128-byte swizzle); values of head_dim 128 are two such blocks
@@ -154,9 +160,9 @@ constexpr int ISSUE_UNROLL = 4;
 constexpr int SEGMENTS = 64;                     // of a CTA at a time
 struct PrefixShared {
   Segment seg[SEGMENTS];
-  unsigned long long raw_full[5], raw_free[5], scaled[16], k_full[3], k_free[3], v_full[3], v_free[3], s_full[4], p_full[4], o_done[4], q_full, end;
+  unsigned long long raw_full[RAWS], raw_free[RAWS], scaled[16], full[2][RING], free[2][RING], s_full[4], p_full[4], o_done[4], q_full, end;      // [2]: keys, values
   int2 scale[16];                                // (ek, ev) by page of the CTA's line; pages are scaled ten ahead of their softmax at most
-  int there[5];                                  // whether a raw page is one
+  int there[RAWS];                                // whether a raw page is one
   float2 ml[2][128];                             // of the two streams, where they share rows
   int segments, more;                            // in hand; whether others follow
   uint32_t tmem;
@@ -333,8 +339,6 @@ template <int D, bool BF>
 __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixArgs p, const uint8_t* __restrict__ book_table) {
   using S = PrefixSmem<D>;
   constexpr int PB = S::PAGE_BYTES, HALF = MZP_TILE_ROWS / 2;
-  // f16 caches: P as value and remainder, as its rounding would be as large as the output's (12 rows of samples: error 3.2e-4 instead of 2.6e-4); bf16's own is eight times that
-  constexpr int P_PARTS = BF ? 1 : 2;
   extern __shared__ uint8_t window[];
   uint8_t* smem = window + (S::ALIGN - smem_u32(window) % S::ALIGN) % S::ALIGN;
   __shared__ PrefixShared x;
@@ -345,9 +349,9 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
   auto everyone = [&]() { asm volatile("bar.sync 0;" ::: "memory"); };
   if (tid == 0) {
     x.failed = p.fail_waits;
-    for (int i = 0; i < S::RAWS; ++i) { bar_init(bar(x.raw_full[i]), 1); bar_init(bar(x.raw_free[i]), 4); }
+    for (int i = 0; i < RAWS; ++i) { bar_init(bar(x.raw_full[i]), 1); bar_init(bar(x.raw_free[i]), 4); }
     for (int i = 0; i < S::SCALES; ++i) bar_init(bar(x.scaled[i]), 1);
-    for (int i = 0; i < S::STAGES; ++i) { bar_init(bar(x.k_full[i]), 4); bar_init(bar(x.k_free[i]), 1); bar_init(bar(x.v_full[i]), 4); bar_init(bar(x.v_free[i]), 1); }
+    for (int i = 0; i < 2 * RING; ++i) { bar_init(bar(x.full[i / RING][i % RING]), 4); bar_init(bar(x.free[i / RING][i % RING]), 1); }
     for (int i = 0; i < 4; ++i) { bar_init(bar(x.s_full[i]), 1); bar_init(bar(x.p_full[i]), 4); bar_init(bar(x.o_done[i]), 1); }
     bar_init(bar(x.q_full), SOFTMAX_WARPS);
     bar_init(bar(x.end), 1);
@@ -391,11 +395,11 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
         }
         *failed = 1;
       };
-      int segment = 0, ahead = 0, behind = 0, k_stage = 0, v_stage = 0;    // of the CTA so far: segments, jobs whose logits, whose outputs were issued
-      uint32_t k_phase = 0, v_phase = 0;
+      // of the CTA so far: segments, jobs whose logits, whose outputs were issued; pages of both, and the block of logits that is the page's where the streams share rows
+      int segment = 0, ahead = 0, behind = 0, k_page = 0, v_page = 0, k_block = 0, v_block = 0;
       const uint32_t keys = same((int)(sbase + S::KEYS) >> 4), values = same((int)(sbase + S::VALUES) >> 4);
       const uint32_t s_full = bar(x.s_full[0]), p_full = bar(x.p_full[0]), o_done = bar(x.o_done[0]), q_full = bar(x.q_full);
-      const uint32_t k_full = bar(x.k_full[0]), k_free = bar(x.k_free[0]), v_full = bar(x.v_full[0]), v_free = bar(x.v_free[0]);
+      const uint32_t k_full = bar(x.full[0][0]), k_free = bar(x.free[0][0]), v_full = bar(x.full[1][0]), v_free = bar(x.free[1][0]);
       for (int n = same(x.segments); n > 0; n = same(x.segments)) {
         for (int i0 = 0; i0 < n; ++i0, ++segment) {
           const bool both = same(x.seg[i0].rows) > HALF;     // two tiles of rows take each page; otherwise the streams take the pages in turn
@@ -403,38 +407,50 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
           for (int i = 0; i < jobs + lead; ++i) {
             const int j = i - lead;
             // the queries' barrier, which was passed or has to be, stands for what a job does not need
-            const uint32_t q_phase = segment & 1, k_bar = i < jobs ? k_full + 8 * k_stage : q_full, k_want = i < jobs ? k_phase : q_phase;
-            if (j >= 0) wait3(v_full + 8 * v_stage, v_phase, p_full + 8 * (behind & 3), behind >> 2 & 1, k_bar, k_want);
+            const uint32_t q_phase = segment & 1, k_bar = i < jobs ? k_full + 8 * (k_page % RING) : q_full, k_want = i < jobs ? k_page / RING & 1 : q_phase;
+            if (j >= 0) wait3(v_full + 8 * (v_page % RING), v_page / RING & 1, p_full + 8 * (behind & 3), behind >> 2 & 1, k_bar, k_want);
             else wait3(q_full, q_phase, q_full, q_phase, k_bar, k_want);
             tm_after();
             // short loops: a scheduler's instruction cache is full of the other duties, and what is executed once a page has to be fetched each time
             if (j >= 0) {
               const bool last = !both || (j & 1);
-              const uint32_t vd = values + v_stage * (S::PLANE >> 4), t_o = S::TM_O + (j & 1) * D, t_s = S::tm_s(both) + (both ? j & 1 : v_stage) * MZP_PAGE;
+              const uint32_t vd = values + v_page % STAGES * (2 * S::PLANE >> 4), t_o = S::TM_O + (j & 1) * D, t_s = S::tm_s(both) + (both ? j & 1 : v_block) * MZP_PAGE;
               if (elect()) {
-#pragma unroll ISSUE_UNROLL
-                for (int k = 0; k < P_PARTS * MZP_PAGE / 16; ++k)      // P, then its remainder
-                  umma16<D>(t_o, t_s + k * 8, vd + k % (MZP_PAGE / 16) * OPERAND_STEP, k > 0 || j > 1);
+#pragma unroll 1
+                for (int part = 0; part < 3; ++part) {       // P and V as value and remainder: all but the remainders' product
+                  const uint32_t p = t_s + (part == 1 ? MZP_PAGE / 2 : 0), v = vd + (part == 2 ? S::PLANE >> 4 : 0);
+#pragma unroll
+                  for (int k = 0; k < MZP_PAGE / 16; ++k) umma16<D>(t_o, p + k * 8, v + k * OPERAND_STEP, part + k > 0 || j > 1);
+                }
                 umma_commit(o_done + 8 * (behind & 3));
-                if (last) umma_commit(v_free + 8 * v_stage);
+                if (last) umma_commit(v_free + 8 * (v_page % RING));
               }
               __syncwarp();
               ++behind;
-              if (last && ++v_stage == S::STAGES) { v_stage = 0; v_phase ^= 1; }
+              if (last) {
+                ++v_page;
+                v_block = v_block == BLOCKS - 1 ? 0 : v_block + 1;
+              }
             }
             if (i < jobs) {
               const bool last = !both || (i & 1);
-              const uint32_t kd = keys + k_stage * (2 * S::PLANE >> 4), t_q = S::TM_Q + (both ? (i & 1) * (D / 2) : 0), t_s = S::tm_s(both) + (both ? i & 1 : k_stage) * MZP_PAGE;
+              const uint32_t kd = keys + k_page % STAGES * (2 * S::PLANE >> 4), t_q = S::TM_Q + (both ? (i & 1) * (D / 2) : 0), t_s = S::tm_s(both) + (both ? i & 1 : k_block) * MZP_PAGE;
               if (elect()) {
+#pragma unroll 1
+                for (int part = 0; part < 2; ++part) {       // remainder, then value: what is summed first is small, and so is what the tensor cores cut off of it
+                  const uint32_t k0 = kd + (part == 0 ? S::PLANE >> 4 : 0);
 #pragma unroll ISSUE_UNROLL
-                for (int k = 0; k < 2 * D / 16; ++k)         // value, then remainder: the second plane stands behind the first
-                  umma16<MZP_PAGE>(t_s, t_q + k % (D / 16) * 8, kd + k * OPERAND_STEP, k > 0);
+                  for (int k = 0; k < D / 16; ++k) umma16<MZP_PAGE>(t_s, t_q + k * 8, k0 + k * OPERAND_STEP, part + k > 0);
+                }
                 umma_commit(s_full + 8 * (ahead & 3));
-                if (last) umma_commit(k_free + 8 * k_stage);
+                if (last) umma_commit(k_free + 8 * (k_page % RING));
               }
               __syncwarp();
               ++ahead;
-              if (last && ++k_stage == S::STAGES) { k_stage = 0; k_phase ^= 1; }
+              if (last) {
+                ++k_page;
+                k_block = k_block == BLOCKS - 1 ? 0 : k_block + 1;
+              }
             }
           }
         }
@@ -453,9 +469,9 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
           for (int at = 0; at < seg.count; at += 32) {
             const int coming = at + 32 + lane < seg.count ? table[at + 32 + lane] : -1;
             for (int k = 0; k < min(32, seg.count - at); ++k, ++pages) {
-              const int slot = pages % S::RAWS, id = __shfl_sync(0xffffffffu, ids, k);
+              const int slot = pages % RAWS, id = __shfl_sync(0xffffffffu, ids, k);
               const bool there = id >= 0 && id < c.pages;    // a page that is not there any more has T = 0
-              bar_wait(bar(x.raw_free[slot]), (pages / S::RAWS & 1) ^ 1, failed);
+              bar_wait(bar(x.raw_free[slot]), (pages / RAWS & 1) ^ 1, failed);
               const bool fine = !*failed;
               if (fine) sent = pages + 1;
               if (fine && elect()) {
@@ -480,8 +496,8 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
         everyone();
       }
       // copies land before the CTA ends, whatever else went wrong
-      for (int j = max(0, sent - S::RAWS); j < sent; ++j)
-        for (int k = 0; k < SPIN_LIMIT && !bar_test(bar(x.raw_full[j % S::RAWS]), j / S::RAWS & 1); ++k) {}
+      for (int j = max(0, sent - RAWS); j < sent; ++j)
+        for (int k = 0; k < SPIN_LIMIT && !bar_test(bar(x.raw_full[j % RAWS]), j / RAWS & 1); ++k) {}
     } else if ((warp & 3) == 3) {
       // ---- words: the powers of two above a page's largest key and value (f16 has them below 2^14), and of every row of codes {scale, 1024 + zero level, anchor (as pairs), place of
       // its book}.  Here, and not where the levels are made, as this scheduler has the least to do
@@ -490,11 +506,11 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
       while (x.segments > 0) {
         for (int i0 = 0; i0 < x.segments; ++i0) pages += x.seg[i0].count;
         for (; page < pages; page += 2) {
-          const int slot = page % S::RAWS;
+          const int slot = page % RAWS;
           const uint32_t raw = sbase + S::RAW + slot * PB + 32 * D;
           // the place's page before this one was the other decoder's: it has been there, so the parity of the next phase is this page's
-          if (page >= S::RAWS) bar_wait(bar(x.scaled[(page - S::RAWS) % S::SCALES]), (page - S::RAWS) / S::SCALES & 1, failed);
-          bar_wait(bar(x.raw_full[slot]), page / S::RAWS & 1, failed);
+          if (page >= RAWS) bar_wait(bar(x.scaled[(page - RAWS) % S::SCALES]), (page - RAWS) / S::SCALES & 1, failed);
+          bar_wait(bar(x.raw_full[slot]), page / RAWS & 1, failed);
           const bool there = x.there[slot];
           int e[2];
 #pragma unroll
@@ -535,27 +551,27 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
       const uint32_t k_at = sbase + S::KEYS + 128 * ch, v_at = sbase + S::VALUES + (D == 128 ? part * MZP_PAGE * 128 : 0) + 128 * token;
       const uint32_t k_turn = (ch & 7) << 4, v_turn = (token & 7) << 4, terms = sbase + S::TERMS;
       const uint32_t sbook = sbase + S::BOOK;                // a place in it is masked: where waits ran out, terms are whatever stood there
-      int page = member >> 2, pages = 0, slot = page, stage = page;
-      uint32_t raw_phase = 0, phase = 1;
-      // A team that waits for a place has waited for what was in it before: its last page went into a place that was free later than that.  So the parity of a phase is enough
-      static_assert(S::RAWS > TEAMS && S::STAGES >= TEAMS, "a wait could take the phase before the last one for its own");
+      int page = member >> 2, pages = 0, slot = page;
+      uint32_t raw_phase = 0;
       while (x.segments > 0) {
         for (int i0 = 0; i0 < x.segments; ++i0) pages += x.seg[i0].count;
         for (; page < pages; page += TEAMS) {
           const uint32_t raw = sbase + S::RAW + slot * PB;
           bar_wait(bar(x.scaled[page % S::SCALES]), page / S::SCALES & 1, failed);
           bar_wait(bar(x.raw_full[slot]), raw_phase, failed);
-          bar_wait(bar(x.k_free[stage]), phase, failed);
-          {
-            const uint4 term = lds128(terms + (slot * 2 * D + k_row) * 16), book = book128(sbook + (term.w & 0x7f0u));
+#pragma unroll 1
+          for (int side = 0; side < 2; ++side) {
+            if (page >= STAGES) bar_wait(bar(x.free[side][(page - STAGES) % RING]), (page - STAGES) / RING & 1, failed);
+            const uint32_t at = (side ? v_at : k_at) + page % STAGES * 2 * S::PLANE, turn = side ? v_turn : k_turn, row = side ? v_row : k_row;
+            const uint4 term = lds128(terms + ((slot * 2 + side) * D + row) * 16), book = book128(sbook + (term.w & 0x7f0u));
+            const uint32_t from = raw + side * 36 * D + 32 * row;
             const __half2 step = bits_half2(term.x), zero = bits_half2(term.y);
-            const uint32_t at = k_at + 2 * stage * S::PLANE;
             if (!__any_sync(0xffffffffu, term.z)) {
 #pragma unroll 1
               for (int piece = piece0; piece < piece0 + PIECES; ++piece) {
-                const uint4 codes = lds128(raw + 32 * k_row + 16 * piece);
+                const uint4 codes = lds128(from + 16 * piece);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {    // eight tokens
+                for (int q = 0; q < 4; ++q) {    // eight values
                   uint32_t u[4], lo[4];
                   levels8((&codes.x)[q], book, u);
 #pragma unroll
@@ -564,7 +580,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
                     u[k] = half2_bits(h);
                     lo[k] = half2_bits(__hfma2(w, step, __hneg2(h)));      // exact
                   }
-                  const uint32_t dst = at + ((64 * piece + 16 * q) ^ k_turn);
+                  const uint32_t dst = at + ((64 * piece + 16 * q) ^ turn);
                   sts128(dst, u[0], u[1], u[2], u[3]);
                   sts128(dst + S::PLANE, lo[0], lo[1], lo[2], lo[3]);
                 }
@@ -573,7 +589,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
               const float unit = __low2float(step), anchor = __low2float(bits_half2(term.z));
 #pragma unroll 1
               for (int piece = piece0; piece < piece0 + PIECES; ++piece) {
-                const uint4 codes = lds128(raw + 32 * k_row + 16 * piece);
+                const uint4 codes = lds128(from + 16 * piece);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                   uint32_t u[4], lo[4];
@@ -587,44 +603,21 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
                     u[k] = half2_bits(h);
                     lo[k] = half2_bits(__floats2half2_rn(a - f.x, b - f.y));
                   }
-                  const uint32_t dst = at + ((64 * piece + 16 * q) ^ k_turn);
+                  const uint32_t dst = at + ((64 * piece + 16 * q) ^ turn);
                   sts128(dst, u[0], u[1], u[2], u[3]);
                   sts128(dst + S::PLANE, lo[0], lo[1], lo[2], lo[3]);
                 }
               }
             }
-          }
-          fence_operands();
-          __syncwarp();
-          if (lane == 0) bar_arrive(bar(x.k_full[stage]));
-          bar_wait(bar(x.v_free[stage]), phase, failed);
-          {
-            const uint4 term = lds128(terms + ((slot * 2 + 1) * D + v_row) * 16), book = book128(sbook + (term.w & 0x7f0u));
-            const __half2 step = bits_half2(term.x), zero = bits_half2(term.y), base = bits_half2(term.z);
-            const uint32_t at = v_at + stage * S::PLANE;
-#pragma unroll 1
-            for (int piece = piece0; piece < piece0 + PIECES; ++piece) {
-              const uint4 codes = lds128(raw + 36 * D + 32 * v_row + 16 * piece);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {      // eight channels
-                uint32_t u[4];
-                levels8((&codes.x)[q], book, u);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) u[k] = half2_bits(__hfma2(__hsub2(bits_half2(u[k]), zero), step, base));
-                sts128(at + ((64 * piece + 16 * q) ^ v_turn), u[0], u[1], u[2], u[3]);
-              }
+            fence_operands();
+            __syncwarp();
+            if (lane == 0) {
+              bar_arrive(bar(x.full[side][page % RING]));
+              if (side) bar_arrive(bar(x.raw_free[slot]));
             }
           }
-          fence_operands();
-          __syncwarp();
-          if (lane == 0) {
-            bar_arrive(bar(x.v_full[stage]));
-            bar_arrive(bar(x.raw_free[slot]));
-          }
           slot += TEAMS;
-          if (slot >= S::RAWS) { slot -= S::RAWS; raw_phase ^= 1; }
-          stage += TEAMS;
-          if (stage >= S::STAGES) { stage -= S::STAGES; phase ^= 1; }
+          if (slot >= RAWS) { slot -= RAWS; raw_phase ^= 1; }
         }
         everyone();
         everyone();
@@ -689,7 +682,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
       const int jobs = both ? 2 * seg.count : seg.count, mine = (jobs + 1 - s) / 2;        // of the segment, of this stream
       for (int j = 0; j < mine; ++j) {
         const int i = 2 * j + s, job = first_job + i, page = pages + (both ? j : i);
-        const uint32_t t_s = lanes + S::tm_s(both) + (both ? s : page % S::STAGES) * MZP_PAGE;
+        const uint32_t t_s = lanes + S::tm_s(both) + (both ? s : page % BLOCKS) * MZP_PAGE;
         bar_wait(bar(x.scaled[page % S::SCALES]), page / S::SCALES & 1, failed);
         bar_wait(bar(x.s_full[job & 3]), job >> 2 & 1, failed);
         tm_after();
@@ -697,7 +690,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
           const int2 sc = x.scale[page % S::SCALES];
           const float f = rowf * pow2(sc.x), ev = (float)sc.y;
           // P under the maximum so far, of the first pages' logits: its sum stays below 2^15 unless that is passed by 8 or so.  Then the maximum is found and P taken once more
-          uint32_t w[32], rest[BF ? 1 : 32];
+          uint32_t w[32], rest[32];
           float total = 0.f;
           bool known = j > 0;
           for (int turn = 0;; ++turn) {
@@ -718,13 +711,13 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
                   const __half2 p0 = __floats2half2_rn(a, b), p1 = __floats2half2_rn(c2, d);
                   w[16 * h + i / 2] = half2_bits(p0);
                   w[16 * h + i / 2 + 1] = half2_bits(p1);
-                  if (!BF) {
-                    const float2 f0 = __half22float2(p0), f1 = __half22float2(p1);
-                    rest[16 * h + i / 2] = half2_bits(__floats2half2_rn(a - f0.x, b - f0.y));
-                    rest[16 * h + i / 2 + 1] = half2_bits(__floats2half2_rn(c2 - f1.x, d - f1.y));
-                  }
                   add2(sum[0], sum[1], a, b);
                   add2(sum[2], sum[3], c2, d);
+                  const float2 f0 = __half22float2(p0), f1 = __half22float2(p1);
+                  fma2(a, b, f0.x, f0.y, -1.f);              // exact
+                  fma2(c2, d, f1.x, f1.y, -1.f);
+                  rest[16 * h + i / 2] = half2_bits(__floats2half2_rn(a, b));
+                  rest[16 * h + i / 2 + 1] = half2_bits(__floats2half2_rn(c2, d));
                 }
               }
               total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -765,7 +758,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
             }
           }
           tm_store32(t_s, w);                    // over logits that have been read
-          if constexpr (!BF) tm_store32(t_s + 32, rest);
+          tm_store32(t_s + 32, rest);
           l = fmaf(total, pow2(-sc.y - 7), l);
           tm_stored();
         }

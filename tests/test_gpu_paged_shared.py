@@ -1,6 +1,8 @@
 """GPU: shared prefixes of the paged cache, where batches are wide and prefixes short, rows stay out of their group, values need more than 16 bits, and runs of pages are long.
 
-Helpers and the tolerance for sharing are those of test_gpu_paged_views.py.
+Helpers and SHARED_TOL are those of test_gpu_paged_views.py.  FINE_TOL, before any run: keys, values and probabilities are two f16 numbers each, 2^-22 of themselves; logits of up to 30 (base 2: 43)
+carry that of their terms and 2^-23 of a running sum for each of 16 products, of which all but the last few are small: 1e-5; the output's sums lose at most 2^-23 in each of 12 products per page, and a
+CTA has at most three pages of these prefixes, a stream two: 3e-6; the exponential 2^-22.  Together below 2e-5, and with the 16-bit window's 1e-5 what ordinary attention is held to: 3e-5.
 """
 import numpy as np
 import pytest
@@ -11,6 +13,7 @@ from test_gpu_paged import DT, f32, ints, make, tokens
 from test_gpu_paged_views import SHARED_TOL, close, grouped, query, shares
 
 pytestmark = pytest.mark.gpu
+FINE_TOL = 3e-5
 
 
 def spoil_workspaces(cache):
@@ -60,3 +63,19 @@ def test_whether_sharing_pays_is_a_matter_of_the_rows_that_share(live, pays):
     assert torch.equal(got, want) != pays
     assert not got[live:].any()
     close(got, want.double().cpu().numpy(), SHARED_TOL)
+
+
+@pytest.mark.parametrize("d, dt, hq, lq", [(128, "bf16", 32, 1), (128, "fp16", 32, 1), (64, "bf16", 32, 1), (64, "fp16", 16, 2), (128, "bf16", 8, 3)])
+def test_shared_attention_is_as_exact_as_ordinary_attention(d, dt, hq, lq):
+    cache, members, kv = grouped([(3000, [3 + i % 70 for i in range(64)])], 8, d, dt, 128)
+    kids = members[0]
+    q = query(64, lq, hq, d, dt, 13)
+    got = cache.attend(0, q, rows=ints(*kids), groups=ints(0, 64), out_dtype=torch.float32)
+    cache.check()
+    assert min(shares(cache, q, kids, ints(0, 64))) >= 44
+    want = cache.attend(0, q, rows=ints(*kids), out_dtype=torch.float32)
+    assert not torch.equal(got, want)
+    close(got, want.double().cpu().numpy(), 2 * FINE_TOL)
+    for i in (0, 31, 63):
+        k, v = plain.held(f32(kv[kids[i]][0]), f32(kv[kids[i]][1]), 128)
+        close(got[i], plain.attention(f32(q[i].cpu()), k, v, d ** -0.5), FINE_TOL)
