@@ -6,6 +6,7 @@
 // Keys and values of a page are scaled into f16's range by powers of two, ek and ev; f takes ek back.  ev is taken back by the softmax itself: M is the running
 // maximum not of the logits t but of t + ev, so P V has one scale whatever the pages' ranges and l sums P 2^-ev in fp32.  P is 2^7 under M itself; M moves when a row's sum of P over a page
 // passes 2^15 (the output in tensor memory is scaled then), so P is a f16 number, and what is lost below its smallest one is under 2^-31 of the largest.
+// The output's running sums are held in fp32 outside the tensor cores (SUM_JOBS).
 // Scales of rows of codes are f16 as well: one below 2^-21 of its page's largest loses bits, 2^-32 of the page's largest value.
 // Measured, the output's error against the call without sharing: 1.4e-6 (64 rows behind 4224 tokens) to 1.3e-5 (32 rows behind 131072); with one f16 number for P and V 2e-4 and 10 to 40 us less,
 // with one for K 1.0e-3 where channels differ by a factor of e^2.5.
@@ -157,6 +158,10 @@ constexpr int OPERAND_STEP = 16 * 128 >> 4;      // 16 rows further
 
 struct alignas(16) Segment { int first, row, head, m0, rows, page, count, pad; long long record; };      // a run of steps of one unit
 constexpr int ISSUE_UNROLL = 4;
+// Jobs of a stream that go into one accumulator.  The tensor cores cut their running sums off, always towards zero: up to 2^-23 of the sum in each of a job's 12 products.  Measured with values of one
+// sign: 2.2e-4 of the output after 432 jobs, 1.1e-4 after 216.  So after this many the sum is added in fp32 to what there is: below 2e-5.  32 rows behind 131072 tokens with 8 / 16 / 32 / all jobs to
+// an accumulator 259 / 253 / 245 / 245 us
+constexpr int SUM_JOBS = 32;
 constexpr int SEGMENTS = 64;                     // of a CTA at a time
 struct PrefixShared {
   Segment seg[SEGMENTS];
@@ -420,7 +425,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
                 for (int part = 0; part < 3; ++part) {       // P and V as value and remainder: all but the remainders' product
                   const uint32_t p = t_s + (part == 1 ? MZP_PAGE / 2 : 0), v = vd + (part == 2 ? S::PLANE >> 4 : 0);
 #pragma unroll
-                  for (int k = 0; k < MZP_PAGE / 16; ++k) umma16<D>(t_o, p + k * 8, v + k * OPERAND_STEP, part + k > 0 || j > 1);
+                  for (int k = 0; k < MZP_PAGE / 16; ++k) umma16<D>(t_o, p + k * 8, v + k * OPERAND_STEP, part + k > 0 || (j >> 1) % SUM_JOBS != 0);
                 }
                 umma_commit(o_done + 8 * (behind & 3));
                 if (last) umma_commit(v_free + 8 * (v_page % RING));
@@ -629,6 +634,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
     const int s = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_o = lanes + S::TM_O + s * D;
     int pages = 0, first_job = 0;                            // of the CTA so far
+    float4* const part = p.out.part + ((long long)blockIdx.x * 2 + s) * (D / 4) * HALF + r;
     while (x.segments > 0) {
     for (int i0 = 0; i0 < x.segments; ++i0) {
       const Segment seg = x.seg[i0];
@@ -678,7 +684,27 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
         __syncwarp();
         if (lane == 0) bar_arrive(bar(x.q_full));
       }
-      float M = -INFINITY, l = 0.f;
+      float M = -INFINITY, l = 0.f, M_part = 0.f;            // M_part: that of the sums so far
+      auto keep = [&](bool more) {                           // adds the accumulator to them
+        const float f = more ? ex2(M_part - (M == -INFINITY ? 0.f : M)) : 0.f;
+        M_part = M;
+#pragma unroll 1
+        for (int h = 0; h < D / 32; ++h) {
+          uint32_t o[32];
+          float4 sum[8];
+          tm_load32(o, t_o + 32 * h);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (more) sum[i] = part[(8 * h + i) * HALF];
+          }
+          tm_loaded(o);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            part[(8 * h + i) * HALF] = make_float4(fmaf(sum[i].x, f, __uint_as_float(o[4 * i])), fmaf(sum[i].y, f, __uint_as_float(o[4 * i + 1])),
+                                                   fmaf(sum[i].z, f, __uint_as_float(o[4 * i + 2])), fmaf(sum[i].w, f, __uint_as_float(o[4 * i + 3])));
+        }
+      };
       const int jobs = both ? 2 * seg.count : seg.count, mine = (jobs + 1 - s) / 2;        // of the segment, of this stream
       for (int j = 0; j < mine; ++j) {
         const int i = 2 * j + s, job = first_job + i, page = pages + (both ? j : i);
@@ -761,6 +787,11 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
           tm_store32(t_s + 32, rest);
           l = fmaf(total, pow2(-sc.y - 7), l);
           tm_stored();
+          if (j > 0 && j % SUM_JOBS == 0) {      // this job's product begins a new sum
+            bar_wait(bar(x.o_done[(job - 2) & 3]), (job - 2) >> 2 & 1, failed);
+            tm_after();
+            keep(j > SUM_JOBS);
+          }
         }
         tm_before();
         __syncwarp();
@@ -772,6 +803,8 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
         bar_wait(bar(x.o_done[job & 3]), job >> 2 & 1, failed);
       }
       tm_after();
+      const bool kept = jobs > 2 * SUM_JOBS;                 // of either stream
+      if (kept && some) keep(mine > SUM_JOBS);
       const bool bad = *failed != 0;
       const long long at = seg.record + m;
       const bool inside = here && MZ_IN_BOUNDS(at, p.out.records, 21);
@@ -797,15 +830,27 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
       }
 #pragma unroll 1
       for (int d = d0; d < d1; d += 32) {
-        uint32_t v[32], u[32];
         float out[32];
-        tm_load32(v, t_o + d);
-        tm_load32(u, t_other + d);
-        tm_loaded(v);
-        tm_loaded(u);
-        // a stream that had no page left nothing in its accumulator
+        if (kept) {
+          const float4* other = part + (s ? -1 : 1) * (D / 4) * HALF;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) out[i] = (mine > 0 ? __uint_as_float(v[i]) * f_mine : 0.f) + (!both && f_other != 0.f ? __uint_as_float(u[i]) * f_other : 0.f);
+          for (int i = 0; i < 8; ++i) {
+            const float4 a = part[(d / 4 + i) * HALF];
+            float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (!both) b = other[(d / 4 + i) * HALF];
+            out[4 * i] = a.x * f_mine + b.x * f_other; out[4 * i + 1] = a.y * f_mine + b.y * f_other;
+            out[4 * i + 2] = a.z * f_mine + b.z * f_other; out[4 * i + 3] = a.w * f_mine + b.w * f_other;
+          }
+        } else {
+          uint32_t v[32], u[32];
+          tm_load32(v, t_o + d);
+          tm_load32(u, t_other + d);
+          tm_loaded(v);
+          tm_loaded(u);
+          // a stream that had no page left nothing in its accumulator
+#pragma unroll
+          for (int i = 0; i < 32; ++i) out[i] = (mine > 0 ? __uint_as_float(v[i]) * f_mine : 0.f) + (!both && f_other != 0.f ? __uint_as_float(u[i]) * f_other : 0.f);
+        }
         if (inside) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) stg256(p.out.acc + at * D + d + i, out + i);
@@ -863,7 +908,8 @@ void mzp_prefix_shape(const mz_paged_cache* c, int batch, int n_groups, int qrow
   s->sums_at = s->groups_at + up(n_groups * sizeof(MzpGroup));
   s->ml_at = s->sums_at + up((n_groups + 1) * sizeof(MzpSums));
   s->acc_at = s->ml_at + up(s->records * sizeof(float2));
-  s->bytes = s->acc_at + s->records * c->head_dim * sizeof(float);
+  s->part_at = s->acc_at + up(s->records * c->head_dim * sizeof(float));
+  s->bytes = s->part_at + (size_t)s->grid * MZP_TILE_ROWS * c->head_dim * sizeof(float);
 }
 
 int mzp_prefix_launch(const mz_paged_cache& c, int layer, const mz_paged_attention_args& args, const mz_paged_view& view, const MzpPrefixShape& s, uint8_t* workspace,
@@ -886,6 +932,7 @@ int mzp_prefix_launch(const mz_paged_cache& c, int layer, const mz_paged_attenti
   p.out.sums = (MzpSums*)(workspace + s.sums_at);
   p.out.ml = (float2*)(workspace + s.ml_at);
   p.out.acc = (float*)(workspace + s.acc_at);
+  p.out.part = (float4*)(workspace + s.part_at);
   p.out.n_groups = view.n_groups;
   p.out.grid = p.out.sms = s.grid;               // a CTA per multiprocessor
   p.out.nr = nr;

@@ -21,6 +21,7 @@ struct MzpPrefix {
   MzpSums* sums;                                 // [n_groups + 1]
   float2* ml;                                    // [record] maximum (base 2) and sum
   float* acc;                                    // [record][D]
+  float4* part;                                  // [CTA][stream][D / 4][128] sums of a long run of pages so far
   int n_groups, grid;
   int nr, passes, sms;                           // of the call without sharing: query rows to a step, steps per page
   long long records;
@@ -81,7 +82,7 @@ struct MzpUnits {
   }
 };
 
-struct MzpPrefixShape { int grid; long long records; size_t skip_at, group_of_at, groups_at, sums_at, ml_at, acc_at, bytes; };
+struct MzpPrefixShape { int grid; long long records; size_t skip_at, group_of_at, groups_at, sums_at, ml_at, acc_at, part_at, bytes; };
 void mzp_prefix_shape(const mz_paged_cache* c, int batch, int n_groups, int qrows, int sms, MzpPrefixShape* s);
 // Finds the prefixes of the groups and takes the attention of their rows over them; fills `out`.  longest: no row is taken for longer.
 int mzp_prefix_launch(const mz_paged_cache& c, int layer, const mz_paged_attention_args& args, const mz_paged_view& view, const MzpPrefixShape& s, uint8_t* workspace,

@@ -79,3 +79,37 @@ def test_shared_attention_is_as_exact_as_ordinary_attention(d, dt, hq, lq):
     for i in (0, 31, 63):
         k, v = plain.held(f32(kv[kids[i]][0]), f32(kv[kids[i]][1]), 128)
         close(got[i], plain.attention(f32(q[i].cpu()), k, v, d ** -0.5), FINE_TOL)
+
+
+@pytest.mark.parametrize("d, dt, group", [(128, "bf16", 4), (128, "fp16", 2), (64, "bf16", 4)])
+def test_long_runs_of_pages_lose_nothing(d, dt, group):
+    """A CTA takes hundreds of pages one after the other, of values that are all of one sign (the tensor cores' sums are cut off towards zero).  A long table needs few pages: it
+    names each of 50 many times, and attention over it is that over 50 with their weights multiplied."""
+    rows, kvh, distinct, times, residual = 64, 8, 50, 160, 64
+    n = distinct * times * 64 + residual
+    cache = make(rows, kvh, d, dt, residual, max_length=n, pages=distinct + 6)
+    g = torch.Generator().manual_seed(3)
+    k = torch.randn(distinct * 64 + residual, kvh, d, generator=g).to(DT[dt])
+    v = (1 + 0.2 * torch.randn(k.shape, generator=g)).to(DT[dt])
+    o = ints(0, k.shape[0])
+    cache.extend(rows=ints(0), offsets=o)
+    cache.append(0, k.cuda(), v.cuda(), rows=ints(0), offsets=o)
+    cache.check()
+    ids = cache.block_table[0, :distinct].clone()
+    cache.block_table[:, :distinct * times] = ids[torch.randperm(distinct * times, generator=g).cuda() % distinct]
+    cache.lengths.fill_(n)
+    cache.tail.copy_(1 + torch.randn(cache.tail.shape, generator=g).to(cache.dtype).cuda() / 8)
+    q = query(rows, 1, group * kvh, d, dt, 14)
+    got = cache.attend(0, q, groups=ints(0, rows), out_dtype=torch.float32)
+    cache.check()
+    assert shares(cache, q, None, ints(0, rows)) == [distinct * times] * rows
+    held_k, held_v = plain.held(f32(k), f32(v), residual)
+    place = [(n - residual + i) % cache.tail.shape[4] for i in range(residual)]
+    ring = cache.tail[0].double().cpu().numpy()[:, :, :, place]
+    for r in (0, 37):
+        for h in range(kvh):
+            kk, vv = (np.concatenate([x[:distinct * 64, h], y]) for x, y in ((held_k, ring[r, 0, h]), (held_v, ring[r, 1, h])))
+            s = q[r, 0, h * group:(h + 1) * group].double().cpu().numpy() @ kk.T * d ** -0.5
+            w = np.exp(s - s.max(-1, keepdims=True))
+            w[:, :distinct * 64] *= times
+            close(got[r, 0, h * group:(h + 1) * group], w @ vv / w.sum(-1, keepdims=True), FINE_TOL)
