@@ -128,7 +128,7 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
   }
   const int entries = end - first, members = s_members;
   const MzpTiles tiles(entries * p.qrows);
-  if (mzp_gain(common, c.kv_heads, (long long)members * p.out.passes, p.out.nr, tiles.weight * tiles.count) == 0) common = 0;
+  if (mzp_gain(common, c.kv_heads, (long long)members * p.out.passes, p.out.nr, tiles.cost()) == 0) common = 0;
   for (int b = first + rank * PLAN_THREADS + tid; b < end; b += PLAN_CTAS * PLAN_THREADS) { p.out.skip[b] = s_member[b - first] ? common : 0; p.out.group_of[b] = g; }
   if (rank == 0 && tid == 0) p.out.groups[g] = {first, (end - first) * p.qrows, end > first ? common : 0, row0, members};
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");      // nobody's shared memory goes while it is read
@@ -258,7 +258,7 @@ struct Lister {
       const MzpGroup info = p.out.groups[i];
       const MzpTiles tiles(info.rows);
       if (info.pages > 0) heaviest = max(heaviest, tiles.weight);
-      gain += mzp_gain(info.pages, p.c.kv_heads, (long long)info.members * p.out.passes, p.out.nr, tiles.weight * tiles.count);
+      gain += mzp_gain(info.pages, p.c.kv_heads, (long long)info.members * p.out.passes, p.out.nr, tiles.cost());
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {

@@ -113,3 +113,48 @@ def test_long_runs_of_pages_lose_nothing(d, dt, group):
             w = np.exp(s - s.max(-1, keepdims=True))
             w[:, :distinct * 64] *= times
             close(got[r, 0, h * group:(h + 1) * group], w @ vv / w.sum(-1, keepdims=True), FINE_TOL)
+
+
+@pytest.mark.parametrize("d, group, rows, pages, pays", [(128, 4, 8, 64, False), (128, 4, 32, 64, True), (128, 4, 4, 600, False), (128, 8, 4, 1000, True), (64, 4, 8, 64, False), (64, 4, 64, 64, True)])
+def test_the_rule_on_both_sides(d, group, rows, pages, pays):
+    """Where sharing was measured to cost more, a call with groups gives what one without does, bit for bit."""
+    cache = make(rows, 8, d, "bf16", 64, max_length=pages * 64 + 64, pages=pages)
+    random_pages(cache, 1)
+    cache.block_table.copy_(torch.arange(pages, dtype=torch.int32).expand(rows, -1))
+    cache.lengths.fill_(pages * 64 + 64)
+    q = query(rows, 1, group * 8, d, "bf16", 15)
+    want = cache.attend(0, q, out_dtype=torch.float32)
+    got = cache.attend(0, q, groups=ints(0, rows), out_dtype=torch.float32)
+    cache.check()
+    assert torch.equal(got, want) != pays
+    close(got, want.double().cpu().numpy(), 2 * FINE_TOL)
+
+
+def random_pages(cache, seed):
+    """Codes as they come, words with moderate scales that straddle zero."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    d = cache.head_dim
+    cache.store.random_(0, 256, generator=gen)
+    for at in (32 * d, 68 * d):
+        w = cache.store[..., at:at + 4 * d].view(torch.int32)
+        w.copy_((torch.randint(64, 128, w.shape, device="cuda", generator=gen, dtype=torch.int32) << 16) | 0x3400)
+    cache.tail.copy_(torch.randn(cache.tail.shape, device="cuda", generator=gen))
+
+
+def test_more_units_than_a_cta_lists_at_a_time():
+    """200 groups of five rows with tables of their own and 64 kv heads: 86 units to a CTA, that share."""
+    kvh, d, rows = 64, 64, 1000
+    cache = make(rows, kvh, d, "bf16", 0, max_length=16 * 64, pages=1400)
+    random_pages(cache, 2)
+    table = torch.full((rows, cache.block_table.shape[1]), -1, dtype=torch.int32)
+    for g in range(200):
+        table[5 * g:5 * g + 5, :7] = torch.arange(7 * g, 7 * g + 7, dtype=torch.int32)
+    cache.block_table.copy_(table)
+    cache.lengths.fill_(7 * 64)
+    q = query(rows, 1, 8 * kvh, d, "bf16", 9)
+    o = torch.arange(0, rows + 1, 5, dtype=torch.int32, device="cuda")
+    got = cache.attend(0, q, groups=o, out_dtype=torch.float32)
+    cache.check()
+    want = cache.attend(0, q, out_dtype=torch.float32)
+    assert set(shares(cache, q, None, o)) == {7} and not torch.equal(got, want)
+    close(got[::7].reshape(-1, d), want[::7].reshape(-1, d).double().cpu().numpy(), 2 * FINE_TOL)
