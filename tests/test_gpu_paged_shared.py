@@ -158,3 +158,28 @@ def test_more_units_than_a_cta_lists_at_a_time():
     want = cache.attend(0, q, out_dtype=torch.float32)
     assert set(shares(cache, q, None, o)) == {7} and not torch.equal(got, want)
     close(got[::7].reshape(-1, d), want[::7].reshape(-1, d).double().cpu().numpy(), 2 * FINE_TOL)
+
+
+@pytest.mark.parametrize("dt, span", [("bf16", 20), ("fp16", 10)])
+def test_scales_that_are_very_unlike_within_a_page(dt, span):
+    """Channels of the keys, and tokens of the values, whose sizes go down to 2^-20 of the largest, and queries that make up for it: every channel weighs the same.  A scale of
+    2^-20 is still a normal f16 number once the page's largest is 2^14, and its remainder has an error of 2^-19."""
+    kvh, d, rows, pages = 8, 128, 64, 46
+    cache = make(rows + 1, kvh, d, dt, 64, max_length=4096, pages=64)
+    g = torch.Generator().manual_seed(6)
+    n = pages * 64 + 64
+    down = torch.exp2(-span * torch.rand(d, generator=g))
+    k = (torch.randn(n, kvh, d, generator=g) * down).to(DT[dt])
+    v = (torch.randn(n, kvh, d, generator=g) * torch.exp2(-span * torch.rand(n, 1, 1, generator=g))).to(DT[dt])
+    o = ints(0, n)
+    cache.extend(rows=ints(rows), offsets=o)
+    cache.append(0, k.cuda(), v.cuda(), rows=ints(rows), offsets=o)
+    kids = list(range(rows))
+    cache.fork(ints(*[rows] * rows), ints(*kids))
+    q = (torch.randn(rows, 1, 4 * kvh, d, generator=g) / down).to(DT[dt]).cuda()
+    got = cache.attend(0, q, rows=ints(*kids), groups=ints(0, rows), out_dtype=torch.float32)
+    cache.check()
+    assert not torch.equal(got, cache.attend(0, q, rows=ints(*kids), out_dtype=torch.float32))
+    kk, vv = plain.held(f32(k), f32(v), 64)
+    for i in (0, 40):
+        close(got[i], plain.attention(f32(q[i].cpu()), kk, vv, d ** -0.5), FINE_TOL)
