@@ -5,8 +5,9 @@
 A stack of attention layers with random projections stands in for a model.  A common prefix is written once and forked into every request's row (pages are
 shared, only the 16-bit window is copied); requests bring prompts of their own, decode until they are done, and make room for the next ones; one
 in eight branches into two continuations half way.  A decode step (extend, then append and attend per layer, the prefix's pages once for all rows) is captured once
-in a CUDA graph: lengths and pages live on the device.  The first sequence that ends, the first branch that does and the prefix are checked in every layer: their attention against dense
-attention over what their pages hold, and of the first one what its pages hold against the keys that were written.
+in a CUDA graph: lengths and pages live on the device.  Reading the prefix once pays from about 3000 tokens on with the default of 32 rows; below, the same call attends row by row.  The first sequence that ends,
+the first branch that does and the prefix are checked in every layer: their attention, and that of the whole batch as a captured step calls it, against dense
+attention over what their pages hold, decoded here; and of the first one what its pages hold against the keys that were written, and against `read`.
 """
 from __future__ import annotations
 
@@ -54,7 +55,7 @@ def main(argv=None) -> dict:
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--rows", type=int, default=32)
-    ap.add_argument("--prefix", type=int, default=2048)
+    ap.add_argument("--prefix", type=int, default=4096)
     ap.add_argument("--requests", type=int, default=96)
     ap.add_argument("--new-tokens", type=int, default=128)
     ap.add_argument("--seed", type=int, default=0)
@@ -116,18 +117,21 @@ def main(argv=None) -> dict:
     with torch.cuda.graph(graph, stream=side):
         y = step()
 
-    def dense_error(row: int) -> float:
-        """The largest error, over the layers, of a row's attention against dense attention over what its pages and ring hold."""
-        q, worst = torch.randn(1, heads, dim, device="cuda", generator=gen).bfloat16(), 0.0
+    def dense_error(row: int, batch: bool = False) -> float:
+        """The largest error, over the layers, of a row's attention against dense attention over what its pages and ring hold; of a row of the whole batch with its groups."""
+        q, worst = torch.randn(a.rows if batch else 1, heads, dim, device="cuda", generator=gen).bfloat16(), 0.0
         for layer in range(a.layers):
-            got = cache.attend(layer, q, rows=index(row)).float()
-            k, v = read_row(cache, layer, row)
-            s = torch.einsum("hd,thd->ht", q[0].float(), k.repeat_interleave(heads // kv_heads, 1)) * dim ** -0.5
+            if batch:
+                got = cache.attend(layer, q, rows=rows, groups=groups)[row].float()
+            else:
+                got = cache.attend(layer, q, rows=index(row))[0].float()
+            k, v = decode_row(cache, layer, row)
+            s = torch.einsum("hd,thd->ht", q[row if batch else 0].float(), k.repeat_interleave(heads // kv_heads, 1)) * dim ** -0.5
             want = torch.einsum("ht,thd->hd", torch.softmax(s, -1), v.repeat_interleave(heads // kv_heads, 1))
-            worst = max(worst, float((got[0] - want).norm() / want.norm()))
+            worst = max(worst, float((got - want).norm() / want.norm()))
         return worst
 
-    errors, branches, held = {}, [], None
+    errors, branches, held, batch = {}, [], None, {}
     done = branched = decoded = moved = 0
     torch.cuda.synchronize()
     began = time.perf_counter()
@@ -152,7 +156,13 @@ def main(argv=None) -> dict:
                 if first:
                     errors["first"] = dense_error(0)
                     _, key, _ = layers[0].project(torch.cat(history))
-                    held = float((read_row(cache, 0, 0)[0] - key.float()).norm() / key.float().norm())
+                    held = float((decode_row(cache, 0, 0)[0] - key.float()).norm() / key.float().norm())
+                    batch["read"] = all(torch.equal(x, y) for i in range(a.layers) for x, y in zip(read_row(cache, i, 0), decode_row(cache, i, 0)))
+                    batch["error"] = dense_error(0, batch=True)
+                    # a prefix that was taken once for all rows is rounded otherwise
+                    q = torch.randn(a.rows, heads, dim, device="cuda", generator=gen).bfloat16()
+                    one, each = (cache.attend(0, q, rows=rows, out_dtype=torch.float32, **kw) for kw in (dict(groups=groups), {}))
+                    batch["shared"] = not torch.equal(one, each)
                 if branch:
                     errors["branch"] = dense_error(min(branch))
                 began += time.perf_counter() - paused
@@ -181,13 +191,40 @@ def main(argv=None) -> dict:
     errors["prefix"] = dense_error(home)
     out = {"requests": done, "branches": branched, "compactions": moved, "tokens": decoded, "seconds": round(seconds, 3),
            "tokens_per_s": round(decoded / seconds, 1), "free_pages": cache.free_pages(), "pages": pages,
-           "error": max(errors.values()), "errors": errors, "held": held}
+           "error": max(errors.values()), "errors": errors, "held": held, "batch": batch}
     print(out)
     return out
 
 
+def decode_row(cache: MuZeroPagedCache, layer: int, row: int):
+    """A row's keys and values as they stand in its pages and ring, [tokens, kv_heads, head_dim] in fp32: from the bytes, as the codec is defined."""
+    import ctypes
+    book = (ctypes.c_ubyte * 2048)()
+    cache._lib.mz_paged_books(book, (ctypes.c_ubyte * 16384)())
+    book = torch.tensor(list(book), device=cache.device).view(128, 16)
+    n, d, h = int(cache.lengths[row]), cache.head_dim, cache.kv_heads
+    np_ = max(0, n - cache.residual_length) // 64
+    raw = cache.store[layer, cache.block_table[row, :np_].long()]
+
+    def side(codes, words):
+        w = words.contiguous().view(torch.int32)
+        t, field = (w & 0xFFFF).short().view(torch.float16).double(), (w >> 16) & 0xFFFF
+        off = (field & 0x7FFF) >= 128
+        anchor = torch.where(off, field.short().view(torch.float16).double(), torch.zeros_like(t))
+        z = torch.where(off, torch.where(anchor < 0, 127, 0), field).long()
+        e = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).long()
+        return (anchor[..., None] + t[..., None] * (book[z[..., None], e] - z[..., None]) / 32).float()
+
+    kc, kw, vc, vw = raw.split([32 * d, 4 * d, 32 * d, 4 * d], -1)
+    k = side(kc.reshape(np_, h, d, 32), kw).permute(0, 3, 1, 2).reshape(np_ * 64, h, d)
+    v = side(vc.reshape(np_, h, d, 32), vw).reshape(np_, h, 64, d).transpose(1, 2).reshape(np_ * 64, h, d)
+    at = torch.arange(np_ * 64, n, device=cache.device) % cache.tail.shape[4]
+    ring = cache.tail[layer, row][:, :, at].float().transpose(1, 2)
+    return torch.cat([k, ring[0]]), torch.cat([v, ring[1]])
+
+
 def read_row(cache: MuZeroPagedCache, layer: int, row: int):
-    """A row's keys and values as they stand in its pages and ring, [tokens, kv_heads, head_dim] in fp32."""
+    """The same by the cache's own call."""
     n = int(cache.lengths[row])
     one = torch.tensor([row], dtype=torch.int32, device=cache.device)
     return cache.read(layer, rows=one, offsets=torch.tensor([0, n], dtype=torch.int32, device=cache.device), tokens=n, out_dtype=torch.float32)

@@ -183,3 +183,17 @@ def test_scales_that_are_very_unlike_within_a_page(dt, span):
     kk, vv = plain.held(f32(k), f32(v), 64)
     for i in (0, 40):
         close(got[i], plain.attention(f32(q[i].cpu()), kk, vv, d ** -0.5), FINE_TOL)
+
+
+@pytest.mark.parametrize("args, shared", [(["--rows", "32", "--requests", "33", "--new-tokens", "6"], True), (["--rows", "8", "--prefix", "500", "--requests", "9", "--new-tokens", "20"], False)])
+def test_the_example_shares_its_prefix(args, shared):
+    """With its default prefix the serving example's batch takes the prefix once; its attention is checked against pages that are decoded in torch (bf16 output), and so is `read`."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_serving.py")
+    spec = importlib.util.spec_from_file_location("paged_serving", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    out = m.main(["--layers", "2", *args])
+    assert out["batch"]["shared"] == shared and out["batch"]["read"]
+    assert max(out["batch"]["error"], out["error"]) <= 2.0 ** -8
