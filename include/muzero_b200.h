@@ -466,7 +466,7 @@ int mz_paged_attention_view(const mz_paged_cache* cache, int layer, const mz_pag
 
 /*
  * Tokens back as ordinary keys and values: entry i's places offsets[i] .. offsets[i+1] - 1 of key and value get the tokens first[i], first[i] + 1, ... (NULL: from
- * 0) of row rows[i] (NULL: row i), as their codes stand for them, rounded once and held to the type's finite range.  Tokens that a row does not have are zero; places that no
+ * 0) of row rows[i] (NULL: row i), as their codes stand for them, rounded once and held to the type's finite range.  Tokens that a row does not have, before its first or behind its last, are zero; places that no
  * entry has, or at or beyond `tokens`, are left as they are.  Rows may be repeated.  batch <= 4096.
  * Replaces: the range dequantizer of muzero/cache/layer.py:303-345 for the paged cache.
  */

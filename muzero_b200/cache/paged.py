@@ -233,7 +233,7 @@ class MuZeroPagedCache:
              tokens: Optional[int] = None, out: Optional[tuple] = None, out_dtype: Optional[torch.dtype] = None) -> tuple:
         """Tokens of rows as ordinary keys and values [tokens, kv_heads, head_dim], what their codes stand for: places ``offsets[i]`` to ``offsets[i+1]`` get the
         tokens from ``first[i]`` on (from 0 without ``first``) of row ``rows[i]`` (row i without ``rows``).  Tokens that a row does not have read as zero, so equal steps
-        of ``offsets`` give a padded batch.  ``tokens``: places in all, which the host has to know; or ``out``: the two tensors to write, of any
+        of ``offsets`` give a padded batch (with a negative ``first`` padded on the left).  ``tokens``: places in all, which the host has to know; or ``out``: the two tensors to write, of any
         strides with whole 16-byte pieces.  Places that no entry has are left as they are.  ``out_dtype``: the cache's type, or float32."""
         n = self._entries(rows, offsets)
         if out is None:

@@ -65,10 +65,12 @@ __global__ void __launch_bounds__(READ_THREADS, READ_CTAS) read_kernel(const Rea
   __shared__ int s_warp[READ_THREADS / 32], s_entry, s_piece;
   if (tid < MZP_BOOKS * MZP_LEVELS / 16) ((uint4*)s_book)[tid] = ((const uint4*)book_table)[tid];
   static_assert(READ_THREADS >= MZP_BOOKS * MZP_LEVELS / 16, "one piece of the books per thread");
-  // ---- the entry and its piece: pieces are the pages that an entry's tokens stand in, or would
+  // ---- the entry and its piece: pieces are the pages that an entry's tokens stand in, or would (before the first token too)
+  auto page_of = [](long long token) { return token >> 6; };           // rounded down
+  static_assert(MZP_PAGE == 64, "page_of");
   auto pieces_of = [&](int i) {
     const long long first = a.first ? a.first[i] : 0, n = (long long)a.offsets[i + 1] - a.offsets[i];
-    return n > 0 && first >= 0 ? (int)((first + n - 1) / MZP_PAGE - first / MZP_PAGE + 1) : 0;
+    return n > 0 ? (int)(page_of(first + n - 1) - page_of(first) + 1) : 0;
   };
   if (tid == 0) s_entry = -1;
   long long before = 0;
@@ -95,14 +97,14 @@ __global__ void __launch_bounds__(READ_THREADS, READ_CTAS) read_kernel(const Rea
     return;
   }
   const long long first = a.first ? a.first[entry] : 0, place0 = a.offsets[entry] - first;       // token t of the row goes to place0 + t
-  const long long t0 = (first / MZP_PAGE + s_piece) * MZP_PAGE;                                    // the page's first token
+  const long long t0 = (page_of(first) + s_piece) * MZP_PAGE;                                      // the page's first token
   const int len = max(0, min(c.lengths[row], p.longest)), packed = mzp_packed(len, c.residual);
   // the page's tokens lo .. hi - 1 are asked for
   const int lo = (int)max(0ll, max(first - t0, -(place0 + t0)));
   const int hi = (int)max(0ll, min((long long)MZP_PAGE, min(a.offsets[entry + 1], a.tokens) - (place0 + t0)));
   const long long k_at = (place0 + t0) * a.k_stride_token, v_at = (place0 + t0) * a.v_stride_token;
   int id = -1;
-  if (t0 < packed) {
+  if (t0 >= 0 && t0 < packed) {
     const long long page = t0 / MZP_PAGE;
     id = page < c.width ? c.block_table[(long long)row * c.width + page] : -1;
     if (id < 0 || id >= c.pages) { id = -1; if (tid == 0) atomicOr(c.status, MZ_PAGED_BAD_INDEX); }
