@@ -28,6 +28,7 @@ from ..kernels._cabi import (MuZeroKernelError, PagedAttentionArgs, PagedCache, 
 
 PAGE_TOKENS = 64
 _STATUS = {1: "the pool has too few free pages", 2: "a sequence outgrew its row of the block table", 4: "a row or page index is outside the cache"}
+_NEEDS = 1024                                        # shapes of calls whose workspaces' sizes are remembered
 _ERRORS = sum(_STATUS)                               # the fourth bit says that the newest extension was refused; the device sets and clears it
 
 
@@ -205,6 +206,8 @@ class MuZeroPagedCache:
                 need = on_device(self.device, self._lib.mz_paged_attention_workspace_bytes, self._ref, b, lq, hq)
             else:
                 need = on_device(self.device, self._lib.mz_paged_attention_view_workspace_bytes, self._ref, ctypes.byref(view), b, lq, hq)
+            if len(self._needs) >= _NEEDS:                # (a window that is another one in each step)
+                self._needs.clear()
             self._needs[key] = need
         ws = self._workspace(need, st)
         # a block per call: another thread may attend another layer meanwhile
