@@ -52,6 +52,10 @@ def _index(t: Optional[torch.Tensor], what: str, device: torch.device, n: Option
     return t.data_ptr()
 
 
+def _capturing(device: torch.device) -> bool:
+    return device.type == "cuda" and on_device(device, torch.cuda.is_current_stream_capturing)
+
+
 class MuZeroPagedCache:
     """The tensors of a paged cache and the calls on them.
 
@@ -59,7 +63,8 @@ class MuZeroPagedCache:
     tail         bf16 or fp16 [layers, rows, 2, kv_heads, ring, head_dim]: the rows' rings, token t at place t % ring
     block_table  int32 [rows, width], lengths int32 [rows], page_refs int32 [pages], status int32 [1]
 
-    ``allocate`` makes them; the constructor takes them as they are.  All calls run on the current stream of the cache's device.
+    ``allocate`` makes them; the constructor takes them as they are.  All calls run on the current stream of the cache's device, each stream with a workspace of its own, and each
+    captured graph.
     """
 
     def __init__(self, *, store: torch.Tensor, tail: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, page_refs: torch.Tensor,
@@ -162,8 +167,11 @@ class MuZeroPagedCache:
                         v.stride(1), r, o, n, shape[0], max_new, stream_ptr(self.device)), "mz_paged_append")
 
     def _workspace(self, nbytes: int, stream: int) -> tuple:
-        # One per stream, grown by replacement.  An outgrown one is kept, as a captured graph may hold its address; one that has to grow at least
-        # doubles, so that its predecessors are smaller than it all together
+        # One per stream, grown by replacement; one that has to grow at least doubles, so that its predecessors are smaller than it all together.  Captured calls take theirs
+        # from the graph's own memory, like any tensor of a capture: two graphs that were captured on one stream may be replayed on two
+        if _capturing(self.device):
+            t = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=self.device)
+            return t.data_ptr(), t.numel(), t
         held = self._workspaces.get(stream)
         if held is None or held[-1][1] < nbytes:
             size = max(nbytes, 1 << 20, 2 * held[-1][1] if held else 0)

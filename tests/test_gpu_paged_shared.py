@@ -197,3 +197,36 @@ def test_the_example_shares_its_prefix(args, shared):
     out = m.main(["--layers", "2", *args])
     assert out["batch"]["shared"] == shared and out["batch"]["read"]
     assert max(out["batch"]["error"], out["error"]) <= 2.0 ** -8
+
+
+def test_graphs_of_one_stream_replayed_on_two():
+    """Two steps of layers, captured on the same stream, are replayed at the same time on two others: each has its own workspace, and so has what runs outside of them meanwhile."""
+    layers, rows, d, pages = 4, 64, 64, 60
+    cache = make(rows, 8, d, "bf16", 64, max_length=pages * 64 + 128, pages=pages, layers=layers)
+    for layer in range(layers):
+        random_pages(cache, 20 + layer)
+    cache.block_table.copy_(torch.arange(cache.block_table.shape[1], dtype=torch.int32) % pages)
+    cache.lengths.copy_(torch.arange(rows, dtype=torch.int32) * 3 + pages * 64 - 200)
+    q = [query(rows, 1, 32, d, "bf16", 16 + i) for i in range(2)]
+    calls = [lambda i=i, kw=kw: [cache.attend(layer, q[i], **kw) for layer in range(layers)] for i, kw in enumerate((dict(groups=ints(0, rows)), dict(window=1500, sinks=70)))]
+    want = [call() for call in calls]
+    capture, streams = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for call in calls + calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=capture):
+            outs.append(call())
+    for _ in range(20):
+        for out in outs:
+            for x in out:
+                x.zero_()
+        torch.cuda.synchronize()
+        for i, (graph, out) in enumerate(zip(graphs, outs)):
+            with torch.cuda.stream(streams[i % 2]):
+                graph.replay()
+        here = [call() for call in calls]
+        torch.cuda.synchronize()
+        for got in (outs[:2], outs[2:], here):
+            assert all(torch.equal(x, y) for a, b in zip(got, want) for x, y in zip(a, b))
+    cache.check()

@@ -40,3 +40,22 @@ def test_a_window_that_changes_in_every_step_does_not_fill_the_handle(cache):
     for window in range(1, 5000):
         cache.attend(0, q, window=window, sinks=window % 3)
     assert len(cache._needs) <= 1024 and len(set(cache.given)) == 1
+
+
+def test_captured_calls_have_workspaces_of_their_graph(cache, monkeypatch):
+    """While a stream is captured the handle keeps nothing: the memory is the graph's, and neither another graph's nor that of calls outside."""
+    q = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    cache.attend(0, q)
+    outside = cache.given[-1]
+    held = []
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: held.append(empty(*a, **kw)) or held[-1])
+    from muzero_b200.cache import paged
+    monkeypatch.setattr(paged, "_capturing", lambda device: True)
+    for kw in ({}, dict(window=5), {}):
+        cache.attend(0, q, **kw)
+        assert cache.given[-1] == (held[-1].data_ptr(), 100)
+    assert [w[:2] for w in cache._workspaces[7]] == [outside] and len({x for x in cache.given}) == 4
+    monkeypatch.setattr(paged, "_capturing", lambda device: False)
+    cache.attend(0, q)
+    assert cache.given[-1] == outside
