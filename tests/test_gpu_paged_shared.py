@@ -230,3 +230,46 @@ def test_graphs_of_one_stream_replayed_on_two():
         for got in (outs[:2], outs[2:], here):
             assert all(torch.equal(x, y) for a, b in zip(got, want) for x, y in zip(a, b))
     cache.check()
+
+
+@pytest.mark.parametrize("prompts, pages, pays", [((2000, 1900, 1500), (30, 22), False), ((6000, 5900, 4500), (92, 69), True)])
+def test_which_groups_share(prompts, pages, pays):
+    """Groups of one batch are weighed each for itself: the pair stays out, the others take their pages once, if what that saves is worth a call that shares (kv heads x pages x
+    (13 x 16 rows - 38 and 13 x 10 - 38) tenths of a row's visit: 57 thousand of 104, and 176)."""
+    groups = [(prompts[0], [3, 70, 9, 200] * 4), (prompts[1], [5, 6]), (prompts[2], [17] * 10)]
+    cache, members, _ = grouped(groups, 8, 128, "fp16", 64)
+    order = [r for kids in members for r in kids]
+    o = ints(0, 16, 18, 28)
+    q = query(len(order), 1, 64, 128, "fp16", 7)
+    want = cache.attend(0, q, rows=ints(*order), out_dtype=torch.float32)
+    got = cache.attend(0, q, rows=ints(*order), groups=o, out_dtype=torch.float32)
+    cache.check()
+    assert shares(cache, q, order, o) == [pages[0]] * 16 + [0] * 2 + [pages[1]] * 10
+    # (where the others share, the pair's steps are cut otherwise, and rounded otherwise)
+    assert all(torch.equal(got[i], want[i]) != pays for i in (*range(16), *range(18, 28))) and (pays or torch.equal(got, want))
+    close(got, want.double().cpu().numpy(), 2 * FINE_TOL)
+
+
+@pytest.mark.parametrize("d, dt, hq, lq, rows, own", [(128, "bf16", 32, 70, 6, [70, 100, 200]), (64, "fp16", 16, 130, 3, [5, 140, 131]), (128, "bf16", 8, 300, 2, [300, 40]),
+                                                      (64, "bf16", 20, 33, 5, [0, 33, 64])])
+def test_blocks_of_query_tokens(d, dt, hq, lq, rows, own):
+    """Tens to hundreds of query tokens of each row, some of them in the prefix, whose last pages then are not whole for every query."""
+    kvh, residual = 4, 64
+    cache, members, kv = grouped([(3300, (own * rows)[:rows])], kvh, d, dt, residual)
+    kids = members[0]
+    q = query(rows, lq, hq, d, dt, 17)
+    o = ints(0, rows)
+    want = cache.attend(0, q, rows=ints(*kids), out_dtype=torch.float32)
+    got = cache.attend(0, q, rows=ints(*kids), groups=o, out_dtype=torch.float32)
+    cache.check()
+    pages = min(min(plain.packed(len(kv[r][0]), residual), len(kv[r][0]) - lq + 1) // 64 for r in kids)
+    table = cache.block_table[kids].cpu()
+    pages = next((i for i in range(pages) if len(set(table[:, i].tolist())) > 1), pages)
+    assert shares(cache, q, kids, o) == [pages] * rows and not torch.equal(got, want)
+    close(got, want.double().cpu().numpy(), 2 * FINE_TOL)
+    r = 1
+    k, v = plain.held(f32(kv[kids[r]][0]), f32(kv[kids[r]][1]), residual)
+    at = [0, lq // 2, lq - 1]
+    n = len(k)
+    for j in at:
+        close(got[r, j:j + 1], plain.attention(f32(q[r, j:j + 1].cpu()), k[:n - lq + j + 1], v[:n - lq + j + 1], d ** -0.5), FINE_TOL)
