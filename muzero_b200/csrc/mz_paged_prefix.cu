@@ -135,16 +135,18 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
 }
 
 // ---- attention over the prefixes
-// Pages as they are, pages as operands, blocks of logits where the streams share their rows.  The barriers of an operand stage go round RING places, so that a team, which is behind its own last
+// Pages as they are, stages of keys and of values, blocks of logits where the streams share their rows.  Values stand longer than keys, until P is there: with 5 raw pages and 2 + 2, 3 + 2 (4 raw pages),
+// 2 + 3 (4) stages 32 rows behind 131072 tokens take 243, 249, 235 us; a sixth raw page, all products of a job written out, keys and values by code of their own 241, 243, 262.
+// The barriers of a stage go round RING places, so that a team, which is behind its own last
 // page by TEAMS pages and knows that what was in that one's stage before has been used, cannot take another phase of a barrier for the one that it waits for
-constexpr int RAWS = 5, STAGES = 2, BLOCKS = 3, RING = 4;
-static_assert(RAWS > TEAMS && RING >= TEAMS && (RING & (RING - 1)) == 0 && RING >= STAGES, "a wait could take another phase for its own");
+constexpr int RAWS = 4, K_STAGES = 2, V_STAGES = 3, BLOCKS = 3, RING = 4;
+static_assert(RAWS > TEAMS && RING >= TEAMS && (RING & (RING - 1)) == 0 && RING >= K_STAGES && RING >= V_STAGES, "a wait could take another phase for its own");
 template <int D>
 struct PrefixSmem {
   static constexpr int PLANE = MZP_PAGE * D * 2;                                 // a page's keys, or values, in 16 bits
   static constexpr int PAGE_BYTES = 72 * D;
   static constexpr int SCALES = 16, ROWS = 2 * D;                                // ROWS: rows of codes of a page
-  static constexpr int KEYS = 0, VALUES = STAGES * 2 * PLANE, RAW = 2 * VALUES, BOOK = RAW + RAWS * PAGE_BYTES, TERMS = BOOK + MZP_BOOKS * MZP_LEVELS;
+  static constexpr int KEYS = 0, VALUES = K_STAGES * 2 * PLANE, RAW = VALUES + V_STAGES * 2 * PLANE, BOOK = RAW + RAWS * PAGE_BYTES, TERMS = BOOK + MZP_BOOKS * MZP_LEVELS;
   static constexpr int ALIGN = 1024, TOTAL = TERMS + RAWS * ROWS * 16 + ALIGN;
   // columns of tensor memory: queries (A operand, two values to a column), logits of two or three jobs (P stands over their first half, its remainder over the other), outputs of the streams.
   // Where the streams have rows of their own there are two blocks of queries and of logits, where they share theirs one and three
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
             // short loops: a scheduler's instruction cache is full of the other duties, and what is executed once a page has to be fetched each time
             if (j >= 0) {
               const bool last = !both || (j & 1);
-              const uint32_t vd = values + v_page % STAGES * (2 * S::PLANE >> 4), t_o = S::TM_O + (j & 1) * D, t_s = S::tm_s(both) + (both ? j & 1 : v_block) * MZP_PAGE;
+              const uint32_t vd = values + v_page % V_STAGES * (2 * S::PLANE >> 4), t_o = S::TM_O + (j & 1) * D, t_s = S::tm_s(both) + (both ? j & 1 : v_block) * MZP_PAGE;
               if (elect()) {
 #pragma unroll 1
                 for (int part = 0; part < 3; ++part) {       // P and V as value and remainder: all but the remainders' product
@@ -439,7 +441,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
             }
             if (i < jobs) {
               const bool last = !both || (i & 1);
-              const uint32_t kd = keys + k_page % STAGES * (2 * S::PLANE >> 4), t_q = S::TM_Q + (both ? (i & 1) * (D / 2) : 0), t_s = S::tm_s(both) + (both ? i & 1 : k_block) * MZP_PAGE;
+              const uint32_t kd = keys + k_page % K_STAGES * (2 * S::PLANE >> 4), t_q = S::TM_Q + (both ? (i & 1) * (D / 2) : 0), t_s = S::tm_s(both) + (both ? i & 1 : k_block) * MZP_PAGE;
               if (elect()) {
 #pragma unroll 1
                 for (int part = 0; part < 2; ++part) {       // remainder, then value: what is summed first is small, and so is what the tensor cores cut off of it
@@ -566,8 +568,9 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
           bar_wait(bar(x.raw_full[slot]), raw_phase, failed);
 #pragma unroll 1
           for (int side = 0; side < 2; ++side) {
-            if (page >= STAGES) bar_wait(bar(x.free[side][(page - STAGES) % RING]), (page - STAGES) / RING & 1, failed);
-            const uint32_t at = (side ? v_at : k_at) + page % STAGES * 2 * S::PLANE, turn = side ? v_turn : k_turn, row = side ? v_row : k_row;
+            const int stages = side ? V_STAGES : K_STAGES;
+            if (page >= stages) bar_wait(bar(x.free[side][(page - stages) % RING]), (page - stages) / RING & 1, failed);
+            const uint32_t at = (side ? v_at : k_at) + page % stages * 2 * S::PLANE, turn = side ? v_turn : k_turn, row = side ? v_row : k_row;
             const uint4 term = lds128(terms + ((slot * 2 + side) * D + row) * 16), book = book128(sbook + (term.w & 0x7f0u));
             const uint32_t from = raw + side * 36 * D + 32 * row;
             const __half2 step = bits_half2(term.x), zero = bits_half2(term.y);
