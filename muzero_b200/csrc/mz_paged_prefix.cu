@@ -8,17 +8,17 @@
 // passes 2^15 (the output in tensor memory is scaled then), so P is a f16 number, and what is lost below its smallest one is under 2^-31 of the largest.
 // The output's running sums are held in fp32 outside the tensor cores (SUM_JOBS).
 // Scales of rows of codes are f16 as well: one below 2^-21 of its page's largest loses bits, 2^-32 of the page's largest value.
-// Measured, the output's error against the call without sharing: 1.4e-6 (64 rows behind 4224 tokens) to 1.3e-5 (32 rows behind 131072); with one f16 number for P and V 2e-4 and 10 to 40 us less,
-// with one for K 1.0e-3 where channels differ by a factor of e^2.5.
+// Measured, the output's error against the call without sharing: 1.4e-6 (64 rows behind 4224 tokens) to 1.0e-5 (32 rows behind 131072; against 64 bits 6.6e-6, without sharing 1.1e-5).  With one f16
+// number for P and V 2e-4 and 10 to 40 us less, with one for K 1.0e-3 where channels differ by a factor of e^2.5.
 //
 // Work.  Groups, tiles, units, the line and its cut: mz_paged_prefix.cuh.  A CTA per SM, its warps by duty: a page is copied as it is (one bulk copy), its rows' words are decoded, its codes become
 // f16 operands (MN-major, 128-byte swizzle: a thread has a row of 64 codes and stores it as 8 pieces of 16 bytes, nothing is transposed), products, softmax.  Queries and P are operands in tensor
 // memory, where 512 columns hold two blocks of queries, two or three of logits with P over them, and two outputs.  Two streams of four softmax warps: with more than 128 rows each has half of
 // the rows, otherwise they take the pages in turn and their outputs are merged at the end.
 //
-// Measured (B200 at 1965 MHz, 8 kv heads, head_dim 128): 32 rows x 4 heads behind 131072 tokens 147 us (its 68.7 GFLOP would take 42 us at the measured cuBLAS rate), 12 prompts of 500 to 16001
-// tokens for 4 rows x 8 heads, f16, 145 us (114 with P as one number).  A page takes 2300 cycles where the tensor cores need 788 and levels and softmax 1240 instructions on the busiest scheduler; no unit is saturated (issue 55 %,
-// logic pipe 40 %, ex2 25 %): jobs go round from products to softmax and back, and instruction fetch is a part of every turn.
+// Measured (B200 at 1965 MHz, 8 kv heads, head_dim 128): 32 rows x 4 heads behind 131072 tokens 202 us (its 68.7 GFLOP would take 42 us at the measured cuBLAS rate), 12 prompts of 500 to 16001
+// tokens for 4 rows x 8 heads, f16, 154 us.  A page takes 3300 cycles where the tensor cores need 1310 (keys 530, values 780); no unit is saturated (issue 51 %, tensor pipe 44 %, logic pipe 35 %, ex2
+// and conversions 21 %): jobs go round from products to softmax and back, and instruction fetch is a part of every turn.
 #include <algorithm>
 #include <atomic>
 

@@ -35,12 +35,12 @@ struct MzpTiles {
     rows = ((m + count - 1) / (count > 0 ? count : 1) + 7) / 8 * 8;
     weight = rows > MZP_TILE_ROWS / 2 ? 2 : 1;
   }
-  __host__ __device__ __forceinline__ int cost() const { return count * (20 + 18 * weight); }      // of a page, in tenths of a row's visit to it without sharing
+  __host__ __device__ __forceinline__ int cost() const { return count * (10 + 24 * weight); }      // of a page, in tenths of a row's visit to it without sharing
 };
-// Whether sharing pays.  A page of a prefix costs one kv head 2.6 ns of the machine per row and pass without sharing (3.5 with 8 query rows to a step; head_dim 64: 1.9 and 2.5) and with it 10 ns per
-// tile of at most 128 query rows, 14.7 above (7.0 and 10.7), and a call that shares takes 28 us more in the first place (24).  In tenths of a row's visit to a page; measured on both sides, 32 query
-// heads on 8 kv heads, without / with: 8 rows of 4096 tokens 38 / 56 us, of 16384 71 / 71, of 65536 201 / 130, 4 rows of 65536 116 / 126, 32 rows of 1024 38 / 56, of 4096 73 / 65, 64 rows of 1024 60 / 73,
-// of 4096 126 / 89; 8 query rows to a step: 4 rows of 65536 148 / 130, 16 of 4096 60 / 63.  cost: of a page's tiles (MzpTiles)
+// Whether sharing pays.  A page of a prefix costs one kv head 2.6 ns of the machine per row and pass without sharing (3.5 with 8 query rows to a step; head_dim 64: 1.9 and 2.5) and with it 9 ns per
+// tile of at most 128 query rows, 15 above (6.3 and 11), and a call that shares takes 28 us more in the first place (24).  In tenths of a row's visit to a page; measured on both sides, 32 query
+// heads on 8 kv heads, without / with: 8 rows of 4096 tokens 37 / 56 us, of 16384 71 / 69, of 65536 200 / 118, 4 rows of 65536 116 / 120, 32 rows of 1024 38 / 56, of 4096 73 / 67, 64 rows of 1024 60 / 73,
+// of 4096 125 / 89; 8 query rows to a step: 4 rows of 65536 149 / 120, 16 of 4096 60 / 65.  cost: of a page's tiles (MzpTiles)
 __host__ __device__ __forceinline__ long long mzp_gain(long long pages, int kv_heads, long long rows_passes, int nr, int cost) {
   const long long each = rows_passes * (nr > 4 ? 13 : 10) - cost;
   return each > 0 ? pages * kv_heads * each : 0;

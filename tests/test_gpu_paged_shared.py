@@ -235,7 +235,7 @@ def test_graphs_of_one_stream_replayed_on_two():
 @pytest.mark.parametrize("prompts, pages, pays", [((2000, 1900, 1500), (30, 22), False), ((6000, 5900, 4500), (92, 69), True)])
 def test_which_groups_share(prompts, pages, pays):
     """Groups of one batch are weighed each for itself: the pair stays out, the others take their pages once, if what that saves is worth a call that shares (kv heads x pages x
-    (13 x 16 rows - 38 and 13 x 10 - 38) tenths of a row's visit: 57 thousand of 104, and 176)."""
+    (13 x 16 rows - 34 and 13 x 10 - 34) tenths of a row's visit: 59 thousand of 104, and 181)."""
     groups = [(prompts[0], [3, 70, 9, 200] * 4), (prompts[1], [5, 6]), (prompts[2], [17] * 10)]
     cache, members, _ = grouped(groups, 8, 128, "fp16", 64)
     order = [r for kids in members for r in kids]
