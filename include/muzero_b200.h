@@ -453,7 +453,7 @@ int mz_paged_attention(const mz_paged_cache* cache, int layer, const mz_paged_at
  *                the group.  The result is that of mz_paged_attention but for rounding: keys, values and probabilities are taken with 22 bits, sums with 24 (about 1e-5 of the
  *                output).  Entries that no group has, groups of one, rows without a common page, and rows
  *                that are empty or without a whole page in sight go as they do there, the latter without keeping the others from sharing.  Numbers that do not ascend from 0
- *                or more to `batch` or less share nothing and set MZ_PAGED_BAD_INDEX.
+ *                or more to `batch` or less share nothing and set MZ_PAGED_BAD_INDEX; where the tables could not hold enough for sharing to pay they are not looked at.
  * Not both.  workspace: mz_paged_attention_view_workspace_bytes() bytes (NULL view: those of mz_paged_attention), 32-byte aligned with groups.
  */
 typedef struct {

@@ -199,6 +199,20 @@ def test_the_example_shares_its_prefix(args, shared):
     assert max(out["batch"]["error"], out["error"]) <= 2.0 ** -8
 
 
+@pytest.mark.parametrize("d, batch, lq, hq", [(128, 64, 1, 32), (64, 9, 40, 20), (128, 64, 512, 32)])
+def test_the_size_of_a_workspace_for_groups(d, batch, lq, hq):
+    """What a call with groups needs beyond one without: records, sums of long runs, and a few numbers per entry and group."""
+    import ctypes
+    from muzero_b200.kernels._cabi import PagedView
+    cache = make(batch, 4, d, "bf16", 64, max_length=1 << 17, pages=8)
+    o = ints(0, batch)
+    view = PagedView(0, 0, o.data_ptr(), 1)
+    lib = cache._lib
+    more = lib.mz_paged_attention_view_workspace_bytes(cache._ref, ctypes.byref(view), batch, lq, hq) - lib.mz_paged_attention_workspace_bytes(cache._ref, batch, lq, hq)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert 0 <= more - ((batch * lq * hq + 256 * sms) * (4 * d + 8) + 1024 * sms * d) <= 1024 + 16 * batch
+
+
 def test_graphs_of_one_stream_replayed_on_two():
     """Two steps of layers, captured on the same stream, are replayed at the same time on two others: each has its own workspace, and so has what runs outside of them meanwhile."""
     layers, rows, d, pages = 4, 64, 64, 60
