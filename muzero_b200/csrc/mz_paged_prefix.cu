@@ -16,9 +16,9 @@
 // memory, where 512 columns hold two blocks of queries, two or three of logits with P over them, and two outputs.  Two streams of four softmax warps: with more than 128 rows each has half of
 // the rows, otherwise they take the pages in turn and their outputs are merged at the end.
 //
-// Measured (B200 at 1965 MHz, 8 kv heads, head_dim 128): 32 rows x 4 heads behind 131072 tokens 202 us (its 68.7 GFLOP would take 42 us at the measured cuBLAS rate), 12 prompts of 500 to 16001
-// tokens for 4 rows x 8 heads, f16, 154 us.  A page takes 3300 cycles where the tensor cores need 1310 (keys 530, values 780); no unit is saturated (issue 51 %, tensor pipe 44 %, logic pipe 35 %, ex2
-// and conversions 21 %): jobs go round from products to softmax and back, and instruction fetch is a part of every turn.
+// Measured (B200 at 1965 MHz, 8 kv heads, head_dim 128): 32 rows x 4 heads behind 131072 tokens 195 us (its 68.7 GFLOP would take 42 us at the measured cuBLAS rate), 12 prompts of 500 to 16001
+// tokens for 4 rows x 8 heads, f16, 147 us.  A page takes 3200 cycles where the tensor cores need 1310 (keys 530, values 780); no unit is saturated (issue 53 %, tensor pipe 46 %, logic pipe 36 %, ex2
+// and conversions 22 %): jobs go round from products to softmax and back, and instruction fetch is a part of every turn.
 #include <algorithm>
 #include <atomic>
 
@@ -162,7 +162,7 @@ struct alignas(16) Segment { int first, row, head, m0, rows, page, count, pad; l
 constexpr int ISSUE_UNROLL = 4;
 // Jobs of a stream that go into one accumulator.  The tensor cores cut their running sums off, always towards zero: up to 2^-23 of the sum in each of a job's 12 products.  Measured with values of one
 // sign: 2.2e-4 of the output after 432 jobs, 1.1e-4 after 216.  So after this many the sum is added in fp32 to what there is: below 2e-5.  32 rows behind 131072 tokens with 8 / 16 / 32 / all jobs to
-// an accumulator 259 / 253 / 245 / 245 us
+// an accumulator 259 / 253 / 245 / 245 us (with two stages of values)
 constexpr int SUM_JOBS = 32;
 constexpr int SEGMENTS = 64;                     // of a CTA at a time
 struct PrefixShared {
@@ -515,8 +515,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_kernel(const PrefixA
         for (; page < pages; page += 2) {
           const int slot = page % RAWS;
           const uint32_t raw = sbase + S::RAW + slot * PB + 32 * D;
-          // the place's page before this one was the other decoder's: it has been there, so the parity of the next phase is this page's
-          if (page >= RAWS) bar_wait(bar(x.scaled[(page - RAWS) % S::SCALES]), (page - RAWS) / S::SCALES & 1, failed);
+          static_assert(RAWS % 2 == 0, "the page before in this place was this decoder's: it has waited for its phase");
           bar_wait(bar(x.raw_full[slot]), page / RAWS & 1, failed);
           const bool there = x.there[slot];
           int e[2];
